@@ -336,6 +336,177 @@ int kg_l2_touch_line(int grid, int workgroup, int thread, int* line);
  * reference: the index map its kernel uses, for host-side checks. */
 int kg_rmsnorm_rows_of(int rows, int channels, int region, int workgroup, int* grid, int* first_row, int* count);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Learning from the network's answers: operators on device buffers. No counterpart in the reference, which only
+ * evaluates. Each call enqueues its kernels on `stream` (a hipStream_t of `device`; NULL is its null stream) and returns
+ * without waiting. It allocates nothing, copies nothing and keeps nothing for a later call, so it may be captured into a
+ * graph, and calls on different streams may overlap as long as their buffers differ. The argument structures are read
+ * before the call returns; every pointer in them is memory of `device` unless it says otherwise, aligned to its elements.
+ * The caller's current device is left as it was. Outputs must not overlap inputs. Element types are KG_PRECISION_F32, _F16
+ * and _BF16; all sums and row statistics are float or wider.
+ * ------------------------------------------------------------------------------------------------------------------ */
+
+/* The clipped policy loss with a KL term of `rows` rows of logits, and its gradient. Row i holds `columns` logits z (362
+ * moves of a network's raw row, columns = 362 and ld = output_row_len; or the tokens of a language policy) and the move a
+ * that was played. Over the legal columns, with p = softmax(logit_scale z) and r the reference's:
+ *   logp = log p[a], ratio = exp(logp - old_logp),
+ *   loss = weight (-min(ratio adv, clamp(ratio, 1 - clip_low, 1 + clip_high) adv) + kl_coef kl),
+ *   kl   = sum p log(p / r) with ref_logits; e^d - d - 1, d = ref_logp - logp, with ref_logp; 0 with neither,
+ * and grad[i] is the gradient of loss[i] with respect to row i's logits (scale weight to scale both). Illegal columns take
+ * no part whatever they hold, and their gradient is 0. A row whose action is outside [0, columns) is padding: loss, logp, kl
+ * and gradient 0. A row whose action is illegal or has the logit -infinity, or that has no legal column, takes no part
+ * either: logp -infinity, the rest 0. At the clip's border the ratio counts as unclipped. NaN in a legal column makes the
+ * row's results NaN. */
+typedef struct {
+  int rows, columns;
+  int type;                    /* of logits, ref_logits and grad */
+  const void* logits;          /* [rows] rows of ld elements */
+  long long ld;
+  const unsigned char* legal;  /* [rows] rows of ld_legal bytes, nonzero where legal; NULL: every column */
+  long long ld_legal;
+  const int* action;           /* [rows] */
+  const float* old_logp;       /* [rows] log-probability of the action when it was played */
+  const float* advantage;      /* [rows] */
+  const float* weight;         /* [rows] or NULL: 1 */
+  const void* ref_logits;      /* [rows] rows of ld_ref, under the same legality and scale; or NULL */
+  long long ld_ref;
+  const float* ref_logp;       /* [rows] or NULL (not with ref_logits) */
+  double logit_scale;          /* 1 / temperature, > 0 */
+  double clip_low, clip_high;  /* >= 0, clip_low < 1 */
+  double kl_coef;
+  float* loss;                 /* [rows] */
+  float* logp;                 /* [rows] */
+  float* kl;                   /* [rows] */
+  void* grad;                  /* [rows] rows of ld_grad (columns past `columns` stay as they are); or NULL */
+  long long ld_grad;
+} kg_policy_loss_args;
+int kg_policy_loss(int device, void* stream, const kg_policy_loss_args* args);
+
+/* The preference loss of `pairs` pairs of lines of moves (or token sequences), and its gradient. The sequences lie packed in
+ * `rows` rows of logits: sequence q is rows [offsets[q], offsets[q + 1]), pair i prefers sequence 2 i to 2 i + 1. A row
+ * whose label is outside [0, columns) (a prompt, a forced move) is not counted. With L(q) the sum of log softmax(z)[label]
+ * over the sequence's counted rows (`average`: their mean; 0 for none),
+ *   margin = beta ((L(2i) - ref_logp[2i]) - (L(2i+1) - ref_logp[2i+1])),
+ *   loss   = weight (-(1 - label_smoothing) log sigmoid(margin) - label_smoothing log sigmoid(-margin)),
+ * and grad is the gradient of the sum of the losses with respect to every logit: 0 in rows that are not counted and in
+ * rows before offsets[0] or from offsets[2 pairs] on. offsets must not decrease; they are cut to [0, rows]. A counted label
+ * whose logit is -infinity makes its pair's results infinite or NaN, as the formula has it. */
+typedef struct {
+  int rows, columns;
+  int type;                 /* of logits and grad */
+  const void* logits;       /* [rows] rows of ld elements */
+  long long ld;
+  const int* label;         /* [rows] */
+  int pairs;
+  const int* offsets;       /* [2 pairs + 1] */
+  const float* ref_logp;    /* [2 pairs] L(q) of the reference policy */
+  const float* weight;      /* [pairs] or NULL: 1 */
+  double beta;              /* > 0 */
+  double label_smoothing;   /* in [0, 0.5] */
+  int average;
+  float* loss;              /* [pairs] */
+  float* margin;            /* [pairs] */
+  float* seq_logp;          /* [2 pairs] L(q) */
+  void* grad;               /* [rows] rows of ld_grad (columns past `columns` stay as they are); or NULL */
+  long long ld_grad;
+  void* workspace;          /* kg_preference_loss_workspace(rows) bytes, 16-byte aligned, this call's own until it has run */
+} kg_preference_loss_args;
+int kg_preference_loss(int device, void* stream, const kg_preference_loss_args* args);
+size_t kg_preference_loss_workspace(int rows);
+
+/* One AdamW step over `count` tensors at once (decoupled weight decay), in float:
+ *   g = grad_scale grad; m = beta1 m + (1 - beta1) g; v = beta2 v + (1 - beta2) g^2;
+ *   p = p (1 - lr weight_decay) - (lr / (1 - beta1^step)) m / (sqrt(v) / sqrt(1 - beta2^step) + eps).
+ * p is the tensor's master copy where it has one (param then gets its rounding), else param itself. 16-bit parameters
+ * without a master lose steps below half their spacing.
+ * The moments of all tensors lie in one state, tensor t's elements from element KG_ADAMW_BLOCK * first_block on, in whole
+ * blocks of KG_ADAMW_BLOCK (the caller chooses first_block so that no two overlap; zero-filled for a new optimizer).
+ * - state_bits 32: m and v, floats.
+ * - state_bits 8: m as sign, 4 exponent and 3 mantissa bits (e4m3) times 2^(m_exp - 135), and sqrt(v) as 3 exponent and 5
+ *   mantissa bits (code c: c below 64, else (c mod 32 + 32) 2^(c / 32 - 1)) times 2^(v_exp - 138), one exponent a block.
+ *   Codes are rounded up with the probability of the part cut off (a moving average of 0.1 % a step would never move
+ *   by nearest rounding), from a hash of `seed` and the element's place in the state: the same seed gives the same bits,
+ *   each step wants another. A positive v never becomes 0, so a tiny one cannot let its m through undamped. A gradient
+ *   that is not finite makes its element NaN, in 8 bits its block's moments.
+ * Gradients may change place from call to call. kg_adamw_values fills the scalars that a step takes; with `values` NULL
+ * the call uses them from `hyper` as it is, so a captured step repeats its lr, step and seed: a program that replays a
+ * captured step gives `values`, device memory that it fills before each replay. */
+#define KG_ADAMW_BLOCK 256
+typedef struct {
+  void* param;
+  const void* grad;
+  float* master;           /* or NULL */
+  long long elements;      /* >= 0 */
+  long long first_block;   /* >= 0 */
+  double weight_decay;
+  int param_type, grad_type;
+} kg_adamw_tensor;
+typedef struct {
+  double lr, beta1, beta2, eps;
+  double grad_scale;
+  long long step;          /* from 1 */
+  unsigned seed;           /* state_bits 8 */
+} kg_adamw_hyper;
+typedef struct {
+  float lr, beta1, beta1_rest, beta2, beta2_rest, eps, grad_scale, step_size, root_scale;
+  unsigned seed;
+} kg_adamw_values_t;
+typedef struct {
+  int state_bits;          /* 8 or 32 */
+  void* m;                 /* floats, or bytes */
+  void* v;
+  unsigned char* m_exp;    /* state_bits 8: one byte a block; else unused */
+  unsigned char* v_exp;
+} kg_adamw_state;
+/* tensors and state are host memory; `values` is device memory or NULL. */
+int kg_adamw_step(int device, void* stream, int count, const kg_adamw_tensor* tensors, const kg_adamw_state* state,
+                  const kg_adamw_hyper* hyper, const kg_adamw_values_t* values);
+/* The scalars of a step (host only). */
+int kg_adamw_values(const kg_adamw_hyper* hyper, kg_adamw_values_t* out);
+/* The moments of `blocks` blocks as numbers: m and sqrt(v) in `type` (exact in KG_PRECISION_BF16 and _F32 for 8-bit states
+ * within their range). */
+int kg_adamw_moments(int device, void* stream, long long blocks, const kg_adamw_state* state, int type, void* m,
+                     void* root);
+
+/* Group norm with an activation on channels-last rows, under the board mask. x is [batch][points] rows of `channels`
+ * elements, row stride ldx, batch stride points ldx; group q is channels [q channels / groups, (q + 1) channels / groups).
+ * Over the points with a nonzero mask (all without one) and the channels of a group, mean and variance:
+ *   rstd = 1 / sqrt(variance + eps), y = act((x - mean) rstd gamma + beta), 0 where the mask is 0.
+ * Masked points take no part whatever they hold. A row without any point gives mean 0, rstd 1 / sqrt(eps) and zeros.
+ * act: KG_ACT_*. The statistics are outputs for the backward pass. */
+#define KG_ACT_IDENTITY 0
+#define KG_ACT_RELU 1
+#define KG_ACT_MISH 2
+#define KG_ACT_SILU 3
+typedef struct {
+  int batch, points, channels, groups;
+  int type;                /* of x, y, dy and dx */
+  int act;
+  double eps;              /* > 0 */
+  const void* x;
+  long long ldx;
+  const float* mask;       /* [batch][points] or NULL */
+  const float* gamma;      /* [channels] or NULL: 1 */
+  const float* beta;       /* [channels] or NULL: 0 */
+  float* mean;             /* [batch][groups]: written by kg_group_norm, read by kg_group_norm_backward */
+  float* rstd;             /* [batch][groups] */
+  void* workspace;         /* kg_group_norm_workspace bytes, 16-byte aligned, this call's own until it has run */
+  /* kg_group_norm */
+  void* y;                 /* rows of ldy */
+  long long ldy;
+  /* kg_group_norm_backward */
+  const void* dy;          /* rows of lddy */
+  long long lddy;
+  void* dx;                /* rows of lddx */
+  long long lddx;
+  float* dgamma;           /* [channels], sums over batch and points; or NULL */
+  float* dbeta;            /* [channels]; or NULL */
+} kg_group_norm_args;
+int kg_group_norm(int device, void* stream, const kg_group_norm_args* args);
+/* The gradients of a loss whose gradient with respect to y is dy (eps and y are not used). */
+int kg_group_norm_backward(int device, void* stream, const kg_group_norm_args* args);
+size_t kg_group_norm_workspace(int batch, int points, int channels, int groups, int backward);
+
 #ifdef __cplusplus
 }
 #endif

@@ -40,6 +40,8 @@ EXPORTS = [
     "kg_conv_geometry", "kg_conv_tile_of", "kg_conv_weight_load", "kg_conv_weight_chunk", "kg_float_tile_of", "kg_small_tile_of",
     "kg_junction_tile_of", "kg_gpool_tile_of", "kg_l2_touch_line", "kg_rmsnorm_rows_of",
     "kg_featurize", "kg_featurize_rows", "kg_evaluate_positions",
+    "kg_policy_loss", "kg_preference_loss", "kg_preference_loss_workspace", "kg_adamw_step", "kg_adamw_values",
+    "kg_adamw_moments", "kg_group_norm", "kg_group_norm_backward", "kg_group_norm_workspace",
 ]
 # Completion callback of kg_get_output_async: (user, status).
 DONE_FN = ctypes.CFUNCTYPE(None, ctypes.c_void_p, ctypes.c_int)
@@ -221,6 +223,18 @@ def lib():
         L.kg_gpool_tile_of.argtypes = [ci, ci, ci, ci] + [ctypes.POINTER(ci)] * 4
         L.kg_l2_touch_line.argtypes = [ci, ci, ci, ctypes.POINTER(ci)]
         L.kg_rmsnorm_rows_of.argtypes = [ci, ci, ci, ci] + [ctypes.POINTER(ci)] * 3
+        # The learning operators (learn.py gives their structures).
+        L.kg_policy_loss.argtypes = [ci, vp, vp]
+        L.kg_preference_loss.argtypes = [ci, vp, vp]
+        L.kg_preference_loss_workspace.argtypes = [ci]
+        L.kg_preference_loss_workspace.restype = ctypes.c_size_t
+        L.kg_adamw_step.argtypes = [ci, vp, ci, vp, vp, vp, vp]
+        L.kg_adamw_values.argtypes = [vp, vp]
+        L.kg_adamw_moments.argtypes = [ci, vp, ctypes.c_longlong, vp, ci, vp, vp]
+        L.kg_group_norm.argtypes = [ci, vp, vp]
+        L.kg_group_norm_backward.argtypes = [ci, vp, vp]
+        L.kg_group_norm_workspace.argtypes = [ci] * 5
+        L.kg_group_norm_workspace.restype = ctypes.c_size_t
         _ = cf
         _lib = L
     return _lib
@@ -397,6 +411,16 @@ def copy_outputs(raw, P: int, S: int, model_version: int, symmetry, policy_optim
     return _output_dicts(outs, owners)
 
 
+class DeviceArray:
+    """Float rows inside device memory that its owner keeps, as torch.as_tensor(..., device="cuda") takes them without a
+    copy (__cuda_array_interface__)."""
+
+    def __init__(self, owner, pointer, shape, strides):
+        self._owner = owner
+        self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": "<f4", "data": (pointer, False),
+                                         "strides": tuple(4 * s for s in strides), "version": 2}
+
+
 class Net:
     """A parsed KataGo model (NeuralNet::load_model_file)."""
 
@@ -477,6 +501,15 @@ class Handle:
         ptrs = [ctypes.c_void_p() for _ in range(4)]
         _check(lib().kg_handle_device_buffers(self._h, *[ctypes.byref(p) for p in ptrs]))
         return tuple(p.value for p in ptrs)
+
+    def policy_rows(self, n: int, channel: int = 0) -> DeviceArray:
+        """Policy channel `channel` of the first n raw rows in the device output buffer, [n, 362] (pass last), in place: what
+        the last pass on the handle left there (run with out=None; wait for it with sync, or order the reader behind
+        `stream`)."""
+        if not 1 <= n <= self.max_batch or not 0 <= channel < self.net.P:
+            raise ValueError(f"policy_rows: n must be in [1, {self.max_batch}] and channel in [0, {self.net.P})")
+        return DeviceArray(self, self.device_buffers()[3] + 4 * channel * MAX_POLICY, (n, MAX_POLICY),
+                           (self.net.row_len, 1))
 
     def run(self, n: int, out: np.ndarray = None):
         """Forward pass on the inputs already in the device buffers; reads back into `out` when given."""

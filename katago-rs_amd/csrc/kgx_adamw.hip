@@ -1,0 +1,319 @@
+// The AdamW step over many tensors at once (kg_adamw_step), with moments in 32 or in 8 bits, and the moments as numbers.
+//
+// Bound by memory: 28 bytes an element in float, 14 with 16-bit parameters and gradients, float masters and 8-bit moments.
+// One launch covers up to kTensors tensors, whose descriptions travel as kernel arguments: nothing has to be uploaded, and a
+// captured launch carries them. Each workgroup takes kChunk consecutive elements of one tensor.
+//
+// 8 bits: a block of 256 elements is one wave, four elements a lane, so that its largest moment is a wave's reduction. A
+// block's unit is a power of two: scaling by it is exact, and so is every step of the rounding (the quotient by a code's
+// spacing, its floor, the comparison with the random part), which makes the codes a function of the moments alone. The file
+// is compiled without contraction into fused multiply-adds, so that the moments before the rounding are each formula's
+// plain sequence of float operations.
+#include "kgx_device.h"
+#include <climits>
+
+#include "kgx_learn.h"
+
+namespace kgx {
+
+namespace {
+
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned short u16x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned int u32_any __attribute__((aligned(1)));
+
+constexpr int kTensors = 72;                 // 48-byte descriptions in the 4 KB of kernel arguments
+constexpr int kBlock = KG_ADAMW_BLOCK;
+constexpr int kUnroll = 4, kWaves = 4;       // blocks a wave, waves a workgroup
+constexpr int kChunk = kBlock * kUnroll * kWaves;
+
+struct AdamTensor {
+  void* param;
+  const void* grad;
+  float* master;
+  long long elements, first_block;
+  float weight_decay;
+  short param_type, grad_type;
+};
+struct AdamArgs {
+  AdamTensor t[kTensors];
+  int start[kTensors];  // first workgroup of tensor i; INT_MAX past the last
+  kg_adamw_values_t values;
+  const kg_adamw_values_t* device_values;
+  void *m, *v;
+  unsigned char *m_exp, *v_exp;
+};
+static_assert(sizeof(AdamArgs) <= 4096, "kernel arguments");
+
+// Four elements at index i of a tensor of any element type; elements from n on read as 0 and are not written.
+__device__ __forceinline__ floatx4 load4(const void* p, int type, long long i, long long n) {
+  floatx4 f = {0.f, 0.f, 0.f, 0.f};
+  if (i + 4 <= n) {
+    if (type == PREC_F32) {
+      f = *(const f32x4_any*)((const float*)p + i);
+    } else {
+      const u16x4_any h = *(const u16x4_any*)((const unsigned short*)p + i);
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        f[j] = type == PREC_BF16 ? __uint_as_float((unsigned)h[j] << 16) : (float)__builtin_bit_cast(f16, (unsigned short)h[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (i + j < n)
+        f[j] = type == PREC_F32 ? ((const float*)p)[i + j]
+                                : type == PREC_BF16 ? (float)((const bf16*)p)[i + j] : (float)((const f16*)p)[i + j];
+  }
+  return f;
+}
+__device__ __forceinline__ void store4_any(void* p, int type, long long i, long long n, floatx4 f) {
+  if (i + 4 <= n) {
+    if (type == PREC_F32) {
+      *(f32x4_any*)((float*)p + i) = f;
+    } else {
+      u16x4_any h;
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        h[j] = type == PREC_BF16 ? __builtin_bit_cast(unsigned short, (bf16)f[j]) : __builtin_bit_cast(unsigned short, (f16)f[j]);
+      *(u16x4_any*)((unsigned short*)p + i) = h;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (i + j < n) {
+        if (type == PREC_F32) ((float*)p)[i + j] = f[j];
+        else if (type == PREC_BF16) ((bf16*)p)[i + j] = (bf16)f[j];
+        else ((f16*)p)[i + j] = (f16)f[j];
+      }
+  }
+}
+
+// A 32-bit hash: two rounds of a shift and an odd multiplier (the fraction of the golden ratio and of e). 16 bits each round
+// the first and the second moment.
+__device__ __forceinline__ unsigned mix32(unsigned x) {
+  x = (x ^ (x >> 16)) * 0x9E3779B9u;
+  x = (x ^ (x >> 15)) * 0xB7E15163u;
+  return x ^ (x >> 16);
+}
+
+__device__ __forceinline__ float exp_bits(int e) { return __uint_as_float((unsigned)e << 23); }
+// The unit of a block: 2^(exp - bias), NaN where the block held something that was no number. (A new state's exponents
+// are 0, below the least that a step writes.)
+__device__ __forceinline__ float unit_of(int exp, int bias) {
+  const int e = exp - bias + 127;
+  return exp == 255 ? __uint_as_float(0x7fc00000u) : exp_bits(e < 1 ? 1 : e);
+}
+// The exponent of a block whose largest magnitude has the bits `top`: the least unit in which it does not pass the largest
+// code (mantissas above it, `carry` short of the next power of two, go there).
+__device__ __forceinline__ int exp_of(unsigned top, unsigned carry, int least) {
+  const int e = (int)((top + carry) >> 23);
+  return e < least ? least : e > 255 ? 255 : e;
+}
+
+constexpr int M_BIAS = 135, M_LEAST = 9, V_BIAS = 138, V_LEAST = 12;
+constexpr unsigned M_CARRY = 0x1FFFFF, V_CARRY = 0x03FFFF;  // largest codes 1.75 and 1.96875 times a power of two
+
+// |x| 2^(bias - exp) as e4m3 without its sign, rounded up where the cut part exceeds the random part u of its spacing.
+__device__ __forceinline__ unsigned encode_m(float y, float u) {
+  int e = (int)(__float_as_uint(y) >> 23) - 127;
+  e = e < -6 ? -6 : e;
+  const float t = y * exp_bits(127 + 3 - e);
+  return (unsigned)((e + 6) << 3) + (unsigned)(t + u);
+}
+// The same as e3m5; a positive value never becomes 0.
+__device__ __forceinline__ unsigned encode_v(float y, float u) {
+  int e = (int)(__float_as_uint(y) >> 23) - 127;
+  e = e < 5 ? 5 : e;
+  const float t = y * exp_bits(127 + 5 - e);
+  unsigned n = (unsigned)(t + u);
+  n = n == 0 && y > 0.f ? 1 : n;
+  return (unsigned)((e - 5) << 5) + n;
+}
+__device__ __forceinline__ float decode_v(unsigned c) {
+  const unsigned n = c < 64 ? c : ((c & 31) | 32) << ((c >> 5) - 1);
+  return (float)n;
+}
+
+__device__ __forceinline__ unsigned wave_max(unsigned v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o));
+  return v;
+}
+
+template <bool BYTES>
+__global__ __launch_bounds__(kWaves * 64) void adamw_kernel(AdamArgs a) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wg = blockIdx.x;
+  // The tensor of this workgroup: the last one that starts at or before it.
+  int ti = __popcll(__ballot(a.start[lane] <= wg));
+  ti += __popcll(__ballot(lane < kTensors - 64 && a.start[64 + (lane < kTensors - 64 ? lane : 0)] <= wg));
+  ti = __builtin_amdgcn_readfirstlane(ti) - 1;
+  const AdamTensor t = a.t[ti];
+  const kg_adamw_values_t h = a.device_values ? *a.device_values : a.values;
+  const float decay = (float)(1.0 - (double)h.lr * (double)t.weight_decay);
+  const long long base = (long long)(wg - a.start[ti]) * kChunk + (wave * kUnroll) * kBlock + lane * 4;
+  const void* weights = t.master ? (const void*)t.master : t.param;
+  const int wtype = t.master ? PREC_F32 : t.param_type;
+  const long long state0 = t.first_block * kBlock;
+
+  floatx4 p[kUnroll], g[kUnroll], m[kUnroll], v[kUnroll];
+  unsigned mc[kUnroll], vc[kUnroll], me[kUnroll], ve[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; u++) {
+    const long long i = base + u * kBlock;
+    if (i - lane * 4 >= t.elements) break;  // (whole blocks: uniform over the wave)
+    p[u] = load4(weights, wtype, i, t.elements);
+    g[u] = load4(t.grad, t.grad_type, i, t.elements);
+    if constexpr (BYTES) {
+      mc[u] = *(const u32_any*)((const unsigned char*)a.m + state0 + i);
+      vc[u] = *(const u32_any*)((const unsigned char*)a.v + state0 + i);
+      me[u] = a.m_exp[(state0 + i) / kBlock];
+      ve[u] = a.v_exp[(state0 + i) / kBlock];
+    } else {
+      m[u] = *(const f32x4_any*)((const float*)a.m + state0 + i);
+      v[u] = *(const f32x4_any*)((const float*)a.v + state0 + i);
+    }
+  }
+  unsigned high = 0;
+  if constexpr (BYTES) high = mix32(h.seed);
+#pragma unroll
+  for (int u = 0; u < kUnroll; u++) {
+    const long long i = base + u * kBlock;
+    if (i - lane * 4 >= t.elements) break;
+    if constexpr (BYTES) {
+      const float mu = unit_of(me[u], M_BIAS), vu = unit_of(ve[u], V_BIAS);
+      m[u] = floatx4{__builtin_amdgcn_cvt_f32_fp8(mc[u], 0), __builtin_amdgcn_cvt_f32_fp8(mc[u], 1),
+                     __builtin_amdgcn_cvt_f32_fp8(mc[u], 2), __builtin_amdgcn_cvt_f32_fp8(mc[u], 3)};
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        m[u][j] *= mu;
+        const float r = decode_v((vc[u] >> (8 * j)) & 0xff) * vu;
+        v[u][j] = r * r;
+      }
+    }
+    floatx4 root;
+    unsigned mtop = 0, vtop = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const bool in = i + j < t.elements;
+      const float gj = g[u][j] * h.grad_scale;
+      m[u][j] = in ? m[u][j] * h.beta1 + gj * h.beta1_rest : 0.f;
+      v[u][j] = in ? v[u][j] * h.beta2 + gj * gj * h.beta2_rest : 0.f;
+      root[j] = sqrtf(v[u][j]);
+      p[u][j] = p[u][j] * decay - h.step_size * m[u][j] / (root[j] * h.root_scale + h.eps);
+      mtop = max(mtop, __float_as_uint(m[u][j]) & 0x7fffffffu);
+      vtop = max(vtop, __float_as_uint(root[j]) & 0x7fffffffu);
+    }
+    if (t.master) store4_any(t.master, PREC_F32, i, t.elements, p[u]);
+    store4_any(t.param, t.param_type, i, t.elements, p[u]);
+    if constexpr (BYTES) {
+      const int em = exp_of(wave_max(mtop), M_CARRY, M_LEAST), ev = exp_of(wave_max(vtop), V_CARRY, V_LEAST);
+      const float ms = exp_bits(127 + M_BIAS - (em > 254 ? 254 : em)), vs = exp_bits(127 + V_BIAS - (ev > 254 ? 254 : ev));
+      const unsigned long long at = (unsigned long long)(state0 + i);
+      const unsigned place = mix32((unsigned)(at >> 32) + high);
+      unsigned mw = 0, vw = 0;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const unsigned r = mix32((unsigned)at + j + place);
+        const unsigned bits = __float_as_uint(m[u][j]);
+        const unsigned cm = encode_m(__uint_as_float(bits & 0x7fffffffu) * ms, (float)(r & 0xffff) * 0x1p-16f) | ((bits >> 24) & 0x80);
+        const unsigned cv = encode_v(root[j] * vs, (float)(r >> 16) * 0x1p-16f);
+        mw |= (cm & 0xff) << (8 * j);
+        vw |= (cv & 0xff) << (8 * j);
+      }
+      *(u32_any*)((unsigned char*)a.m + at) = mw;
+      *(u32_any*)((unsigned char*)a.v + at) = vw;
+      if (lane == 0) {
+        a.m_exp[at / kBlock] = (unsigned char)em;
+        a.v_exp[at / kBlock] = (unsigned char)ev;
+      }
+    } else {
+      *(f32x4_any*)((float*)a.m + state0 + i) = m[u];
+      *(f32x4_any*)((float*)a.v + state0 + i) = v[u];
+    }
+  }
+}
+
+// A block a wave, four elements a lane.
+template <bool BYTES>
+__global__ __launch_bounds__(256) void adamw_moments_kernel(const void* m, const void* v, const unsigned char* m_exp,
+                                                            const unsigned char* v_exp, long long blocks, int type,
+                                                            void* out_m, void* out_root) {
+  const int lane = threadIdx.x & 63;
+  for (long long b = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); b < blocks; b += (long long)gridDim.x * 4) {
+    const long long i = b * kBlock + lane * 4;
+    floatx4 fm, fr;
+    if constexpr (BYTES) {
+      const unsigned mc = *(const u32_any*)((const unsigned char*)m + i), vc = *(const u32_any*)((const unsigned char*)v + i);
+      const float mu = unit_of(m_exp[b], M_BIAS), vu = unit_of(v_exp[b], V_BIAS);
+      fm = floatx4{__builtin_amdgcn_cvt_f32_fp8(mc, 0), __builtin_amdgcn_cvt_f32_fp8(mc, 1),
+                   __builtin_amdgcn_cvt_f32_fp8(mc, 2), __builtin_amdgcn_cvt_f32_fp8(mc, 3)} * mu;
+#pragma unroll
+      for (int j = 0; j < 4; j++) fr[j] = decode_v((vc >> (8 * j)) & 0xff) * vu;
+    } else {
+      fm = *(const f32x4_any*)((const float*)m + i);
+      fr = *(const f32x4_any*)((const float*)v + i);
+#pragma unroll
+      for (int j = 0; j < 4; j++) fr[j] = sqrtf(fr[j]);
+    }
+    store4_any(out_m, type, i, blocks * kBlock, fm);
+    store4_any(out_root, type, i, blocks * kBlock, fr);
+  }
+}
+
+}  // namespace
+
+void launch_adamw(int count, const kg_adamw_tensor* tensors, const kg_adamw_state& state, const kg_adamw_values_t& values,
+                  const kg_adamw_values_t* device_values, hipStream_t s) {
+  AdamArgs a;
+  a.values = values;
+  a.device_values = device_values;
+  a.m = state.m; a.v = state.v;
+  a.m_exp = state.m_exp; a.v_exp = state.v_exp;
+  int n = 0;
+  long long groups = 0;
+  auto flush = [&] {
+    if (!n) return;
+    for (int i = n; i < kTensors; i++) a.start[i] = INT_MAX;
+    if (state.state_bits == 8) launch_k(adamw_kernel<true>, dim3((unsigned)groups), kWaves * 64, 0, s, a);
+    else launch_k(adamw_kernel<false>, dim3((unsigned)groups), kWaves * 64, 0, s, a);
+    KGX_CHECK_LAUNCH();
+    n = 0;
+    groups = 0;
+  };
+  for (int i = 0; i < count; i++) {
+    const kg_adamw_tensor& t = tensors[i];
+    // (A launch takes up to 2^22 workgroups, 2^34 elements: a larger tensor goes in pieces of whole blocks.)
+    constexpr long long most = 1ll << 22;
+    for (long long done = 0; done < t.elements;) {
+      if (n == kTensors || groups == most) flush();
+      const long long left = t.elements - done, room = (most - groups) * kChunk, take = left < room ? left : room;
+      AdamTensor& d = a.t[n];
+      const long long ps = t.param_type == PREC_F32 ? 4 : 2, gs = t.grad_type == PREC_F32 ? 4 : 2;
+      d.param = (char*)t.param + done * ps;
+      d.grad = (const char*)t.grad + done * gs;
+      d.master = t.master ? t.master + done : nullptr;
+      d.elements = take;
+      d.first_block = t.first_block + done / kBlock;
+      d.weight_decay = (float)t.weight_decay;
+      d.param_type = (short)t.param_type;
+      d.grad_type = (short)t.grad_type;
+      a.start[n++] = (int)groups;
+      groups += (take + kChunk - 1) / kChunk;
+      done += take;
+    }
+  }
+  flush();
+}
+
+void launch_adamw_moments(long long blocks, const kg_adamw_state& state, int type, void* m, void* root, hipStream_t s) {
+  if (blocks <= 0) return;
+  const long long groups = (blocks + 3) / 4;
+  const dim3 grid((unsigned)(groups < (1 << 20) ? groups : (1 << 20)));
+  if (state.state_bits == 8)
+    launch_k(adamw_moments_kernel<true>, grid, 256, 0, s, state.m, state.v, state.m_exp, state.v_exp, blocks, type, m, root);
+  else
+    launch_k(adamw_moments_kernel<false>, grid, 256, 0, s, state.m, state.v, state.m_exp, state.v_exp, blocks, type, m, root);
+  KGX_CHECK_LAUNCH();
+}
+
+}  // namespace kgx

@@ -14,6 +14,7 @@
 #include <thread>
 #include <vector>
 
+#include "kgx_error.h"
 #include "kgx_model.h"
 #include "kgx_net.h"
 
@@ -71,20 +72,7 @@ namespace {
 
 thread_local std::string g_last_error;
 
-int fail(const std::string& msg) {
-  g_last_error = msg;
-  return 1;
-}
-
-template <typename F>
-int guarded(F&& f) {
-  try {
-    f();
-    return 0;
-  } catch (const std::exception& e) {
-    return fail(e.what());
-  }
-}
+using kgx::guarded;
 
 constexpr int POS = 19;
 constexpr int HW = POS * POS;
@@ -365,6 +353,11 @@ void enqueue_featurize(kg_handle* h, int n, const kg_position* rows, const int* 
 }
 
 }  // namespace
+
+int kgx::set_last_error(const std::string& msg) {
+  g_last_error = msg;
+  return 1;
+}
 
 extern "C" {
 

@@ -1,0 +1,529 @@
+// The policy and preference losses with their gradients (kg_policy_loss, kg_preference_loss).
+//
+// Both are softmax cross-entropies whose gradient factor depends on the whole row (the clip, the KL term) or on whole
+// sequences (the margin): a row's maximum, sum and chosen log-probability come first, then grad = factor (onehot - p), plus
+// the KL term's p (log p/r - KL). One pass over a row keeps the running maximum and the sum of exp relative to it; with a
+// reference row also the reference's and sum e^(z - max) ((z - max) - (r - max_r)), from which KL = sum p ((z - max) -
+// (r - max_r)) - log(sum / sum_r) follows without a second look (both rows relative to their maxima: no cancellation
+// between rows far from 0, and none with a mask of the type's lowest value). A second pass writes the gradient.
+//
+// A row's few scalars are computed in double: logp decides on which side of the clip the row is, and the losses of a
+// sequence are differences of sums of thousands. (A comparison of logp - old_logp with log(1 +- clip) needs no exp.)
+#include "kgx_device.h"
+#include "kgx_learn.h"
+
+namespace kgx {
+
+namespace {
+
+// 16 bytes of a row at its elements' alignment: rows of odd strides and columns of a larger row start anywhere. (Global
+// loads and stores of any width need no more than that on this hardware.)
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned short u16x8_any __attribute__((ext_vector_type(8), aligned(2)));
+typedef unsigned int u32_any __attribute__((aligned(1)));
+typedef unsigned long long u64_any __attribute__((aligned(1)));
+
+template <typename T> constexpr int kVec = 16 / sizeof(T);
+
+template <typename T> struct RowVec { typedef u16x8_any type; };
+template <> struct RowVec<float> { typedef f32x4_any type; };
+
+template <typename T>
+__device__ __forceinline__ float widen(typename RowVec<T>::type v, int j) {
+  if constexpr (std::is_same<T, float>::value) return v[j];
+  else if constexpr (std::is_same<T, bf16>::value) return __uint_as_float((unsigned)v[j] << 16);
+  else return (float)__builtin_bit_cast(f16, (unsigned short)v[j]);
+}
+
+// Elements [c kVec, (c + 1) kVec) of a row as floats, -infinity past `columns`.
+template <typename T>
+__device__ __forceinline__ void load_chunk(const T* row, int c, int columns, float (&f)[kVec<T>]) {
+  const T* p = row + (size_t)c * kVec<T>;
+  const int left = columns - c * kVec<T>;
+  if (left >= kVec<T>) {
+    const typename RowVec<T>::type v = *(const typename RowVec<T>::type*)p;
+#pragma unroll
+    for (int j = 0; j < kVec<T>; j++) f[j] = widen<T>(v, j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kVec<T>; j++) f[j] = j < left ? (float)p[j] : -INFINITY;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_chunk(T* row, int c, int columns, const float (&f)[kVec<T>]) {
+  T* p = row + (size_t)c * kVec<T>;
+  const int left = columns - c * kVec<T>;
+  T t[kVec<T>];
+#pragma unroll
+  for (int j = 0; j < kVec<T>; j++) t[j] = to_t<T>(f[j]);
+  if (left >= kVec<T>) {
+    *(typename RowVec<T>::type*)p = __builtin_bit_cast(typename RowVec<T>::type, t);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kVec<T>; j++)
+      if (j < left) p[j] = t[j];
+  }
+}
+
+// The legality bytes of a chunk, 0 past `columns`.
+template <int V>
+__device__ __forceinline__ unsigned long long load_legal(const unsigned char* row, int c, int columns) {
+  const unsigned char* p = row + (size_t)c * V;
+  const int left = columns - c * V;
+  if (left >= V) {
+    if constexpr (V == 4) return *(const u32_any*)p;
+    else return *(const u64_any*)p;
+  }
+  unsigned long long b = 0;
+#pragma unroll
+  for (int j = 0; j < V; j++)
+    if (j < left) b |= (unsigned long long)p[j] << (8 * j);
+  return b;
+}
+
+// Reductions over the NT threads of a row: a wave, or the whole workgroup through `red` (16 floats a value).
+template <int NT, bool MAX>
+__device__ __forceinline__ float row_reduce(float v, float* red) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    const float w = __shfl_xor(v, o);
+    v = MAX ? fmaxf(v, w) : v + w;
+  }
+  if constexpr (NT > 64) {
+    __syncthreads();  // (the last reduction's values have been read)
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0];
+#pragma unroll
+    for (int k = 1; k < NT / 64; k++) v = MAX ? fmaxf(v, red[k]) : v + red[k];
+  }
+  return v;
+}
+
+// log(s) in double for a float s >= 1, from s = 2^k f, f in [0.7, 1.42): log f = 2 atanh(t) = 2 (t + t^3/3 + ...),
+// t = (f - 1) / (f + 1), |t| < 0.172, so that the terms to t^13 leave 1e-12. NaN and infinity stay.
+__device__ __forceinline__ double log_sum(float s) {
+  int k;
+  float f = frexpf(s, &k);
+  if (f < 0.70710678f) { f *= 2.f; k--; }
+  const double t = ((double)f - 1.0) / ((double)f + 1.0), q = t * t;
+  double p = 1.0 / 13;
+  p = __builtin_fma(p, q, 1.0 / 11);
+  p = __builtin_fma(p, q, 1.0 / 9);
+  p = __builtin_fma(p, q, 1.0 / 7);
+  p = __builtin_fma(p, q, 1.0 / 5);
+  p = __builtin_fma(p, q, 1.0 / 3);
+  p = __builtin_fma(p, q, 1.0);
+  return __builtin_fma((double)k, 0.69314718055994530942, 2.0 * t * p);
+}
+
+// s log2 e in two floats: the first alone is off by up to 2^-25, relative, the same way in every term of a row. A sequence's
+// log-probability sums that error over its rows, and the margin is a small difference of such sums (0.15 of 5000 in a case of
+// 500 tokens: the margin was off by 7e-6, with both parts by 4e-7).
+struct Base2 {
+  float hi, lo;
+  __device__ __forceinline__ explicit Base2(double s) {
+    hi = (float)(s * 1.44269504088896340736);
+    lo = (float)(s * 1.44269504088896340736 - (double)hi);
+  }
+};
+__device__ __forceinline__ float exp_of(float x, Base2 c) {
+  return __builtin_amdgcn_exp2f(__builtin_fmaf(x, c.hi, x * c.lo));
+}
+
+// The running maximum and sum of e^((z - top) s) over a thread's share of a row.
+struct Running {
+  float top = -INFINITY, sum = 0.f;
+  // Takes V values, which become z - top; e: their exponentials. Returns what the sum so far was scaled by, and in `moved`
+  // how far the maximum it is relative to went down (old minus new).
+  template <int V>
+  __device__ __forceinline__ float add(float (&z)[V], Base2 c, float (&e)[V], float& moved) {
+    float t = z[0];
+#pragma unroll
+    for (int j = 1; j < V; j++) t = fmaxf(t, z[j]);
+    const float up = fmaxf(top, t);
+    // (Nothing but -infinity so far: keep the sums at 0 rather than take -infinity from itself.)
+    const float base = up == -INFINITY ? 0.f : up;
+    moved = top - base;
+    const float keep = exp_of(moved, c);
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      z[j] -= base;
+      e[j] = exp_of(z[j], c);
+      s += e[j];
+    }
+    sum = __builtin_fmaf(sum, keep, s);
+    top = up;
+    return keep;
+  }
+  template <int V>
+  __device__ __forceinline__ void add(float (&z)[V], Base2 c) {
+    float e[V], moved;
+    add<V>(z, c, e, moved);
+  }
+  template <int NT>
+  __device__ __forceinline__ float join(Base2 c, float* red, float& moved) {  // over the row; returns as add does
+    const float all = row_reduce<NT, true>(top, red);
+    moved = top - all;
+    const float keep = top == -INFINITY ? 0.f : exp_of(moved, c);
+    sum = row_reduce<NT, false>(sum * keep, red);
+    top = all;
+    return keep;
+  }
+};
+
+struct PolicyRows {
+  const void* logits;
+  const unsigned char* legal;
+  const void* ref;
+  void* grad;
+  long long ld, ld_legal, ld_ref, ld_grad;
+  const int* action;
+  const float *old_logp, *advantage, *weight, *ref_logp;
+  float *loss, *logp, *kl;
+  int rows, columns;
+  double scale, low, high, log_low, log_high;  // clip_low, clip_high; log(1 - clip_low), log(1 + clip_high)
+  float kl_coef;
+};
+
+template <typename T, int NT, bool LEGAL, bool FULL>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void policy_loss_kernel(PolicyRows a) {
+  constexpr int V = kVec<T>, PER = NT < 256 ? 256 / NT : 1;
+  __shared__ float red[16];
+  const int tid = threadIdx.x % NT, columns = a.columns, chunks = (columns + V - 1) / V;
+  const float s = (float)a.scale;
+  const Base2 c2(a.scale);
+  for (int row = blockIdx.x * PER + threadIdx.x / NT; row < a.rows; row += gridDim.x * PER) {
+    const T* z = (const T*)a.logits + (size_t)row * a.ld;
+    const T* r = FULL ? (const T*)a.ref + (size_t)row * a.ld_ref : nullptr;
+    const unsigned char* lg = LEGAL ? a.legal + (size_t)row * a.ld_legal : nullptr;
+    T* g = a.grad ? (T*)a.grad + (size_t)row * a.ld_grad : nullptr;
+    const int act = a.action[row];
+    const bool padding = (unsigned)act >= (unsigned)columns;
+
+    Running run, ref;
+    float cross = 0.f;  // sum e^(z - top) ((z - top) - (r - its top))
+    if (!padding) {
+      for (int c = tid; c < chunks; c += NT) {
+        float zf[V], e[V];
+        load_chunk<T>(z, c, columns, zf);
+        unsigned long long ok = ~0ull;
+        if constexpr (LEGAL) {
+          ok = load_legal<V>(lg, c, columns);
+#pragma unroll
+          for (int j = 0; j < V; j++)
+            if (!((ok >> (8 * j)) & 0xff)) zf[j] = -INFINITY;
+        }
+        const float before = run.sum;
+        float moved, r_moved;
+        const float keep = run.add<V>(zf, c2, e, moved);
+        if constexpr (FULL) {
+          float rf[V], er[V];
+          load_chunk<T>(r, c, columns, rf);
+#pragma unroll
+          for (int j = 0; j < V; j++)
+            if (LEGAL && !((ok >> (8 * j)) & 0xff)) rf[j] = -INFINITY;
+          ref.add<V>(rf, c2, er, r_moved);
+          float x = 0.f;
+#pragma unroll
+          for (int j = 0; j < V; j++) x += e[j] == 0.f ? 0.f : e[j] * (zf[j] - rf[j]);
+          cross = keep == 0.f ? x : __builtin_fmaf(__builtin_fmaf(before, moved - r_moved, cross), keep, x);
+        }
+      }
+      const float before = run.sum;
+      float moved, r_moved;
+      const float keep = run.join<NT>(c2, red, moved);
+      if constexpr (FULL) {
+        ref.join<NT>(c2, red, r_moved);
+        cross = row_reduce<NT, false>(keep == 0.f ? 0.f : __builtin_fmaf(before, moved - r_moved, cross) * keep, red);
+      }
+    }
+
+    float za = -INFINITY;
+    if (!padding && (!LEGAL || lg[act])) za = (float)z[act];
+    const double log_s = log_sum(run.sum);
+    const double lp = za == -INFINITY ? -(double)INFINITY : ((double)za - (double)run.top) * a.scale - log_s;
+    const bool part = !padding && !(lp == -(double)INFINITY);
+    float hot = 0.f, f_p = 0.f, f_kl = 0.f, shift = 0.f;
+    if (part) {
+      const float w = a.weight ? a.weight[row] : 1.f, adv = a.advantage[row], inv = 1.f / run.sum;
+      const double delta = lp - (double)a.old_logp[row];
+      const float ratio = expf((float)delta);
+      const bool held = adv > 0.f ? delta > a.log_high : adv < 0.f ? delta < a.log_low : false;
+      const float bounded = fminf(fmaxf(ratio, (float)(1.0 - a.low)), (float)(1.0 + a.high));
+      const float obj = held ? bounded * adv : ratio * adv;
+      float c = held ? 0.f : -ratio * adv;
+      float kl = 0.f;
+      if constexpr (FULL) {
+        const double gap = log_s - log_sum(ref.sum);
+        const double k = (double)cross * a.scale * (double)inv - gap;
+        kl = (float)k;
+        shift = (float)(gap + k);
+      } else if (a.ref_logp) {
+        const float d = (float)((double)a.ref_logp[row] - lp), em = expm1f(d);
+        kl = em - d;
+        c -= a.kl_coef * em;
+      }
+      const float gw = w * s;
+      hot = gw * c;
+      f_p = -hot * inv;
+      f_kl = FULL ? a.kl_coef * gw * inv : 0.f;
+      if (tid == 0) {
+        a.loss[row] = w * (a.kl_coef * kl - obj);
+        a.logp[row] = (float)lp;
+        a.kl[row] = kl;
+      }
+    } else if (tid == 0) {
+      a.loss[row] = 0.f;
+      a.logp[row] = padding ? 0.f : -INFINITY;
+      a.kl[row] = 0.f;
+    }
+    if (!g) continue;
+    for (int c = tid; c < chunks; c += NT) {
+      float gf[V];
+      if (part) {
+        float zf[V], rf[V];
+        load_chunk<T>(z, c, columns, zf);
+        if constexpr (FULL) load_chunk<T>(r, c, columns, rf);
+        unsigned long long ok = ~0ull;
+        if constexpr (LEGAL) ok = load_legal<V>(lg, c, columns);
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          const float e = __builtin_amdgcn_exp2f((zf[j] - run.top) * c2.hi);
+          float f = f_p;
+          if constexpr (FULL) f += f_kl * (((zf[j] - run.top) - (rf[j] - ref.top)) * s - shift);
+          gf[j] = FULL && e == 0.f ? 0.f : e * f;
+          if (LEGAL && !((ok >> (8 * j)) & 0xff)) gf[j] = 0.f;
+        }
+        if (c == act / V) {
+#pragma unroll
+          for (int j = 0; j < V; j++)
+            if (j == act % V) gf[j] += hot;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; j++) gf[j] = 0.f;
+      }
+      store_chunk<T>(g, c, columns, gf);
+    }
+  }
+}
+
+// Workgroups of a launch over rows, `per` at a time: the grid's threads stay below 2^32 and each workgroup strides on.
+inline int row_grid(int rows, int per) {
+  const long long n = ((long long)rows + per - 1) / per;
+  return (int)(n < (1 << 20) ? n : (1 << 20));
+}
+
+template <typename T, int NT>
+void policy_on(const PolicyRows& p, hipStream_t s) {
+  const int per = NT < 256 ? 256 / NT : 1, threads = NT < 256 ? 256 : NT;
+  const dim3 grid(row_grid(p.rows, per));
+  if (p.legal) {
+    if (p.ref) launch_k(policy_loss_kernel<T, NT, true, true>, grid, threads, 0, s, p);
+    else launch_k(policy_loss_kernel<T, NT, true, false>, grid, threads, 0, s, p);
+  } else {
+    if (p.ref) launch_k(policy_loss_kernel<T, NT, false, true>, grid, threads, 0, s, p);
+    else launch_k(policy_loss_kernel<T, NT, false, false>, grid, threads, 0, s, p);
+  }
+}
+
+template <typename T>
+void policy_typed(const PolicyRows& p, hipStream_t s) {
+  if (p.columns <= 2048) policy_on<T, 64>(p, s);
+  else if (p.columns <= 16384) policy_on<T, 256>(p, s);
+  else policy_on<T, 1024>(p, s);
+}
+
+struct PrefRows {
+  const void* logits;
+  void* grad;
+  long long ld, ld_grad;
+  const int *label, *offsets;
+  const float *ref_logp, *weight;
+  PrefRow* row;
+  float* coef;
+  float *loss, *margin, *seq_logp;
+  int rows, columns, pairs, average;
+  double beta, smooth;
+};
+
+// Row t's softmax maximum, reciprocal sum and log-probability of its label, where it counts; its gradient's factor starts
+// at 0.
+template <typename T, int NT>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void pref_rows_kernel(PrefRows a) {
+  constexpr int V = kVec<T>, PER = NT < 256 ? 256 / NT : 1;
+  __shared__ float red[16];
+  const int tid = threadIdx.x % NT, columns = a.columns, chunks = (columns + V - 1) / V;
+  const int first = a.offsets[0], last = a.offsets[2 * a.pairs];
+  const Base2 c2(1.0);
+  for (int row = blockIdx.x * PER + threadIdx.x / NT; row < a.rows; row += gridDim.x * PER) {
+    const int label = a.label[row];
+    if (tid == 0) a.coef[row] = 0.f;
+    if (row < first || row >= last || (unsigned)label >= (unsigned)columns) continue;
+    const T* z = (const T*)a.logits + (size_t)row * a.ld;
+    Running run;
+    for (int c = tid; c < chunks; c += NT) {
+      float zf[V];
+      load_chunk<T>(z, c, columns, zf);
+      run.add<V>(zf, c2);
+    }
+    float moved;
+    run.join<NT>(c2, red, moved);
+    if (tid == 0) {
+      const float za = (float)z[label];
+      a.row[row] = PrefRow{za == -INFINITY ? -(double)INFINITY : (double)za - (double)run.top - log_sum(run.sum), run.top,
+                           1.f / run.sum};
+    }
+  }
+}
+
+// One workgroup a pair: the sequences' sums in a fixed order, the loss, and the factor of each counted row's gradient.
+__global__ __launch_bounds__(256) void pref_pairs_kernel(PrefRows a) {
+  __shared__ double sums[4][2];
+  __shared__ int counts[4][2];
+  const int tid = threadIdx.x, w = tid >> 6;
+  for (int pair = blockIdx.x; pair < a.pairs; pair += gridDim.x) {
+    int at[3];
+    for (int k = 0; k < 3; k++) at[k] = min(max(a.offsets[2 * pair + k], 0), a.rows);
+    double sum[2] = {0, 0};
+    int count[2] = {0, 0};
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+      for (int t = at[q] + tid; t < at[q + 1]; t += 256)
+        if ((unsigned)a.label[t] < (unsigned)a.columns) {
+          sum[q] += a.row[t].logp;
+          count[q]++;
+        }
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) {
+        sum[q] += __shfl_xor(sum[q], o);
+        count[q] += __shfl_xor(count[q], o);
+      }
+    }
+    __syncthreads();
+    if ((tid & 63) == 0)
+      for (int q = 0; q < 2; q++) { sums[w][q] = sum[q]; counts[w][q] = count[q]; }
+    __syncthreads();
+    double part[2];
+    for (int q = 0; q < 2; q++) {
+      const int n = counts[0][q] + counts[1][q] + counts[2][q] + counts[3][q];
+      part[q] = a.average ? 1.0 / max(n, 1) : 1.0;
+      sum[q] = (sums[0][q] + sums[1][q] + sums[2][q] + sums[3][q]) * part[q];
+    }
+    const double h = a.beta * ((sum[0] - (double)a.ref_logp[2 * pair]) - (sum[1] - (double)a.ref_logp[2 * pair + 1]));
+    const double wt = a.weight ? (double)a.weight[pair] : 1.0;
+    // -log sigmoid(h) = log1p(e^-|h|) + max(-h, 0); the sigmoids from the same exponential.
+    const double e = exp(-fabs(h)), soft = log1p(e), near = 1.0 / (1.0 + e), far = e / (1.0 + e);
+    const double up = h >= 0 ? near : far, down = h >= 0 ? far : near;  // sigmoid(h), sigmoid(-h)
+    if (tid == 0) {
+      a.loss[pair] = (float)(wt * ((1 - a.smooth) * (soft + fmax(-h, 0.0)) + a.smooth * (soft + fmax(h, 0.0))));
+      a.margin[pair] = (float)h;
+      a.seq_logp[2 * pair] = (float)sum[0];
+      a.seq_logp[2 * pair + 1] = (float)sum[1];
+    }
+    if (a.grad) {
+      const double dh = wt * a.beta * (a.smooth * up - (1 - a.smooth) * down);
+      for (int q = 0; q < 2; q++)
+        for (int t = at[q] + tid; t < at[q + 1]; t += 256)
+          if ((unsigned)a.label[t] < (unsigned)a.columns) a.coef[t] = (float)((q ? -dh : dh) * part[q]);
+    }
+  }
+}
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void pref_grad_kernel(PrefRows a) {
+  constexpr int V = kVec<T>, PER = NT < 256 ? 256 / NT : 1;
+  const int tid = threadIdx.x % NT, columns = a.columns, chunks = (columns + V - 1) / V;
+  const int first = a.offsets[0], last = a.offsets[2 * a.pairs];
+  for (int row = blockIdx.x * PER + threadIdx.x / NT; row < a.rows; row += gridDim.x * PER) {
+    const int label = a.label[row];
+    const bool counted = row >= first && row < last && (unsigned)label < (unsigned)columns;
+    const T* z = (const T*)a.logits + (size_t)row * a.ld;
+    T* g = (T*)a.grad + (size_t)row * a.ld_grad;
+    float hot = 0.f, f = 0.f, top = 0.f;
+    if (counted) {
+      hot = a.coef[row];
+      top = a.row[row].top;
+      f = -hot * a.row[row].inv_sum;
+    }
+    for (int c = tid; c < chunks; c += NT) {
+      float zf[V];
+      if (counted) {
+        load_chunk<T>(z, c, columns, zf);
+#pragma unroll
+        for (int j = 0; j < V; j++) zf[j] = __builtin_amdgcn_exp2f((zf[j] - top) * 1.44269504088896340736f) * f;
+        if (c == label / V) {
+#pragma unroll
+          for (int j = 0; j < V; j++)
+            if (j == label % V) zf[j] += hot;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; j++) zf[j] = 0.f;
+      }
+      store_chunk<T>(g, c, columns, zf);
+    }
+  }
+}
+
+template <typename T, int NT>
+void pref_on(const PrefRows& p, hipStream_t s) {
+  const int per = NT < 256 ? 256 / NT : 1, threads = NT < 256 ? 256 : NT;
+  const dim3 grid(row_grid(p.rows, per));
+  if (p.rows > 0) launch_k(pref_rows_kernel<T, NT>, grid, threads, 0, s, p);
+  if (p.pairs > 0) launch_k(pref_pairs_kernel, dim3(p.pairs < 65536 ? p.pairs : 65536), 256, 0, s, p);
+  if (p.rows > 0 && p.grad) launch_k(pref_grad_kernel<T, NT>, grid, threads, 0, s, p);
+}
+
+template <typename T>
+void pref_typed(const PrefRows& p, hipStream_t s) {
+  if (p.columns <= 2048) pref_on<T, 64>(p, s);
+  else if (p.columns <= 16384) pref_on<T, 256>(p, s);
+  else pref_on<T, 1024>(p, s);
+}
+
+}  // namespace
+
+void launch_policy_loss(const kg_policy_loss_args& a, hipStream_t s) {
+  PolicyRows p;
+  p.logits = a.logits; p.ld = a.ld;
+  p.legal = a.legal; p.ld_legal = a.ld_legal;
+  p.ref = a.ref_logits; p.ld_ref = a.ld_ref;
+  p.grad = a.grad; p.ld_grad = a.ld_grad;
+  p.action = a.action; p.old_logp = a.old_logp; p.advantage = a.advantage; p.weight = a.weight; p.ref_logp = a.ref_logp;
+  p.loss = a.loss; p.logp = a.logp; p.kl = a.kl;
+  p.rows = a.rows; p.columns = a.columns;
+  p.scale = a.logit_scale;
+  p.low = a.clip_low; p.high = a.clip_high;
+  p.log_low = log1p(-a.clip_low); p.log_high = log1p(a.clip_high);
+  p.kl_coef = (float)a.kl_coef;
+  switch (a.type) {
+    case PREC_F32: policy_typed<float>(p, s); break;
+    case PREC_F16: policy_typed<f16>(p, s); break;
+    default: policy_typed<bf16>(p, s); break;
+  }
+  KGX_CHECK_LAUNCH();
+}
+
+void launch_preference_loss(const kg_preference_loss_args& a, hipStream_t s) {
+  PrefRows p;
+  p.logits = a.logits; p.ld = a.ld;
+  p.grad = a.grad; p.ld_grad = a.ld_grad;
+  p.label = a.label; p.offsets = a.offsets; p.ref_logp = a.ref_logp; p.weight = a.weight;
+  p.row = (PrefRow*)a.workspace;
+  p.coef = (float*)(p.row + a.rows);
+  p.loss = a.loss; p.margin = a.margin; p.seq_logp = a.seq_logp;
+  p.rows = a.rows; p.columns = a.columns; p.pairs = a.pairs; p.average = a.average;
+  p.beta = a.beta; p.smooth = a.label_smoothing;
+  switch (a.type) {
+    case PREC_F32: pref_typed<float>(p, s); break;
+    case PREC_F16: pref_typed<f16>(p, s); break;
+    default: pref_typed<bf16>(p, s); break;
+  }
+  KGX_CHECK_LAUNCH();
+}
+
+}  // namespace kgx

@@ -1,10 +1,16 @@
 // Group norm with an activation on channels-last rows under the board mask, forward and backward (kg_group_norm,
 // kg_group_norm_backward).
 //
-// Bound by memory. A workgroup takes a share of one batch row's points with all their channels, so that every access runs
-// along whole rows however wide or odd the groups are; a thread keeps its column of 16 bytes for all its points, with the
-// channels' parameters in registers. The statistics of a group cross workgroups, so each direction is a reduction launch
-// and an elementwise one; the second reading of the same rows comes from the caches where they fit.
+// Bound by memory: x read and y written once, or dy and x read and dx written once.
+// - Where a slab of whole groups over all points of a batch row fits the registers of one workgroup (up to 128 KB: the
+//   boards of every network here, images of 64 x 64), it is read once, the statistics meet in LDS, and the result is
+//   written from the registers. Slabs are as narrow as keeps whole 16-byte columns, 64 bytes where that fits, so that few
+//   rows fill the chip; neighbouring slabs, which share cache lines, run on one XCD.
+// - Larger rows are cut along the points: a reduction launch and an elementwise one, whose second reading of the rows comes
+//   from the caches where they fit. Every access runs along whole rows however wide or odd the groups are.
+// A thread keeps its column of 16 bytes for all its points, with the channels' parameters in registers.
+#include <algorithm>
+
 #include "kgx_device.h"
 #include "kgx_learn.h"
 
@@ -23,15 +29,17 @@ template <typename T> struct RowVec { typedef u16x8_any type; };
 template <> struct RowVec<float> { typedef f32x4_any type; };
 
 template <typename T>
+__device__ __forceinline__ float widen1(const typename RowVec<T>::type& v, int j) {
+  if constexpr (std::is_same<T, float>::value) return v[j];
+  else if constexpr (std::is_same<T, bf16>::value) return __uint_as_float((unsigned)v[j] << 16);
+  else return (float)__builtin_bit_cast(f16, (unsigned short)v[j]);
+}
+template <typename T>
 __device__ __forceinline__ void load_vec(const T* p, int left, float (&f)[kVec<T>]) {
   if (left >= kVec<T>) {
     const typename RowVec<T>::type v = *(const typename RowVec<T>::type*)p;
 #pragma unroll
-    for (int j = 0; j < kVec<T>; j++) {
-      if constexpr (std::is_same<T, float>::value) f[j] = v[j];
-      else if constexpr (std::is_same<T, bf16>::value) f[j] = __uint_as_float((unsigned)v[j] << 16);
-      else f[j] = (float)__builtin_bit_cast(f16, (unsigned short)v[j]);
-    }
+    for (int j = 0; j < kVec<T>; j++) f[j] = widen1<T>(v, j);
   } else {
 #pragma unroll
     for (int j = 0; j < kVec<T>; j++) f[j] = j < left ? (float)p[j] : 0.f;
@@ -61,6 +69,7 @@ struct NormArgs {
   float* counts;   // backward: [batch][splits] points
   float* sums;     // backward: [batch][2][groups]
   int batch, points, channels, groups, width, splits;  // width: channels of a group
+  int slab_groups;  // groups of a slab (fused launches)
   float eps;
 };
 
@@ -179,26 +188,33 @@ __global__ __launch_bounds__(GT) void norm_apply_kernel(NormArgs a) {
   const int b = blockIdx.x / a.splits, k = blockIdx.x % a.splits, tid = threadIdx.x;
   int p0, p1;
   split_range(a, k, p0, p1);
-  for (int g = tid; g < a.groups; g += GT) {
-    const float* in = a.part + (size_t)b * a.splits * 3 * a.groups + g;
+  int share = 64;
+  while (share > 1 && share * a.groups > GT) share >>= 1;
+  for (int gb = 0; gb < a.groups; gb += GT / share) {
+    const int g = gb + tid / share, sub = tid % share;
+    const float* in = a.part + (size_t)b * a.splits * 3 * a.groups + min(g, a.groups - 1);
     float n = 0.f, s = 0.f, m2 = 0.f;
-    for (int i = 0; i < a.splits; i++) {
+    for (int i = sub; i < a.splits; i += share) {
       const float* q = in + (size_t)i * 3 * a.groups;
       n += q[0];
       s = __builtin_fmaf(q[0], q[a.groups], s);
     }
+    for (int o = share >> 1; o >= 1; o >>= 1) { n += __shfl_xor(n, o); s += __shfl_xor(s, o); }
     const float mean = n > 0.f ? s / n : 0.f;
-    for (int i = 0; i < a.splits; i++) {
+    for (int i = sub; i < a.splits; i += share) {
       const float* q = in + (size_t)i * 3 * a.groups;
       const float d = q[a.groups] - mean;
       m2 += q[2 * a.groups] + (q[0] > 0.f ? q[0] * d * d : 0.f);
     }
-    const float rstd = 1.f / sqrtf((n > 0.f ? m2 / n : 0.f) + a.eps);
-    g_mean[g] = mean;
-    g_rstd[g] = rstd;
-    if (k == 0) {
-      a.mean[(size_t)b * a.groups + g] = mean;
-      a.rstd[(size_t)b * a.groups + g] = rstd;
+    for (int o = share >> 1; o >= 1; o >>= 1) m2 += __shfl_xor(m2, o);
+    if (g < a.groups && sub == 0) {
+      const float rstd = 1.f / sqrtf((n > 0.f ? m2 / n : 0.f) + a.eps);
+      g_mean[g] = mean;
+      g_rstd[g] = rstd;
+      if (k == 0) {
+        a.mean[(size_t)b * a.groups + g] = mean;
+        a.rstd[(size_t)b * a.groups + g] = rstd;
+      }
     }
   }
   __syncthreads();
@@ -233,14 +249,15 @@ __global__ __launch_bounds__(GT) void norm_apply_kernel(NormArgs a) {
 }
 
 // d act(a) / d a. Mish: with e = exp(a) and n = e (e + 2), tanh(softplus) = n / (n + 2) and 1 - tanh^2 = 4 (e + 1)^2 /
-// (n + 2)^2, so the derivative n / (n + 2) + 4 a e (e + 1) / (n + 2)^2 has no cancellation but its own sign's.
+// (n + 2)^2, so the derivative n / (n + 2) + 4 a e (e + 1) / (n + 2)^2 has no cancellation but its own sign's. From a = 20 on
+// it is 1 in float, as it is at 20: the argument is held there, with no branch.
 template <int ACT>
 __device__ __forceinline__ float act_slope(float v) {
   if constexpr (ACT == ACT_RELU) {
     return v > 0.f ? 1.f : 0.f;
   } else if constexpr (ACT == ACT_MISH) {
-    const float e = __expf(fminf(v, 20.f)), n = e * (e + 2.f), r = __builtin_amdgcn_rcpf(n + 2.f);
-    return v > 20.f ? 1.f : n * r + 4.f * v * (e * r) * ((e + 1.f) * r);
+    const float u = fminf(v, 20.f), e = __expf(u), n = e * (e + 2.f), r = __builtin_amdgcn_rcpf(n + 2.f);
+    return n * r + 4.f * u * (e * r) * ((e + 1.f) * r);
   } else if constexpr (ACT == ACT_SILU) {
     const float q = __builtin_amdgcn_rcpf(1.f + __expf(-v));
     return q * (1.f + v * (1.f - q));
@@ -249,32 +266,56 @@ __device__ __forceinline__ float act_slope(float v) {
   }
 }
 
-// A column's parameters in the backward pass, and the gradient at the norm's output: da = dy act'(xh gamma + beta).
-template <typename T, int ACT>
+// A column's parameters in the backward pass, and with xc = x - mean (xh = xc rstd) the gradient at the norm's output: da =
+// dy act'(xh gamma + beta). The channels' sums are taken of da xc and multiplied by rstd at the end: three values a channel
+// in registers rather than four (128 KB of 16-bit x and dy leave no more).
+template <typename T, int ACT, int V = kVec<T>>
 struct BackColumn {
-  static constexpr int V = kVec<T>;
-  float mean[V], rstd[V], gamma[V], beta[V];
+  static constexpr bool kExactSide = ACT == ACT_RELU && sizeof(T) == 4;
+  float mean[V], mul[V], beta[V];
+  double scale[kExactSide ? V : 1];
   __device__ __forceinline__ void load(const NormArgs& a, int b, int c0) {
 #pragma unroll
     for (int j = 0; j < V; j++) {
       const int c = min(c0 + j, a.channels - 1), g = c / a.width;
+      const float rstd = a.rstd[(size_t)b * a.groups + g], gamma = a.gamma ? a.gamma[c] : 1.f;
       mean[j] = a.mean[(size_t)b * a.groups + g];
-      rstd[j] = a.rstd[(size_t)b * a.groups + g];
-      gamma[j] = a.gamma ? a.gamma[c] : 1.f;
+      mul[j] = rstd * gamma;
       beta[j] = a.beta ? a.beta[c] : 0.f;
+      if constexpr (kExactSide) scale[j] = (double)rstd * (double)gamma;
     }
   }
-  __device__ __forceinline__ void grad(float x, float dy, int j, float& xh, float& da) const {
-    xh = (x - mean[j]) * rstd[j];
-    if constexpr (ACT == ACT_RELU && sizeof(T) == 4) {
+  // The same from a fused workgroup's copy in LDS, channels c .. c + V - 1 of its slab.
+  template <int NT>
+  __device__ __forceinline__ void read(const float* c_mean, const float* c_mul, const float* c_beta, const double* c_scale, int c) {
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {
+      const floatx4 m = *(const floatx4*)(c_mean + c + j), u = *(const floatx4*)(c_mul + c + j), t = *(const floatx4*)(c_beta + c + j);
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        mean[j + k] = m[k];
+        mul[j + k] = u[k];
+        beta[j + k] = t[k];
+        if constexpr (kExactSide) scale[j + k] = c_scale[c + j + k];
+      }
+    }
+  }
+  __device__ __forceinline__ void grad(float x, float dy, int j, float& xc, float& da) const {
+    xc = x - mean[j];
+    if constexpr (kExactSide) {
       // The side of 0 in double: a float's rounding there would switch a whole gradient.
-      const double v = __builtin_fma(((double)x - (double)mean[j]) * (double)rstd[j], (double)gamma[j], (double)beta[j]);
-      da = v > 0.0 ? dy : 0.f;
+      da = __builtin_fma((double)x - (double)mean[j], scale[j], (double)beta[j]) > 0.0 ? dy : 0.f;
     } else {
-      da = dy * act_slope<ACT>(__builtin_fmaf(xh, gamma[j], beta[j]));
+      da = dy * act_slope<ACT>(__builtin_fmaf(xc, mul[j], beta[j]));
     }
   }
 };
+
+// What dx takes besides: dx = rstd (da gamma - m1 - xh m2) = da mul - k1 - xc k2, with m1 and m2 the group's means of da gamma
+// and da gamma xh.
+__device__ __forceinline__ float back_dx(float da, float xc, float mul, float k1, float k2) {
+  return __builtin_fmaf(da, mul, __builtin_fmaf(-xc, k2, -k1));
+}
 
 // Backward, first launch: sums of da and da xh over the workgroup's points, per channel.
 template <typename T, int ACT>
@@ -305,10 +346,10 @@ __global__ __launch_bounds__(GT) void norm_back_sums_kernel(NormArgs a) {
         load_vec<T>(dy + (size_t)p * a.lddy, left, d);
 #pragma unroll
         for (int j = 0; j < V; j++) {
-          float xh, da;
-          col.grad(f[j], d[j], j, xh, da);
+          float xc, da;
+          col.grad(f[j], d[j], j, xc, da);
           sb[j] += da;
-          sg[j] = __builtin_fmaf(da, xh, sg[j]);
+          sg[j] = __builtin_fmaf(da, xc, sg[j]);
         }
       }
     }
@@ -325,7 +366,7 @@ __global__ __launch_bounds__(GT) void norm_back_sums_kernel(NormArgs a) {
         tg += s_g[t];
       }
       out[first * V + c] = tb;
-      out[a.channels + first * V + c] = tg;
+      out[a.channels + first * V + c] = tg * a.rstd[(size_t)b * a.groups + (first * V + c) / a.width];
     }
     if (first == 0 && tid == 0) {
       float t = 0.f;
@@ -336,58 +377,35 @@ __global__ __launch_bounds__(GT) void norm_back_sums_kernel(NormArgs a) {
   }
 }
 
-// Second launch. Workgroups [0, batch): a batch row's group sums, divided by the group's elements. The others: dgamma and
-// dbeta of 64 channels each, four waves over the parts.
+// Second launch: a wave a group of a batch row, its sums divided by its elements.
 __global__ __launch_bounds__(GT) void norm_back_join_kernel(NormArgs a) {
-  const int tid = threadIdx.x;
-  if ((int)blockIdx.x < a.batch) {
-    const int b = blockIdx.x;
-    float n = 0.f;
-    for (int k = 0; k < a.splits; k++) n += a.counts[(size_t)b * a.splits + k];
+  const int lane = threadIdx.x & 63, id = (int)blockIdx.x * (GT / 64) + (threadIdx.x >> 6);
+  if (id >= a.batch * a.groups) return;
+  const int b = id / a.groups, g = id % a.groups;
+  float n = 0.f, s1 = 0.f, s2 = 0.f;
+  for (int k = lane; k < a.splits; k += 64) n += a.counts[(size_t)b * a.splits + k];
+#pragma unroll 4
+  for (int i = lane; i < a.width * a.splits; i += 64) {
+    const int c = g * a.width + i % a.width, k = i / a.width;
+    const float* q = a.part + ((size_t)b * a.splits + k) * 2 * a.channels + c;
+    const float gm = a.gamma ? a.gamma[c] : 1.f;
+    s1 = __builtin_fmaf(gm, q[0], s1);
+    s2 = __builtin_fmaf(gm, q[a.channels], s2);
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    n += __shfl_xor(n, o);
+    s1 += __shfl_xor(s1, o);
+    s2 += __shfl_xor(s2, o);
+  }
+  if (lane == 0) {
     const float inv = n > 0.f ? 1.f / (n * (float)a.width) : 0.f;
-    int share = 64;
-    while (share > 1 && share * a.groups > GT) share >>= 1;
-    const int sub = tid % share, per = GT / share;
-    for (int gb = 0; gb < a.groups; gb += per) {
-      const int g = gb + tid / share;
-      float s1 = 0.f, s2 = 0.f;
-      if (g < a.groups) {
-        for (int i = sub; i < a.width * a.splits; i += share) {
-          const int c = g * a.width + i % a.width, k = i / a.width;
-          const float* q = a.part + ((size_t)b * a.splits + k) * 2 * a.channels + c;
-          const float gm = a.gamma ? a.gamma[c] : 1.f;
-          s1 = __builtin_fmaf(gm, q[0], s1);
-          s2 = __builtin_fmaf(gm, q[a.channels], s2);
-        }
-      }
-      for (int o = share >> 1; o >= 1; o >>= 1) { s1 += __shfl_xor(s1, o); s2 += __shfl_xor(s2, o); }
-      if (g < a.groups && sub == 0) {
-        a.sums[(size_t)b * 2 * a.groups + g] = s1 * inv;
-        a.sums[(size_t)b * 2 * a.groups + a.groups + g] = s2 * inv;
-      }
-    }
-  } else {
-    __shared__ float red[4][2][64];
-    const int c = ((int)blockIdx.x - a.batch) * 64 + (tid & 63), wave = tid >> 6, parts = a.batch * a.splits;
-    float sb = 0.f, sg = 0.f;
-    if (c < a.channels) {
-      for (int i = wave; i < parts; i += 4) {
-        const float* q = a.part + (size_t)i * 2 * a.channels + c;
-        sb += q[0];
-        sg += q[a.channels];
-      }
-    }
-    red[wave][0][tid & 63] = sb;
-    red[wave][1][tid & 63] = sg;
-    __syncthreads();
-    if (wave == 0 && c < a.channels) {
-      if (a.dbeta) a.dbeta[c] = (red[0][0][tid] + red[1][0][tid]) + (red[2][0][tid] + red[3][0][tid]);
-      if (a.dgamma) a.dgamma[c] = (red[0][1][tid] + red[1][1][tid]) + (red[2][1][tid] + red[3][1][tid]);
-    }
+    a.sums[(size_t)b * 2 * a.groups + g] = s1 * inv;
+    a.sums[(size_t)b * 2 * a.groups + a.groups + g] = s2 * inv;
   }
 }
 
-// Third launch: dx = rstd (da gamma - mean(da gamma) - xh mean(da gamma xh)).
+// Third launch: dx.
 template <typename T, int ACT>
 __global__ __launch_bounds__(GT) void norm_back_apply_kernel(NormArgs a) {
   constexpr int V = kVec<T>;
@@ -401,12 +419,13 @@ __global__ __launch_bounds__(GT) void norm_back_apply_kernel(NormArgs a) {
     const int c0 = (first + w.col) * V, left = a.channels - c0;
     BackColumn<T, ACT> col;
     col.load(a, b, c0);
-    float m1[V], m2[V];
+    float k1[V], k2[V];
 #pragma unroll
     for (int j = 0; j < V; j++) {
       const int g = min(c0 + j, a.channels - 1) / a.width;
-      m1[j] = a.sums[(size_t)b * 2 * a.groups + g];
-      m2[j] = a.sums[(size_t)b * 2 * a.groups + a.groups + g];
+      const float rstd = a.rstd[(size_t)b * a.groups + g];
+      k1[j] = rstd * a.sums[(size_t)b * 2 * a.groups + g];
+      k2[j] = rstd * rstd * a.sums[(size_t)b * 2 * a.groups + a.groups + g];
     }
     const T* x = (const T*)a.x + (size_t)b * a.points * a.ldx + c0;
     const T* dy = (const T*)a.dy + (size_t)b * a.points * a.lddy + c0;
@@ -422,14 +441,446 @@ __global__ __launch_bounds__(GT) void norm_back_apply_kernel(NormArgs a) {
         load_vec<T>(dy + (size_t)p * a.lddy, left, d);
 #pragma unroll
         for (int j = 0; j < V; j++) {
-          float xh, da;
-          col.grad(f[j], d[j], j, xh, da);
-          f[j] = col.rstd[j] * (da * col.gamma[j] - m1[j] - xh * m2[j]);
+          float xc, da;
+          col.grad(f[j], d[j], j, xc, da);
+          f[j] = back_dx(da, xc, col.mul[j], k1[j], k2[j]);
         }
       }
       store_vec<T>(dx + (size_t)p * a.lddx, left, f);
     }
   }
+}
+
+// The slab of a fused launch's workgroup: neighbouring slabs (which share cache lines) are on one XCD, workgroup g running
+// on XCD g mod 8. False past the last.
+__device__ __forceinline__ bool slab_of(const NormArgs& a, int& b, int& c0) {
+  const int slabs = a.groups / a.slab_groups, n = a.batch * slabs, per = (n + 7) / 8;
+  const int id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+  if (id >= n) return false;
+  // (Scalar registers: every address is one of them plus a 32-bit offset.)
+  b = __builtin_amdgcn_readfirstlane(id / slabs);
+  c0 = __builtin_amdgcn_readfirstlane((id % slabs) * a.slab_groups * a.width);
+  return true;
+}
+
+// A fused workgroup's points: thread (col, lane) takes points lane + e lanes, e < E, of 16-byte column col. Threads and
+// points past the end read the last one's address, so that no load is behind a branch.
+template <typename T, int NT, int E>
+struct Slab {
+  static constexpr int V = kVec<T>;
+  int b, c0, width, cols, lanes, col, lane, last;  // width: the slab's channels, whole columns
+  unsigned in, on;  // bit e: the point exists; and is not masked
+  __device__ __forceinline__ Slab(const NormArgs& a, int b_, int c0_) : b(b_), c0(c0_) {
+    width = a.slab_groups * a.width;
+    cols = width / V;
+    lanes = NT / cols;
+    lane = threadIdx.x / cols;
+    col = threadIdx.x - lane * cols;
+    last = a.points - 1;
+    in = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) in |= (lane < lanes && lane + e * lanes <= last ? 1u : 0u) << e;
+    on = in;
+    if (a.mask) {
+      const float* mask = a.mask + (size_t)b * a.points;
+      float mk[E];
+#pragma unroll
+      for (int e = 0; e < E; e++) mk[e] = mask[point(e)];
+#pragma unroll
+      for (int e = 0; e < E; e++) on &= ~((mk[e] == 0.f ? 1u : 0u) << e);
+    }
+  }
+  __device__ __forceinline__ unsigned point(int e) const { return min(lane + e * lanes, last); }
+  // Byte offset of point e's column in the batch row's slab (below 2^31: fused_shape).
+  __device__ __forceinline__ unsigned at(int e, unsigned ld) const { return (point(e) * ld + col * V) * (unsigned)sizeof(T); }
+};
+
+// A column's 16 bytes as words; element j of them as a float, and back.
+template <typename T>
+__device__ __forceinline__ float element(const u32x4& w, int j) {
+  if constexpr (std::is_same<T, float>::value) {
+    return __uint_as_float(w[j]);
+  } else {
+    const unsigned x = w[j >> 1];
+    if constexpr (std::is_same<T, bf16>::value) return __uint_as_float(j & 1 ? x & 0xffff0000u : x << 16);
+    else return (float)__builtin_bit_cast(f16, (unsigned short)(j & 1 ? x >> 16 : x));
+  }
+}
+template <typename T>
+__device__ __forceinline__ unsigned word_of(float lo, float hi) {  // (float: hi is not used)
+  if constexpr (std::is_same<T, float>::value) return __float_as_uint(lo);
+  else return __builtin_bit_cast(unsigned short, to_t<T>(lo)) | (unsigned)__builtin_bit_cast(unsigned short, to_t<T>(hi)) << 16;
+}
+template <typename T> struct AnyWords;  // 16 bytes at their elements' alignment
+typedef unsigned int u32x4_any2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned int u32x4_any4 __attribute__((ext_vector_type(4), aligned(4)));
+template <> struct AnyWords<float> { typedef u32x4_any4 type; };
+template <> struct AnyWords<f16> { typedef u32x4_any2 type; };
+template <> struct AnyWords<bf16> { typedef u32x4_any2 type; };
+
+// Makes the words new to the compiler: what was computed from them before is computed again rather than kept in registers.
+template <int E>
+__device__ __forceinline__ void forget(u32x4 (&raw)[E]) {
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      unsigned w = raw[e][k];
+      asm("" : "+v"(w));
+      raw[e][k] = w;
+    }
+  }
+}
+// Zeros in the place of points that are not `on`.
+template <int E>
+__device__ __forceinline__ void clear_off(u32x4 (&raw)[E], unsigned on) {
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) raw[e][k] = on >> e & 1 ? raw[e][k] : 0u;
+  }
+}
+template <int N>
+__device__ __forceinline__ void read_lds(const float* p, float (&f)[N]) {  // (N floats at a multiple of 16 bytes)
+#pragma unroll
+  for (int j = 0; j < N; j += 4) {
+    const floatx4 v = *(const floatx4*)(p + j);
+#pragma unroll
+    for (int k = 0; k < 4; k++) f[j + k] = v[k];
+  }
+}
+
+// All loads of a thread's column, issued before any is used (masked points too: what they hold is not looked at).
+template <typename T, int NT, int E>
+__device__ __forceinline__ void load_slab(const NormArgs& a, const Slab<T, NT, E>& s, const void* from, long long ld, u32x4 (&raw)[E]) {
+  const char* base = (const char*)((const T*)from + (size_t)s.b * a.points * ld + s.c0);
+#pragma unroll
+  for (int e = 0; e < E; e++) raw[e] = *(const typename AnyWords<T>::type*)(base + s.at(e, (unsigned)ld));
+}
+template <typename T, int NT, int E>
+__device__ __forceinline__ void store_slab(const NormArgs& a, const Slab<T, NT, E>& s, void* to, long long ld, int e, const u32x4& raw) {
+  char* base = (char*)((T*)to + (size_t)s.b * a.points * ld + s.c0);
+  if (s.in >> e & 1) *(typename AnyWords<T>::type*)(base + s.at(e, (unsigned)ld)) = raw;
+}
+
+// The lanes that share a group in a join over `groups` groups by NT threads.
+template <int NT>
+__device__ __forceinline__ int join_share(int groups) {
+  int share = 64;
+  while (share > 1 && share * groups > NT) share >>= 1;
+  return share;
+}
+
+template <typename T, int ACT, int NT, int E>
+__global__ __launch_bounds__(NT) void norm_fused_kernel(NormArgs a) {
+  constexpr int V = kVec<T>;
+  __shared__ float s_mean[V * NT], s_m2[V * NT], s_n[NT];
+  __shared__ float r_n[NT], r_mean[NT], r_m2[NT], g_mean[NT], g_rstd[NT];
+  __shared__ __align__(16) float c_mean[NT], c_mul[NT], c_add[NT];
+  int b, c0;
+  if (!slab_of(a, b, c0)) return;
+  Slab<T, NT, E> s(a, b, c0);
+  const int tid = threadIdx.x;
+  u32x4 raw[E];
+  load_slab<T, NT, E>(a, s, a.x, a.ldx, raw);
+  const float gamma = a.gamma && tid < s.width ? a.gamma[c0 + tid] : 1.f, beta = a.beta && tid < s.width ? a.beta[c0 + tid] : 0.f;
+  clear_off<E>(raw, s.on);
+
+  // A thread's own count, means, and squared deviations from them.
+  const float n = (float)__builtin_popcount(s.on), inv = s.on ? 1.f / n : 0.f;
+  float m[V], m2[V];
+#pragma unroll
+  for (int j = 0; j < V; j++) m[j] = m2[j] = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+#pragma unroll
+    for (int j = 0; j < V; j++) m[j] += element<T>(raw[e], j);
+  }
+#pragma unroll
+  for (int j = 0; j < V; j++) m[j] *= inv;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      const float d = s.on >> e & 1 ? element<T>(raw[e], j) - m[j] : 0.f;
+      m2[j] = __builtin_fmaf(d, d, m2[j]);
+    }
+  }
+  if (s.lane < s.lanes) {
+    if (s.col == 0) s_n[s.lane] = n;
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      s_mean[j * NT + tid] = m[j];
+      s_m2[j * NT + tid] = m2[j];
+    }
+  }
+  __syncthreads();
+  // Joined over the lanes: R rows of the slab's channels, then over a group's channels and those rows. Each join is
+  // exact: the mean first, then M2 = sum M2_i + n_i (mean_i - mean)^2.
+  const int R = min(NT / s.width, s.lanes);
+  if (tid < R * s.width) {
+    const int c = tid % s.width, r = tid / s.width;
+    const float* qm = s_mean + (c % V) * NT + c / V;
+    const float* q2 = s_m2 + (c % V) * NT + c / V;
+    float cn = 0.f, cs = 0.f, c2 = 0.f;
+    for (int l = r; l < s.lanes; l += R) {
+      cn += s_n[l];
+      cs = __builtin_fmaf(s_n[l], qm[l * s.cols], cs);
+    }
+    const float mean = cn > 0.f ? cs / cn : 0.f;
+    for (int l = r; l < s.lanes; l += R) {
+      const float d = qm[l * s.cols] - mean;
+      c2 += q2[l * s.cols] + s_n[l] * d * d;
+    }
+    r_n[tid] = cn;
+    r_mean[tid] = mean;
+    r_m2[tid] = c2;
+  }
+  __syncthreads();
+  {
+    const int share = join_share<NT>(a.slab_groups), sub = tid % share, g = tid / share;
+    const bool mine = g < a.slab_groups;
+    const int items = mine ? a.width * R : 0, first = mine ? g * a.width : 0;
+    float cn = 0.f, cs = 0.f, c2 = 0.f;
+    for (int i = sub; i < items; i += share) {
+      const int at = (i / a.width) * s.width + first + i % a.width;
+      cn += r_n[at];
+      cs = __builtin_fmaf(r_n[at], r_mean[at], cs);
+    }
+    for (int o = share >> 1; o >= 1; o >>= 1) { cn += __shfl_xor(cn, o); cs += __shfl_xor(cs, o); }
+    const float mean = cn > 0.f ? cs / cn : 0.f;
+    for (int i = sub; i < items; i += share) {
+      const int at = (i / a.width) * s.width + first + i % a.width;
+      const float d = r_mean[at] - mean;
+      c2 += r_m2[at] + r_n[at] * d * d;
+    }
+    for (int o = share >> 1; o >= 1; o >>= 1) c2 += __shfl_xor(c2, o);
+    if (mine && sub == 0) {
+      const float rstd = 1.f / sqrtf((cn > 0.f ? c2 / cn : 0.f) + a.eps);
+      g_mean[g] = mean;
+      g_rstd[g] = rstd;
+      const size_t out = (size_t)b * a.groups + c0 / a.width + g;
+      a.mean[out] = mean;
+      a.rstd[out] = rstd;
+    }
+  }
+  __syncthreads();
+  if (tid < s.width) {
+    const int g = tid / a.width;
+    c_mean[tid] = g_mean[g];
+    c_mul[tid] = g_rstd[g] * gamma;
+    c_add[tid] = beta;
+  }
+  __syncthreads();
+  asm("" : "+v"(s.lane));  // (addresses too are computed again)
+  forget<E>(raw);
+  float mean[V], mul[V], add[V];
+  read_lds<V>(c_mean + s.col * V, mean);
+  read_lds<V>(c_mul + s.col * V, mul);
+  read_lds<V>(c_add + s.col * V, add);
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    float f[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) f[j] = act_f<ACT>(__builtin_fmaf(element<T>(raw[e], j) - mean[j], mul[j], add[j]));
+    u32x4 w;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      w[k] = sizeof(T) == 4 ? word_of<T>(f[k], 0.f) : word_of<T>(f[(2 * k) % V], f[(2 * k + 1) % V]);
+      w[k] = s.on >> e & 1 ? w[k] : 0u;
+    }
+    store_slab<T, NT, E>(a, s, a.y, a.ldy, e, w);
+  }
+}
+
+// Backward over a slab. The channels' sums over the slab's points go to part [batch][2][channels] for dgamma and dbeta. x and
+// dy take 64 of a thread's 128 registers, so a column's channels are taken four at a time with their parameters from LDS, and
+// dx replaces dy in place. dy is 0 at masked points, and with it da.
+template <typename T, int ACT, int NT, int E>
+__global__ __launch_bounds__(NT) void norm_back_fused_kernel(NormArgs a) {
+  constexpr int V = kVec<T>, H = 4;
+  constexpr bool kExactSide = BackColumn<T, ACT>::kExactSide;
+  __shared__ float s_b[V * NT], s_g[V * NT], s_n[NT];
+  __shared__ float r_b[NT], r_g[NT], g_1[NT], g_2[NT];
+  __shared__ __align__(16) float c_mean[NT], c_mul[NT], c_beta[NT], c_k1[NT], c_k2[NT];
+  __shared__ double c_scale[kExactSide ? NT : 1];
+  int b, c0;
+  if (!slab_of(a, b, c0)) return;
+  Slab<T, NT, E> s(a, b, c0);
+  const int tid = threadIdx.x;
+  u32x4 rx[E], rd[E];
+  load_slab<T, NT, E>(a, s, a.x, a.ldx, rx);
+  load_slab<T, NT, E>(a, s, a.dy, a.lddy, rd);
+  float gamma = 1.f, rstd = 0.f;  // of channel c0 + tid
+  if (tid < s.width) {
+    const size_t g = (size_t)b * a.groups + (c0 + tid) / a.width;
+    rstd = a.rstd[g];
+    if (a.gamma) gamma = a.gamma[c0 + tid];
+    c_mean[tid] = a.mean[g];
+    c_mul[tid] = rstd * gamma;
+    c_beta[tid] = a.beta ? a.beta[c0 + tid] : 0.f;
+    if constexpr (kExactSide) c_scale[tid] = (double)rstd * (double)gamma;
+  }
+  if (s.lane < s.lanes && s.col == 0) s_n[s.lane] = (float)__builtin_popcount(s.on);
+  clear_off<E>(rx, s.on);
+  clear_off<E>(rd, s.on);
+  __syncthreads();
+#pragma unroll
+  for (int h = 0; h < V; h += H) {
+    BackColumn<T, ACT, H> col;
+    col.template read<NT>(c_mean, c_mul, c_beta, c_scale, s.col * V + h);
+    float sb[H], sg[H];
+#pragma unroll
+    for (int j = 0; j < H; j++) sb[j] = sg[j] = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+#pragma unroll
+      for (int j = 0; j < H; j++) {
+        float xc, da;
+        col.grad(element<T>(rx[e], h + j), element<T>(rd[e], h + j), j, xc, da);
+        sb[j] += da;
+        sg[j] = __builtin_fmaf(da, xc, sg[j]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (s.lane < s.lanes) {
+#pragma unroll
+      for (int j = 0; j < H; j++) { s_b[(h + j) * NT + tid] = sb[j]; s_g[(h + j) * NT + tid] = sg[j]; }
+    }
+  }
+  __syncthreads();
+  const int R = min(NT / s.width, s.lanes);
+  if (tid < R * s.width) {
+    const int c = tid % s.width, r = tid / s.width, from = (c % V) * NT + c / V;
+    float tb = 0.f, tg = 0.f;
+    for (int l = r; l < s.lanes; l += R) {
+      tb += s_b[from + l * s.cols];
+      tg += s_g[from + l * s.cols];
+    }
+    r_b[tid] = tb;
+    r_g[tid] = tg;
+  }
+  __syncthreads();
+  if (tid < s.width) {
+    float tb = 0.f, tg = 0.f;
+    for (int r = 0; r < R; r++) {
+      tb += r_b[r * s.width + tid];
+      tg += r_g[r * s.width + tid];
+    }
+    tg *= rstd;
+    float* out = a.part + (size_t)b * 2 * a.channels + c0 + tid;
+    out[0] = tb;
+    out[a.channels] = tg;
+    s_b[tid] = tb * gamma;  // (the lanes' sums have been read)
+    s_g[tid] = tg * gamma;
+  }
+  __syncthreads();
+  {
+    const int share = join_share<NT>(a.slab_groups), sub = tid % share, g = tid / share;
+    const bool mine = g < a.slab_groups;
+    float t1 = 0.f, t2 = 0.f, cn = 0.f;
+    for (int i = sub; i < (mine ? a.width : 0); i += share) {
+      t1 += s_b[g * a.width + i];
+      t2 += s_g[g * a.width + i];
+    }
+    for (int i = sub; i < (mine ? s.lanes : 0); i += share) cn += s_n[i];
+    for (int o = share >> 1; o >= 1; o >>= 1) {
+      t1 += __shfl_xor(t1, o);
+      t2 += __shfl_xor(t2, o);
+      cn += __shfl_xor(cn, o);
+    }
+    if (mine && sub == 0) {
+      const float inv = cn > 0.f ? 1.f / (cn * (float)a.width) : 0.f;
+      g_1[g] = t1 * inv;
+      g_2[g] = t2 * inv;
+    }
+  }
+  __syncthreads();
+  if (tid < s.width) {
+    c_k1[tid] = rstd * g_1[tid / a.width];
+    c_k2[tid] = rstd * rstd * g_2[tid / a.width];
+  }
+  __syncthreads();
+  asm("" : "+v"(s.lane));  // (addresses too are computed again)
+  forget<E>(rx);
+  forget<E>(rd);
+#pragma unroll
+  for (int h = 0; h < V; h += H) {
+    BackColumn<T, ACT, H> col;
+    col.template read<NT>(c_mean, c_mul, c_beta, c_scale, s.col * V + h);
+    float k1[H], k2[H];
+    read_lds<H>(c_k1 + s.col * V + h, k1);
+    read_lds<H>(c_k2 + s.col * V + h, k2);
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      float dx[H];
+#pragma unroll
+      for (int j = 0; j < H; j++) {
+        float xc, da;
+        col.grad(element<T>(rx[e], h + j), element<T>(rd[e], h + j), j, xc, da);
+        dx[j] = back_dx(da, xc, col.mul[j], k1[j], k2[j]);
+      }
+#pragma unroll
+      for (int k = 0; k < H * (int)sizeof(T) / 4; k++)
+        rd[e][h * (int)sizeof(T) / 4 + k] = sizeof(T) == 4 ? word_of<T>(dx[k], 0.f) : word_of<T>(dx[(2 * k) % H], dx[(2 * k + 1) % H]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  clear_off<E>(rd, s.on);
+#pragma unroll
+  for (int e = 0; e < E; e++) store_slab<T, NT, E>(a, s, a.dx, a.lddx, e, rd[e]);
+}
+
+// dgamma and dbeta of 64 channels a workgroup from `parts` rows of channel sums, one wave a sixteenth of them.
+__global__ __launch_bounds__(1024) void norm_back_params_kernel(NormArgs a, int parts) {
+  __shared__ float red[16][2][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = (int)blockIdx.x * 64 + lane;
+  float sb = 0.f, sg = 0.f;
+  if (c < a.channels) {
+#pragma unroll 4
+    for (int i = wave; i < parts; i += 16) {
+      const float* q = a.part + (size_t)i * 2 * a.channels + c;
+      sb += q[0];
+      sg += q[a.channels];
+    }
+  }
+  red[wave][0][lane] = sb;
+  red[wave][1][lane] = sg;
+  __syncthreads();
+  if (wave < 2 && c < a.channels) {
+    float t = 0.f;
+    for (int w = 0; w < 16; w++) t += red[w][wave][lane];
+    float* out = wave ? a.dgamma : a.dbeta;
+    if (out) out[c] = t;
+  }
+}
+
+// The threads and points a thread of the fused launch for slabs of `width` channels, 0 where none fits: the
+// slab's channels meet in one row of threads, and a thread holds up to 8 points (128 KB of 16-bit values over 1024 threads).
+struct FusedShape {
+  int groups = 0, threads = 0, each = 0;
+};
+inline int fused_each(int points, int cols, int threads) {
+  const int lanes = threads / cols;
+  return lanes ? (points + lanes - 1) / lanes : 1 << 30;
+}
+FusedShape fused_shape(const NormArgs& n, int size) {
+  const int points = n.points, groups = n.groups, width = n.width, vec = 16 / size;
+  FusedShape best;
+  // (A batch row has a point, whose address the threads past the end read, and its byte offsets have 31 bits.)
+  const long long ld = std::max(std::max(n.ldx, n.ldy), std::max(n.lddy, n.lddx));
+  if (points < 1 || points * ld >= (1ll << 31) / size) return best;
+  for (int sg = 1; sg <= groups; sg++) {
+    if (groups % sg) continue;
+    const int w = sg * width, cols = (w + vec - 1) / vec;
+    if (w > 1024) break;
+    if (w % vec) continue;
+    const int t = fused_each(points, cols, 256) <= 4 && w <= 256 ? 256 : 1024, e = fused_each(points, cols, t);
+    if (e > 8) break;
+    best = {sg, t, e <= 4 ? 4 : 8};
+    if (w >= 4 * vec) break;
+  }
+  return best;
 }
 
 NormArgs norm_args(const kg_group_norm_args& a) {
@@ -449,28 +900,58 @@ NormArgs norm_args(const kg_group_norm_args& a) {
   return n;
 }
 
-template <typename T>
-void norm_forward(const NormArgs& n, int act, hipStream_t s) {
+template <typename T, int ACT>
+void norm_forward_act(NormArgs& n, hipStream_t s) {
+  const FusedShape f = fused_shape(n, sizeof(T));
+  if (f.groups) {
+    n.slab_groups = f.groups;
+    const dim3 grid((n.batch * (n.groups / f.groups) + 7) / 8 * 8);
+    if (f.threads == 256) launch_k(norm_fused_kernel<T, ACT, 256, 4>, grid, 256, 0, s, n);
+    else if (f.each == 4) launch_k(norm_fused_kernel<T, ACT, 1024, 4>, grid, 1024, 0, s, n);
+    else launch_k(norm_fused_kernel<T, ACT, 1024, 8>, grid, 1024, 0, s, n);
+    return;
+  }
   const dim3 grid(n.batch * n.splits);
   launch_k(norm_stats_kernel<T>, grid, GT, 0, s, n);
+  launch_k(norm_apply_kernel<T, ACT>, grid, GT, 0, s, n);
+}
+
+template <typename T>
+void norm_forward(NormArgs& n, int act, hipStream_t s) {
   switch (act) {
-    case ACT_RELU: launch_k(norm_apply_kernel<T, ACT_RELU>, grid, GT, 0, s, n); break;
-    case ACT_MISH: launch_k(norm_apply_kernel<T, ACT_MISH>, grid, GT, 0, s, n); break;
-    case ACT_SILU: launch_k(norm_apply_kernel<T, ACT_SILU>, grid, GT, 0, s, n); break;
-    default: launch_k(norm_apply_kernel<T, ACT_ID>, grid, GT, 0, s, n); break;
+    case ACT_RELU: norm_forward_act<T, ACT_RELU>(n, s); break;
+    case ACT_MISH: norm_forward_act<T, ACT_MISH>(n, s); break;
+    case ACT_SILU: norm_forward_act<T, ACT_SILU>(n, s); break;
+    default: norm_forward_act<T, ACT_ID>(n, s); break;
   }
 }
 
 template <typename T, int ACT>
-void norm_backward_act(const NormArgs& n, hipStream_t s) {
+void norm_backward_act(NormArgs& n, hipStream_t s) {
+  const FusedShape f = fused_shape(n, sizeof(T));
+  const dim3 columns((n.channels + 63) / 64);
+  if (f.groups) {
+    n.slab_groups = f.groups;
+    const dim3 grid((n.batch * (n.groups / f.groups) + 7) / 8 * 8);
+    if (n.batch) {
+      if (f.threads == 256) launch_k(norm_back_fused_kernel<T, ACT, 256, 4>, grid, 256, 0, s, n);
+      else if (f.each == 4) launch_k(norm_back_fused_kernel<T, ACT, 1024, 4>, grid, 1024, 0, s, n);
+      else launch_k(norm_back_fused_kernel<T, ACT, 1024, 8>, grid, 1024, 0, s, n);
+    }
+    if (n.dgamma || n.dbeta) launch_k(norm_back_params_kernel, columns, 1024, 0, s, n, n.batch);
+    return;
+  }
   const dim3 grid(n.batch * n.splits);
-  if (n.batch) launch_k(norm_back_sums_kernel<T, ACT>, grid, GT, 0, s, n);
-  launch_k(norm_back_join_kernel, dim3(n.batch + (n.channels + 63) / 64), GT, 0, s, n);
-  if (n.batch) launch_k(norm_back_apply_kernel<T, ACT>, grid, GT, 0, s, n);
+  if (n.batch) {
+    launch_k(norm_back_sums_kernel<T, ACT>, grid, GT, 0, s, n);
+    launch_k(norm_back_join_kernel, dim3((n.batch * n.groups + GT / 64 - 1) / (GT / 64)), GT, 0, s, n);
+    launch_k(norm_back_apply_kernel<T, ACT>, grid, GT, 0, s, n);
+  }
+  if (n.dgamma || n.dbeta) launch_k(norm_back_params_kernel, columns, 1024, 0, s, n, n.batch * n.splits);
 }
 
 template <typename T>
-void norm_backward(const NormArgs& n, int act, hipStream_t s) {
+void norm_backward(NormArgs& n, int act, hipStream_t s) {
   switch (act) {
     case ACT_RELU: norm_backward_act<T, ACT_RELU>(n, s); break;
     case ACT_MISH: norm_backward_act<T, ACT_MISH>(n, s); break;
@@ -483,7 +964,7 @@ void norm_backward(const NormArgs& n, int act, hipStream_t s) {
 
 int group_norm_splits(int batch, int points, int channels) {
   const long long want = ((long long)points * channels + kSplitTarget - 1) / kSplitTarget;
-  const long long most = batch > 0 ? (4096 + batch - 1) / batch : 1;
+  const long long most = batch > 0 ? (2048 + batch - 1) / batch : 1;
   long long n = want < most ? want : most;
   if (n > points) n = points;
   return n < 1 ? 1 : (int)n;
@@ -496,7 +977,7 @@ size_t group_norm_workspace(int batch, int points, int channels, int groups, boo
 }
 
 void launch_group_norm(const kg_group_norm_args& a, hipStream_t s) {
-  const NormArgs n = norm_args(a);
+  NormArgs n = norm_args(a);
   switch (a.type) {
     case PREC_F32: norm_forward<float>(n, a.act, s); break;
     case PREC_F16: norm_forward<f16>(n, a.act, s); break;

@@ -133,7 +133,8 @@ void check_norm(const kg_group_norm_args& a, bool backward) {
   need(a.batch >= 0 && a.points >= 0, op, "batch and points must be at least 0");
   need(a.channels >= 1 && a.groups >= 1 && a.channels % a.groups == 0, op, "channels must be a multiple of groups");
   need(a.groups <= kMaxNormGroups, op, "at most 2048 groups are supported");
-  need((long long)a.batch * a.points <= std::numeric_limits<int>::max(), op, "batch x points is out of range");
+  need((long long)a.batch * a.points <= std::numeric_limits<int>::max() && (long long)a.batch * a.groups <= std::numeric_limits<int>::max(),
+       op, "batch x points or batch x groups is out of range");
   check_type(a.type, op);
   need(a.act >= KG_ACT_IDENTITY && a.act <= KG_ACT_SILU, op, "unknown activation");
   const long long rows = (long long)a.batch * a.points;

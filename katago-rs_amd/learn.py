@@ -19,6 +19,8 @@ runtime.
 
 import collections
 import ctypes
+import math
+import struct
 
 import numpy as np
 import torch
@@ -28,6 +30,7 @@ from . import KgError, PRECISION_BF16, PRECISION_F16, PRECISION_F32, _check, lib
 TYPES = {torch.float32: PRECISION_F32, torch.float16: PRECISION_F16, torch.bfloat16: PRECISION_BF16}
 ACTS = {"identity": 0, "relu": 1, "mish": 2, "silu": 3}
 BLOCK = 256  # KG_ADAMW_BLOCK
+_BYTES = (torch.bool, torch.uint8)
 
 PolicyLoss = collections.namedtuple("PolicyLoss", ["loss", "logp", "kl", "grad"])
 PreferenceLoss = collections.namedtuple("PreferenceLoss", ["loss", "margin", "seq_logp", "grad"])
@@ -35,26 +38,11 @@ PreferenceLoss = collections.namedtuple("PreferenceLoss", ["loss", "margin", "se
 _vp, _ci, _ll, _cd = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_double
 
 
-class _PolicyArgs(ctypes.Structure):
-    _fields_ = [("rows", _ci), ("columns", _ci), ("type", _ci), ("logits", _vp), ("ld", _ll), ("legal", _vp),
-                ("ld_legal", _ll), ("action", _vp), ("old_logp", _vp), ("advantage", _vp), ("weight", _vp),
-                ("ref_logits", _vp), ("ld_ref", _ll), ("ref_logp", _vp), ("logit_scale", _cd), ("clip_low", _cd),
-                ("clip_high", _cd), ("kl_coef", _cd), ("loss", _vp), ("logp", _vp), ("kl", _vp), ("grad", _vp),
-                ("ld_grad", _ll)]
-
-
-class _PreferenceArgs(ctypes.Structure):
-    _fields_ = [("rows", _ci), ("columns", _ci), ("type", _ci), ("logits", _vp), ("ld", _ll), ("label", _vp),
-                ("pairs", _ci), ("offsets", _vp), ("ref_logp", _vp), ("weight", _vp), ("beta", _cd),
-                ("label_smoothing", _cd), ("average", _ci), ("loss", _vp), ("margin", _vp), ("seq_logp", _vp),
-                ("grad", _vp), ("ld_grad", _ll), ("workspace", _vp)]
-
-
-class _NormArgs(ctypes.Structure):
-    _fields_ = [("batch", _ci), ("points", _ci), ("channels", _ci), ("groups", _ci), ("type", _ci), ("act", _ci),
-                ("eps", _cd), ("x", _vp), ("ldx", _ll), ("mask", _vp), ("gamma", _vp), ("beta", _vp), ("mean", _vp),
-                ("rstd", _vp), ("workspace", _vp), ("y", _vp), ("ldy", _ll), ("dy", _vp), ("lddy", _ll), ("dx", _vp),
-                ("lddx", _ll), ("dgamma", _vp), ("dbeta", _vp)]
+# The argument structures of include/kgx.h, packed at their natural alignment: a third of a ctypes structure's time, and a small
+# batch's call is its host time.
+_POLICY_ARGS = struct.Struct("@3iPqPqPPPPPqPddddPPPPq0q")
+_PREFERENCE_ARGS = struct.Struct("@3iPqPiPPPddiPPPPqP0q")
+_NORM_ARGS = struct.Struct("@6idPqPPPPPPPqPqPqPP0q")
 
 
 class _AdamTensor(ctypes.Structure):
@@ -94,27 +82,28 @@ def _library():
     return L
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+# The handle of torch's current stream of a device, without the Stream object around it where torch offers that.
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _rows(t, name, like=None):
     """(pointer, row stride) of a matrix on the GPU with unit column stride; `like`: of that shape, type and device."""
-    if t.dim() != 2 or t.dtype not in TYPES or (t.stride(1) != 1 and t.shape[1] > 1):
+    ld = t.stride()
+    if len(ld) != 2 or t.dtype not in TYPES or (ld[1] != 1 and t.shape[1] > 1):
         raise ValueError(f"{name} must be [rows, columns] of float32, float16 or bfloat16 with contiguous columns")
     if not t.is_cuda:
         raise ValueError(f"{name} must be on the GPU")
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+    if like is not None and (t.shape != like.shape or t.dtype is not like.dtype or t.get_device() != like.get_device()):
         raise ValueError(f"{name} must have the shape, type and device of the logits")
-    return t.data_ptr(), t.stride(0)
+    return t.data_ptr(), ld[0]
 
 
 def _vector(t, n, dtype, name, device):
-    """Pointer of a contiguous vector of n elements on `device`; None for None."""
+    """Pointer of a contiguous vector of n elements on GPU number `device`; 0 for None."""
     if t is None:
-        return None
-    if t.shape != (n,) or t.dtype != dtype or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous vector of {n} {str(dtype)[6:]} on {device}")
+        return 0
+    if t.dtype is not dtype or t.shape != (n,) or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous vector of {n} {str(dtype)[6:]} on GPU {device}")
     return t.data_ptr()
 
 
@@ -128,28 +117,30 @@ def policy_loss(logits, actions, old_logp, advantage, *, legal=None, weight=None
     the logits' type (into `grad` when given; None without want_grad)."""
     ptr, ld = _rows(logits, "logits")
     n, v = logits.shape
-    dev = logits.device
-    lg, ld_lg = None, 0
+    dev = logits.get_device()
+    lg = ld_lg = ref = ld_ref = g = ld_g = 0
     if legal is not None:
-        if legal.shape != (n, v) or legal.dtype not in (torch.bool, torch.uint8) or legal.device != dev or \
-                (legal.stride(1) != 1 and v > 1):
-            raise ValueError(f"legal must be [{n}, {v}] bool or uint8 on {dev} with contiguous columns")
+        if legal.shape != (n, v) or legal.dtype not in _BYTES or legal.get_device() != dev or (legal.stride(1) != 1 and v > 1):
+            raise ValueError(f"legal must be [{n}, {v}] bool or uint8 on GPU {dev} with contiguous columns")
         lg, ld_lg = legal.data_ptr(), legal.stride(0)
-    ref, ld_ref = (None, 0) if ref_logits is None else _rows(ref_logits, "ref_logits", logits)
-    if grad is None and want_grad:
-        grad = torch.empty(n, v, dtype=logits.dtype, device=dev)
-    g, ld_g = (None, 0) if grad is None else _rows(grad, "grad", logits)
-    out = torch.empty(3, n, dtype=torch.float32, device=dev)
-    o = out.data_ptr()
-    low, high = clip
-    args = _PolicyArgs(n, v, TYPES[logits.dtype], ptr, ld, lg, ld_lg, _vector(actions, n, torch.int32, "actions", dev),
-                       _vector(old_logp, n, torch.float32, "old_logp", dev),
-                       _vector(advantage, n, torch.float32, "advantage", dev),
-                       _vector(weight, n, torch.float32, "weight", dev), ref, ld_ref,
-                       _vector(ref_logp, n, torch.float32, "ref_logp", dev), logit_scale, low, high, kl_coef, o, o + 4 * n,
-                       o + 8 * n, g, ld_g)
-    _check(_library().kg_policy_loss(dev.index, _stream(dev), ctypes.byref(args)))
-    return PolicyLoss(out[0], out[1], out[2], grad)
+    if ref_logits is not None:
+        ref, ld_ref = _rows(ref_logits, "ref_logits", logits)
+    if grad is not None:
+        g, ld_g = _rows(grad, "grad", logits)
+    elif want_grad:
+        grad = torch.empty((n, v), dtype=logits.dtype, device=logits.device)
+        g, ld_g = grad.data_ptr(), v
+    loss, logp, kl = torch.empty((3, n), dtype=torch.float32, device=logits.device).unbind()
+    o = loss.data_ptr()
+    args = _POLICY_ARGS.pack(n, v, TYPES[logits.dtype], ptr, ld, lg, ld_lg, _vector(actions, n, torch.int32, "actions", dev),
+                             _vector(old_logp, n, torch.float32, "old_logp", dev),
+                             _vector(advantage, n, torch.float32, "advantage", dev),
+                             _vector(weight, n, torch.float32, "weight", dev), ref, ld_ref,
+                             _vector(ref_logp, n, torch.float32, "ref_logp", dev), logit_scale, clip[0], clip[1], kl_coef, o,
+                             o + 4 * n, o + 8 * n, g, ld_g)
+    if _library().kg_policy_loss(dev, _stream(dev), args):
+        _check(1)
+    return PolicyLoss(loss, logp, kl, grad)
 
 
 def preference_loss(logits, labels, offsets, ref_logp, *, beta=0.1, label_smoothing=0.0, average=False, weight=None,
@@ -162,106 +153,124 @@ def preference_loss(logits, labels, offsets, ref_logp, *, beta=0.1, label_smooth
     seq_logp [2 p] and grad [t, v] of the logits' type (into `grad` when given; None without want_grad)."""
     ptr, ld = _rows(logits, "logits")
     t, v = logits.shape
-    dev = logits.device
+    dev = logits.get_device()
+    g = ld_g = 0
     if offsets.dim() != 1 or offsets.shape[0] % 2 == 0:
         raise ValueError("offsets must be a vector of an odd length")
     p = offsets.shape[0] // 2
-    if grad is None and want_grad:
-        grad = torch.empty(t, v, dtype=logits.dtype, device=dev)
-    g, ld_g = (None, 0) if grad is None else _rows(grad, "grad", logits)
+    if grad is not None:
+        g, ld_g = _rows(grad, "grad", logits)
+    elif want_grad:
+        grad = torch.empty((t, v), dtype=logits.dtype, device=logits.device)
+        g, ld_g = grad.data_ptr(), v
     L = _library()
-    out = torch.empty(4 * p, dtype=torch.float32, device=dev)
-    work = torch.empty(L.kg_preference_loss_workspace(t), dtype=torch.uint8, device=dev)
+    # (One allocation: the pairs' results, then the workspace at a multiple of 256 bytes.)
+    room = -(-16 * p // 256) * 256
+    out = torch.empty(room // 4 + L.kg_preference_loss_workspace(t) // 4, dtype=torch.float32, device=logits.device)
+    loss, margin, seq_logp, _ = out.split_with_sizes((p, p, 2 * p, out.numel() - 4 * p))
     o = out.data_ptr()
-    args = _PreferenceArgs(t, v, TYPES[logits.dtype], ptr, ld, _vector(labels, t, torch.int32, "labels", dev), p,
-                           _vector(offsets, 2 * p + 1, torch.int32, "offsets", dev),
-                           _vector(ref_logp, 2 * p, torch.float32, "ref_logp", dev),
-                           _vector(weight, p, torch.float32, "weight", dev), beta, label_smoothing, bool(average), o, o + 4 * p,
-                           o + 8 * p, g, ld_g, work.data_ptr())
-    _check(L.kg_preference_loss(dev.index, _stream(dev), ctypes.byref(args)))
-    return PreferenceLoss(out[:p], out[p:2 * p], out[2 * p:], grad)
+    args = _PREFERENCE_ARGS.pack(t, v, TYPES[logits.dtype], ptr, ld, _vector(labels, t, torch.int32, "labels", dev), p,
+                                 _vector(offsets, 2 * p + 1, torch.int32, "offsets", dev),
+                                 _vector(ref_logp, 2 * p, torch.float32, "ref_logp", dev),
+                                 _vector(weight, p, torch.float32, "weight", dev), beta, label_smoothing, bool(average), o,
+                                 o + 4 * p, o + 8 * p, g, ld_g, o + room)
+    if L.kg_preference_loss(dev, _stream(dev), args):
+        _check(1)
+    return PreferenceLoss(loss, margin, seq_logp, grad)
 
 
 def _points(t, name):
     """(pointer, row stride) of [batch, ..., channels] whose points lie evenly spaced."""
-    if t.dim() < 2 or t.dtype not in TYPES:
+    shape = t.shape
+    if len(shape) < 2 or t.dtype not in TYPES:
         raise ValueError(f"{name} must be [batch, ..., channels] of float32, float16 or bfloat16")
     if not t.is_cuda:
         raise ValueError(f"{name} must be on the GPU")
-    if not t.numel():
-        return t.data_ptr(), t.shape[-1]
+    if t.is_contiguous() or not t.numel():
+        return t.data_ptr(), shape[-1]
     ld = None
     span = 1
-    for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+    for size, stride in zip(reversed(shape[:-1]), reversed(t.stride()[:-1])):
         if size != 1:
             if ld is None:
                 ld = stride
             elif stride != ld * span:
                 raise ValueError(f"the points of {name} must be evenly spaced")
             span *= size
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    if shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name} must have contiguous channels")
-    return t.data_ptr(), t.shape[-1] if ld is None else ld
+    return t.data_ptr(), shape[-1] if ld is None else ld
 
 
 def _norm_shape(x, groups, gamma, beta, mask, act):
-    if x.dim() < 2 or act not in ACTS:
-        raise ValueError(f"x must be [batch, ..., channels] and act one of {', '.join(ACTS)}")
-    batch, channels = x.shape[0], x.shape[-1]
-    points = 1
-    for s in x.shape[1:-1]:
-        points *= s
-    dev = x.device
+    shape, dev = x.shape, x.get_device()
+    if act not in ACTS:
+        raise ValueError(f"act must be one of {', '.join(ACTS)}")
+    batch, channels = shape[0], shape[-1]
+    points = shape[1] if len(shape) == 3 else math.prod(shape[1:-1])
+    mk = 0
     if mask is not None:
-        if mask.shape != x.shape[:-1] or mask.dtype != torch.float32 or mask.device != dev or not mask.is_contiguous():
-            raise ValueError(f"mask must be contiguous float32 of shape {tuple(x.shape[:-1])} on {dev}")
-        mask = mask.data_ptr()
-    return (batch, points, channels, int(groups), mask, _vector(gamma, channels, torch.float32, "gamma", dev),
+        if mask.dtype is not torch.float32 or mask.shape != shape[:-1] or mask.get_device() != dev or not mask.is_contiguous():
+            raise ValueError(f"mask must be contiguous float32 of shape {tuple(shape[:-1])} on GPU {dev}")
+        mk = mask.data_ptr()
+    return (dev, batch, points, channels, int(groups), mk, _vector(gamma, channels, torch.float32, "gamma", dev),
             _vector(beta, channels, torch.float32, "beta", dev))
+
+
+def _like(t, x, name):
+    if t.shape != x.shape or t.dtype is not x.dtype or t.get_device() != x.get_device():
+        raise ValueError(f"{name} must have the shape, type and device of x")
+    return _points(t, name)
 
 
 def group_norm(x, groups, gamma=None, beta=None, *, mask=None, eps=1e-5, act="identity", y=None):
     """act(group norm of x) on channels-last x [batch, ..., channels] over the points with a nonzero mask [batch, ...]
     (kg_group_norm). Returns y (into `y` when given; 0 where the mask is 0), and mean and rstd [batch, groups]."""
     ptr, ld = _points(x, "x")
-    b, p, c, g, mk, gm, bt = _norm_shape(x, groups, gamma, beta, mask, act)
+    dev, b, p, c, g, mk, gm, bt = _norm_shape(x, groups, gamma, beta, mask, act)
     if y is None:
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    elif y.shape != x.shape or y.dtype != x.dtype or y.device != x.device:
-        raise ValueError("y must have the shape, type and device of x")
-    yp, ldy = _points(y, "y")
+        yp, ldy = y.data_ptr(), c
+    else:
+        yp, ldy = _like(y, x, "y")
     L = _library()
-    stats = torch.empty(2, b, max(g, 0), dtype=torch.float32, device=x.device)
-    work = torch.empty(L.kg_group_norm_workspace(b, p, c, g, 0), dtype=torch.uint8, device=x.device)
-    args = _NormArgs(b, p, c, g, TYPES[x.dtype], ACTS[act], eps, ptr, ld, mk, gm, bt, stats.data_ptr(),
-                     stats.data_ptr() + 4 * b * g, work.data_ptr(), yp, ldy, None, 0, None, 0, None, None)
-    _check(L.kg_group_norm(x.device.index, _stream(x.device), ctypes.byref(args)))
-    return y, stats[0], stats[1]
+    stats = torch.empty((2, b, max(g, 0)), dtype=torch.float32, device=x.device)
+    bytes_ = L.kg_group_norm_workspace(b, p, c, g, 0)
+    work = torch.empty(bytes_, dtype=torch.uint8, device=x.device).data_ptr() if bytes_ else 0
+    mean, rstd = stats.unbind()
+    o = stats.data_ptr()
+    args = _NORM_ARGS.pack(b, p, c, g, TYPES[x.dtype], ACTS[act], eps, ptr, ld, mk, gm, bt, o, o + 4 * b * g, work, yp, ldy, 0, 0,
+                           0, 0, 0, 0)
+    if L.kg_group_norm(dev, _stream(dev), args):
+        _check(1)
+    return y, mean, rstd
 
 
 def group_norm_backward(dy, x, mean, rstd, groups, gamma=None, beta=None, *, mask=None, act="identity", dx=None):
     """The gradients (dx, dgamma, dbeta) of a loss whose gradient with respect to group_norm's y is dy, from its mean and rstd
     (kg_group_norm_backward); dx into `dx` when given."""
     ptr, ld = _points(x, "x")
-    b, p, c, g, mk, gm, bt = _norm_shape(x, groups, gamma, beta, mask, act)
-    dev = x.device
+    dev, b, p, c, g, mk, gm, bt = _norm_shape(x, groups, gamma, beta, mask, act)
+    dyp, lddy = _like(dy, x, "dy")
     if dx is None:
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    for t, name in ((dy, "dy"), (dx, "dx")):
-        if t.shape != x.shape or t.dtype != x.dtype or t.device != dev:
-            raise ValueError(f"{name} must have the shape, type and device of x")
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dxp, lddx = dx.data_ptr(), c
+    else:
+        dxp, lddx = _like(dx, x, "dx")
     for t, name in ((mean, "mean"), (rstd, "rstd")):
-        if t.shape != (b, g) or t.dtype != torch.float32 or t.device != dev or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous float32 of shape ({b}, {g}) on {dev}")
-    dyp, lddy = _points(dy, "dy")
-    dxp, lddx = _points(dx, "dx")
+        if t.dtype is not torch.float32 or t.shape != (b, g) or t.get_device() != dev or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous float32 of shape ({b}, {g}) on GPU {dev}")
     L = _library()
-    out = torch.empty(2, c, dtype=torch.float32, device=dev)
-    work = torch.empty(L.kg_group_norm_workspace(b, p, c, g, 1), dtype=torch.uint8, device=dev)
-    args = _NormArgs(b, p, c, g, TYPES[x.dtype], ACTS[act], 0.0, ptr, ld, mk, gm, bt, mean.data_ptr(), rstd.data_ptr(),
-                     work.data_ptr(), None, 0, dyp, lddy, dxp, lddx, out.data_ptr(), out.data_ptr() + 4 * c)
-    _check(L.kg_group_norm_backward(dev.index, _stream(dev), ctypes.byref(args)))
-    return dx, out[0], out[1]
+    bytes_ = L.kg_group_norm_workspace(b, p, c, g, 1)
+    work = torch.empty(bytes_, dtype=torch.uint8, device=x.device).data_ptr() if bytes_ else 0
+    out = torch.empty((2, c), dtype=torch.float32, device=x.device)
+    dgamma, dbeta = out.unbind()
+    o = out.data_ptr()
+    args = _NORM_ARGS.pack(b, p, c, g, TYPES[x.dtype], ACTS[act], 0.0, ptr, ld, mk, gm, bt, mean.data_ptr(), rstd.data_ptr(),
+                           work, 0, 0, dyp, lddy, dxp, lddx, o, o + 4 * c)
+    if L.kg_group_norm_backward(dev, _stream(dev), args):
+        _check(1)
+    return dx, dgamma, dbeta
 
 
 class AdamW:
@@ -290,6 +299,7 @@ class AdamW:
         self.params, self.masters, self.state_bits = params, masters, state_bits
         self.lr, self.betas, self.eps = lr, tuple(betas), eps
         self.step_count = 0
+        self._sizes = [p.numel() for p in params]
         blocks = [-(-p.numel() // BLOCK) for p in params]
         self.first_block = np.concatenate([[0], np.cumsum(blocks)]).astype(np.int64)
         total = int(self.first_block[-1])
@@ -315,14 +325,21 @@ class AdamW:
         grads = list(grads)
         if len(grads) != len(self.params):
             raise ValueError(f"AdamW needs {len(self.params)} gradients, got {len(grads)}")
-        for i, (g, p) in enumerate(zip(grads, self.params)):
-            if g is not None and (g.dtype not in TYPES or g.shape != p.shape or g.device != self.device or
-                                  not g.is_contiguous()):
-                raise ValueError(f"gradient {i} must be contiguous float32, float16 or bfloat16 of its parameter's shape "
-                                 "and device")
-        self._rec["grad"] = [0 if g is None else g.data_ptr() for g in grads]
-        self._rec["grad_type"] = [0 if g is None else TYPES[g.dtype] for g in grads]
-        self._rec["elements"] = [0 if g is None else g.numel() for g in grads]
+        some = [g for g in grads if g is not None]
+        sizes = self._sizes if len(some) == len(grads) else [n for g, n in zip(grads, self._sizes) if g is not None]
+        # (Whole lists at once: a network has hundreds of gradients, and a step's time on the GPU is near this one's.)
+        dev = self.device.index
+        if [g.numel() for g in some] != sizes or not all([g.is_contiguous() for g in some]) or \
+                any([g.get_device() != dev for g in some]) or not all([g.dtype in TYPES for g in some]):
+            raise ValueError("each gradient must be contiguous float32, float16 or bfloat16 of its parameter's size and GPU")
+        if len(some) == len(grads):
+            self._rec["grad"] = [g.data_ptr() for g in grads]
+            self._rec["grad_type"] = [TYPES[g.dtype] for g in grads]
+            self._rec["elements"] = sizes
+        else:
+            self._rec["grad"] = [0 if g is None else g.data_ptr() for g in grads]
+            self._rec["grad_type"] = [0 if g is None else TYPES[g.dtype] for g in grads]
+            self._rec["elements"] = [0 if g is None else g.numel() for g in grads]
         self.grads = grads
 
     def _hyper(self, lr, step, grad_scale, seed):
@@ -341,7 +358,8 @@ class AdamW:
                                    values.numel() * values.element_size() < ctypes.sizeof(AdamValues)):
             raise ValueError(f"values must be {ctypes.sizeof(AdamValues)} bytes on {self.device}")
         number = self.step_count + 1 if step is None else step
-        _check(_library().kg_adamw_step(self.device.index, _stream(self.device), len(self.params),
+        dev = self.device.index
+        _check(_library().kg_adamw_step(dev, _stream(dev), len(self.params),
                                         ctypes.byref(self._tensors), ctypes.byref(self._state),
                                         ctypes.byref(self._hyper(lr, number, grad_scale, seed)), None if values is None else values.data_ptr()))
         self.step_count = number
@@ -360,8 +378,8 @@ class AdamW:
         dtype = dtype or (torch.float32 if self.state_bits == 32 else torch.bfloat16)
         if dtype not in TYPES:
             raise ValueError("moments are given as float32, float16 or bfloat16")
-        m, root = (torch.empty(self.m.numel(), dtype=dtype, device=self.device) for _ in range(2))
-        _check(_library().kg_adamw_moments(self.device.index, _stream(self.device), self.m.numel() // BLOCK,
+        m, root = torch.empty((2, self.m.numel()), dtype=dtype, device=self.device).unbind()
+        _check(_library().kg_adamw_moments(self.device.index, _stream(self.device.index), self.m.numel() // BLOCK,
                                            ctypes.byref(self._state),
                                            TYPES[dtype], m.data_ptr(), root.data_ptr()))
         return m, root

@@ -7,6 +7,7 @@ import numpy as np
 import pytest
 import torch
 
+import learn_abi as abi
 import learn_ref as ref
 
 
@@ -19,7 +20,7 @@ def _policy_args(learn, **change):
     base = dict(rows=4, columns=9, type=0, logits=4096, ld=9, legal=None, ld_legal=0, action=4096, old_logp=4096,
                 advantage=4096, weight=None, ref_logits=None, ld_ref=0, ref_logp=None, logit_scale=1.0, clip_low=0.2,
                 clip_high=0.2, kl_coef=0.0, loss=4096, logp=4096, kl=4096, grad=8192, ld_grad=9)
-    return learn._PolicyArgs(**{**base, **change})
+    return abi.PolicyArgs(**{**base, **change})
 
 
 @pytest.mark.parametrize("change,text", [
@@ -35,6 +36,14 @@ def _policy_args(learn, **change):
 def test_policy_loss_refuses(kgx, learn, change, text):
     assert kgx.lib().kg_policy_loss(0, None, ctypes.byref(_policy_args(learn, **change))) == 1
     assert text in kgx.lib().kg_last_error().decode()
+
+
+@pytest.mark.parametrize("name", ["POLICY", "PREFERENCE", "NORM"])
+def test_packed_arguments_lie_as_the_structures_do(learn, name):
+    packed, kind = getattr(learn, f"_{name}_ARGS"), getattr(abi, {"POLICY": "PolicyArgs", "PREFERENCE": "PreferenceArgs", "NORM": "NormArgs"}[name])
+    values = [0.5 + i if t is ctypes.c_double else 3 + i for i, (_, t) in enumerate(kind._fields_)]
+    got = kind.from_buffer_copy(packed.pack(*values))
+    assert packed.size == ctypes.sizeof(kind) and [getattr(got, f) for f, _ in kind._fields_] == values
 
 
 def test_null_structures_are_refused(kgx, learn):
@@ -56,7 +65,7 @@ def test_preference_loss_refuses(kgx, learn, change, text):
     base = dict(rows=4, columns=9, type=1, logits=4096, ld=9, label=4096, pairs=1, offsets=4096, ref_logp=4096, weight=None,
                 beta=0.1, label_smoothing=0.0, average=0, loss=4096, margin=4096, seq_logp=4096, grad=8192, ld_grad=9,
                 workspace=4096)
-    args = learn._PreferenceArgs(**{**base, **change})
+    args = abi.PreferenceArgs(**{**base, **change})
     assert kgx.lib().kg_preference_loss(0, None, ctypes.byref(args)) == 1
     assert text in kgx.lib().kg_last_error().decode()
 
@@ -73,14 +82,14 @@ def test_group_norm_refuses(kgx, learn, change, text, backward):
     base = dict(batch=2, points=9, channels=12, groups=3, type=0, act=2, eps=1e-5, x=4096, ldx=12, mask=None, gamma=None,
                 beta=None, mean=4096, rstd=4096, workspace=4096, y=8192, ldy=12, dy=16384, lddy=12, dx=8192, lddx=12,
                 dgamma=None, dbeta=None)
-    args = learn._NormArgs(**{**base, **change})
+    args = abi.NormArgs(**{**base, **change})
     L = kgx.lib()
     assert (L.kg_group_norm_backward if backward else L.kg_group_norm)(0, None, ctypes.byref(args)) == 1
     assert text in L.kg_last_error().decode()
 
 
 def test_group_norm_refuses_eps(kgx, learn):
-    args = learn._NormArgs(2, 9, 12, 3, 0, 2, 0.0, 4096, 12)
+    args = abi.NormArgs(2, 9, 12, 3, 0, 2, 0.0, 4096, 12)
     assert kgx.lib().kg_group_norm(0, None, ctypes.byref(args)) == 1
     assert "eps" in kgx.lib().kg_last_error().decode()
 

@@ -69,7 +69,7 @@ struct NormArgs {
   float* counts;   // backward: [batch][splits] points
   float* sums;     // backward: [batch][2][groups]
   int batch, points, channels, groups, width, splits;  // width: channels of a group
-  int slab_groups;  // groups of a slab (fused launches)
+  int slab_groups, each;  // fused launches: groups of a slab, points a thread takes
   float eps;
 };
 
@@ -463,17 +463,17 @@ __device__ __forceinline__ bool slab_of(const NormArgs& a, int& b, int& c0) {
   return true;
 }
 
-// A fused workgroup's points: thread (col, lane) takes points lane + e lanes, e < E, of 16-byte column col. Threads and
-// points past the end read the last one's address, so that no load is behind a branch.
-template <typename T, int NT, int E>
+// A fused workgroup's points: thread (col, lane) takes points lane + e lanes, e < each (at most E), of 16-byte column col.
+// Threads and points past the end read the last one's address, so that no load is behind a branch of its own.
+template <typename T, int E>
 struct Slab {
   static constexpr int V = kVec<T>;
-  int b, c0, width, cols, lanes, col, lane, last;  // width: the slab's channels, whole columns
+  int b, c0, each, threads, width, cols, lanes, col, lane, last;  // width: the slab's channels, whole columns
   unsigned in, on;  // bit e: the point exists; and is not masked
-  __device__ __forceinline__ Slab(const NormArgs& a, int b_, int c0_) : b(b_), c0(c0_) {
+  __device__ __forceinline__ Slab(const NormArgs& a, int b_, int c0_) : b(b_), c0(c0_), each(a.each), threads(blockDim.x) {
     width = a.slab_groups * a.width;
     cols = width / V;
-    lanes = NT / cols;
+    lanes = threads / cols;
     lane = threadIdx.x / cols;
     col = threadIdx.x - lane * cols;
     last = a.points - 1;
@@ -551,38 +551,41 @@ __device__ __forceinline__ void read_lds(const float* p, float (&f)[N]) {  // (N
 }
 
 // All loads of a thread's column, issued before any is used (masked points too: what they hold is not looked at).
-template <typename T, int NT, int E>
-__device__ __forceinline__ void load_slab(const NormArgs& a, const Slab<T, NT, E>& s, const void* from, long long ld, u32x4 (&raw)[E]) {
+template <typename T, int E>
+__device__ __forceinline__ void load_slab(const NormArgs& a, const Slab<T, E>& s, const void* from, long long ld, u32x4 (&raw)[E]) {
   const char* base = (const char*)((const T*)from + (size_t)s.b * a.points * ld + s.c0);
 #pragma unroll
-  for (int e = 0; e < E; e++) raw[e] = *(const typename AnyWords<T>::type*)(base + s.at(e, (unsigned)ld));
+  for (int e = 0; e < E; e++) {
+    raw[e] = u32x4{0, 0, 0, 0};
+    if (e < s.each) raw[e] = *(const typename AnyWords<T>::type*)(base + s.at(e, (unsigned)ld));
+  }
 }
-template <typename T, int NT, int E>
-__device__ __forceinline__ void store_slab(const NormArgs& a, const Slab<T, NT, E>& s, void* to, long long ld, int e, const u32x4& raw) {
+template <typename T, int E>
+__device__ __forceinline__ void store_slab(const NormArgs& a, const Slab<T, E>& s, void* to, long long ld, int e, const u32x4& raw) {
   char* base = (char*)((T*)to + (size_t)s.b * a.points * ld + s.c0);
   if (s.in >> e & 1) *(typename AnyWords<T>::type*)(base + s.at(e, (unsigned)ld)) = raw;
 }
 
-// The lanes that share a group in a join over `groups` groups by NT threads.
-template <int NT>
-__device__ __forceinline__ int join_share(int groups) {
+// The lanes that share a group in a join over `groups` groups by `threads` threads (groups <= threads).
+__device__ __forceinline__ int join_share(int groups, int threads) {
   int share = 64;
-  while (share > 1 && share * groups > NT) share >>= 1;
+  while (share > 1 && share * groups > threads) share >>= 1;
   return share;
 }
 
 template <typename T, int ACT, int NT, int E>
 __global__ __launch_bounds__(NT) void norm_fused_kernel(NormArgs a) {
   constexpr int V = kVec<T>;
-  __shared__ float s_mean[V * NT], s_m2[V * NT], s_n[NT];
+  constexpr int P = NT + 8;  // (the eight channels of a column lie in different banks)
+  __shared__ float s_mean[V * P], s_m2[V * P], s_n[NT];
   __shared__ float r_n[NT], r_mean[NT], r_m2[NT], g_mean[NT], g_rstd[NT];
   __shared__ __align__(16) float c_mean[NT], c_mul[NT], c_add[NT];
   int b, c0;
   if (!slab_of(a, b, c0)) return;
-  Slab<T, NT, E> s(a, b, c0);
+  Slab<T, E> s(a, b, c0);
   const int tid = threadIdx.x;
   u32x4 raw[E];
-  load_slab<T, NT, E>(a, s, a.x, a.ldx, raw);
+  load_slab<T, E>(a, s, a.x, a.ldx, raw);
   const float gamma = a.gamma && tid < s.width ? a.gamma[c0 + tid] : 1.f, beta = a.beta && tid < s.width ? a.beta[c0 + tid] : 0.f;
   clear_off<E>(raw, s.on);
 
@@ -593,13 +596,16 @@ __global__ __launch_bounds__(NT) void norm_fused_kernel(NormArgs a) {
   for (int j = 0; j < V; j++) m[j] = m2[j] = 0.f;
 #pragma unroll
   for (int e = 0; e < E; e++) {
+    if (e >= s.each) break;
 #pragma unroll
     for (int j = 0; j < V; j++) m[j] += element<T>(raw[e], j);
   }
 #pragma unroll
   for (int j = 0; j < V; j++) m[j] *= inv;
+  forget<E>(raw);
 #pragma unroll
   for (int e = 0; e < E; e++) {
+    if (e >= s.each) break;
 #pragma unroll
     for (int j = 0; j < V; j++) {
       const float d = s.on >> e & 1 ? element<T>(raw[e], j) - m[j] : 0.f;
@@ -610,18 +616,18 @@ __global__ __launch_bounds__(NT) void norm_fused_kernel(NormArgs a) {
     if (s.col == 0) s_n[s.lane] = n;
 #pragma unroll
     for (int j = 0; j < V; j++) {
-      s_mean[j * NT + tid] = m[j];
-      s_m2[j * NT + tid] = m2[j];
+      s_mean[j * P + tid] = m[j];
+      s_m2[j * P + tid] = m2[j];
     }
   }
   __syncthreads();
   // Joined over the lanes: R rows of the slab's channels, then over a group's channels and those rows. Each join is
   // exact: the mean first, then M2 = sum M2_i + n_i (mean_i - mean)^2.
-  const int R = min(NT / s.width, s.lanes);
+  const int R = min(s.threads / s.width, s.lanes);
   if (tid < R * s.width) {
     const int c = tid % s.width, r = tid / s.width;
-    const float* qm = s_mean + (c % V) * NT + c / V;
-    const float* q2 = s_m2 + (c % V) * NT + c / V;
+    const float* qm = s_mean + (c % V) * P + c / V;
+    const float* q2 = s_m2 + (c % V) * P + c / V;
     float cn = 0.f, cs = 0.f, c2 = 0.f;
     for (int l = r; l < s.lanes; l += R) {
       cn += s_n[l];
@@ -638,7 +644,7 @@ __global__ __launch_bounds__(NT) void norm_fused_kernel(NormArgs a) {
   }
   __syncthreads();
   {
-    const int share = join_share<NT>(a.slab_groups), sub = tid % share, g = tid / share;
+    const int share = join_share(a.slab_groups, s.threads), sub = tid % share, g = tid / share;
     const bool mine = g < a.slab_groups;
     const int items = mine ? a.width * R : 0, first = mine ? g * a.width : 0;
     float cn = 0.f, cs = 0.f, c2 = 0.f;
@@ -680,6 +686,7 @@ __global__ __launch_bounds__(NT) void norm_fused_kernel(NormArgs a) {
   read_lds<V>(c_add + s.col * V, add);
 #pragma unroll
   for (int e = 0; e < E; e++) {
+    if (e >= s.each) break;
     float f[V];
 #pragma unroll
     for (int j = 0; j < V; j++) f[j] = act_f<ACT>(__builtin_fmaf(element<T>(raw[e], j) - mean[j], mul[j], add[j]));
@@ -689,7 +696,7 @@ __global__ __launch_bounds__(NT) void norm_fused_kernel(NormArgs a) {
       w[k] = sizeof(T) == 4 ? word_of<T>(f[k], 0.f) : word_of<T>(f[(2 * k) % V], f[(2 * k + 1) % V]);
       w[k] = s.on >> e & 1 ? w[k] : 0u;
     }
-    store_slab<T, NT, E>(a, s, a.y, a.ldy, e, w);
+    store_slab<T, E>(a, s, a.y, a.ldy, e, w);
   }
 }
 
@@ -700,17 +707,18 @@ template <typename T, int ACT, int NT, int E>
 __global__ __launch_bounds__(NT) void norm_back_fused_kernel(NormArgs a) {
   constexpr int V = kVec<T>, H = 4;
   constexpr bool kExactSide = BackColumn<T, ACT>::kExactSide;
-  __shared__ float s_b[V * NT], s_g[V * NT], s_n[NT];
+  constexpr int P = NT + 8;
+  __shared__ float s_b[V * P], s_g[V * P], s_n[NT];
   __shared__ float r_b[NT], r_g[NT], g_1[NT], g_2[NT];
   __shared__ __align__(16) float c_mean[NT], c_mul[NT], c_beta[NT], c_k1[NT], c_k2[NT];
   __shared__ double c_scale[kExactSide ? NT : 1];
   int b, c0;
   if (!slab_of(a, b, c0)) return;
-  Slab<T, NT, E> s(a, b, c0);
+  Slab<T, E> s(a, b, c0);
   const int tid = threadIdx.x;
   u32x4 rx[E], rd[E];
-  load_slab<T, NT, E>(a, s, a.x, a.ldx, rx);
-  load_slab<T, NT, E>(a, s, a.dy, a.lddy, rd);
+  load_slab<T, E>(a, s, a.x, a.ldx, rx);
+  load_slab<T, E>(a, s, a.dy, a.lddy, rd);
   float gamma = 1.f, rstd = 0.f;  // of channel c0 + tid
   if (tid < s.width) {
     const size_t g = (size_t)b * a.groups + (c0 + tid) / a.width;
@@ -722,9 +730,9 @@ __global__ __launch_bounds__(NT) void norm_back_fused_kernel(NormArgs a) {
     if constexpr (kExactSide) c_scale[tid] = (double)rstd * (double)gamma;
   }
   if (s.lane < s.lanes && s.col == 0) s_n[s.lane] = (float)__builtin_popcount(s.on);
+  lds_barrier();  // (the parameters; x and dy may still be on their way)
   clear_off<E>(rx, s.on);
   clear_off<E>(rd, s.on);
-  __syncthreads();
 #pragma unroll
   for (int h = 0; h < V; h += H) {
     BackColumn<T, ACT, H> col;
@@ -734,6 +742,7 @@ __global__ __launch_bounds__(NT) void norm_back_fused_kernel(NormArgs a) {
     for (int j = 0; j < H; j++) sb[j] = sg[j] = 0.f;
 #pragma unroll
     for (int e = 0; e < E; e++) {
+      if (e >= s.each) break;
 #pragma unroll
       for (int j = 0; j < H; j++) {
         float xc, da;
@@ -745,13 +754,13 @@ __global__ __launch_bounds__(NT) void norm_back_fused_kernel(NormArgs a) {
     }
     if (s.lane < s.lanes) {
 #pragma unroll
-      for (int j = 0; j < H; j++) { s_b[(h + j) * NT + tid] = sb[j]; s_g[(h + j) * NT + tid] = sg[j]; }
+      for (int j = 0; j < H; j++) { s_b[(h + j) * P + tid] = sb[j]; s_g[(h + j) * P + tid] = sg[j]; }
     }
   }
   __syncthreads();
-  const int R = min(NT / s.width, s.lanes);
+  const int R = min(s.threads / s.width, s.lanes);
   if (tid < R * s.width) {
-    const int c = tid % s.width, r = tid / s.width, from = (c % V) * NT + c / V;
+    const int c = tid % s.width, r = tid / s.width, from = (c % V) * P + c / V;
     float tb = 0.f, tg = 0.f;
     for (int l = r; l < s.lanes; l += R) {
       tb += s_b[from + l * s.cols];
@@ -776,7 +785,7 @@ __global__ __launch_bounds__(NT) void norm_back_fused_kernel(NormArgs a) {
   }
   __syncthreads();
   {
-    const int share = join_share<NT>(a.slab_groups), sub = tid % share, g = tid / share;
+    const int share = join_share(a.slab_groups, s.threads), sub = tid % share, g = tid / share;
     const bool mine = g < a.slab_groups;
     float t1 = 0.f, t2 = 0.f, cn = 0.f;
     for (int i = sub; i < (mine ? a.width : 0); i += share) {
@@ -813,6 +822,7 @@ __global__ __launch_bounds__(NT) void norm_back_fused_kernel(NormArgs a) {
     read_lds<H>(c_k2 + s.col * V + h, k2);
 #pragma unroll
     for (int e = 0; e < E; e++) {
+      if (e >= s.each) break;
       float dx[H];
 #pragma unroll
       for (int j = 0; j < H; j++) {
@@ -828,7 +838,7 @@ __global__ __launch_bounds__(NT) void norm_back_fused_kernel(NormArgs a) {
   }
   clear_off<E>(rd, s.on);
 #pragma unroll
-  for (int e = 0; e < E; e++) store_slab<T, NT, E>(a, s, a.dx, a.lddx, e, rd[e]);
+  for (int e = 0; e < E; e++) store_slab<T, E>(a, s, a.dx, a.lddx, e, rd[e]);
 }
 
 // dgamma and dbeta of 64 channels a workgroup from `parts` rows of channel sums, one wave a sixteenth of them.
@@ -855,29 +865,27 @@ __global__ __launch_bounds__(1024) void norm_back_params_kernel(NormArgs a, int 
   }
 }
 
-// The threads and points a thread of the fused launch for slabs of `width` channels, 0 where none fits: the
-// slab's channels meet in one row of threads, and a thread holds up to 8 points (128 KB of 16-bit values over 1024 threads).
+// The fused launch's slab (groups 0: none fits), the threads of a workgroup and the points that each takes: as few points as
+// 1024 threads allow (up to 8: 128 KB of 16-bit values), then no more threads than those take. (361 points of 6 columns: 3
+// points and 768 threads, where 1024 threads left a third of the work to empty points.)
 struct FusedShape {
   int groups = 0, threads = 0, each = 0;
 };
-inline int fused_each(int points, int cols, int threads) {
-  const int lanes = threads / cols;
-  return lanes ? (points + lanes - 1) / lanes : 1 << 30;
-}
 FusedShape fused_shape(const NormArgs& n, int size) {
-  const int points = n.points, groups = n.groups, width = n.width, vec = 16 / size;
+  const int vec = 16 / size;
   FusedShape best;
   // (A batch row has a point, whose address the threads past the end read, and its byte offsets have 31 bits.)
   const long long ld = std::max(std::max(n.ldx, n.ldy), std::max(n.lddy, n.lddx));
-  if (points < 1 || points * ld >= (1ll << 31) / size) return best;
-  for (int sg = 1; sg <= groups; sg++) {
-    if (groups % sg) continue;
-    const int w = sg * width, cols = (w + vec - 1) / vec;
+  if (n.points < 1 || n.points * ld >= (1ll << 31) / size) return best;
+  for (int sg = 1; sg <= n.groups; sg++) {
+    if (n.groups % sg) continue;
+    const int w = sg * n.width, cols = w / vec;
     if (w > 1024) break;
     if (w % vec) continue;
-    const int t = fused_each(points, cols, 256) <= 4 && w <= 256 ? 256 : 1024, e = fused_each(points, cols, t);
-    if (e > 8) break;
-    best = {sg, t, e <= 4 ? 4 : 8};
+    const int lanes = 1024 / cols, each = (n.points + lanes - 1) / lanes;
+    if (each > 8) break;
+    // (The slab's channels meet in one row of threads.)
+    best = {sg, std::max(round_up((n.points + each - 1) / each * cols, 64), round_up(w, 64)), each};
     if (w >= 4 * vec) break;
   }
   return best;
@@ -905,10 +913,11 @@ void norm_forward_act(NormArgs& n, hipStream_t s) {
   const FusedShape f = fused_shape(n, sizeof(T));
   if (f.groups) {
     n.slab_groups = f.groups;
+    n.each = f.each;
     const dim3 grid((n.batch * (n.groups / f.groups) + 7) / 8 * 8);
-    if (f.threads == 256) launch_k(norm_fused_kernel<T, ACT, 256, 4>, grid, 256, 0, s, n);
-    else if (f.each == 4) launch_k(norm_fused_kernel<T, ACT, 1024, 4>, grid, 1024, 0, s, n);
-    else launch_k(norm_fused_kernel<T, ACT, 1024, 8>, grid, 1024, 0, s, n);
+    if (f.threads <= 256 && f.each <= 4) launch_k(norm_fused_kernel<T, ACT, 256, 4>, grid, f.threads, 0, s, n);
+    else if (f.each <= 4) launch_k(norm_fused_kernel<T, ACT, 1024, 4>, grid, f.threads, 0, s, n);
+    else launch_k(norm_fused_kernel<T, ACT, 1024, 8>, grid, f.threads, 0, s, n);
     return;
   }
   const dim3 grid(n.batch * n.splits);
@@ -932,11 +941,12 @@ void norm_backward_act(NormArgs& n, hipStream_t s) {
   const dim3 columns((n.channels + 63) / 64);
   if (f.groups) {
     n.slab_groups = f.groups;
+    n.each = f.each;
     const dim3 grid((n.batch * (n.groups / f.groups) + 7) / 8 * 8);
     if (n.batch) {
-      if (f.threads == 256) launch_k(norm_back_fused_kernel<T, ACT, 256, 4>, grid, 256, 0, s, n);
-      else if (f.each == 4) launch_k(norm_back_fused_kernel<T, ACT, 1024, 4>, grid, 1024, 0, s, n);
-      else launch_k(norm_back_fused_kernel<T, ACT, 1024, 8>, grid, 1024, 0, s, n);
+      if (f.threads <= 256 && f.each <= 4) launch_k(norm_back_fused_kernel<T, ACT, 256, 4>, grid, f.threads, 0, s, n);
+      else if (f.each <= 4) launch_k(norm_back_fused_kernel<T, ACT, 1024, 4>, grid, f.threads, 0, s, n);
+      else launch_k(norm_back_fused_kernel<T, ACT, 1024, 8>, grid, f.threads, 0, s, n);
     }
     if (n.dgamma || n.dbeta) launch_k(norm_back_params_kernel, columns, 1024, 0, s, n, n.batch);
     return;

@@ -82,18 +82,33 @@ __device__ __forceinline__ unsigned long long load_legal(const unsigned char* ro
   return b;
 }
 
-// Reductions over the NT threads of a row: a wave, or the whole workgroup through `red` (16 floats a value).
+// A wave's sum or maximum, in every lane: within each row of 16 lanes by the lanes' crossbar of the vector unit, then the four
+// rows through scalar registers (six exchanges through LDS, before, were most of a narrow row's time).
+template <int CTRL>
+__device__ __forceinline__ float crossed(float v) {
+  return __uint_as_float((unsigned)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float lane_of(float v, int lane) {
+  return __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(v), lane));
+}
+template <bool MAX>
+__device__ __forceinline__ float wave_reduce(float v) {
+  auto join = [](float a, float b) { return MAX ? fmaxf(a, b) : a + b; };
+  v = join(v, crossed<0xB1>(v));   // lane ^ 1
+  v = join(v, crossed<0x4E>(v));   // lane ^ 2
+  v = join(v, crossed<0x141>(v));  // mirrored within 8
+  v = join(v, crossed<0x140>(v));  // mirrored within 16
+  return join(join(lane_of(v, 0), lane_of(v, 16)), join(lane_of(v, 32), lane_of(v, 48)));
+}
+
+// Reductions over the NT threads of a row: a wave, or the whole workgroup through `red` (16 floats).
 template <int NT, bool MAX>
 __device__ __forceinline__ float row_reduce(float v, float* red) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const float w = __shfl_xor(v, o);
-    v = MAX ? fmaxf(v, w) : v + w;
-  }
+  v = wave_reduce<MAX>(v);
   if constexpr (NT > 64) {
-    __syncthreads();  // (the last reduction's values have been read)
+    lds_barrier();  // (the last reduction's values have been read)
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
+    lds_barrier();
     v = red[0];
 #pragma unroll
     for (int k = 1; k < NT / 64; k++) v = MAX ? fmaxf(v, red[k]) : v + red[k];
@@ -174,6 +189,13 @@ struct Running {
   }
 };
 
+// Which of a workgroup's rows this thread's is, in a scalar register where a row is a wave.
+template <int NT>
+__device__ __forceinline__ int wave_row() {
+  static_assert(NT == 64 || NT >= 256, "a wave a row, or a workgroup");
+  return NT == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+}
+
 struct PolicyRows {
   const void* logits;
   const unsigned char* legal;
@@ -188,14 +210,79 @@ struct PolicyRows {
   float kl_coef;
 };
 
+// What a row's gradient takes from its sums: grad_j = e_j (f_p + f_kl (d_j - shift)) with e_j = e^((z_j - top) s) and d_j the
+// difference of z - top and the reference's, times s; plus hot at the action. part: the row takes part.
+struct PolicyFactors {
+  float hot, f_p, f_kl, shift;
+  int part;
+};
+
+// The row's results and factors from its sums, the action's logit (-infinity where it is illegal) and cross = sum e^(z -
+// top) ((z - top) - (r - its top)). Every lane of a wave computes them; `writes`: this one stores the results.
+template <bool FULL>
+__device__ __forceinline__ PolicyFactors policy_row(const PolicyRows& a, int row, bool padding, float za, float top, float sum,
+                                                    float ref_sum, float cross, bool writes) {
+  const double log_s = log_sum(sum);
+  const double lp = za == -INFINITY ? -(double)INFINITY : ((double)za - (double)top) * a.scale - log_s;
+  PolicyFactors f = {0.f, 0.f, 0.f, 0.f, !padding && !(lp == -(double)INFINITY)};
+  float loss = 0.f, logp = padding ? 0.f : -INFINITY, kl = 0.f;
+  if (f.part) {
+    const float w = a.weight ? a.weight[row] : 1.f, adv = a.advantage[row], inv = __builtin_amdgcn_rcpf(sum);
+    const double delta = lp - (double)a.old_logp[row];
+    const float ratio = exp_of((float)delta, Base2(1.0));
+    const bool held = adv > 0.f ? delta > a.log_high : adv < 0.f ? delta < a.log_low : false;
+    const float bounded = fminf(fmaxf(ratio, (float)(1.0 - a.low)), (float)(1.0 + a.high));
+    float c = held ? 0.f : -ratio * adv;
+    if constexpr (FULL) {
+      const double gap = log_s - log_sum(ref_sum);
+      const double k = (double)cross * a.scale * (double)inv - gap;
+      kl = (float)k;
+      f.shift = (float)(gap + k);
+    } else if (a.ref_logp) {
+      const float d = (float)((double)a.ref_logp[row] - lp), em = expm1f(d);
+      kl = em - d;
+      c -= a.kl_coef * em;
+    }
+    const float gw = w * (float)a.scale;
+    f.hot = gw * c;
+    f.f_p = -f.hot * inv;
+    f.f_kl = FULL ? a.kl_coef * gw * inv : 0.f;
+    loss = w * (a.kl_coef * kl - (held ? bounded : ratio) * adv);
+    logp = (float)lp;
+  }
+  if (writes) {
+    a.loss[row] = loss;
+    a.logp[row] = logp;
+    a.kl[row] = kl;
+  }
+  return f;
+}
+
+// The same for a row of NT threads: one wave computes, the others read its factors.
+template <int NT, bool FULL>
+__device__ __forceinline__ PolicyFactors policy_row_shared(const PolicyRows& a, int row, bool padding, float za, float top, float sum,
+                                                           float ref_sum, float cross, PolicyFactors* box) {
+  if constexpr (NT <= 64) {
+    return policy_row<FULL>(a, row, padding, za, top, sum, ref_sum, cross, (threadIdx.x & 63) == 0);
+  } else {
+    if (threadIdx.x < 64) {
+      const PolicyFactors f = policy_row<FULL>(a, row, padding, za, top, sum, ref_sum, cross, threadIdx.x == 0);
+      if (threadIdx.x == 0) *box = f;
+    }
+    lds_barrier();
+    return *box;  // (the next row's reductions lie between this and the next writing)
+  }
+}
+
 template <typename T, int NT, bool LEGAL, bool FULL>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void policy_loss_kernel(PolicyRows a) {
   constexpr int V = kVec<T>, PER = NT < 256 ? 256 / NT : 1;
   __shared__ float red[16];
+  __shared__ PolicyFactors box;
   const int tid = threadIdx.x % NT, columns = a.columns, chunks = (columns + V - 1) / V;
   const float s = (float)a.scale;
   const Base2 c2(a.scale);
-  for (int row = blockIdx.x * PER + threadIdx.x / NT; row < a.rows; row += gridDim.x * PER) {
+  for (int row = blockIdx.x * PER + wave_row<NT>(); row < a.rows; row += gridDim.x * PER) {
     const T* z = (const T*)a.logits + (size_t)row * a.ld;
     const T* r = FULL ? (const T*)a.ref + (size_t)row * a.ld_ref : nullptr;
     const unsigned char* lg = LEGAL ? a.legal + (size_t)row * a.ld_legal : nullptr;
@@ -243,47 +330,11 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void policy_loss_kernel(Policy
 
     float za = -INFINITY;
     if (!padding && (!LEGAL || lg[act])) za = (float)z[act];
-    const double log_s = log_sum(run.sum);
-    const double lp = za == -INFINITY ? -(double)INFINITY : ((double)za - (double)run.top) * a.scale - log_s;
-    const bool part = !padding && !(lp == -(double)INFINITY);
-    float hot = 0.f, f_p = 0.f, f_kl = 0.f, shift = 0.f;
-    if (part) {
-      const float w = a.weight ? a.weight[row] : 1.f, adv = a.advantage[row], inv = 1.f / run.sum;
-      const double delta = lp - (double)a.old_logp[row];
-      const float ratio = expf((float)delta);
-      const bool held = adv > 0.f ? delta > a.log_high : adv < 0.f ? delta < a.log_low : false;
-      const float bounded = fminf(fmaxf(ratio, (float)(1.0 - a.low)), (float)(1.0 + a.high));
-      const float obj = held ? bounded * adv : ratio * adv;
-      float c = held ? 0.f : -ratio * adv;
-      float kl = 0.f;
-      if constexpr (FULL) {
-        const double gap = log_s - log_sum(ref.sum);
-        const double k = (double)cross * a.scale * (double)inv - gap;
-        kl = (float)k;
-        shift = (float)(gap + k);
-      } else if (a.ref_logp) {
-        const float d = (float)((double)a.ref_logp[row] - lp), em = expm1f(d);
-        kl = em - d;
-        c -= a.kl_coef * em;
-      }
-      const float gw = w * s;
-      hot = gw * c;
-      f_p = -hot * inv;
-      f_kl = FULL ? a.kl_coef * gw * inv : 0.f;
-      if (tid == 0) {
-        a.loss[row] = w * (a.kl_coef * kl - obj);
-        a.logp[row] = (float)lp;
-        a.kl[row] = kl;
-      }
-    } else if (tid == 0) {
-      a.loss[row] = 0.f;
-      a.logp[row] = padding ? 0.f : -INFINITY;
-      a.kl[row] = 0.f;
-    }
+    const PolicyFactors f = policy_row_shared<NT, FULL>(a, row, padding, za, run.top, run.sum, ref.sum, cross, &box);
     if (!g) continue;
     for (int c = tid; c < chunks; c += NT) {
       float gf[V];
-      if (part) {
+      if (f.part) {
         float zf[V], rf[V];
         load_chunk<T>(z, c, columns, zf);
         if constexpr (FULL) load_chunk<T>(r, c, columns, rf);
@@ -292,15 +343,15 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void policy_loss_kernel(Policy
 #pragma unroll
         for (int j = 0; j < V; j++) {
           const float e = __builtin_amdgcn_exp2f((zf[j] - run.top) * c2.hi);
-          float f = f_p;
-          if constexpr (FULL) f += f_kl * (((zf[j] - run.top) - (rf[j] - ref.top)) * s - shift);
-          gf[j] = FULL && e == 0.f ? 0.f : e * f;
+          float k = f.f_p;
+          if constexpr (FULL) k += f.f_kl * (((zf[j] - run.top) - (rf[j] - ref.top)) * s - f.shift);
+          gf[j] = FULL && e == 0.f ? 0.f : e * k;
           if (LEGAL && !((ok >> (8 * j)) & 0xff)) gf[j] = 0.f;
         }
         if (c == act / V) {
 #pragma unroll
           for (int j = 0; j < V; j++)
-            if (j == act % V) gf[j] += hot;
+            if (j == act % V) gf[j] += f.hot;
         }
       } else {
 #pragma unroll
@@ -311,30 +362,284 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void policy_loss_kernel(Policy
   }
 }
 
+// ---- Rows that fit the registers of their threads: one read. ----
+
+// A thread's chunk c of a row as words. The row's last chunk, where it is not whole, is read from the row's last 16 bytes, and
+// chunks past the end too, so that no load is behind a branch; first(c) of its elements belong to the chunk before (all, past
+// the end).
+template <typename T>
+struct Chunks {
+  static constexpr int V = kVec<T>;
+  int columns;
+  __device__ __forceinline__ int start(int c) const { return min(c * V, columns - V); }
+  __device__ __forceinline__ int first(int c) const { return min(c * V - start(c), V); }
+};
+typedef unsigned int u32x4_any2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned int u32x4_any4 __attribute__((ext_vector_type(4), aligned(4)));
+template <typename T> struct AnyWords { typedef u32x4_any2 type; };
+template <> struct AnyWords<float> { typedef u32x4_any4 type; };
+
+template <typename T>
+__device__ __forceinline__ float element(const u32x4& w, int j) {
+  if constexpr (std::is_same<T, float>::value) {
+    return __uint_as_float(w[j]);
+  } else {
+    const unsigned x = w[j >> 1];
+    if constexpr (std::is_same<T, bf16>::value) return __uint_as_float(j & 1 ? x & 0xffff0000u : x << 16);
+    else return (float)__builtin_bit_cast(f16, (unsigned short)(j & 1 ? x >> 16 : x));
+  }
+}
+// -infinity in the place of element j.
+template <typename T>
+__device__ __forceinline__ void remove(u32x4& w, int j, bool gone) {
+  if constexpr (std::is_same<T, float>::value) {
+    w[j] = gone ? 0xff800000u : w[j];
+  } else {
+    constexpr unsigned inf = std::is_same<T, bf16>::value ? 0xff80u : 0xfc00u;
+    const unsigned x = w[j >> 1];
+    w[j >> 1] = gone ? (j & 1 ? (x & 0xffffu) | inf << 16 : (x & 0xffff0000u) | inf) : x;
+  }
+}
+template <typename T>
+__device__ __forceinline__ u32x4 words_of(const float (&f)[kVec<T>]) {
+  u32x4 w;
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    if constexpr (std::is_same<T, float>::value) w[k] = __float_as_uint(f[k]);
+    else w[k] = __builtin_bit_cast(unsigned short, to_t<T>(f[2 * k])) | (unsigned)__builtin_bit_cast(unsigned short, to_t<T>(f[2 * k + 1])) << 16;
+  }
+  return w;
+}
+// Makes the words new to the compiler: what was computed from them before is computed again rather than kept in registers.
+template <int E>
+__device__ __forceinline__ void forget(u32x4 (&raw)[E]) {
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      unsigned w = raw[e][k];
+      asm("" : "+v"(w));
+      raw[e][k] = w;
+    }
+  }
+}
+// A value that the compiler takes for new: what follows from it is computed here rather than kept over the loop of rows.
+__device__ __forceinline__ int fresh(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+template <typename T, int NT, int E>
+__device__ __forceinline__ void load_row(const T* row, int tid, const Chunks<T>& at, u32x4 (&raw)[E]) {
+  tid = fresh(tid);
+#pragma unroll
+  for (int e = 0; e < E; e++) raw[e] = *(const typename AnyWords<T>::type*)(row + at.start(tid + e * NT));
+}
+template <typename T, int NT, int E>
+__device__ __forceinline__ void remove_past(int tid, const Chunks<T>& at, u32x4 (&raw)[E]) {
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    if ((e + 1) * NT * kVec<T> <= at.columns) continue;  // (whole chunks in every thread)
+    const int first = at.first(fresh(tid) + e * NT);
+    if (first > 0) {
+#pragma unroll
+      for (int j = 0; j < kVec<T>; j++) remove<T>(raw[e], j, j < first);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // (here and below: a chunk at a time, so that registers hold little beside the row)
+  }
+}
+template <typename T, int NT, int E>
+__device__ __forceinline__ float max_of(const u32x4 (&raw)[E], float* red) {
+  float top = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+#pragma unroll
+    for (int j = 0; j < kVec<T>; j++) top = fmaxf(top, element<T>(raw[e], j));
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  return row_reduce<NT, true>(top, red);
+}
+template <typename T>
+__device__ __forceinline__ void store_gradient(T* row, int c, const Chunks<T>& at, const float (&f)[kVec<T>]) {
+  const int first = at.first(c);
+  if (first == 0) {
+    *(typename AnyWords<T>::type*)(row + at.start(c)) = words_of<T>(f);
+  } else if (first < kVec<T>) {
+    T* p = row + at.start(c);
+#pragma unroll
+    for (int j = 0; j < kVec<T>; j++)
+      if (j >= first) p[j] = to_t<T>(f[j]);
+  }
+}
+
+// Illegal columns and chunk elements past the row become -infinity in the words once, and from there on need no test: their
+// exponential is 0, and with it their gradient.
+template <typename T, int NT, int E, bool FULL, bool LEGAL>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void policy_row_kernel(PolicyRows a) {
+  constexpr int V = kVec<T>, PER = NT < 256 ? 256 / NT : 1;
+  __shared__ float red[16];
+  __shared__ PolicyFactors box;
+  const int tid = threadIdx.x % NT;
+  const float s = (float)a.scale;
+  const Base2 c2(a.scale);
+  const Chunks<T> at{a.columns};
+  for (int row = blockIdx.x * PER + wave_row<NT>(); row < a.rows; row += gridDim.x * PER) {
+    const T* z = (const T*)a.logits + (size_t)row * a.ld;
+    const unsigned char* lg = LEGAL && a.legal ? a.legal + (size_t)row * a.ld_legal : nullptr;
+    T* g = a.grad ? (T*)a.grad + (size_t)row * a.ld_grad : nullptr;
+    const int act = a.action[row];
+    const bool padding = (unsigned)act >= (unsigned)a.columns;
+    PolicyFactors f = {0.f, 0.f, 0.f, 0.f, 0};
+    float top = 0.f, ref_top = 0.f;
+    u32x4 raw[E], ref[FULL ? E : 1];
+    if (!padding) {
+      load_row<T, NT, E>(z, tid, at, raw);
+      if constexpr (FULL) load_row<T, NT, E>((const T*)a.ref + (size_t)row * a.ld_ref, tid, at, ref);
+      float za = (float)z[act];
+      if (lg) {
+        unsigned long long ok[E];
+        const int t = fresh(tid);
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+          const unsigned char* p = lg + at.start(t + e * NT);
+          if constexpr (V == 4) ok[e] = *(const u32_any*)p;
+          else ok[e] = *(const u64_any*)p;
+        }
+        if (!lg[act]) za = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+#pragma unroll
+          for (int j = 0; j < V; j++) {
+            const bool gone = ((ok[e] >> (8 * j)) & 0xff) == 0;
+            remove<T>(raw[e], j, gone);
+            if constexpr (FULL) remove<T>(ref[e], j, gone);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      remove_past<T, NT, E>(tid, at, raw);
+      if constexpr (FULL) remove_past<T, NT, E>(tid, at, ref);
+      top = max_of<T, NT, E>(raw, red);
+      if constexpr (FULL) ref_top = max_of<T, NT, E>(ref, red);
+      if (top == -INFINITY) top = 0.f;
+      if (FULL && ref_top == -INFINITY) ref_top = 0.f;
+      float sum = 0.f, ref_sum = 0.f, cross = 0.f;
+      forget<E>(raw);
+      if constexpr (FULL) forget<E>(ref);
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        float t = 0.f, tr = 0.f, tx = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          const float x = element<T>(raw[e], j) - top, ex = exp_of(x, c2);
+          t += ex;
+          if constexpr (FULL) {
+            const float rx = element<T>(ref[e], j) - ref_top;
+            tr += exp_of(rx, c2);
+            tx += ex == 0.f ? 0.f : ex * (x - rx);
+          }
+        }
+        sum += t;
+        ref_sum += tr;
+        cross += tx;
+        // (Here, and not behind the first sum's reduction.)
+        asm volatile("" : "+v"(sum), "+v"(ref_sum), "+v"(cross));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      sum = row_reduce<NT, false>(sum, red);
+      if constexpr (FULL) {
+        ref_sum = row_reduce<NT, false>(ref_sum, red);
+        cross = row_reduce<NT, false>(cross, red);
+      }
+      f = policy_row_shared<NT, FULL>(a, row, false, za, top, sum, ref_sum, cross, &box);
+      forget<E>(raw);
+      if constexpr (FULL) forget<E>(ref);
+    } else if (tid == 0) {
+      a.loss[row] = a.logp[row] = a.kl[row] = 0.f;
+    }
+    if (!g) continue;
+    if (!__builtin_amdgcn_readfirstlane(f.part)) {
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const float none[V] = {};
+        store_gradient<T>(g, fresh(tid) + e * NT, at, none);
+      }
+      continue;
+    }
+    const int hot_chunk = act / V;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const int c = fresh(tid) + e * NT;
+      float gf[V];
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        const float x = element<T>(raw[e], j) - top, ex = __builtin_amdgcn_exp2f(x * c2.hi);
+        float k = f.f_p;
+        if constexpr (FULL) k += f.f_kl * ((x - (element<T>(ref[e], j) - ref_top)) * s - f.shift);
+        gf[j] = FULL && ex == 0.f ? 0.f : ex * k;
+      }
+      if (c == hot_chunk) {
+        const int hot = act - at.start(c);
+#pragma unroll
+        for (int j = 0; j < V; j++) gf[j] += j == hot ? f.hot : 0.f;
+      }
+      if ((e + 1) * NT * V <= a.columns) *(typename AnyWords<T>::type*)(g + c * V) = words_of<T>(gf);
+      else store_gradient<T>(g, c, at, gf);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
 // Workgroups of a launch over rows, `per` at a time: the grid's threads stay below 2^32 and each workgroup strides on.
 inline int row_grid(int rows, int per) {
   const long long n = ((long long)rows + per - 1) / per;
   return (int)(n < (1 << 20) ? n : (1 << 20));
 }
 
-template <typename T, int NT>
-void policy_on(const PolicyRows& p, hipStream_t s) {
-  const int per = NT < 256 ? 256 / NT : 1, threads = NT < 256 ? 256 : NT;
-  const dim3 grid(row_grid(p.rows, per));
-  if (p.legal) {
-    if (p.ref) launch_k(policy_loss_kernel<T, NT, true, true>, grid, threads, 0, s, p);
-    else launch_k(policy_loss_kernel<T, NT, true, false>, grid, threads, 0, s, p);
-  } else {
-    if (p.ref) launch_k(policy_loss_kernel<T, NT, false, true>, grid, threads, 0, s, p);
-    else launch_k(policy_loss_kernel<T, NT, false, false>, grid, threads, 0, s, p);
-  }
+// The threads and chunks a thread of a row of `columns` elements of 16 / vec bytes that stays in registers; threads 0 where it
+// does not fit: a row shorter than a chunk, or of more than `most` chunks. A wave a row up to 512 chunks needs no barrier;
+// beyond, the fewest threads that hold it in 8 chunks each, and 16 at 1024 threads (131072 16-bit elements).
+struct RowShape {
+  int threads = 0, each = 0;
+};
+inline RowShape row_shape(int columns, int vec, int most) {
+  const int chunks = (int)(((long long)columns + vec - 1) / vec);
+  if (columns < vec || chunks > most) return {};
+  if (chunks <= 128) return {64, 2};
+  if (chunks <= 512) return {64, 8};
+  if (chunks <= 2048) return {256, 8};
+  if (chunks <= 4096) return {512, 8};
+  if (chunks <= 8192) return {1024, 8};
+  return {1024, 16};
+}
+
+template <typename T, bool FULL, bool LEGAL>
+void policy_rows(const PolicyRows& p, hipStream_t s) {
+  // (128 registers a thread at 1024 threads hold 8 chunks and their legality, or 16 without, but not a reference row's too.)
+  const RowShape r = row_shape(p.columns, kVec<T>, FULL ? 4096 : LEGAL ? 8192 : 16384);
+  const dim3 waves(row_grid(p.rows, 4)), groups(row_grid(p.rows, 1));
+  if (r.threads == 64 && r.each == 2) launch_k(policy_row_kernel<T, 64, 2, FULL, LEGAL>, waves, 256, 0, s, p);
+  else if (r.threads == 64) launch_k(policy_row_kernel<T, 64, 8, FULL, LEGAL>, waves, 256, 0, s, p);
+  else if (r.threads == 256) launch_k(policy_row_kernel<T, 256, 8, FULL, LEGAL>, groups, 256, 0, s, p);
+  else if (r.threads == 512) launch_k(policy_row_kernel<T, 512, 8, FULL, LEGAL>, groups, 512, 0, s, p);
+  else if (r.threads == 1024) {
+    if constexpr (!FULL) {
+      if (r.each == 8) launch_k(policy_row_kernel<T, 1024, 8, false, LEGAL>, groups, 1024, 0, s, p);
+      if constexpr (!LEGAL)
+        if (r.each == 16) launch_k(policy_row_kernel<T, 1024, 16, false, false>, groups, 1024, 0, s, p);
+    }
+  } else if (p.columns < kVec<T>) launch_k(policy_loss_kernel<T, 64, LEGAL, FULL>, waves, 256, 0, s, p);
+  else launch_k(policy_loss_kernel<T, 1024, LEGAL, FULL>, groups, 1024, 0, s, p);
 }
 
 template <typename T>
 void policy_typed(const PolicyRows& p, hipStream_t s) {
-  if (p.columns <= 2048) policy_on<T, 64>(p, s);
-  else if (p.columns <= 16384) policy_on<T, 256>(p, s);
-  else policy_on<T, 1024>(p, s);
+  if (p.ref) {
+    if (p.legal) policy_rows<T, true, true>(p, s);
+    else policy_rows<T, true, false>(p, s);
+  } else {
+    if (p.legal) policy_rows<T, false, true>(p, s);
+    else policy_rows<T, false, false>(p, s);
+  }
 }
 
 struct PrefRows {
@@ -359,7 +664,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void pref_rows_kernel(PrefRows
   const int tid = threadIdx.x % NT, columns = a.columns, chunks = (columns + V - 1) / V;
   const int first = a.offsets[0], last = a.offsets[2 * a.pairs];
   const Base2 c2(1.0);
-  for (int row = blockIdx.x * PER + threadIdx.x / NT; row < a.rows; row += gridDim.x * PER) {
+  for (int row = blockIdx.x * PER + wave_row<NT>(); row < a.rows; row += gridDim.x * PER) {
     const int label = a.label[row];
     if (tid == 0) a.coef[row] = 0.f;
     if (row < first || row >= last || (unsigned)label >= (unsigned)columns) continue;
@@ -377,6 +682,41 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void pref_rows_kernel(PrefRows
       a.row[row] = PrefRow{za == -INFINITY ? -(double)INFINITY : (double)za - (double)run.top - log_sum(run.sum), run.top,
                            1.f / run.sum};
     }
+  }
+}
+
+// The same where the row fits its threads' registers (E chunks each): all loads before any sum, two operations fewer an element.
+template <typename T, int NT, int E>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void pref_rows_held_kernel(PrefRows a) {
+  constexpr int V = kVec<T>, PER = NT < 256 ? 256 / NT : 1;
+  __shared__ float red[16];
+  const int tid = threadIdx.x % NT;
+  const int first = a.offsets[0], last = a.offsets[2 * a.pairs];
+  const Base2 c2(1.0);
+  const Chunks<T> at{a.columns};
+  for (int row = blockIdx.x * PER + wave_row<NT>(); row < a.rows; row += gridDim.x * PER) {
+    const int label = a.label[row];
+    if (tid == 0) a.coef[row] = 0.f;
+    if (row < first || row >= last || (unsigned)label >= (unsigned)a.columns) continue;
+    const T* z = (const T*)a.logits + (size_t)row * a.ld;
+    u32x4 raw[E];
+    load_row<T, NT, E>(z, tid, at, raw);
+    const float za = (float)z[label];
+    remove_past<T, NT, E>(tid, at, raw);
+    const float top = max_of<T, NT, E>(raw, red), base = top == -INFINITY ? 0.f : top;
+    forget<E>(raw);
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      float t = 0.f;
+#pragma unroll
+      for (int j = 0; j < V; j++) t += exp_of(element<T>(raw[e], j) - base, c2);
+      sum += t;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    sum = row_reduce<NT, false>(sum, red);
+    if (tid == 0)
+      a.row[row] = PrefRow{za == -INFINITY ? -(double)INFINITY : (double)za - (double)base - log_sum(sum), base, 1.f / sum};
   }
 }
 
@@ -438,7 +778,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void pref_grad_kernel(PrefRows
   constexpr int V = kVec<T>, PER = NT < 256 ? 256 / NT : 1;
   const int tid = threadIdx.x % NT, columns = a.columns, chunks = (columns + V - 1) / V;
   const int first = a.offsets[0], last = a.offsets[2 * a.pairs];
-  for (int row = blockIdx.x * PER + threadIdx.x / NT; row < a.rows; row += gridDim.x * PER) {
+  for (int row = blockIdx.x * PER + wave_row<NT>(); row < a.rows; row += gridDim.x * PER) {
     const int label = a.label[row];
     const bool counted = row >= first && row < last && (unsigned)label < (unsigned)columns;
     const T* z = (const T*)a.logits + (size_t)row * a.ld;
@@ -472,8 +812,18 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void pref_grad_kernel(PrefRows
 template <typename T, int NT>
 void pref_on(const PrefRows& p, hipStream_t s) {
   const int per = NT < 256 ? 256 / NT : 1, threads = NT < 256 ? 256 : NT;
-  const dim3 grid(row_grid(p.rows, per));
-  if (p.rows > 0) launch_k(pref_rows_kernel<T, NT>, grid, threads, 0, s, p);
+  const dim3 grid(row_grid(p.rows, per)), waves(row_grid(p.rows, 4)), groups(row_grid(p.rows, 1));
+  if (p.rows > 0) {
+    const RowShape r = row_shape(p.columns, kVec<T>, 16384);
+    if (r.threads == 64 && r.each == 2) launch_k(pref_rows_held_kernel<T, 64, 2>, waves, 256, 0, s, p);
+    else if (r.threads == 64) launch_k(pref_rows_held_kernel<T, 64, 8>, waves, 256, 0, s, p);
+    else if (r.threads == 256) launch_k(pref_rows_held_kernel<T, 256, 8>, groups, 256, 0, s, p);
+    else if (r.threads == 512) launch_k(pref_rows_held_kernel<T, 512, 8>, groups, 512, 0, s, p);
+    else if (r.threads == 1024 && r.each == 8) launch_k(pref_rows_held_kernel<T, 1024, 8>, groups, 1024, 0, s, p);
+    else if (r.threads == 1024) launch_k(pref_rows_held_kernel<T, 1024, 16>, groups, 1024, 0, s, p);
+    else if (p.columns < kVec<T>) launch_k(pref_rows_kernel<T, 64>, waves, 256, 0, s, p);
+    else launch_k(pref_rows_kernel<T, 1024>, groups, 1024, 0, s, p);
+  }
   if (p.pairs > 0) launch_k(pref_pairs_kernel, dim3(p.pairs < 65536 ? p.pairs : 65536), 256, 0, s, p);
   if (p.rows > 0 && p.grad) launch_k(pref_grad_kernel<T, NT>, grid, threads, 0, s, p);
 }

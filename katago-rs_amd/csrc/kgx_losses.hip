@@ -18,69 +18,14 @@ namespace {
 
 // 16 bytes of a row at its elements' alignment: rows of odd strides and columns of a larger row start anywhere. (Global
 // loads and stores of any width need no more than that on this hardware.)
-typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
-typedef unsigned short u16x8_any __attribute__((ext_vector_type(8), aligned(2)));
+typedef unsigned int u32x4_any2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned int u32x4_any4 __attribute__((ext_vector_type(4), aligned(4)));
+template <typename T> struct AnyWords { typedef u32x4_any2 type; };
+template <> struct AnyWords<float> { typedef u32x4_any4 type; };
 typedef unsigned int u32_any __attribute__((aligned(1)));
 typedef unsigned long long u64_any __attribute__((aligned(1)));
 
 template <typename T> constexpr int kVec = 16 / sizeof(T);
-
-template <typename T> struct RowVec { typedef u16x8_any type; };
-template <> struct RowVec<float> { typedef f32x4_any type; };
-
-template <typename T>
-__device__ __forceinline__ float widen(typename RowVec<T>::type v, int j) {
-  if constexpr (std::is_same<T, float>::value) return v[j];
-  else if constexpr (std::is_same<T, bf16>::value) return __uint_as_float((unsigned)v[j] << 16);
-  else return (float)__builtin_bit_cast(f16, (unsigned short)v[j]);
-}
-
-// Elements [c kVec, (c + 1) kVec) of a row as floats, -infinity past `columns`.
-template <typename T>
-__device__ __forceinline__ void load_chunk(const T* row, int c, int columns, float (&f)[kVec<T>]) {
-  const T* p = row + (size_t)c * kVec<T>;
-  const int left = columns - c * kVec<T>;
-  if (left >= kVec<T>) {
-    const typename RowVec<T>::type v = *(const typename RowVec<T>::type*)p;
-#pragma unroll
-    for (int j = 0; j < kVec<T>; j++) f[j] = widen<T>(v, j);
-  } else {
-#pragma unroll
-    for (int j = 0; j < kVec<T>; j++) f[j] = j < left ? (float)p[j] : -INFINITY;
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void store_chunk(T* row, int c, int columns, const float (&f)[kVec<T>]) {
-  T* p = row + (size_t)c * kVec<T>;
-  const int left = columns - c * kVec<T>;
-  T t[kVec<T>];
-#pragma unroll
-  for (int j = 0; j < kVec<T>; j++) t[j] = to_t<T>(f[j]);
-  if (left >= kVec<T>) {
-    *(typename RowVec<T>::type*)p = __builtin_bit_cast(typename RowVec<T>::type, t);
-  } else {
-#pragma unroll
-    for (int j = 0; j < kVec<T>; j++)
-      if (j < left) p[j] = t[j];
-  }
-}
-
-// The legality bytes of a chunk, 0 past `columns`.
-template <int V>
-__device__ __forceinline__ unsigned long long load_legal(const unsigned char* row, int c, int columns) {
-  const unsigned char* p = row + (size_t)c * V;
-  const int left = columns - c * V;
-  if (left >= V) {
-    if constexpr (V == 4) return *(const u32_any*)p;
-    else return *(const u64_any*)p;
-  }
-  unsigned long long b = 0;
-#pragma unroll
-  for (int j = 0; j < V; j++)
-    if (j < left) b |= (unsigned long long)p[j] << (8 * j);
-  return b;
-}
 
 // A wave's sum or maximum, in every lane: within each row of 16 lanes by the lanes' crossbar of the vector unit, then the four
 // rows through scalar registers (six exchanges through LDS, before, were most of a narrow row's time).
@@ -274,90 +219,34 @@ __device__ __forceinline__ PolicyFactors policy_row_shared(const PolicyRows& a, 
   }
 }
 
-template <typename T, int NT, bool LEGAL, bool FULL>
-__global__ __launch_bounds__(NT < 256 ? 256 : NT) void policy_loss_kernel(PolicyRows a) {
-  constexpr int V = kVec<T>, PER = NT < 256 ? 256 / NT : 1;
-  __shared__ float red[16];
-  __shared__ PolicyFactors box;
-  const int tid = threadIdx.x % NT, columns = a.columns, chunks = (columns + V - 1) / V;
-  const float s = (float)a.scale;
+// Rows shorter than 16 bytes: a wave a row, a lane a column.
+template <typename T, bool FULL, bool LEGAL>
+__global__ __launch_bounds__(256) void policy_short_kernel(PolicyRows a) {
+  const int lane = threadIdx.x & 63;
   const Base2 c2(a.scale);
-  for (int row = blockIdx.x * PER + wave_row<NT>(); row < a.rows; row += gridDim.x * PER) {
-    const T* z = (const T*)a.logits + (size_t)row * a.ld;
-    const T* r = FULL ? (const T*)a.ref + (size_t)row * a.ld_ref : nullptr;
-    const unsigned char* lg = LEGAL ? a.legal + (size_t)row * a.ld_legal : nullptr;
-    T* g = a.grad ? (T*)a.grad + (size_t)row * a.ld_grad : nullptr;
+  for (int row = blockIdx.x * 4 + wave_row<64>(); row < a.rows; row += gridDim.x * 4) {
     const int act = a.action[row];
-    const bool padding = (unsigned)act >= (unsigned)columns;
-
-    Running run, ref;
-    float cross = 0.f;  // sum e^(z - top) ((z - top) - (r - its top))
-    if (!padding) {
-      for (int c = tid; c < chunks; c += NT) {
-        float zf[V], e[V];
-        load_chunk<T>(z, c, columns, zf);
-        unsigned long long ok = ~0ull;
-        if constexpr (LEGAL) {
-          ok = load_legal<V>(lg, c, columns);
-#pragma unroll
-          for (int j = 0; j < V; j++)
-            if (!((ok >> (8 * j)) & 0xff)) zf[j] = -INFINITY;
-        }
-        const float before = run.sum;
-        float moved, r_moved;
-        const float keep = run.add<V>(zf, c2, e, moved);
-        if constexpr (FULL) {
-          float rf[V], er[V];
-          load_chunk<T>(r, c, columns, rf);
-#pragma unroll
-          for (int j = 0; j < V; j++)
-            if (LEGAL && !((ok >> (8 * j)) & 0xff)) rf[j] = -INFINITY;
-          ref.add<V>(rf, c2, er, r_moved);
-          float x = 0.f;
-#pragma unroll
-          for (int j = 0; j < V; j++) x += e[j] == 0.f ? 0.f : e[j] * (zf[j] - rf[j]);
-          cross = keep == 0.f ? x : __builtin_fmaf(__builtin_fmaf(before, moved - r_moved, cross), keep, x);
-        }
-      }
-      const float before = run.sum;
-      float moved, r_moved;
-      const float keep = run.join<NT>(c2, red, moved);
-      if constexpr (FULL) {
-        ref.join<NT>(c2, red, r_moved);
-        cross = row_reduce<NT, false>(keep == 0.f ? 0.f : __builtin_fmaf(before, moved - r_moved, cross) * keep, red);
-      }
+    const bool padding = (unsigned)act >= (unsigned)a.columns;
+    const bool in = !padding && lane < a.columns && (!LEGAL || a.legal[(size_t)row * a.ld_legal + lane]);
+    const float z = in ? (float)((const T*)a.logits)[(size_t)row * a.ld + lane] : -INFINITY;
+    float top = wave_reduce<true>(z), x = 0.f, ref_sum = 0.f, cross = 0.f;
+    if (top == -INFINITY) top = 0.f;
+    const float e = exp_of(z - top, c2);
+    if constexpr (FULL) {
+      const float r = in ? (float)((const T*)a.ref)[(size_t)row * a.ld_ref + lane] : -INFINITY;
+      float ref_top = wave_reduce<true>(r);
+      if (ref_top == -INFINITY) ref_top = 0.f;
+      ref_sum = wave_reduce<false>(exp_of(r - ref_top, c2));
+      x = (z - top) - (r - ref_top);
+      cross = wave_reduce<false>(e == 0.f ? 0.f : e * x);
     }
-
-    float za = -INFINITY;
-    if (!padding && (!LEGAL || lg[act])) za = (float)z[act];
-    const PolicyFactors f = policy_row_shared<NT, FULL>(a, row, padding, za, run.top, run.sum, ref.sum, cross, &box);
-    if (!g) continue;
-    for (int c = tid; c < chunks; c += NT) {
-      float gf[V];
-      if (f.part) {
-        float zf[V], rf[V];
-        load_chunk<T>(z, c, columns, zf);
-        if constexpr (FULL) load_chunk<T>(r, c, columns, rf);
-        unsigned long long ok = ~0ull;
-        if constexpr (LEGAL) ok = load_legal<V>(lg, c, columns);
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-          const float e = __builtin_amdgcn_exp2f((zf[j] - run.top) * c2.hi);
-          float k = f.f_p;
-          if constexpr (FULL) k += f.f_kl * (((zf[j] - run.top) - (rf[j] - ref.top)) * s - f.shift);
-          gf[j] = FULL && e == 0.f ? 0.f : e * k;
-          if (LEGAL && !((ok >> (8 * j)) & 0xff)) gf[j] = 0.f;
-        }
-        if (c == act / V) {
-#pragma unroll
-          for (int j = 0; j < V; j++)
-            if (j == act % V) gf[j] += f.hot;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; j++) gf[j] = 0.f;
-      }
-      store_chunk<T>(g, c, columns, gf);
+    const float sum = wave_reduce<false>(e), za = padding ? -INFINITY : lane_of(z, act);
+    const PolicyFactors f = policy_row<FULL>(a, row, padding, za, top, sum, ref_sum, cross, lane == 0);
+    if (a.grad && lane < a.columns) {
+      float g = 0.f;
+      if (f.part && !(FULL && e == 0.f)) g = e * (FULL ? f.f_p + f.f_kl * (x * (float)a.scale - f.shift) : f.f_p);
+      if (f.part && lane == act) g += f.hot;
+      ((T*)a.grad)[(size_t)row * a.ld_grad + lane] = to_t<T>(g);
     }
   }
 }
@@ -374,10 +263,6 @@ struct Chunks {
   __device__ __forceinline__ int start(int c) const { return min(c * V, columns - V); }
   __device__ __forceinline__ int first(int c) const { return min(c * V - start(c), V); }
 };
-typedef unsigned int u32x4_any2 __attribute__((ext_vector_type(4), aligned(2)));
-typedef unsigned int u32x4_any4 __attribute__((ext_vector_type(4), aligned(4)));
-template <typename T> struct AnyWords { typedef u32x4_any2 type; };
-template <> struct AnyWords<float> { typedef u32x4_any4 type; };
 
 template <typename T>
 __device__ __forceinline__ float element(const u32x4& w, int j) {
@@ -429,17 +314,21 @@ __device__ __forceinline__ int fresh(int v) {
   return v;
 }
 template <typename T, int NT, int E>
-__device__ __forceinline__ void load_row(const T* row, int tid, const Chunks<T>& at, u32x4 (&raw)[E]) {
-  tid = fresh(tid);
-#pragma unroll
-  for (int e = 0; e < E; e++) raw[e] = *(const typename AnyWords<T>::type*)(row + at.start(tid + e * NT));
-}
-template <typename T, int NT, int E>
-__device__ __forceinline__ void remove_past(int tid, const Chunks<T>& at, u32x4 (&raw)[E]) {
+__device__ __forceinline__ void load_row(const T* row, int tid, const Chunks<T>& at, u32x4 (&raw)[E], int c0 = 0) {
+  tid = fresh(tid + c0);
 #pragma unroll
   for (int e = 0; e < E; e++) {
-    if ((e + 1) * NT * kVec<T> <= at.columns) continue;  // (whole chunks in every thread)
-    const int first = at.first(fresh(tid) + e * NT);
+    if ((c0 + e * NT) * kVec<T> >= at.columns) break;  // (here and below: no thread has such a chunk)
+    raw[e] = *(const typename AnyWords<T>::type*)(row + at.start(tid + e * NT));
+  }
+}
+template <typename T, int NT, int E>
+__device__ __forceinline__ void remove_past(int tid, const Chunks<T>& at, u32x4 (&raw)[E], int c0 = 0) {
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    if ((c0 + e * NT) * kVec<T> >= at.columns) break;
+    if ((c0 + (e + 1) * NT) * kVec<T> <= at.columns) continue;  // (whole chunks in every thread)
+    const int first = at.first(fresh(tid) + c0 + e * NT);
     if (first > 0) {
 #pragma unroll
       for (int j = 0; j < kVec<T>; j++) remove<T>(raw[e], j, j < first);
@@ -447,11 +336,39 @@ __device__ __forceinline__ void remove_past(int tid, const Chunks<T>& at, u32x4 
     __builtin_amdgcn_sched_barrier(0);  // (here and below: a chunk at a time, so that registers hold little beside the row)
   }
 }
+// -infinity in the place of illegal elements, of the row and of the reference's (where FULL).
+template <typename T, int NT, int E, bool FULL>
+__device__ __forceinline__ void remove_illegal(const unsigned char* legal, int tid, const Chunks<T>& at, u32x4 (&raw)[E],
+                                               u32x4 (&ref)[FULL ? E : 1], int c0 = 0) {
+  constexpr int V = kVec<T>;
+  unsigned long long ok[E];
+  const int t = fresh(tid + c0);
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    ok[e] = ~0ull;
+    if ((c0 + e * NT) * V >= at.columns) continue;
+    const unsigned char* p = legal + at.start(t + e * NT);
+    if constexpr (V == 4) ok[e] = *(const u32_any*)p;
+    else ok[e] = *(const u64_any*)p;
+  }
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    if ((c0 + e * NT) * V >= at.columns) break;
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      const bool gone = ((ok[e] >> (8 * j)) & 0xff) == 0;
+      remove<T>(raw[e], j, gone);
+      if constexpr (FULL) remove<T>(ref[e], j, gone);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
 template <typename T, int NT, int E>
-__device__ __forceinline__ float max_of(const u32x4 (&raw)[E], float* red) {
+__device__ __forceinline__ float max_of(const u32x4 (&raw)[E], const Chunks<T>& at, float* red) {
   float top = -INFINITY;
 #pragma unroll
   for (int e = 0; e < E; e++) {
+    if (e * NT * kVec<T> >= at.columns) break;
 #pragma unroll
     for (int j = 0; j < kVec<T>; j++) top = fmaxf(top, element<T>(raw[e], j));
     __builtin_amdgcn_sched_barrier(0);
@@ -496,30 +413,13 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void policy_row_kernel(PolicyR
       if constexpr (FULL) load_row<T, NT, E>((const T*)a.ref + (size_t)row * a.ld_ref, tid, at, ref);
       float za = (float)z[act];
       if (lg) {
-        unsigned long long ok[E];
-        const int t = fresh(tid);
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-          const unsigned char* p = lg + at.start(t + e * NT);
-          if constexpr (V == 4) ok[e] = *(const u32_any*)p;
-          else ok[e] = *(const u64_any*)p;
-        }
         if (!lg[act]) za = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-#pragma unroll
-          for (int j = 0; j < V; j++) {
-            const bool gone = ((ok[e] >> (8 * j)) & 0xff) == 0;
-            remove<T>(raw[e], j, gone);
-            if constexpr (FULL) remove<T>(ref[e], j, gone);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
+        remove_illegal<T, NT, E, FULL>(lg, tid, at, raw, ref);
       }
       remove_past<T, NT, E>(tid, at, raw);
       if constexpr (FULL) remove_past<T, NT, E>(tid, at, ref);
-      top = max_of<T, NT, E>(raw, red);
-      if constexpr (FULL) ref_top = max_of<T, NT, E>(ref, red);
+      top = max_of<T, NT, E>(raw, at, red);
+      if constexpr (FULL) ref_top = max_of<T, NT, E>(ref, at, red);
       if (top == -INFINITY) top = 0.f;
       if (FULL && ref_top == -INFINITY) ref_top = 0.f;
       float sum = 0.f, ref_sum = 0.f, cross = 0.f;
@@ -527,6 +427,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void policy_row_kernel(PolicyR
       if constexpr (FULL) forget<E>(ref);
 #pragma unroll
       for (int e = 0; e < E; e++) {
+        if (e * NT * V >= a.columns) break;
         float t = 0.f, tr = 0.f, tx = 0.f;
 #pragma unroll
         for (int j = 0; j < V; j++) {
@@ -560,6 +461,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void policy_row_kernel(PolicyR
     if (!__builtin_amdgcn_readfirstlane(f.part)) {
 #pragma unroll
       for (int e = 0; e < E; e++) {
+        if (e * NT * V >= a.columns) break;
         const float none[V] = {};
         store_gradient<T>(g, fresh(tid) + e * NT, at, none);
       }
@@ -568,6 +470,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void policy_row_kernel(PolicyR
     const int hot_chunk = act / V;
 #pragma unroll
     for (int e = 0; e < E; e++) {
+      if (e * NT * V >= a.columns) break;
       const int c = fresh(tid) + e * NT;
       float gf[V];
 #pragma unroll
@@ -589,6 +492,104 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void policy_row_kernel(PolicyR
   }
 }
 
+// Longer rows: E chunks of each thread at a time relative to the running maxima, and again for the gradient, whose second
+// reading comes from the caches. (Held by 1024 threads in 16 chunks each, a row has a CU to itself, whose loads,
+// exponentials and stores wait for each other.)
+template <typename T, int NT, int E, bool FULL, bool LEGAL>
+__global__ __launch_bounds__(NT) void policy_long_kernel(PolicyRows a) {
+  constexpr int V = kVec<T>;
+  __shared__ float red[16];
+  __shared__ PolicyFactors box;
+  const int tid = threadIdx.x;
+  const float s = (float)a.scale;
+  const Base2 c2(a.scale);
+  const Chunks<T> at{a.columns};
+  for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* z = (const T*)a.logits + (size_t)row * a.ld;
+    const T* r = FULL ? (const T*)a.ref + (size_t)row * a.ld_ref : nullptr;
+    const unsigned char* lg = LEGAL ? a.legal + (size_t)row * a.ld_legal : nullptr;
+    T* g = a.grad ? (T*)a.grad + (size_t)row * a.ld_grad : nullptr;
+    const int act = a.action[row];
+    const bool padding = (unsigned)act >= (unsigned)a.columns;
+    Running run, ref;
+    float cross = 0.f;
+    // The words of E chunks of the row (and of the reference's) from chunk c0 on, with -infinity where nothing is.
+    auto piece = [&](int c0, u32x4(&raw)[E], u32x4(&raw_r)[FULL ? E : 1]) {
+      load_row<T, NT, E>(z, tid, at, raw, c0);
+      if constexpr (FULL) load_row<T, NT, E>(r, tid, at, raw_r, c0);
+      if constexpr (LEGAL) remove_illegal<T, NT, E, FULL>(lg, tid, at, raw, raw_r, c0);
+      remove_past<T, NT, E>(tid, at, raw, c0);
+      if constexpr (FULL) remove_past<T, NT, E>(tid, at, raw_r, c0);
+    };
+    if (!padding) {
+      for (int c0 = 0; c0 * V < a.columns; c0 += NT * E) {
+        u32x4 raw[E], raw_r[FULL ? E : 1];
+        piece(c0, raw, raw_r);
+        float f[E * V], e[E * V], moved;
+#pragma unroll
+        for (int k = 0; k < E; k++) {
+#pragma unroll
+          for (int j = 0; j < V; j++) f[k * V + j] = (c0 + k * NT) * V < a.columns ? element<T>(raw[k], j) : -INFINITY;
+        }
+        const float before = run.sum;
+        const float keep = run.add<E * V>(f, c2, e, moved);
+        if constexpr (FULL) {
+          float fr[E * V], er[E * V], r_moved;
+#pragma unroll
+          for (int k = 0; k < E; k++) {
+#pragma unroll
+            for (int j = 0; j < V; j++) fr[k * V + j] = (c0 + k * NT) * V < a.columns ? element<T>(raw_r[k], j) : -INFINITY;
+          }
+          ref.add<E * V>(fr, c2, er, r_moved);
+          float x = 0.f;
+#pragma unroll
+          for (int j = 0; j < E * V; j++) x += e[j] == 0.f ? 0.f : e[j] * (f[j] - fr[j]);
+          cross = keep == 0.f ? x : __builtin_fmaf(__builtin_fmaf(before, moved - r_moved, cross), keep, x);
+        }
+      }
+      const float before = run.sum;
+      float moved, r_moved;
+      const float keep = run.join<NT>(c2, red, moved);
+      if constexpr (FULL) {
+        ref.join<NT>(c2, red, r_moved);
+        cross = row_reduce<NT, false>(keep == 0.f ? 0.f : __builtin_fmaf(before, moved - r_moved, cross) * keep, red);
+      }
+    }
+    float za = -INFINITY;
+    if (!padding && (!LEGAL || lg[act])) za = (float)z[act];
+    const PolicyFactors f = policy_row_shared<NT, FULL>(a, row, padding, za, run.top, run.sum, ref.sum, cross, &box);
+    if (!g) continue;
+    const bool part = __builtin_amdgcn_readfirstlane(f.part);
+    const int hot_chunk = part ? act / V : -1;
+    for (int c0 = 0; c0 * V < a.columns; c0 += NT * E) {
+      u32x4 raw[E], raw_r[FULL ? E : 1];
+      if (part) piece(c0, raw, raw_r);
+#pragma unroll
+      for (int k = 0; k < E; k++) {
+        if ((c0 + k * NT) * V >= a.columns) break;
+        const int c = fresh(tid) + c0 + k * NT;
+        float gf[V] = {};
+        if (part) {
+#pragma unroll
+          for (int j = 0; j < V; j++) {
+            const float x = element<T>(raw[k], j) - run.top, ex = __builtin_amdgcn_exp2f(x * c2.hi);
+            float m = f.f_p;
+            if constexpr (FULL) m += f.f_kl * ((x - (element<T>(raw_r[k], j) - ref.top)) * s - f.shift);
+            gf[j] = FULL && ex == 0.f ? 0.f : ex * m;
+          }
+          if (c == hot_chunk) {
+            const int hot = act - at.start(c);
+#pragma unroll
+            for (int j = 0; j < V; j++) gf[j] += j == hot ? f.hot : 0.f;
+          }
+        }
+        if ((c0 + (k + 1) * NT) * V <= a.columns) *(typename AnyWords<T>::type*)(g + c * V) = words_of<T>(gf);
+        else store_gradient<T>(g, c, at, gf);
+      }
+    }
+  }
+}
+
 // Workgroups of a launch over rows, `per` at a time: the grid's threads stay below 2^32 and each workgroup strides on.
 inline int row_grid(int rows, int per) {
   const long long n = ((long long)rows + per - 1) / per;
@@ -596,39 +597,30 @@ inline int row_grid(int rows, int per) {
 }
 
 // The threads and chunks a thread of a row of `columns` elements of 16 / vec bytes that stays in registers; threads 0 where it
-// does not fit: a row shorter than a chunk, or of more than `most` chunks. A wave a row up to 512 chunks needs no barrier;
-// beyond, the fewest threads that hold it in 8 chunks each, and 16 at 1024 threads (131072 16-bit elements).
+// does not fit: a row shorter than a chunk, or longer than 4096 chunks. A wave a row up to 512 chunks needs no barrier;
+// beyond, the fewest threads that hold it in 8 chunks each.
 struct RowShape {
   int threads = 0, each = 0;
 };
-inline RowShape row_shape(int columns, int vec, int most) {
+inline RowShape row_shape(int columns, int vec) {
   const int chunks = (int)(((long long)columns + vec - 1) / vec);
-  if (columns < vec || chunks > most) return {};
+  if (columns < vec || chunks > 4096) return {};
   if (chunks <= 128) return {64, 2};
   if (chunks <= 512) return {64, 8};
   if (chunks <= 2048) return {256, 8};
-  if (chunks <= 4096) return {512, 8};
-  if (chunks <= 8192) return {1024, 8};
-  return {1024, 16};
+  return {512, 8};
 }
 
 template <typename T, bool FULL, bool LEGAL>
 void policy_rows(const PolicyRows& p, hipStream_t s) {
-  // (128 registers a thread at 1024 threads hold 8 chunks and their legality, or 16 without, but not a reference row's too.)
-  const RowShape r = row_shape(p.columns, kVec<T>, FULL ? 4096 : LEGAL ? 8192 : 16384);
+  const RowShape r = row_shape(p.columns, kVec<T>);
   const dim3 waves(row_grid(p.rows, 4)), groups(row_grid(p.rows, 1));
   if (r.threads == 64 && r.each == 2) launch_k(policy_row_kernel<T, 64, 2, FULL, LEGAL>, waves, 256, 0, s, p);
   else if (r.threads == 64) launch_k(policy_row_kernel<T, 64, 8, FULL, LEGAL>, waves, 256, 0, s, p);
   else if (r.threads == 256) launch_k(policy_row_kernel<T, 256, 8, FULL, LEGAL>, groups, 256, 0, s, p);
   else if (r.threads == 512) launch_k(policy_row_kernel<T, 512, 8, FULL, LEGAL>, groups, 512, 0, s, p);
-  else if (r.threads == 1024) {
-    if constexpr (!FULL) {
-      if (r.each == 8) launch_k(policy_row_kernel<T, 1024, 8, false, LEGAL>, groups, 1024, 0, s, p);
-      if constexpr (!LEGAL)
-        if (r.each == 16) launch_k(policy_row_kernel<T, 1024, 16, false, false>, groups, 1024, 0, s, p);
-    }
-  } else if (p.columns < kVec<T>) launch_k(policy_loss_kernel<T, 64, LEGAL, FULL>, waves, 256, 0, s, p);
-  else launch_k(policy_loss_kernel<T, 1024, LEGAL, FULL>, groups, 1024, 0, s, p);
+  else if (p.columns < kVec<T>) launch_k(policy_short_kernel<T, FULL, LEGAL>, waves, 256, 0, s, p);
+  else launch_k(policy_long_kernel<T, 512, FULL ? 2 : 4, FULL, LEGAL>, groups, 512, 0, s, p);
 }
 
 template <typename T>
@@ -656,32 +648,21 @@ struct PrefRows {
 };
 
 // Row t's softmax maximum, reciprocal sum and log-probability of its label, where it counts; its gradient's factor starts
-// at 0.
-template <typename T, int NT>
-__global__ __launch_bounds__(NT < 256 ? 256 : NT) void pref_rows_kernel(PrefRows a) {
-  constexpr int V = kVec<T>, PER = NT < 256 ? 256 / NT : 1;
-  __shared__ float red[16];
-  const int tid = threadIdx.x % NT, columns = a.columns, chunks = (columns + V - 1) / V;
-  const int first = a.offsets[0], last = a.offsets[2 * a.pairs];
+// at 0. Here for rows shorter than 16 bytes: a wave a row, a lane a column.
+template <typename T>
+__global__ __launch_bounds__(256) void pref_rows_short_kernel(PrefRows a) {
+  const int lane = threadIdx.x & 63, first = a.offsets[0], last = a.offsets[2 * a.pairs];
   const Base2 c2(1.0);
-  for (int row = blockIdx.x * PER + wave_row<NT>(); row < a.rows; row += gridDim.x * PER) {
+  for (int row = blockIdx.x * 4 + wave_row<64>(); row < a.rows; row += gridDim.x * 4) {
     const int label = a.label[row];
-    if (tid == 0) a.coef[row] = 0.f;
-    if (row < first || row >= last || (unsigned)label >= (unsigned)columns) continue;
-    const T* z = (const T*)a.logits + (size_t)row * a.ld;
-    Running run;
-    for (int c = tid; c < chunks; c += NT) {
-      float zf[V];
-      load_chunk<T>(z, c, columns, zf);
-      run.add<V>(zf, c2);
-    }
-    float moved;
-    run.join<NT>(c2, red, moved);
-    if (tid == 0) {
-      const float za = (float)z[label];
-      a.row[row] = PrefRow{za == -INFINITY ? -(double)INFINITY : (double)za - (double)run.top - log_sum(run.sum), run.top,
-                           1.f / run.sum};
-    }
+    if (lane == 0) a.coef[row] = 0.f;
+    if (row < first || row >= last || (unsigned)label >= (unsigned)a.columns) continue;
+    const float z = lane < a.columns ? (float)((const T*)a.logits)[(size_t)row * a.ld + lane] : -INFINITY;
+    float top = wave_reduce<true>(z);
+    if (top == -INFINITY) top = 0.f;
+    const float sum = wave_reduce<false>(exp_of(z - top, c2)), za = lane_of(z, label);
+    if (lane == 0)
+      a.row[row] = PrefRow{za == -INFINITY ? -(double)INFINITY : (double)za - (double)top - log_sum(sum), top, 1.f / sum};
   }
 }
 
@@ -703,11 +684,12 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void pref_rows_held_kernel(Pre
     load_row<T, NT, E>(z, tid, at, raw);
     const float za = (float)z[label];
     remove_past<T, NT, E>(tid, at, raw);
-    const float top = max_of<T, NT, E>(raw, red), base = top == -INFINITY ? 0.f : top;
+    const float top = max_of<T, NT, E>(raw, at, red), base = top == -INFINITY ? 0.f : top;
     forget<E>(raw);
     float sum = 0.f;
 #pragma unroll
     for (int e = 0; e < E; e++) {
+      if (e * NT * V >= a.columns) break;
       float t = 0.f;
 #pragma unroll
       for (int j = 0; j < V; j++) t += exp_of(element<T>(raw[e], j) - base, c2);
@@ -720,10 +702,52 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void pref_rows_held_kernel(Pre
   }
 }
 
+// The same for longer rows, E chunks of each thread at a time relative to the running maximum. (Held by 1024 threads in 16
+// chunks each, such a row has a CU to itself, whose loads and exponentials wait for each other: 297 us for 2430 rows of
+// 100003 f16, against TODO here.)
+template <typename T, int NT, int E>
+__global__ __launch_bounds__(NT) void pref_rows_long_kernel(PrefRows a) {
+  constexpr int V = kVec<T>;
+  __shared__ float red[16];
+  const int tid = threadIdx.x;
+  const int first = a.offsets[0], last = a.offsets[2 * a.pairs];
+  const Base2 c2(1.0);
+  const Chunks<T> at{a.columns};
+  for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const int label = a.label[row];
+    if (tid == 0) a.coef[row] = 0.f;
+    if (row < first || row >= last || (unsigned)label >= (unsigned)a.columns) continue;
+    const T* z = (const T*)a.logits + (size_t)row * a.ld;
+    Running run;
+    for (int c0 = 0; c0 * V < a.columns; c0 += NT * E) {
+      u32x4 raw[E];
+      load_row<T, NT, E>(z, tid, at, raw, c0);
+      remove_past<T, NT, E>(tid, at, raw, c0);
+      float f[E * V];
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const bool in = (c0 + e * NT) * V < a.columns;
+#pragma unroll
+        for (int j = 0; j < V; j++) f[e * V + j] = in ? element<T>(raw[e], j) : -INFINITY;
+      }
+      run.add<E * V>(f, c2);
+    }
+    float moved;
+    run.join<NT>(c2, red, moved);
+    if (tid == 0) {
+      const float za = (float)z[label];
+      a.row[row] = PrefRow{za == -INFINITY ? -(double)INFINITY : (double)za - (double)run.top - log_sum(run.sum), run.top,
+                           1.f / run.sum};
+    }
+  }
+}
+
+constexpr int PT = 512;  // threads of a pair's workgroup
+
 // One workgroup a pair: the sequences' sums in a fixed order, the loss, and the factor of each counted row's gradient.
-__global__ __launch_bounds__(256) void pref_pairs_kernel(PrefRows a) {
-  __shared__ double sums[4][2];
-  __shared__ int counts[4][2];
+__global__ __launch_bounds__(PT) void pref_pairs_kernel(PrefRows a) {
+  __shared__ double sums[PT / 64][2];
+  __shared__ int counts[PT / 64][2];
   const int tid = threadIdx.x, w = tid >> 6;
   for (int pair = blockIdx.x; pair < a.pairs; pair += gridDim.x) {
     int at[3];
@@ -732,11 +756,14 @@ __global__ __launch_bounds__(256) void pref_pairs_kernel(PrefRows a) {
     int count[2] = {0, 0};
 #pragma unroll
     for (int q = 0; q < 2; q++) {
-      for (int t = at[q] + tid; t < at[q + 1]; t += 256)
-        if ((unsigned)a.label[t] < (unsigned)a.columns) {
-          sum[q] += a.row[t].logp;
-          count[q]++;
-        }
+#pragma unroll 4
+      for (int t = at[q] + tid; t < at[q + 1]; t += PT) {
+        // (Every row's place is the workspace's own: read whether it counts or not, so that the loads run ahead.)
+        const bool counted = (unsigned)a.label[t] < (unsigned)a.columns;
+        const double lp = a.row[t].logp;
+        sum[q] += counted ? lp : 0.0;
+        count[q] += counted;
+      }
 #pragma unroll
       for (int o = 32; o >= 1; o >>= 1) {
         sum[q] += __shfl_xor(sum[q], o);
@@ -749,9 +776,14 @@ __global__ __launch_bounds__(256) void pref_pairs_kernel(PrefRows a) {
     __syncthreads();
     double part[2];
     for (int q = 0; q < 2; q++) {
-      const int n = counts[0][q] + counts[1][q] + counts[2][q] + counts[3][q];
+      int n = 0;
+      double total = 0.0;
+      for (int k = 0; k < PT / 64; k++) {
+        n += counts[k][q];
+        total += sums[k][q];
+      }
       part[q] = a.average ? 1.0 / max(n, 1) : 1.0;
-      sum[q] = (sums[0][q] + sums[1][q] + sums[2][q] + sums[3][q]) * part[q];
+      sum[q] = total * part[q];
     }
     const double h = a.beta * ((sum[0] - (double)a.ref_logp[2 * pair]) - (sum[1] - (double)a.ref_logp[2 * pair + 1]));
     const double wt = a.weight ? (double)a.weight[pair] : 1.0;
@@ -767,20 +799,22 @@ __global__ __launch_bounds__(256) void pref_pairs_kernel(PrefRows a) {
     if (a.grad) {
       const double dh = wt * a.beta * (a.smooth * up - (1 - a.smooth) * down);
       for (int q = 0; q < 2; q++)
-        for (int t = at[q] + tid; t < at[q + 1]; t += 256)
+        for (int t = at[q] + tid; t < at[q + 1]; t += PT)
           if ((unsigned)a.label[t] < (unsigned)a.columns) a.coef[t] = (float)((q ? -dh : dh) * part[q]);
     }
   }
 }
 
-template <typename T, int NT>
+// The gradient of every row, from the last to the first: what the sums read last is still in the caches.
+template <typename T, int NT, int E>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void pref_grad_kernel(PrefRows a) {
   constexpr int V = kVec<T>, PER = NT < 256 ? 256 / NT : 1;
-  const int tid = threadIdx.x % NT, columns = a.columns, chunks = (columns + V - 1) / V;
+  const int tid = threadIdx.x % NT;
   const int first = a.offsets[0], last = a.offsets[2 * a.pairs];
-  for (int row = blockIdx.x * PER + wave_row<NT>(); row < a.rows; row += gridDim.x * PER) {
-    const int label = a.label[row];
-    const bool counted = row >= first && row < last && (unsigned)label < (unsigned)columns;
+  const Chunks<T> at{a.columns};
+  for (int r = blockIdx.x * PER + wave_row<NT>(); r < a.rows; r += gridDim.x * PER) {
+    const int row = a.rows - 1 - r, label = a.label[row];
+    const bool counted = row >= first && row < last && (unsigned)label < (unsigned)a.columns;
     const T* z = (const T*)a.logits + (size_t)row * a.ld;
     T* g = (T*)a.grad + (size_t)row * a.ld_grad;
     float hot = 0.f, f = 0.f, top = 0.f;
@@ -789,50 +823,66 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void pref_grad_kernel(PrefRows
       top = a.row[row].top;
       f = -hot * a.row[row].inv_sum;
     }
-    for (int c = tid; c < chunks; c += NT) {
-      float zf[V];
-      if (counted) {
-        load_chunk<T>(z, c, columns, zf);
+    const int hot_chunk = counted ? label / V : -1;
+    for (int c0 = 0; c0 * V < a.columns; c0 += NT * E) {
+      u32x4 raw[E];
+      if (counted) load_row<T, NT, E>(z, tid, at, raw, c0);
 #pragma unroll
-        for (int j = 0; j < V; j++) zf[j] = __builtin_amdgcn_exp2f((zf[j] - top) * 1.44269504088896340736f) * f;
-        if (c == label / V) {
+      for (int e = 0; e < E; e++) {
+        if ((c0 + e * NT) * V >= a.columns) break;
+        const int c = fresh(tid) + c0 + e * NT;
+        float gf[V] = {};
+        if (counted) {
 #pragma unroll
-          for (int j = 0; j < V; j++)
-            if (j == label % V) zf[j] += hot;
+          for (int j = 0; j < V; j++) gf[j] = __builtin_amdgcn_exp2f((element<T>(raw[e], j) - top) * 1.44269504088896340736f) * f;
+          if (c == hot_chunk) {
+            const int at_j = label - at.start(c);
+#pragma unroll
+            for (int j = 0; j < V; j++) gf[j] += j == at_j ? hot : 0.f;
+          }
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; j++) zf[j] = 0.f;
+        if ((c0 + (e + 1) * NT) * V <= a.columns) *(typename AnyWords<T>::type*)(g + c * V) = words_of<T>(gf);
+        else store_gradient<T>(g, c, at, gf);
       }
-      store_chunk<T>(g, c, columns, zf);
     }
   }
 }
 
-template <typename T, int NT>
-void pref_on(const PrefRows& p, hipStream_t s) {
-  const int per = NT < 256 ? 256 / NT : 1, threads = NT < 256 ? 256 : NT;
-  const dim3 grid(row_grid(p.rows, per)), waves(row_grid(p.rows, 4)), groups(row_grid(p.rows, 1));
-  if (p.rows > 0) {
-    const RowShape r = row_shape(p.columns, kVec<T>, 16384);
-    if (r.threads == 64 && r.each == 2) launch_k(pref_rows_held_kernel<T, 64, 2>, waves, 256, 0, s, p);
-    else if (r.threads == 64) launch_k(pref_rows_held_kernel<T, 64, 8>, waves, 256, 0, s, p);
-    else if (r.threads == 256) launch_k(pref_rows_held_kernel<T, 256, 8>, groups, 256, 0, s, p);
-    else if (r.threads == 512) launch_k(pref_rows_held_kernel<T, 512, 8>, groups, 512, 0, s, p);
-    else if (r.threads == 1024 && r.each == 8) launch_k(pref_rows_held_kernel<T, 1024, 8>, groups, 1024, 0, s, p);
-    else if (r.threads == 1024) launch_k(pref_rows_held_kernel<T, 1024, 16>, groups, 1024, 0, s, p);
-    else if (p.columns < kVec<T>) launch_k(pref_rows_kernel<T, 64>, waves, 256, 0, s, p);
-    else launch_k(pref_rows_kernel<T, 1024>, groups, 1024, 0, s, p);
+// The same for rows shorter than a chunk.
+template <typename T>
+__global__ __launch_bounds__(256) void pref_grad_short_kernel(PrefRows a) {
+  const int first = a.offsets[0], last = a.offsets[2 * a.pairs];
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)a.rows * a.columns; i += (long long)gridDim.x * 256) {
+    const int row = (int)(i / a.columns), c = (int)(i % a.columns), label = a.label[row];
+    float g = 0.f;
+    if (row >= first && row < last && (unsigned)label < (unsigned)a.columns) {
+      const float e = __builtin_amdgcn_exp2f(((float)((const T*)a.logits)[(size_t)row * a.ld + c] - a.row[row].top) * 1.44269504088896340736f);
+      g = a.coef[row] * ((c == label ? 1.f : 0.f) - e * a.row[row].inv_sum);
+    }
+    ((T*)a.grad)[(size_t)row * a.ld_grad + c] = to_t<T>(g);
   }
-  if (p.pairs > 0) launch_k(pref_pairs_kernel, dim3(p.pairs < 65536 ? p.pairs : 65536), 256, 0, s, p);
-  if (p.rows > 0 && p.grad) launch_k(pref_grad_kernel<T, NT>, grid, threads, 0, s, p);
 }
 
 template <typename T>
 void pref_typed(const PrefRows& p, hipStream_t s) {
-  if (p.columns <= 2048) pref_on<T, 64>(p, s);
-  else if (p.columns <= 16384) pref_on<T, 256>(p, s);
-  else pref_on<T, 1024>(p, s);
+  const dim3 waves(row_grid(p.rows, 4)), groups(row_grid(p.rows, 1));
+  const bool tiny = p.columns < kVec<T>;  // rows shorter than a chunk
+  if (p.rows > 0) {
+    const RowShape r = row_shape(p.columns, kVec<T>);
+    if (r.threads == 64 && r.each == 2) launch_k(pref_rows_held_kernel<T, 64, 2>, waves, 256, 0, s, p);
+    else if (r.threads == 64) launch_k(pref_rows_held_kernel<T, 64, 8>, waves, 256, 0, s, p);
+    else if (r.threads == 256) launch_k(pref_rows_held_kernel<T, 256, 8>, groups, 256, 0, s, p);
+    else if (r.threads == 512) launch_k(pref_rows_held_kernel<T, 512, 8>, groups, 512, 0, s, p);
+    else if (tiny) launch_k(pref_rows_short_kernel<T>, waves, 256, 0, s, p);
+    else launch_k(pref_rows_long_kernel<T, 512, 4>, groups, 512, 0, s, p);
+  }
+  if (p.pairs > 0) launch_k(pref_pairs_kernel, dim3(p.pairs < 65536 ? p.pairs : 65536), PT, 0, s, p);
+  if (p.rows > 0 && p.grad) {
+    if (tiny) launch_k(pref_grad_short_kernel<T>, dim3(row_grid(p.rows, 32)), 256, 0, s, p);
+    else if (p.columns <= 512 * kVec<T>) launch_k(pref_grad_kernel<T, 64, 4>, waves, 256, 0, s, p);
+    else if (p.columns <= 2048 * kVec<T>) launch_k(pref_grad_kernel<T, 256, 4>, groups, 256, 0, s, p);
+    else launch_k(pref_grad_kernel<T, 512, 4>, groups, 512, 0, s, p);
+  }
 }
 
 }  // namespace

@@ -45,14 +45,17 @@ struct AdamArgs {
 };
 static_assert(sizeof(AdamArgs) <= 4096, "kernel arguments");
 
-// Four elements at index i of a tensor of any element type; elements from n on read as 0 and are not written.
+// Four elements at index i of a tensor of any element type. WHOLE: they are all there; else elements from n on read as 0 and
+// are not written. (Past the caches: every byte of a step is touched once, and with 29M float elements that took 157 us
+// where plain accesses took 180.)
+template <bool WHOLE>
 __device__ __forceinline__ floatx4 load4(const void* p, int type, long long i, long long n) {
   floatx4 f = {0.f, 0.f, 0.f, 0.f};
-  if (i + 4 <= n) {
+  if (WHOLE || i + 4 <= n) {
     if (type == PREC_F32) {
-      f = *(const f32x4_any*)((const float*)p + i);
+      f = __builtin_nontemporal_load((const f32x4_any*)((const float*)p + i));
     } else {
-      const u16x4_any h = *(const u16x4_any*)((const unsigned short*)p + i);
+      const u16x4_any h = __builtin_nontemporal_load((const u16x4_any*)((const unsigned short*)p + i));
 #pragma unroll
       for (int j = 0; j < 4; j++)
         f[j] = type == PREC_BF16 ? __uint_as_float((unsigned)h[j] << 16) : (float)__builtin_bit_cast(f16, (unsigned short)h[j]);
@@ -66,16 +69,17 @@ __device__ __forceinline__ floatx4 load4(const void* p, int type, long long i, l
   }
   return f;
 }
+template <bool WHOLE>
 __device__ __forceinline__ void store4_any(void* p, int type, long long i, long long n, floatx4 f) {
-  if (i + 4 <= n) {
+  if (WHOLE || i + 4 <= n) {
     if (type == PREC_F32) {
-      *(f32x4_any*)((float*)p + i) = f;
+      __builtin_nontemporal_store((f32x4_any)f, (f32x4_any*)((float*)p + i));
     } else {
       u16x4_any h;
 #pragma unroll
       for (int j = 0; j < 4; j++)
         h[j] = type == PREC_BF16 ? __builtin_bit_cast(unsigned short, (bf16)f[j]) : __builtin_bit_cast(unsigned short, (f16)f[j]);
-      *(u16x4_any*)((unsigned short*)p + i) = h;
+      __builtin_nontemporal_store(h, (u16x4_any*)((unsigned short*)p + i));
     }
   } else {
 #pragma unroll
@@ -110,83 +114,98 @@ __device__ __forceinline__ int exp_of(unsigned top, unsigned carry, int least) {
   return e < least ? least : e > 255 ? 255 : e;
 }
 
+// The correctly rounded root: the hardware's (an ulp), or the neighbour below or above it by the sign of what their product with
+// it leaves of v. 0, infinity and NaN keep the hardware's: every comparison fails. (Without the scaling of arguments below
+// 2^-96, whose roots are nothing beside any eps: seven of nineteen operations.)
+__device__ __forceinline__ float root_of(float v) {
+  const float s = __builtin_amdgcn_sqrtf(v);
+  const float below = __uint_as_float(__float_as_uint(s) - 1), above = __uint_as_float(__float_as_uint(s) + 1);
+  float r = __builtin_fmaf(-below, s, v) <= 0.f ? below : s;
+  return __builtin_fmaf(-above, s, v) > 0.f ? above : r;
+}
+
 constexpr int M_BIAS = 135, M_LEAST = 9, V_BIAS = 138, V_LEAST = 12;
 constexpr unsigned M_CARRY = 0x1FFFFF, V_CARRY = 0x03FFFF;  // largest codes 1.75 and 1.96875 times a power of two
 
-// |x| 2^(bias - exp) as e4m3 without its sign, rounded up where the cut part exceeds the random part u of its spacing.
-__device__ __forceinline__ unsigned encode_m(float y, float u) {
-  int e = (int)(__float_as_uint(y) >> 23) - 127;
-  e = e < -6 ? -6 : e;
-  const float t = y * exp_bits(127 + 3 - e);
-  return (unsigned)((e + 6) << 3) + (unsigned)(t + u);
-}
-// The same as e3m5; a positive value never becomes 0.
-__device__ __forceinline__ unsigned encode_v(float y, float u) {
-  int e = (int)(__float_as_uint(y) >> 23) - 127;
-  e = e < 5 ? 5 : e;
-  const float t = y * exp_bits(127 + 5 - e);
-  unsigned n = (unsigned)(t + u);
-  n = n == 0 && y > 0.f ? 1 : n;
-  return (unsigned)((e - 5) << 5) + n;
-}
-__device__ __forceinline__ float decode_v(unsigned c) {
-  const unsigned n = c < 64 ? c : ((c & 31) | 32) << ((c >> 5) - 1);
-  return (float)n;
+// A code is the quotient of its value y, in the block's units, by the spacing there, rounded up where the cut part exceeds
+// u / 2^16, u its random part. In the codes' normal range the quotient is the top of y's mantissa and the code the top of its
+// bits, less the bias: one addition rounds. Below it the spacing is that of the least codes.
+// e4m3 without its sign; normal from 2^-6 on.
+__device__ __forceinline__ unsigned encode_m_normal(float y, unsigned u) { return ((__float_as_uint(y) + (u << 4)) >> 20) - (120u << 3); }
+__device__ __forceinline__ unsigned encode_m_low(float y, unsigned u) { return (unsigned)(y * 512.f + (float)u * 0x1p-16f); }
+// e3m5; normal from 32 on. A positive value never becomes 0.
+__device__ __forceinline__ unsigned encode_v_normal(float y, unsigned u) { return ((__float_as_uint(y) + (u << 2)) >> 18) - (131u << 5); }
+__device__ __forceinline__ unsigned encode_v_low(float y, unsigned u) {
+  const unsigned n = (unsigned)(y + (float)u * 0x1p-16f);
+  return n == 0 && y > 0.f ? 1 : n;
 }
 
+// Four e3m5 codes of a word: code << 18 is a float's exponent and mantissa, 2^-131 of the code's value, its least codes as
+// subnormal floats; the unit, with 2^31 of that, follows 2^100.
+__device__ __forceinline__ float v_unit_of(int exp) {
+  return exp == 255 ? __uint_as_float(0x7fc00000u) : exp_bits(exp + 31 - V_BIAS + 127 < 254 ? exp + 31 - V_BIAS + 127 : 254);
+}
+__device__ __forceinline__ float decode_v(unsigned word, int j, float unit) {
+  const unsigned bits = (j == 0 ? word << 18 : j == 1 ? word << 10 : j == 2 ? word << 2 : word >> 6) & 0x03fc0000u;
+  return __uint_as_float(bits) * 0x1p100f * unit;
+}
+
+// A wave's maximum, in a scalar register: within each row of 16 lanes by the vector unit's crossbar, then the four rows.
+template <int CTRL>
+__device__ __forceinline__ unsigned crossed(unsigned v) {
+  return (unsigned)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
+}
 __device__ __forceinline__ unsigned wave_max(unsigned v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o));
-  return v;
+  v = max(v, crossed<0xB1>(v));   // lane ^ 1
+  v = max(v, crossed<0x4E>(v));   // lane ^ 2
+  v = max(v, crossed<0x141>(v));  // mirrored within 8
+  v = max(v, crossed<0x140>(v));  // mirrored within 16
+  unsigned m = (unsigned)__builtin_amdgcn_readlane((int)v, 0);
+  m = max(m, (unsigned)__builtin_amdgcn_readlane((int)v, 16));
+  m = max(m, (unsigned)__builtin_amdgcn_readlane((int)v, 32));
+  return max(m, (unsigned)__builtin_amdgcn_readlane((int)v, 48));
 }
 
-template <bool BYTES>
-__global__ __launch_bounds__(kWaves * 64) void adamw_kernel(AdamArgs a) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wg = blockIdx.x;
-  // The tensor of this workgroup: the last one that starts at or before it.
-  int ti = __popcll(__ballot(a.start[lane] <= wg));
-  ti += __popcll(__ballot(lane < kTensors - 64 && a.start[64 + (lane < kTensors - 64 ? lane : 0)] <= wg));
-  ti = __builtin_amdgcn_readfirstlane(ti) - 1;
-  const AdamTensor t = a.t[ti];
-  const kg_adamw_values_t h = a.device_values ? *a.device_values : a.values;
+// A workgroup's elements of tensor t from `base` on (this lane's first). WHOLE: the tensor holds the whole chunk.
+template <bool BYTES, bool WHOLE>
+__device__ __forceinline__ void adamw_chunk(const AdamArgs& a, const AdamTensor& t, const kg_adamw_values_t& h, long long base) {
+  const int lane = threadIdx.x & 63;
   const float decay = (float)(1.0 - (double)h.lr * (double)t.weight_decay);
-  const long long base = (long long)(wg - a.start[ti]) * kChunk + (wave * kUnroll) * kBlock + lane * 4;
   const void* weights = t.master ? (const void*)t.master : t.param;
   const int wtype = t.master ? PREC_F32 : t.param_type;
   const long long state0 = t.first_block * kBlock;
+  const unsigned high = BYTES ? mix32(h.seed) : 0;
 
   floatx4 p[kUnroll], g[kUnroll], m[kUnroll], v[kUnroll];
   unsigned mc[kUnroll], vc[kUnroll], me[kUnroll], ve[kUnroll];
 #pragma unroll
   for (int u = 0; u < kUnroll; u++) {
     const long long i = base + u * kBlock;
-    if (i - lane * 4 >= t.elements) break;  // (whole blocks: uniform over the wave)
-    p[u] = load4(weights, wtype, i, t.elements);
-    g[u] = load4(t.grad, t.grad_type, i, t.elements);
+    if (!WHOLE && i - lane * 4 >= t.elements) break;  // (whole blocks: uniform over the wave)
+    p[u] = load4<WHOLE>(weights, wtype, i, t.elements);
+    g[u] = load4<WHOLE>(t.grad, t.grad_type, i, t.elements);
     if constexpr (BYTES) {
       mc[u] = *(const u32_any*)((const unsigned char*)a.m + state0 + i);
       vc[u] = *(const u32_any*)((const unsigned char*)a.v + state0 + i);
       me[u] = a.m_exp[(state0 + i) / kBlock];
       ve[u] = a.v_exp[(state0 + i) / kBlock];
     } else {
-      m[u] = *(const f32x4_any*)((const float*)a.m + state0 + i);
-      v[u] = *(const f32x4_any*)((const float*)a.v + state0 + i);
+      m[u] = __builtin_nontemporal_load((const f32x4_any*)((const float*)a.m + state0 + i));
+      v[u] = __builtin_nontemporal_load((const f32x4_any*)((const float*)a.v + state0 + i));
     }
   }
-  unsigned high = 0;
-  if constexpr (BYTES) high = mix32(h.seed);
 #pragma unroll
   for (int u = 0; u < kUnroll; u++) {
     const long long i = base + u * kBlock;
-    if (i - lane * 4 >= t.elements) break;
+    if (!WHOLE && i - lane * 4 >= t.elements) break;
     if constexpr (BYTES) {
-      const float mu = unit_of(me[u], M_BIAS), vu = unit_of(ve[u], V_BIAS);
+      const float mu = unit_of(me[u], M_BIAS), vu = v_unit_of(ve[u]);
       m[u] = floatx4{__builtin_amdgcn_cvt_f32_fp8(mc[u], 0), __builtin_amdgcn_cvt_f32_fp8(mc[u], 1),
                      __builtin_amdgcn_cvt_f32_fp8(mc[u], 2), __builtin_amdgcn_cvt_f32_fp8(mc[u], 3)};
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         m[u][j] *= mu;
-        const float r = decode_v((vc[u] >> (8 * j)) & 0xff) * vu;
+        const float r = decode_v(vc[u], j, vu);
         v[u][j] = r * r;
       }
     }
@@ -194,31 +213,47 @@ __global__ __launch_bounds__(kWaves * 64) void adamw_kernel(AdamArgs a) {
     unsigned mtop = 0, vtop = 0;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const bool in = i + j < t.elements;
       const float gj = g[u][j] * h.grad_scale;
-      m[u][j] = in ? m[u][j] * h.beta1 + gj * h.beta1_rest : 0.f;
-      v[u][j] = in ? v[u][j] * h.beta2 + gj * gj * h.beta2_rest : 0.f;
-      root[j] = sqrtf(v[u][j]);
-      p[u][j] = p[u][j] * decay - h.step_size * m[u][j] / (root[j] * h.root_scale + h.eps);
+      m[u][j] = m[u][j] * h.beta1 + gj * h.beta1_rest;
+      v[u][j] = v[u][j] * h.beta2 + gj * gj * h.beta2_rest;
+      if (!WHOLE && i + j >= t.elements) m[u][j] = v[u][j] = 0.f;
+      root[j] = root_of(v[u][j]);
+      // (The quotient by the hardware's reciprocal: an ulp of the update, where the parameter keeps an ulp of itself.)
+      p[u][j] = p[u][j] * decay - h.step_size * m[u][j] * __builtin_amdgcn_rcpf(root[j] * h.root_scale + h.eps);
       mtop = max(mtop, __float_as_uint(m[u][j]) & 0x7fffffffu);
       vtop = max(vtop, __float_as_uint(root[j]) & 0x7fffffffu);
     }
-    if (t.master) store4_any(t.master, PREC_F32, i, t.elements, p[u]);
-    store4_any(t.param, t.param_type, i, t.elements, p[u]);
+    if (t.master) store4_any<WHOLE>(t.master, PREC_F32, i, t.elements, p[u]);
+    store4_any<WHOLE>(t.param, t.param_type, i, t.elements, p[u]);
     if constexpr (BYTES) {
       const int em = exp_of(wave_max(mtop), M_CARRY, M_LEAST), ev = exp_of(wave_max(vtop), V_CARRY, V_LEAST);
       const float ms = exp_bits(127 + M_BIAS - (em > 254 ? 254 : em)), vs = exp_bits(127 + V_BIAS - (ev > 254 ? 254 : ev));
       const unsigned long long at = (unsigned long long)(state0 + i);
       const unsigned place = mix32((unsigned)(at >> 32) + high);
+      unsigned r[4], cm[4], cv[4];
+      float ym[4], yv[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        r[j] = mix32((unsigned)at + j + place);
+        ym[j] = fabsf(m[u][j]) * ms;
+        yv[j] = root[j] * vs;
+        cm[j] = encode_m_normal(ym[j], r[j] & 0xffff);
+        cv[j] = encode_v_normal(yv[j], r[j] >> 16);
+      }
+      // (Few blocks hold a moment so small; a lane that has one takes this for all its four.)
+      if (!(fminf(fminf(ym[0], ym[1]), fminf(ym[2], ym[3])) >= 0x1p-6f)) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) cm[j] = ym[j] >= 0x1p-6f ? cm[j] : encode_m_low(ym[j], r[j] & 0xffff);
+      }
+      if (!(fminf(fminf(yv[0], yv[1]), fminf(yv[2], yv[3])) >= 32.f)) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) cv[j] = yv[j] >= 32.f ? cv[j] : encode_v_low(yv[j], r[j] >> 16);
+      }
       unsigned mw = 0, vw = 0;
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const unsigned r = mix32((unsigned)at + j + place);
-        const unsigned bits = __float_as_uint(m[u][j]);
-        const unsigned cm = encode_m(__uint_as_float(bits & 0x7fffffffu) * ms, (float)(r & 0xffff) * 0x1p-16f) | ((bits >> 24) & 0x80);
-        const unsigned cv = encode_v(root[j] * vs, (float)(r >> 16) * 0x1p-16f);
-        mw |= (cm & 0xff) << (8 * j);
-        vw |= (cv & 0xff) << (8 * j);
+        mw |= ((cm[j] & 0x7f) | ((__float_as_uint(m[u][j]) >> 24) & 0x80)) << (8 * j);
+        vw |= (cv[j] & 0xff) << (8 * j);
       }
       *(u32_any*)((unsigned char*)a.m + at) = mw;
       *(u32_any*)((unsigned char*)a.v + at) = vw;
@@ -227,10 +262,24 @@ __global__ __launch_bounds__(kWaves * 64) void adamw_kernel(AdamArgs a) {
         a.v_exp[at / kBlock] = (unsigned char)ev;
       }
     } else {
-      *(f32x4_any*)((float*)a.m + state0 + i) = m[u];
-      *(f32x4_any*)((float*)a.v + state0 + i) = v[u];
+      __builtin_nontemporal_store((f32x4_any)m[u], (f32x4_any*)((float*)a.m + state0 + i));
+      __builtin_nontemporal_store((f32x4_any)v[u], (f32x4_any*)((float*)a.v + state0 + i));
     }
   }
+}
+
+template <bool BYTES>
+__global__ __launch_bounds__(kWaves * 64) void adamw_kernel(AdamArgs a) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wg = blockIdx.x;
+  // The tensor of this workgroup: the last one that starts at or before it.
+  int ti = __popcll(__ballot(a.start[lane] <= wg));
+  ti += __popcll(__ballot(lane < kTensors - 64 && a.start[64 + (lane < kTensors - 64 ? lane : 0)] <= wg));
+  ti = __builtin_amdgcn_readfirstlane(ti) - 1;
+  const AdamTensor t = a.t[ti];
+  const kg_adamw_values_t h = a.device_values ? *a.device_values : a.values;
+  const long long first = (long long)(wg - a.start[ti]) * kChunk, base = first + (wave * kUnroll) * kBlock + lane * 4;
+  if (first + kChunk <= t.elements) adamw_chunk<BYTES, true>(a, t, h, base);
+  else adamw_chunk<BYTES, false>(a, t, h, base);
 }
 
 // A block a wave, four elements a lane.
@@ -244,19 +293,19 @@ __global__ __launch_bounds__(256) void adamw_moments_kernel(const void* m, const
     floatx4 fm, fr;
     if constexpr (BYTES) {
       const unsigned mc = *(const u32_any*)((const unsigned char*)m + i), vc = *(const u32_any*)((const unsigned char*)v + i);
-      const float mu = unit_of(m_exp[b], M_BIAS), vu = unit_of(v_exp[b], V_BIAS);
+      const float mu = unit_of(m_exp[b], M_BIAS), vu = v_unit_of(v_exp[b]);
       fm = floatx4{__builtin_amdgcn_cvt_f32_fp8(mc, 0), __builtin_amdgcn_cvt_f32_fp8(mc, 1),
                    __builtin_amdgcn_cvt_f32_fp8(mc, 2), __builtin_amdgcn_cvt_f32_fp8(mc, 3)} * mu;
 #pragma unroll
-      for (int j = 0; j < 4; j++) fr[j] = decode_v((vc >> (8 * j)) & 0xff) * vu;
+      for (int j = 0; j < 4; j++) fr[j] = decode_v(vc, j, vu);
     } else {
       fm = *(const f32x4_any*)((const float*)m + i);
       fr = *(const f32x4_any*)((const float*)v + i);
 #pragma unroll
       for (int j = 0; j < 4; j++) fr[j] = sqrtf(fr[j]);
     }
-    store4_any(out_m, type, i, blocks * kBlock, fm);
-    store4_any(out_root, type, i, blocks * kBlock, fr);
+    store4_any<true>(out_m, type, i, blocks * kBlock, fm);
+    store4_any<true>(out_root, type, i, blocks * kBlock, fr);
   }
 }
 

@@ -141,6 +141,11 @@ __device__ __forceinline__ int wave_row() {
   return NT == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
 }
 
+// Gradients of more bytes than this are stored past the caches, which then keep logits for the second reading and no lines
+// that a later launch has to write back: 4093 x 32768 bf16 106 -> 97 us, 8192 x 32768 preference rows 200 -> 174. Smaller ones
+// stay where the next operator finds them.
+constexpr long long kPastBytes = 64ll << 20;
+
 struct PolicyRows {
   const void* logits;
   const unsigned char* legal;
@@ -150,7 +155,7 @@ struct PolicyRows {
   const int* action;
   const float *old_logp, *advantage, *weight, *ref_logp;
   float *loss, *logp, *kl;
-  int rows, columns;
+  int rows, columns, past;
   double scale, low, high, log_low, log_high;  // clip_low, clip_high; log(1 - clip_low), log(1 + clip_high)
   float kl_coef;
 };
@@ -253,15 +258,25 @@ __global__ __launch_bounds__(256) void policy_short_kernel(PolicyRows a) {
 
 // ---- Rows that fit the registers of their threads: one read. ----
 
-// A thread's chunk c of a row as words. The row's last chunk, where it is not whole, is read from the row's last 16 bytes, and
-// chunks past the end too, so that no load is behind a branch; first(c) of its elements belong to the chunk before (all, past
-// the end).
+// A row's chunks of 16 bytes, laid so that `along`, the row that is written (or else read), has them at multiples of 16 bytes,
+// and in rows from 4 KB on the first at a multiple of 128, so that a wave's chunks are whole cache lines: chunk c is elements
+// [c V - back, (c + 1) V - back) of the row, back the elements from such a multiple to its start. (Rows of odd strides: stores
+// across 16 bytes cost a quarter of the time over 2700 x 100003 f16, and parts of lines a tenth when stored past the
+// caches.) A chunk that reaches over either end of the row, and one past the end, is read from the row's first or last 16
+// bytes instead, so that no load is behind a branch: of what is read there, elements [first, limit) are the chunk's.
 template <typename T>
 struct Chunks {
   static constexpr int V = kVec<T>;
-  int columns;
-  __device__ __forceinline__ int start(int c) const { return min(c * V, columns - V); }
-  __device__ __forceinline__ int first(int c) const { return min(c * V - start(c), V); }
+  int columns, back;
+  __device__ __forceinline__ Chunks(int columns_, const T* along)
+      : columns(columns_), back(__builtin_amdgcn_readfirstlane((int)((uintptr_t)along & (line(columns_) - 1)) / (int)sizeof(T))) {}
+  static __host__ __device__ __forceinline__ int line(int columns) { return columns < 4096 / (int)sizeof(T) ? 16 : 128; }
+  __device__ __forceinline__ int start(int c) const { return max(min(c * V - back, columns - V), 0); }
+  __device__ __forceinline__ int first(int c) const { return min(max(c * V - back - start(c), 0), V); }
+  __device__ __forceinline__ int limit(int c) const { return min((c + 1) * V - back - start(c), V); }
+  __device__ __forceinline__ int of(int column) const { return (column + back) / V; }
+  __device__ __forceinline__ bool none(int c) const { return c * V - back >= columns; }                  // c and all behind it
+  __device__ __forceinline__ bool whole(int c, int n) const { return c * V >= back && (c + n) * V - back <= columns; }  // n from c on
 };
 
 template <typename T>
@@ -318,7 +333,7 @@ __device__ __forceinline__ void load_row(const T* row, int tid, const Chunks<T>&
   tid = fresh(tid + c0);
 #pragma unroll
   for (int e = 0; e < E; e++) {
-    if ((c0 + e * NT) * kVec<T> >= at.columns) break;  // (here and below: no thread has such a chunk)
+    if (at.none(c0 + e * NT)) break;  // (here and below: no thread has such a chunk)
     raw[e] = *(const typename AnyWords<T>::type*)(row + at.start(tid + e * NT));
   }
 }
@@ -326,12 +341,12 @@ template <typename T, int NT, int E>
 __device__ __forceinline__ void remove_past(int tid, const Chunks<T>& at, u32x4 (&raw)[E], int c0 = 0) {
 #pragma unroll
   for (int e = 0; e < E; e++) {
-    if ((c0 + e * NT) * kVec<T> >= at.columns) break;
-    if ((c0 + (e + 1) * NT) * kVec<T> <= at.columns) continue;  // (whole chunks in every thread)
-    const int first = at.first(fresh(tid) + c0 + e * NT);
-    if (first > 0) {
+    if (at.none(c0 + e * NT)) break;
+    if (at.whole(c0 + e * NT, NT)) continue;
+    const int c = fresh(tid) + c0 + e * NT, first = at.first(c), limit = at.limit(c);
+    if (first > 0 || limit < kVec<T>) {
 #pragma unroll
-      for (int j = 0; j < kVec<T>; j++) remove<T>(raw[e], j, j < first);
+      for (int j = 0; j < kVec<T>; j++) remove<T>(raw[e], j, j < first || j >= limit);
     }
     __builtin_amdgcn_sched_barrier(0);  // (here and below: a chunk at a time, so that registers hold little beside the row)
   }
@@ -346,14 +361,14 @@ __device__ __forceinline__ void remove_illegal(const unsigned char* legal, int t
 #pragma unroll
   for (int e = 0; e < E; e++) {
     ok[e] = ~0ull;
-    if ((c0 + e * NT) * V >= at.columns) continue;
+    if (at.none(c0 + e * NT)) continue;
     const unsigned char* p = legal + at.start(t + e * NT);
     if constexpr (V == 4) ok[e] = *(const u32_any*)p;
     else ok[e] = *(const u64_any*)p;
   }
 #pragma unroll
   for (int e = 0; e < E; e++) {
-    if ((c0 + e * NT) * V >= at.columns) break;
+    if (at.none(c0 + e * NT)) break;
 #pragma unroll
     for (int j = 0; j < V; j++) {
       const bool gone = ((ok[e] >> (8 * j)) & 0xff) == 0;
@@ -368,23 +383,32 @@ __device__ __forceinline__ float max_of(const u32x4 (&raw)[E], const Chunks<T>& 
   float top = -INFINITY;
 #pragma unroll
   for (int e = 0; e < E; e++) {
-    if (e * NT * kVec<T> >= at.columns) break;
+    if (at.none(e * NT)) break;
 #pragma unroll
     for (int j = 0; j < kVec<T>; j++) top = fmaxf(top, element<T>(raw[e], j));
     __builtin_amdgcn_sched_barrier(0);
   }
   return row_reduce<NT, true>(top, red);
 }
+// past: past the caches (kPastBytes).
 template <typename T>
-__device__ __forceinline__ void store_gradient(T* row, int c, const Chunks<T>& at, const float (&f)[kVec<T>]) {
-  const int first = at.first(c);
-  if (first == 0) {
-    *(typename AnyWords<T>::type*)(row + at.start(c)) = words_of<T>(f);
-  } else if (first < kVec<T>) {
-    T* p = row + at.start(c);
+__device__ __forceinline__ void store_gradient(T* row, int c, bool whole, bool past, const Chunks<T>& at, const float (&f)[kVec<T>]) {
+  typedef typename AnyWords<T>::type words_t;
+  const int first = whole ? 0 : at.first(c), limit = whole ? kVec<T> : at.limit(c);
+  T* p = row + at.start(c);
+  if (whole || (first == 0 && limit == kVec<T>)) {
+    const words_t w = words_of<T>(f);
+    if (past) {
+      asm volatile("");  // (or the two stores become one, a plain one)
+      __builtin_nontemporal_store(w, (words_t*)p);
+      asm volatile("");
+    } else {
+      *(words_t*)p = w;
+    }
+  } else {
 #pragma unroll
     for (int j = 0; j < kVec<T>; j++)
-      if (j >= first) p[j] = to_t<T>(f[j]);
+      if (j >= first && j < limit) p[j] = to_t<T>(f[j]);
   }
 }
 
@@ -398,11 +422,11 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void policy_row_kernel(PolicyR
   const int tid = threadIdx.x % NT;
   const float s = (float)a.scale;
   const Base2 c2(a.scale);
-  const Chunks<T> at{a.columns};
   for (int row = blockIdx.x * PER + wave_row<NT>(); row < a.rows; row += gridDim.x * PER) {
     const T* z = (const T*)a.logits + (size_t)row * a.ld;
     const unsigned char* lg = LEGAL && a.legal ? a.legal + (size_t)row * a.ld_legal : nullptr;
     T* g = a.grad ? (T*)a.grad + (size_t)row * a.ld_grad : nullptr;
+    const Chunks<T> at(a.columns, g ? g : z);
     const int act = a.action[row];
     const bool padding = (unsigned)act >= (unsigned)a.columns;
     PolicyFactors f = {0.f, 0.f, 0.f, 0.f, 0};
@@ -427,7 +451,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void policy_row_kernel(PolicyR
       if constexpr (FULL) forget<E>(ref);
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        if (e * NT * V >= a.columns) break;
+        if (at.none(e * NT)) break;
         float t = 0.f, tr = 0.f, tx = 0.f;
 #pragma unroll
         for (int j = 0; j < V; j++) {
@@ -461,16 +485,16 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void policy_row_kernel(PolicyR
     if (!__builtin_amdgcn_readfirstlane(f.part)) {
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        if (e * NT * V >= a.columns) break;
+        if (at.none(e * NT)) break;
         const float none[V] = {};
-        store_gradient<T>(g, fresh(tid) + e * NT, at, none);
+        store_gradient<T>(g, fresh(tid) + e * NT, at.whole(e * NT, NT), a.past, at, none);
       }
       continue;
     }
-    const int hot_chunk = act / V;
+    const int hot_chunk = at.of(act);
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      if (e * NT * V >= a.columns) break;
+      if (at.none(e * NT)) break;
       const int c = fresh(tid) + e * NT;
       float gf[V];
 #pragma unroll
@@ -485,8 +509,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void policy_row_kernel(PolicyR
 #pragma unroll
         for (int j = 0; j < V; j++) gf[j] += j == hot ? f.hot : 0.f;
       }
-      if ((e + 1) * NT * V <= a.columns) *(typename AnyWords<T>::type*)(g + c * V) = words_of<T>(gf);
-      else store_gradient<T>(g, c, at, gf);
+      store_gradient<T>(g, c, at.whole(e * NT, NT), a.past, at, gf);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -503,12 +526,12 @@ __global__ __launch_bounds__(NT) void policy_long_kernel(PolicyRows a) {
   const int tid = threadIdx.x;
   const float s = (float)a.scale;
   const Base2 c2(a.scale);
-  const Chunks<T> at{a.columns};
   for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* z = (const T*)a.logits + (size_t)row * a.ld;
     const T* r = FULL ? (const T*)a.ref + (size_t)row * a.ld_ref : nullptr;
     const unsigned char* lg = LEGAL ? a.legal + (size_t)row * a.ld_legal : nullptr;
     T* g = a.grad ? (T*)a.grad + (size_t)row * a.ld_grad : nullptr;
+    const Chunks<T> at(a.columns, g ? g : z);
     const int act = a.action[row];
     const bool padding = (unsigned)act >= (unsigned)a.columns;
     Running run, ref;
@@ -522,14 +545,14 @@ __global__ __launch_bounds__(NT) void policy_long_kernel(PolicyRows a) {
       if constexpr (FULL) remove_past<T, NT, E>(tid, at, raw_r, c0);
     };
     if (!padding) {
-      for (int c0 = 0; c0 * V < a.columns; c0 += NT * E) {
+      for (int c0 = 0; !at.none(c0); c0 += NT * E) {
         u32x4 raw[E], raw_r[FULL ? E : 1];
         piece(c0, raw, raw_r);
         float f[E * V], e[E * V], moved;
 #pragma unroll
         for (int k = 0; k < E; k++) {
 #pragma unroll
-          for (int j = 0; j < V; j++) f[k * V + j] = (c0 + k * NT) * V < a.columns ? element<T>(raw[k], j) : -INFINITY;
+          for (int j = 0; j < V; j++) f[k * V + j] = !at.none(c0 + k * NT) ? element<T>(raw[k], j) : -INFINITY;
         }
         const float before = run.sum;
         const float keep = run.add<E * V>(f, c2, e, moved);
@@ -538,7 +561,7 @@ __global__ __launch_bounds__(NT) void policy_long_kernel(PolicyRows a) {
 #pragma unroll
           for (int k = 0; k < E; k++) {
 #pragma unroll
-            for (int j = 0; j < V; j++) fr[k * V + j] = (c0 + k * NT) * V < a.columns ? element<T>(raw_r[k], j) : -INFINITY;
+            for (int j = 0; j < V; j++) fr[k * V + j] = !at.none(c0 + k * NT) ? element<T>(raw_r[k], j) : -INFINITY;
           }
           ref.add<E * V>(fr, c2, er, r_moved);
           float x = 0.f;
@@ -560,13 +583,13 @@ __global__ __launch_bounds__(NT) void policy_long_kernel(PolicyRows a) {
     const PolicyFactors f = policy_row_shared<NT, FULL>(a, row, padding, za, run.top, run.sum, ref.sum, cross, &box);
     if (!g) continue;
     const bool part = __builtin_amdgcn_readfirstlane(f.part);
-    const int hot_chunk = part ? act / V : -1;
-    for (int c0 = 0; c0 * V < a.columns; c0 += NT * E) {
+    const int hot_chunk = part ? at.of(act) : -1;
+    for (int c0 = 0; !at.none(c0); c0 += NT * E) {
       u32x4 raw[E], raw_r[FULL ? E : 1];
       if (part) piece(c0, raw, raw_r);
 #pragma unroll
       for (int k = 0; k < E; k++) {
-        if ((c0 + k * NT) * V >= a.columns) break;
+        if (at.none(c0 + k * NT)) break;
         const int c = fresh(tid) + c0 + k * NT;
         float gf[V] = {};
         if (part) {
@@ -583,8 +606,7 @@ __global__ __launch_bounds__(NT) void policy_long_kernel(PolicyRows a) {
             for (int j = 0; j < V; j++) gf[j] += j == hot ? f.hot : 0.f;
           }
         }
-        if ((c0 + (k + 1) * NT) * V <= a.columns) *(typename AnyWords<T>::type*)(g + c * V) = words_of<T>(gf);
-        else store_gradient<T>(g, c, at, gf);
+        store_gradient<T>(g, c, at.whole(c0 + k * NT, NT), a.past, at, gf);
       }
     }
   }
@@ -599,11 +621,16 @@ inline int row_grid(int rows, int per) {
 // The threads and chunks a thread of a row of `columns` elements of 16 / vec bytes that stays in registers; threads 0 where it
 // does not fit: a row shorter than a chunk, or longer than 4096 chunks. A wave a row up to 512 chunks needs no barrier;
 // beyond, the fewest threads that hold it in 8 chunks each.
+// (Rows that do not start at a line's multiple may reach into as many chunks more as a line has.)
 struct RowShape {
   int threads = 0, each = 0;
 };
-inline RowShape row_shape(int columns, int vec) {
-  const int chunks = (int)(((long long)columns + vec - 1) / vec);
+template <typename T>
+RowShape row_shape(int columns, const void* p, long long ld, int rows) {
+  constexpr int vec = kVec<T>;
+  const int line = Chunks<T>::line(columns);
+  const bool aligned = (uintptr_t)p % line == 0 && (rows == 1 || ld * (long long)sizeof(T) % line == 0);
+  const int chunks = (int)(((long long)columns + vec - 1) / vec) + (aligned ? 0 : line / 16);
   if (columns < vec || chunks > 4096) return {};
   if (chunks <= 128) return {64, 2};
   if (chunks <= 512) return {64, 8};
@@ -613,13 +640,17 @@ inline RowShape row_shape(int columns, int vec) {
 
 template <typename T, bool FULL, bool LEGAL>
 void policy_rows(const PolicyRows& p, hipStream_t s) {
-  const RowShape r = row_shape(p.columns, kVec<T>);
+  const RowShape r = p.grad ? row_shape<T>(p.columns, p.grad, p.ld_grad, p.rows) : row_shape<T>(p.columns, p.logits, p.ld, p.rows);
   const dim3 waves(row_grid(p.rows, 4)), groups(row_grid(p.rows, 1));
   if (r.threads == 64 && r.each == 2) launch_k(policy_row_kernel<T, 64, 2, FULL, LEGAL>, waves, 256, 0, s, p);
   else if (r.threads == 64) launch_k(policy_row_kernel<T, 64, 8, FULL, LEGAL>, waves, 256, 0, s, p);
   else if (r.threads == 256) launch_k(policy_row_kernel<T, 256, 8, FULL, LEGAL>, groups, 256, 0, s, p);
   else if (r.threads == 512) launch_k(policy_row_kernel<T, 512, 8, FULL, LEGAL>, groups, 512, 0, s, p);
   else if (p.columns < kVec<T>) launch_k(policy_short_kernel<T, FULL, LEGAL>, waves, 256, 0, s, p);
+  // (Float rows over 160 KB on 1024 threads: with four workgroups of 512 a CU, more rows are under way than the caches hold
+  // for the second reading: 614 against 477 us with gradient at 2700 x 100000, 431 against 442 at 8192 x 32768. 16-bit rows, half
+  // as long, stay on 512: 274 against 292 us.)
+  else if (sizeof(T) == 4 && p.columns > 40960) launch_k(policy_long_kernel<T, 1024, 2, FULL, LEGAL>, groups, 1024, 0, s, p);
   else launch_k(policy_long_kernel<T, 512, FULL ? 2 : 4, FULL, LEGAL>, groups, 512, 0, s, p);
 }
 
@@ -643,7 +674,7 @@ struct PrefRows {
   PrefRow* row;
   float* coef;
   float *loss, *margin, *seq_logp;
-  int rows, columns, pairs, average;
+  int rows, columns, past, pairs, average;
   double beta, smooth;
 };
 
@@ -674,12 +705,12 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void pref_rows_held_kernel(Pre
   const int tid = threadIdx.x % NT;
   const int first = a.offsets[0], last = a.offsets[2 * a.pairs];
   const Base2 c2(1.0);
-  const Chunks<T> at{a.columns};
   for (int row = blockIdx.x * PER + wave_row<NT>(); row < a.rows; row += gridDim.x * PER) {
     const int label = a.label[row];
     if (tid == 0) a.coef[row] = 0.f;
     if (row < first || row >= last || (unsigned)label >= (unsigned)a.columns) continue;
     const T* z = (const T*)a.logits + (size_t)row * a.ld;
+    const Chunks<T> at(a.columns, z);
     u32x4 raw[E];
     load_row<T, NT, E>(z, tid, at, raw);
     const float za = (float)z[label];
@@ -689,7 +720,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void pref_rows_held_kernel(Pre
     float sum = 0.f;
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      if (e * NT * V >= a.columns) break;
+      if (at.none(e * NT)) break;
       float t = 0.f;
 #pragma unroll
       for (int j = 0; j < V; j++) t += exp_of(element<T>(raw[e], j) - base, c2);
@@ -712,21 +743,21 @@ __global__ __launch_bounds__(NT) void pref_rows_long_kernel(PrefRows a) {
   const int tid = threadIdx.x;
   const int first = a.offsets[0], last = a.offsets[2 * a.pairs];
   const Base2 c2(1.0);
-  const Chunks<T> at{a.columns};
   for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const int label = a.label[row];
     if (tid == 0) a.coef[row] = 0.f;
     if (row < first || row >= last || (unsigned)label >= (unsigned)a.columns) continue;
     const T* z = (const T*)a.logits + (size_t)row * a.ld;
+    const Chunks<T> at(a.columns, z);
     Running run;
-    for (int c0 = 0; c0 * V < a.columns; c0 += NT * E) {
+    for (int c0 = 0; !at.none(c0); c0 += NT * E) {
       u32x4 raw[E];
       load_row<T, NT, E>(z, tid, at, raw, c0);
       remove_past<T, NT, E>(tid, at, raw, c0);
       float f[E * V];
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        const bool in = (c0 + e * NT) * V < a.columns;
+        const bool in = !at.none(c0 + e * NT);
 #pragma unroll
         for (int j = 0; j < V; j++) f[e * V + j] = in ? element<T>(raw[e], j) : -INFINITY;
       }
@@ -805,31 +836,34 @@ __global__ __launch_bounds__(PT) void pref_pairs_kernel(PrefRows a) {
   }
 }
 
-// The gradient of every row, from the last to the first: what the sums read last is still in the caches.
+// The gradient of every row: first the sequences' rows, from the last to the first (what the sums read last is still in the
+// caches), then the others, whose zeros would drive it out.
 template <typename T, int NT, int E>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void pref_grad_kernel(PrefRows a) {
   constexpr int V = kVec<T>, PER = NT < 256 ? 256 / NT : 1;
   const int tid = threadIdx.x % NT;
-  const int first = a.offsets[0], last = a.offsets[2 * a.pairs];
-  const Chunks<T> at{a.columns};
+  // (Cut to the rows, so that each row comes once.)
+  const int last = min(max(a.offsets[2 * a.pairs], 0), a.rows), first = min(max(a.offsets[0], 0), last);
   for (int r = blockIdx.x * PER + wave_row<NT>(); r < a.rows; r += gridDim.x * PER) {
-    const int row = a.rows - 1 - r, label = a.label[row];
+    const int row = r < last - first ? last - 1 - r : r - (last - first) < first ? r - (last - first) : r;
+    const int label = a.label[row];
     const bool counted = row >= first && row < last && (unsigned)label < (unsigned)a.columns;
     const T* z = (const T*)a.logits + (size_t)row * a.ld;
     T* g = (T*)a.grad + (size_t)row * a.ld_grad;
+    const Chunks<T> at(a.columns, g);
     float hot = 0.f, f = 0.f, top = 0.f;
     if (counted) {
       hot = a.coef[row];
       top = a.row[row].top;
       f = -hot * a.row[row].inv_sum;
     }
-    const int hot_chunk = counted ? label / V : -1;
-    for (int c0 = 0; c0 * V < a.columns; c0 += NT * E) {
+    const int hot_chunk = counted ? at.of(label) : -1;
+    for (int c0 = 0; !at.none(c0); c0 += NT * E) {
       u32x4 raw[E];
       if (counted) load_row<T, NT, E>(z, tid, at, raw, c0);
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        if ((c0 + e * NT) * V >= a.columns) break;
+        if (at.none(c0 + e * NT)) break;
         const int c = fresh(tid) + c0 + e * NT;
         float gf[V] = {};
         if (counted) {
@@ -841,8 +875,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void pref_grad_kernel(PrefRows
             for (int j = 0; j < V; j++) gf[j] += j == at_j ? hot : 0.f;
           }
         }
-        if ((c0 + (e + 1) * NT) * V <= a.columns) *(typename AnyWords<T>::type*)(g + c * V) = words_of<T>(gf);
-        else store_gradient<T>(g, c, at, gf);
+        store_gradient<T>(g, c, at.whole(c0 + e * NT, NT), a.past, at, gf);
       }
     }
   }
@@ -868,7 +901,7 @@ void pref_typed(const PrefRows& p, hipStream_t s) {
   const dim3 waves(row_grid(p.rows, 4)), groups(row_grid(p.rows, 1));
   const bool tiny = p.columns < kVec<T>;  // rows shorter than a chunk
   if (p.rows > 0) {
-    const RowShape r = row_shape(p.columns, kVec<T>);
+    const RowShape r = row_shape<T>(p.columns, p.logits, p.ld, p.rows);
     if (r.threads == 64 && r.each == 2) launch_k(pref_rows_held_kernel<T, 64, 2>, waves, 256, 0, s, p);
     else if (r.threads == 64) launch_k(pref_rows_held_kernel<T, 64, 8>, waves, 256, 0, s, p);
     else if (r.threads == 256) launch_k(pref_rows_held_kernel<T, 256, 8>, groups, 256, 0, s, p);
@@ -885,6 +918,8 @@ void pref_typed(const PrefRows& p, hipStream_t s) {
   }
 }
 
+bool gradient_past(int rows, int columns, int type) { return (long long)rows * columns * (type == PREC_F32 ? 4 : 2) > kPastBytes; }
+
 }  // namespace
 
 void launch_policy_loss(const kg_policy_loss_args& a, hipStream_t s) {
@@ -896,6 +931,7 @@ void launch_policy_loss(const kg_policy_loss_args& a, hipStream_t s) {
   p.action = a.action; p.old_logp = a.old_logp; p.advantage = a.advantage; p.weight = a.weight; p.ref_logp = a.ref_logp;
   p.loss = a.loss; p.logp = a.logp; p.kl = a.kl;
   p.rows = a.rows; p.columns = a.columns;
+  p.past = gradient_past(a.rows, a.columns, a.type);
   p.scale = a.logit_scale;
   p.low = a.clip_low; p.high = a.clip_high;
   p.log_low = log1p(-a.clip_low); p.log_high = log1p(a.clip_high);
@@ -917,6 +953,7 @@ void launch_preference_loss(const kg_preference_loss_args& a, hipStream_t s) {
   p.coef = (float*)(p.row + a.rows);
   p.loss = a.loss; p.margin = a.margin; p.seq_logp = a.seq_logp;
   p.rows = a.rows; p.columns = a.columns; p.pairs = a.pairs; p.average = a.average;
+  p.past = gradient_past(a.rows, a.columns, a.type);
   p.beta = a.beta; p.smooth = a.label_smoothing;
   switch (a.type) {
     case PREC_F32: pref_typed<float>(p, s); break;

@@ -4,11 +4,13 @@
 // Bound by memory: x read and y written once, or dy and x read and dx written once.
 // - Where a slab of whole groups over all points of a batch row fits the registers of one workgroup (up to 128 KB: the
 //   boards of every network here, images of 64 x 64), it is read once, the statistics meet in LDS, and the result is
-//   written from the registers. Slabs are as narrow as keeps whole 16-byte columns, 64 bytes where that fits, so that few
-//   rows fill the chip; neighbouring slabs, which share cache lines, run on one XCD.
-// - Larger rows are cut along the points: a reduction launch and an elementwise one, whose second reading of the rows comes
-//   from the caches where they fit. Every access runs along whole rows however wide or odd the groups are.
-// A thread keeps its column of 16 bytes for all its points, with the channels' parameters in registers.
+//   written from the registers. Slabs are narrow, so that few rows fill the chip; neighbouring slabs, which share cache lines,
+//   run on one XCD.
+// - Longer rows are cut into shares of the points: the same slabs, once for their part of the statistics and once for the
+//   result, whose second reading comes from the caches where they fit.
+// - Channels fewer than a 16-byte column's, and groups wider than a workgroup joins, go by rows: simple kernels that take any
+//   width.
+// A thread keeps its column of 16 bytes for all its points.
 #include <algorithm>
 
 #include "kgx_device.h"
@@ -21,6 +23,7 @@ namespace {
 constexpr int GT = 256;         // threads of a workgroup
 constexpr int kSplitTarget = 16384;  // elements a workgroup, about
 constexpr int kMaxGroups = 2048;     // group statistics in LDS
+constexpr int kCUs = 256;
 
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned short u16x8_any __attribute__((ext_vector_type(8), aligned(2)));
@@ -69,7 +72,7 @@ struct NormArgs {
   float* counts;   // backward: [batch][splits] points
   float* sums;     // backward: [batch][2][groups]
   int batch, points, channels, groups, width, splits;  // width: channels of a group
-  int slab_groups, each;  // fused launches: groups of a slab, points a thread takes
+  int slab_groups, each;  // slabs: their groups, the points a thread takes
   float eps;
 };
 
@@ -285,8 +288,7 @@ struct BackColumn {
       if constexpr (kExactSide) scale[j] = (double)rstd * (double)gamma;
     }
   }
-  // The same from a fused workgroup's copy in LDS, channels c .. c + V - 1 of its slab.
-  template <int NT>
+  // The same from a slab's copy in LDS, in column order.
   __device__ __forceinline__ void read(const float* c_mean, const float* c_mul, const float* c_beta, const double* c_scale, int c) {
 #pragma unroll
     for (int j = 0; j < V; j += 4) {
@@ -451,48 +453,57 @@ __global__ __launch_bounds__(GT) void norm_back_apply_kernel(NormArgs a) {
   }
 }
 
-// The slab of a fused launch's workgroup: neighbouring slabs (which share cache lines) are on one XCD, workgroup g running
-// on XCD g mod 8. False past the last.
-__device__ __forceinline__ bool slab_of(const NormArgs& a, int& b, int& c0) {
-  const int slabs = a.groups / a.slab_groups, n = a.batch * slabs, per = (n + 7) / 8;
-  const int id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-  if (id >= n) return false;
-  // (Scalar registers: every address is one of them plus a 32-bit offset.)
-  b = __builtin_amdgcn_readfirstlane(id / slabs);
-  c0 = __builtin_amdgcn_readfirstlane((id % slabs) * a.slab_groups * a.width);
-  return true;
-}
+// ---- Slabs: whole groups over the points of a batch row, or over one of its shares, in a workgroup's registers. ----
 
-// A fused workgroup's points: thread (col, lane) takes points lane + e lanes, e < each (at most E), of 16-byte column col.
-// Threads and points past the end read the last one's address, so that no load is behind a branch of its own.
+// A workgroup's slab: thread (col, lane) takes points p0 + lane + e lanes, e < each (at most E), of the slab's 16-byte column
+// col. A last column that is not whole starts earlier: its first `skip` channels are the column's before, and both threads
+// compute the same for them. Threads and points past the end read the last one's address, so that no load is behind a
+// branch of its own.
 template <typename T, int E>
 struct Slab {
   static constexpr int V = kVec<T>;
-  int b, c0, each, threads, width, cols, lanes, col, lane, last;  // width: the slab's channels, whole columns
+  int b, k, c0, p0, each, threads, width, cols, lanes, col, lane, start, skip, last;  // width: the slab's channels
   unsigned in, on;  // bit e: the point exists; and is not masked
-  __device__ __forceinline__ Slab(const NormArgs& a, int b_, int c0_) : b(b_), c0(c0_), each(a.each), threads(blockDim.x) {
+  // Neighbouring slabs (which share cache lines) are on one XCD, workgroup g running on XCD g mod 8. False past the last.
+  __device__ __forceinline__ bool take(const NormArgs& a) {
+    const int slabs = a.groups / a.slab_groups, n = a.batch * a.splits * slabs, per = (n + 7) / 8;
+    const int id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+    if (id >= n) return false;
+    // (Scalar registers: every address is one of them plus a 32-bit offset.)
+    const int row = __builtin_amdgcn_readfirstlane(id / slabs);
+    c0 = __builtin_amdgcn_readfirstlane((id - row * slabs) * a.slab_groups * a.width);
+    b = __builtin_amdgcn_readfirstlane(row / a.splits);
+    k = row - b * a.splits;
+    each = a.each;
+    threads = blockDim.x;
     width = a.slab_groups * a.width;
-    cols = width / V;
+    cols = (width + V - 1) / V;
     lanes = threads / cols;
     lane = threadIdx.x / cols;
     col = threadIdx.x - lane * cols;
-    last = a.points - 1;
+    start = min(col * V, width - V);
+    skip = col * V - start;
+    p0 = k * lanes * each;
+    last = min(a.points - p0, lanes * each) - 1;
     in = 0;
 #pragma unroll
-    for (int e = 0; e < E; e++) in |= (lane < lanes && lane + e * lanes <= last ? 1u : 0u) << e;
+    for (int e = 0; e < E; e++) in |= (lane < lanes && e < each && lane + e * lanes <= last ? 1u : 0u) << e;
     on = in;
     if (a.mask) {
-      const float* mask = a.mask + (size_t)b * a.points;
+      const float* mask = a.mask + (size_t)b * a.points + p0;
       float mk[E];
 #pragma unroll
       for (int e = 0; e < E; e++) mk[e] = mask[point(e)];
 #pragma unroll
       for (int e = 0; e < E; e++) on &= ~((mk[e] == 0.f ? 1u : 0u) << e);
     }
+    return true;
   }
   __device__ __forceinline__ unsigned point(int e) const { return min(lane + e * lanes, last); }
-  // Byte offset of point e's column in the batch row's slab (below 2^31: fused_shape).
-  __device__ __forceinline__ unsigned at(int e, unsigned ld) const { return (point(e) * ld + col * V) * (unsigned)sizeof(T); }
+  // In column order (an entry a thread, columns * V <= threads): the channel of the slab.
+  __device__ __forceinline__ int channel() const { return min((int)threadIdx.x / V * V, width - V) + (int)threadIdx.x % V; }
+  // Byte offset of point e's column from the slab's first element (below 2^31: slab_shape).
+  __device__ __forceinline__ unsigned at(int e, unsigned ld) const { return (point(e) * ld + start) * (unsigned)sizeof(T); }
 };
 
 // A column's 16 bytes as words; element j of them as a float, and back.
@@ -553,7 +564,7 @@ __device__ __forceinline__ void read_lds(const float* p, float (&f)[N]) {  // (N
 // All loads of a thread's column, issued before any is used (masked points too: what they hold is not looked at).
 template <typename T, int E>
 __device__ __forceinline__ void load_slab(const NormArgs& a, const Slab<T, E>& s, const void* from, long long ld, u32x4 (&raw)[E]) {
-  const char* base = (const char*)((const T*)from + (size_t)s.b * a.points * ld + s.c0);
+  const char* base = (const char*)((const T*)from + ((size_t)s.b * a.points + s.p0) * ld + s.c0);
 #pragma unroll
   for (int e = 0; e < E; e++) {
     raw[e] = u32x4{0, 0, 0, 0};
@@ -562,7 +573,7 @@ __device__ __forceinline__ void load_slab(const NormArgs& a, const Slab<T, E>& s
 }
 template <typename T, int E>
 __device__ __forceinline__ void store_slab(const NormArgs& a, const Slab<T, E>& s, void* to, long long ld, int e, const u32x4& raw) {
-  char* base = (char*)((T*)to + (size_t)s.b * a.points * ld + s.c0);
+  char* base = (char*)((T*)to + ((size_t)s.b * a.points + s.p0) * ld + s.c0);
   if (s.in >> e & 1) *(typename AnyWords<T>::type*)(base + s.at(e, (unsigned)ld)) = raw;
 }
 
@@ -573,20 +584,79 @@ __device__ __forceinline__ int join_share(int groups, int threads) {
   return share;
 }
 
-template <typename T, int ACT, int NT, int E>
-__global__ __launch_bounds__(NT) void norm_fused_kernel(NormArgs a) {
+extern __shared__ __align__(16) float slab_lds[];
+// Floats of LDS: the threads' sums (two a channel of a column, at a stride that puts a column's channels in different banks),
+// later the columns' parameters; then what the joins pass on.
+__host__ __device__ __forceinline__ int slab_stride(int threads) { return threads + 8; }
+inline size_t slab_lds_bytes(int vec, int threads, int cols, int groups, bool backward) {
+  const int sums = std::max(2 * vec * slab_stride(threads), 3 * vec * cols);
+  return (size_t)(backward ? sums + 3 * threads + 2 * groups + 2 + 5 * vec * cols : sums + 4 * threads + 2 * groups) * 4;
+}
+
+// The parameters that a thread puts into LDS for all, loaded early.
+struct ColumnEntry {
+  bool mine;
+  int group;
+  float gamma, beta;
+  template <typename T, int E>
+  __device__ __forceinline__ ColumnEntry(const NormArgs& a, const Slab<T, E>& s) {
+    mine = (int)threadIdx.x < s.cols * kVec<T>;
+    const int c = mine ? s.channel() : 0;
+    group = c / a.width;
+    gamma = a.gamma ? a.gamma[s.c0 + c] : 1.f;
+    beta = a.beta ? a.beta[s.c0 + c] : 0.f;
+  }
+};
+
+// y from the words of x, with the groups' mean and rstd in LDS: the columns' parameters first (over the threads' sums, which
+// have been read).
+template <typename T, int ACT, int E>
+__device__ __forceinline__ void slab_forward(const NormArgs& a, Slab<T, E>& s, const ColumnEntry& entry, u32x4 (&raw)[E],
+                                             const float* g_mean, const float* g_rstd) {
   constexpr int V = kVec<T>;
-  constexpr int P = NT + 8;  // (the eight channels of a column lie in different banks)
-  __shared__ float s_mean[V * P], s_m2[V * P], s_n[NT];
-  __shared__ float r_n[NT], r_mean[NT], r_m2[NT], g_mean[NT], g_rstd[NT];
-  __shared__ __align__(16) float c_mean[NT], c_mul[NT], c_add[NT];
-  int b, c0;
-  if (!slab_of(a, b, c0)) return;
-  Slab<T, E> s(a, b, c0);
-  const int tid = threadIdx.x;
+  const int all = s.cols * V;
+  float *c_mean = slab_lds, *c_mul = c_mean + all, *c_add = c_mul + all;
+  if (entry.mine) {
+    c_mean[threadIdx.x] = g_mean[entry.group];
+    c_mul[threadIdx.x] = g_rstd[entry.group] * entry.gamma;
+    c_add[threadIdx.x] = entry.beta;
+  }
+  __syncthreads();
+  asm("" : "+v"(s.lane));  // (addresses too are computed again)
+  forget<E>(raw);
+  float mean[V], mul[V], add[V];
+  read_lds<V>(c_mean + s.col * V, mean);
+  read_lds<V>(c_mul + s.col * V, mul);
+  read_lds<V>(c_add + s.col * V, add);
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    if (e >= s.each) break;
+    float f[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) f[j] = act_f<ACT>(__builtin_fmaf(element<T>(raw[e], j) - mean[j], mul[j], add[j]));
+    u32x4 w;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      w[k] = sizeof(T) == 4 ? word_of<T>(f[k], 0.f) : word_of<T>(f[(2 * k) % V], f[(2 * k + 1) % V]);
+      w[k] = s.on >> e & 1 ? w[k] : 0u;
+    }
+    store_slab<T, E>(a, s, a.y, a.ldy, e, w);
+  }
+}
+
+// Forward over a slab. PART: its groups' count, mean and squared deviations over the workgroup's share of the points, for
+// norm_slab_apply_kernel; else y.
+template <typename T, int ACT, int NT, int E, bool PART>
+__global__ __launch_bounds__(NT) void norm_slab_kernel(NormArgs a) {
+  constexpr int V = kVec<T>;
+  Slab<T, E> s;
+  if (!s.take(a)) return;
+  const int tid = threadIdx.x, P = slab_stride(s.threads);
+  float *s_mean = slab_lds, *s_m2 = s_mean + V * P, *s_n = slab_lds + max(2 * V * P, 3 * V * s.cols), *r_n = s_n + s.threads,
+        *r_mean = r_n + s.threads, *r_m2 = r_mean + s.threads, *g_mean = r_m2 + s.threads, *g_rstd = g_mean + a.slab_groups;
   u32x4 raw[E];
   load_slab<T, E>(a, s, a.x, a.ldx, raw);
-  const float gamma = a.gamma && tid < s.width ? a.gamma[c0 + tid] : 1.f, beta = a.beta && tid < s.width ? a.beta[c0 + tid] : 0.f;
+  const ColumnEntry entry(a, s);
   clear_off<E>(raw, s.on);
 
   // A thread's own count, means, and squared deviations from them.
@@ -615,10 +685,11 @@ __global__ __launch_bounds__(NT) void norm_fused_kernel(NormArgs a) {
   if (s.lane < s.lanes) {
     if (s.col == 0) s_n[s.lane] = n;
 #pragma unroll
-    for (int j = 0; j < V; j++) {
-      s_mean[j * P + tid] = m[j];
-      s_m2[j * P + tid] = m2[j];
-    }
+    for (int j = 0; j < V; j++)
+      if (j >= s.skip) {
+        s_mean[(j - s.skip) * P + tid] = m[j];
+        s_m2[(j - s.skip) * P + tid] = m2[j];
+      }
   }
   __syncthreads();
   // Joined over the lanes: R rows of the slab's channels, then over a group's channels and those rows. Each join is
@@ -662,81 +733,169 @@ __global__ __launch_bounds__(NT) void norm_fused_kernel(NormArgs a) {
     }
     for (int o = share >> 1; o >= 1; o >>= 1) c2 += __shfl_xor(c2, o);
     if (mine && sub == 0) {
-      const float rstd = 1.f / sqrtf((cn > 0.f ? c2 / cn : 0.f) + a.eps);
-      g_mean[g] = mean;
-      g_rstd[g] = rstd;
-      const size_t out = (size_t)b * a.groups + c0 / a.width + g;
-      a.mean[out] = mean;
-      a.rstd[out] = rstd;
+      if constexpr (PART) {
+        float* out = a.part + (size_t)(s.b * a.splits + s.k) * 3 * a.groups + s.c0 / a.width + g;
+        out[0] = cn;
+        out[a.groups] = mean;
+        out[2 * a.groups] = c2;
+      } else {
+        const float rstd = 1.f / sqrtf((cn > 0.f ? c2 / cn : 0.f) + a.eps);
+        g_mean[g] = mean;
+        g_rstd[g] = rstd;
+        const size_t out = (size_t)s.b * a.groups + s.c0 / a.width + g;
+        a.mean[out] = mean;
+        a.rstd[out] = rstd;
+      }
     }
   }
-  __syncthreads();
-  if (tid < s.width) {
-    const int g = tid / a.width;
-    c_mean[tid] = g_mean[g];
-    c_mul[tid] = g_rstd[g] * gamma;
-    c_add[tid] = beta;
-  }
-  __syncthreads();
-  asm("" : "+v"(s.lane));  // (addresses too are computed again)
-  forget<E>(raw);
-  float mean[V], mul[V], add[V];
-  read_lds<V>(c_mean + s.col * V, mean);
-  read_lds<V>(c_mul + s.col * V, mul);
-  read_lds<V>(c_add + s.col * V, add);
-#pragma unroll
-  for (int e = 0; e < E; e++) {
-    if (e >= s.each) break;
-    float f[V];
-#pragma unroll
-    for (int j = 0; j < V; j++) f[j] = act_f<ACT>(__builtin_fmaf(element<T>(raw[e], j) - mean[j], mul[j], add[j]));
-    u32x4 w;
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-      w[k] = sizeof(T) == 4 ? word_of<T>(f[k], 0.f) : word_of<T>(f[(2 * k) % V], f[(2 * k + 1) % V]);
-      w[k] = s.on >> e & 1 ? w[k] : 0u;
-    }
-    store_slab<T, E>(a, s, a.y, a.ldy, e, w);
+  if constexpr (!PART) {
+    __syncthreads();
+    slab_forward<T, ACT, E>(a, s, entry, raw, g_mean, g_rstd);
   }
 }
 
-// Backward over a slab. The channels' sums over the slab's points go to part [batch][2][channels] for dgamma and dbeta. x and
-// dy take 64 of a thread's 128 registers, so a column's channels are taken four at a time with their parameters from LDS, and
-// dx replaces dy in place. dy is 0 at masked points, and with it da.
+// y over a slab's share of the points, from the shares' statistics (a.part).
 template <typename T, int ACT, int NT, int E>
-__global__ __launch_bounds__(NT) void norm_back_fused_kernel(NormArgs a) {
-  constexpr int V = kVec<T>, H = 4;
-  constexpr bool kExactSide = BackColumn<T, ACT>::kExactSide;
-  constexpr int P = NT + 8;
-  __shared__ float s_b[V * P], s_g[V * P], s_n[NT];
-  __shared__ float r_b[NT], r_g[NT], g_1[NT], g_2[NT];
-  __shared__ __align__(16) float c_mean[NT], c_mul[NT], c_beta[NT], c_k1[NT], c_k2[NT];
-  __shared__ double c_scale[kExactSide ? NT : 1];
-  int b, c0;
-  if (!slab_of(a, b, c0)) return;
-  Slab<T, E> s(a, b, c0);
+__global__ __launch_bounds__(NT) void norm_slab_apply_kernel(NormArgs a) {
+  Slab<T, E> s;
+  if (!s.take(a)) return;
   const int tid = threadIdx.x;
+  float *g_mean = slab_lds + 3 * kVec<T> * s.cols, *g_rstd = g_mean + a.slab_groups;
+  u32x4 raw[E];
+  load_slab<T, E>(a, s, a.x, a.ldx, raw);
+  const ColumnEntry entry(a, s);
+  const int share = join_share(a.slab_groups, s.threads), sub = tid % share, g = tid / share;
+  const bool mine = g < a.slab_groups;
+  const float* in = a.part + (size_t)s.b * a.splits * 3 * a.groups + s.c0 / a.width + (mine ? g : 0);
+  float n = 0.f, sum = 0.f, m2 = 0.f;
+  for (int i = sub; i < a.splits; i += share) {
+    const float* q = in + (size_t)i * 3 * a.groups;
+    n += q[0];
+    sum = __builtin_fmaf(q[0], q[a.groups], sum);
+  }
+  for (int o = share >> 1; o >= 1; o >>= 1) { n += __shfl_xor(n, o); sum += __shfl_xor(sum, o); }
+  const float mean = n > 0.f ? sum / n : 0.f;
+  for (int i = sub; i < a.splits; i += share) {
+    const float* q = in + (size_t)i * 3 * a.groups;
+    const float d = q[a.groups] - mean;
+    m2 += q[2 * a.groups] + (q[0] > 0.f ? q[0] * d * d : 0.f);
+  }
+  for (int o = share >> 1; o >= 1; o >>= 1) m2 += __shfl_xor(m2, o);
+  if (mine && sub == 0) {
+    const float rstd = 1.f / sqrtf((n > 0.f ? m2 / n : 0.f) + a.eps);
+    g_mean[g] = mean;
+    g_rstd[g] = rstd;
+    if (s.k == 0) {
+      a.mean[(size_t)s.b * a.groups + s.c0 / a.width + g] = mean;
+      a.rstd[(size_t)s.b * a.groups + s.c0 / a.width + g] = rstd;
+    }
+  }
+  __syncthreads();
+  slab_forward<T, ACT, E>(a, s, entry, raw, g_mean, g_rstd);
+}
+
+// The backward pass's parameters in LDS, in column order: mean, rstd gamma and beta; for float ReLU also their exact product.
+struct BackLds {
+  float *mean, *mul, *beta;
+  double* scale;
+};
+template <typename T, int ACT, int E>
+__device__ __forceinline__ void back_params(const NormArgs& a, const Slab<T, E>& s, const BackLds& c) {
+  const ColumnEntry entry(a, s);
+  if (entry.mine) {
+    const int i = threadIdx.x;
+    const size_t g = (size_t)s.b * a.groups + s.c0 / a.width + entry.group;
+    const float rstd = a.rstd[g];
+    c.mean[i] = a.mean[g];
+    c.mul[i] = rstd * entry.gamma;
+    c.beta[i] = entry.beta;
+    if constexpr (BackColumn<T, ACT>::kExactSide) c.scale[i] = (double)rstd * (double)entry.gamma;
+  }
+}
+
+// KEEP: the first pass's da stay in registers for the second (at most four points a thread). They take those of a second
+// workgroup on the CU, so only launches that have none keep them: mish, 361 points of 384 bf16 channels, 32 boards 14.3 us
+// and 18.0 without, 128 boards 50.4 us and 46.3.
+// dx from the words of x and dy (0 at masked points; or da, KEEP), with the groups' k1 and k2 in LDS.
+template <typename T, int ACT, int E, bool KEEP>
+__device__ __forceinline__ void slab_backward(const NormArgs& a, Slab<T, E>& s, u32x4 (&rx)[E], u32x4 (&rd)[E],
+                                              float (&da)[KEEP ? E : 1][kVec<T>], const BackLds& c, const float* g_1, const float* g_2) {
+  constexpr int V = kVec<T>, H = 4;
+  const int all = s.cols * V;
+  float *c_k1 = slab_lds, *c_k2 = c_k1 + all;
+  if ((int)threadIdx.x < all) {
+    const int g = s.channel() / a.width;
+    c_k1[threadIdx.x] = g_1[g];
+    c_k2[threadIdx.x] = g_2[g];
+  }
+  __syncthreads();
+  asm("" : "+v"(s.lane));  // (addresses too are computed again)
+  forget<E>(rx);
+  if constexpr (!KEEP) forget<E>(rd);
+#pragma unroll
+  for (int h = 0; h < V; h += H) {
+    BackColumn<T, ACT, H> col;
+    float k1[H], k2[H];
+    if constexpr (KEEP) {
+      read_lds<H>(c.mean + s.col * V + h, col.mean);
+      read_lds<H>(c.mul + s.col * V + h, col.mul);
+    } else col.read(c.mean, c.mul, c.beta, c.scale, s.col * V + h);
+    read_lds<H>(c_k1 + s.col * V + h, k1);
+    read_lds<H>(c_k2 + s.col * V + h, k2);
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      if (e >= s.each) break;
+      float dx[H];
+#pragma unroll
+      for (int j = 0; j < H; j++) {
+        float xc, d;
+        if constexpr (KEEP) {
+          xc = element<T>(rx[e], h + j) - col.mean[j];
+          d = da[e][h + j];
+        } else col.grad(element<T>(rx[e], h + j), element<T>(rd[e], h + j), j, xc, d);
+        dx[j] = back_dx(d, xc, col.mul[j], k1[j], k2[j]);
+      }
+#pragma unroll
+      for (int k = 0; k < H * (int)sizeof(T) / 4; k++)
+        rd[e][h * (int)sizeof(T) / 4 + k] = sizeof(T) == 4 ? word_of<T>(dx[k], 0.f) : word_of<T>(dx[(2 * k) % H], dx[(2 * k + 1) % H]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  clear_off<E>(rd, s.on);
+#pragma unroll
+  for (int e = 0; e < E; e++) store_slab<T, E>(a, s, a.dx, a.lddx, e, rd[e]);
+}
+
+// Backward over a slab. The channels' sums over the workgroup's points go to part [batch][splits][2][channels] for dgamma and
+// dbeta; PART: for norm_back_join_kernel too, else dx follows. x and dy take 64 of a thread's 128 registers, so a column's
+// channels are taken four at a time with their parameters from LDS, and dx replaces dy in place. dy is 0 at masked points,
+// and with it da.
+template <typename T, int ACT, int NT, int E, bool PART, bool KEEP>
+__global__ __launch_bounds__(NT) void norm_back_slab_kernel(NormArgs a) {
+  constexpr int V = kVec<T>, H = 4;
+  Slab<T, E> s;
+  if (!s.take(a)) return;
+  const int tid = threadIdx.x, P = slab_stride(s.threads), all = s.cols * V;
+  float *s_b = slab_lds, *s_g = s_b + V * P, *c_mean = slab_lds + max(2 * V * P, 3 * all), *s_n = c_mean + 3 * all,
+        *r_b = s_n + s.threads, *r_g = r_b + s.threads, *g_1 = r_g + s.threads, *g_2 = g_1 + a.slab_groups;
+  // (An even number of floats lies before it: threads and all are even, and the groups come twice.)
+  const BackLds c = {c_mean, c_mean + all, c_mean + 2 * all, (double*)(g_2 + a.slab_groups)};
   u32x4 rx[E], rd[E];
   load_slab<T, E>(a, s, a.x, a.ldx, rx);
   load_slab<T, E>(a, s, a.dy, a.lddy, rd);
-  float gamma = 1.f, rstd = 0.f;  // of channel c0 + tid
-  if (tid < s.width) {
-    const size_t g = (size_t)b * a.groups + (c0 + tid) / a.width;
-    rstd = a.rstd[g];
-    if (a.gamma) gamma = a.gamma[c0 + tid];
-    c_mean[tid] = a.mean[g];
-    c_mul[tid] = rstd * gamma;
-    c_beta[tid] = a.beta ? a.beta[c0 + tid] : 0.f;
-    if constexpr (kExactSide) c_scale[tid] = (double)rstd * (double)gamma;
-  }
+  back_params<T, ACT, E>(a, s, c);
+  const int own = min(tid, s.width - 1), share = join_share(a.slab_groups, s.threads), sub = tid % share, g = tid / share;
+  const float* rstd = a.rstd + (size_t)s.b * a.groups + s.c0 / a.width;
+  const float own_rstd = rstd[own / a.width], own_gamma = a.gamma ? a.gamma[s.c0 + own] : 1.f, g_rstd = rstd[min(g, a.slab_groups - 1)];
   if (s.lane < s.lanes && s.col == 0) s_n[s.lane] = (float)__builtin_popcount(s.on);
   lds_barrier();  // (the parameters; x and dy may still be on their way)
   clear_off<E>(rx, s.on);
   clear_off<E>(rd, s.on);
+  float kept[KEEP ? E : 1][V];
 #pragma unroll
   for (int h = 0; h < V; h += H) {
     BackColumn<T, ACT, H> col;
-    col.template read<NT>(c_mean, c_mul, c_beta, c_scale, s.col * V + h);
+    col.read(c.mean, c.mul, c.beta, c.scale, s.col * V + h);
     float sb[H], sg[H];
 #pragma unroll
     for (int j = 0; j < H; j++) sb[j] = sg[j] = 0.f;
@@ -749,18 +908,23 @@ __global__ __launch_bounds__(NT) void norm_back_fused_kernel(NormArgs a) {
         col.grad(element<T>(rx[e], h + j), element<T>(rd[e], h + j), j, xc, da);
         sb[j] += da;
         sg[j] = __builtin_fmaf(da, xc, sg[j]);
+        if constexpr (KEEP) kept[e][h + j] = da;
       }
       __builtin_amdgcn_sched_barrier(0);
     }
     if (s.lane < s.lanes) {
 #pragma unroll
-      for (int j = 0; j < H; j++) { s_b[(h + j) * P + tid] = sb[j]; s_g[(h + j) * P + tid] = sg[j]; }
+      for (int j = 0; j < H; j++)
+        if (h + j >= s.skip) {
+          s_b[(h + j - s.skip) * P + tid] = sb[j];
+          s_g[(h + j - s.skip) * P + tid] = sg[j];
+        }
     }
   }
   __syncthreads();
   const int R = min(s.threads / s.width, s.lanes);
   if (tid < R * s.width) {
-    const int c = tid % s.width, r = tid / s.width, from = (c % V) * P + c / V;
+    const int ch = tid % s.width, r = tid / s.width, from = (ch % V) * P + ch / V;
     float tb = 0.f, tg = 0.f;
     for (int l = r; l < s.lanes; l += R) {
       tb += s_b[from + l * s.cols];
@@ -776,16 +940,25 @@ __global__ __launch_bounds__(NT) void norm_back_fused_kernel(NormArgs a) {
       tb += r_b[r * s.width + tid];
       tg += r_g[r * s.width + tid];
     }
-    tg *= rstd;
-    float* out = a.part + (size_t)b * 2 * a.channels + c0 + tid;
+    tg *= own_rstd;
+    float* out = a.part + (size_t)(s.b * a.splits + s.k) * 2 * a.channels + s.c0 + tid;
     out[0] = tb;
     out[a.channels] = tg;
-    s_b[tid] = tb * gamma;  // (the lanes' sums have been read)
-    s_g[tid] = tg * gamma;
+    if constexpr (!PART) {
+      s_b[tid] = tb * own_gamma;  // (the lanes' sums have been read)
+      s_g[tid] = tg * own_gamma;
+    }
   }
-  __syncthreads();
-  {
-    const int share = join_share(a.slab_groups, s.threads), sub = tid % share, g = tid / share;
+  if constexpr (PART) {
+    if (s.c0 == 0 && tid < 64) {
+      float n = 0.f;
+      for (int l = tid; l < s.lanes; l += 64) n += s_n[l];
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) n += __shfl_xor(n, o);
+      if (tid == 0) a.counts[s.b * a.splits + s.k] = n;
+    }
+  } else {
+    __syncthreads();
     const bool mine = g < a.slab_groups;
     float t1 = 0.f, t2 = 0.f, cn = 0.f;
     for (int i = sub; i < (mine ? a.width : 0); i += share) {
@@ -800,45 +973,38 @@ __global__ __launch_bounds__(NT) void norm_back_fused_kernel(NormArgs a) {
     }
     if (mine && sub == 0) {
       const float inv = cn > 0.f ? 1.f / (cn * (float)a.width) : 0.f;
-      g_1[g] = t1 * inv;
-      g_2[g] = t2 * inv;
+      g_1[g] = g_rstd * (t1 * inv);
+      g_2[g] = g_rstd * g_rstd * (t2 * inv);
     }
+    __syncthreads();
+    slab_backward<T, ACT, E, KEEP>(a, s, rx, rd, kept, c, g_1, g_2);
   }
-  __syncthreads();
-  if (tid < s.width) {
-    c_k1[tid] = rstd * g_1[tid / a.width];
-    c_k2[tid] = rstd * rstd * g_2[tid / a.width];
+}
+
+// dx over a slab's share of the points, from the groups' means (a.sums).
+template <typename T, int ACT, int NT, int E>
+__global__ __launch_bounds__(NT) void norm_back_slab_apply_kernel(NormArgs a) {
+  constexpr int V = kVec<T>;
+  Slab<T, E> s;
+  if (!s.take(a)) return;
+  const int all = s.cols * V;
+  float *c_mean = slab_lds + 3 * all, *g_1 = c_mean + 3 * all, *g_2 = g_1 + a.slab_groups;
+  const BackLds c = {c_mean, c_mean + all, c_mean + 2 * all, (double*)(g_2 + a.slab_groups)};
+  u32x4 rx[E], rd[E];
+  load_slab<T, E>(a, s, a.x, a.ldx, rx);
+  load_slab<T, E>(a, s, a.dy, a.lddy, rd);
+  back_params<T, ACT, E>(a, s, c);
+  for (int g = threadIdx.x; g < a.slab_groups; g += s.threads) {
+    const float* q = a.sums + (size_t)s.b * 2 * a.groups + s.c0 / a.width + g;
+    const float rstd = a.rstd[(size_t)s.b * a.groups + s.c0 / a.width + g];
+    g_1[g] = rstd * q[0];
+    g_2[g] = rstd * rstd * q[a.groups];
   }
-  __syncthreads();
-  asm("" : "+v"(s.lane));  // (addresses too are computed again)
-  forget<E>(rx);
-  forget<E>(rd);
-#pragma unroll
-  for (int h = 0; h < V; h += H) {
-    BackColumn<T, ACT, H> col;
-    col.template read<NT>(c_mean, c_mul, c_beta, c_scale, s.col * V + h);
-    float k1[H], k2[H];
-    read_lds<H>(c_k1 + s.col * V + h, k1);
-    read_lds<H>(c_k2 + s.col * V + h, k2);
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      if (e >= s.each) break;
-      float dx[H];
-#pragma unroll
-      for (int j = 0; j < H; j++) {
-        float xc, da;
-        col.grad(element<T>(rx[e], h + j), element<T>(rd[e], h + j), j, xc, da);
-        dx[j] = back_dx(da, xc, col.mul[j], k1[j], k2[j]);
-      }
-#pragma unroll
-      for (int k = 0; k < H * (int)sizeof(T) / 4; k++)
-        rd[e][h * (int)sizeof(T) / 4 + k] = sizeof(T) == 4 ? word_of<T>(dx[k], 0.f) : word_of<T>(dx[(2 * k) % H], dx[(2 * k + 1) % H]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  }
+  lds_barrier();
+  clear_off<E>(rx, s.on);
   clear_off<E>(rd, s.on);
-#pragma unroll
-  for (int e = 0; e < E; e++) store_slab<T, E>(a, s, a.dx, a.lddx, e, rd[e]);
+  float none[1][V];
+  slab_backward<T, ACT, E, false>(a, s, rx, rd, none, c, g_1, g_2);
 }
 
 // dgamma and dbeta of 64 channels a workgroup from `parts` rows of channel sums, one wave a sixteenth of them.
@@ -865,30 +1031,44 @@ __global__ __launch_bounds__(1024) void norm_back_params_kernel(NormArgs a, int 
   }
 }
 
-// The fused launch's slab (groups 0: none fits), the threads of a workgroup and the points that each takes: as few points as
-// 1024 threads allow (up to 8: 128 KB of 16-bit values), then no more threads than those take. (361 points of 6 columns: 3
-// points and 768 threads, where 1024 threads left a third of the work to empty points.)
-struct FusedShape {
-  int groups = 0, threads = 0, each = 0;
+// How a call runs. groups 0: by rows (channels fewer than a column's, or groups wider than a workgroup joins); else on slabs of
+// that many groups, `threads` threads a workgroup with up to `each` points each, the row's points in `splits` shares: 1 where a
+// batch row's slab fits the registers of 1024 threads with 8 points each (128 KB of 16-bit values). A slab is the fewest groups
+// that give four whole columns where such fit.
+struct SlabShape {
+  int groups = 0, threads = 0, each = 0, splits = 1;
 };
-FusedShape fused_shape(const NormArgs& n, int size) {
-  const int vec = 16 / size;
-  FusedShape best;
-  // (A batch row has a point, whose address the threads past the end read, and its byte offsets have 31 bits.)
-  const long long ld = std::max(std::max(n.ldx, n.ldy), std::max(n.lddy, n.lddx));
-  if (n.points < 1 || n.points * ld >= (1ll << 31) / size) return best;
-  for (int sg = 1; sg <= n.groups; sg++) {
-    if (n.groups % sg) continue;
-    const int w = sg * n.width, cols = w / vec;
+SlabShape slab_shape(int points, int groups, int width, int vec) {
+  SlabShape best;
+  if (points < 1) return best;
+  for (int sg = 1; sg <= groups; sg++) {
+    if (groups % sg || sg * width < vec) continue;
+    const int w = sg * width, cols = (w + vec - 1) / vec;
     if (w > 1024) break;
-    if (w % vec) continue;
-    const int lanes = 1024 / cols, each = (n.points + lanes - 1) / lanes;
+    const int lanes = 1024 / cols, each = (points + lanes - 1) / lanes;
     if (each > 8) break;
-    // (The slab's channels meet in one row of threads.)
-    best = {sg, std::max(round_up((n.points + each - 1) / each * cols, 64), round_up(w, 64)), each};
+    // As few points a thread as 1024 threads allow, and no more threads than those take (361 points of 6 columns: 3 points and
+    // 768 threads, where 1024 threads left a third of the work to empty points).
+    best = {sg, std::max(round_up((points + each - 1) / each * cols, 64), round_up(w, 64)), each, 1};
+    if (w >= 4 * vec) break;
+  }
+  if (best.groups) return best;
+  for (int sg = 1; sg <= groups; sg++) {
+    if (groups % sg || sg * width < vec) continue;
+    const int w = sg * width, cols = (w + vec - 1) / vec;
+    if (w > 512) break;
+    const int share = 512 / cols * 8;
+    best = {sg, 512, 8, (points + share - 1) / share};
     if (w >= 4 * vec) break;
   }
   return best;
+}
+// The same for a call: byte offsets within a share have 31 bits.
+SlabShape slab_shape(const NormArgs& n, int size) {
+  const SlabShape f = slab_shape(n.points, n.groups, n.width, 16 / size);
+  const long long ld = std::max(std::max(n.ldx, n.ldy), std::max(n.lddy, n.lddx));
+  const long long share = f.splits == 1 ? n.points : 8 * 512;
+  return share * ld < (1ll << 31) / size ? f : SlabShape();
 }
 
 NormArgs norm_args(const kg_group_norm_args& a) {
@@ -910,19 +1090,23 @@ NormArgs norm_args(const kg_group_norm_args& a) {
 
 template <typename T, int ACT>
 void norm_forward_act(NormArgs& n, hipStream_t s) {
-  const FusedShape f = fused_shape(n, sizeof(T));
-  if (f.groups) {
-    n.slab_groups = f.groups;
-    n.each = f.each;
-    const dim3 grid((n.batch * (n.groups / f.groups) + 7) / 8 * 8);
-    if (f.threads <= 256 && f.each <= 4) launch_k(norm_fused_kernel<T, ACT, 256, 4>, grid, f.threads, 0, s, n);
-    else if (f.each <= 4) launch_k(norm_fused_kernel<T, ACT, 1024, 4>, grid, f.threads, 0, s, n);
-    else launch_k(norm_fused_kernel<T, ACT, 1024, 8>, grid, f.threads, 0, s, n);
+  const SlabShape f = slab_shape(n, sizeof(T));
+  if (!f.groups) {
+    const dim3 grid(n.batch * n.splits);
+    launch_k(norm_stats_kernel<T>, grid, GT, 0, s, n);
+    launch_k(norm_apply_kernel<T, ACT>, grid, GT, 0, s, n);
     return;
   }
-  const dim3 grid(n.batch * n.splits);
-  launch_k(norm_stats_kernel<T>, grid, GT, 0, s, n);
-  launch_k(norm_apply_kernel<T, ACT>, grid, GT, 0, s, n);
+  n.slab_groups = f.groups;
+  n.each = f.each;
+  n.splits = f.splits;
+  const dim3 grid((n.batch * f.splits * (n.groups / f.groups) + 7) / 8 * 8);
+  const size_t lds = slab_lds_bytes(kVec<T>, f.threads, (f.groups * n.width + kVec<T> - 1) / kVec<T>, f.groups, false);
+  if (f.splits > 1) {
+    launch_k(norm_slab_kernel<T, ACT_ID, 512, 8, true>, grid, f.threads, lds, s, n);
+    launch_k(norm_slab_apply_kernel<T, ACT, 512, 8>, grid, f.threads, lds, s, n);
+  } else if (f.each <= 4) launch_k(norm_slab_kernel<T, ACT, 1024, 4, false>, grid, f.threads, lds, s, n);
+  else launch_k(norm_slab_kernel<T, ACT, 1024, 8, false>, grid, f.threads, lds, s, n);
 }
 
 template <typename T>
@@ -937,25 +1121,32 @@ void norm_forward(NormArgs& n, int act, hipStream_t s) {
 
 template <typename T, int ACT>
 void norm_backward_act(NormArgs& n, hipStream_t s) {
-  const FusedShape f = fused_shape(n, sizeof(T));
-  const dim3 columns((n.channels + 63) / 64);
+  const SlabShape f = slab_shape(n, sizeof(T));
+  const dim3 columns((n.channels + 63) / 64), join((n.batch * n.groups + GT / 64 - 1) / (GT / 64));
   if (f.groups) {
     n.slab_groups = f.groups;
     n.each = f.each;
-    const dim3 grid((n.batch * (n.groups / f.groups) + 7) / 8 * 8);
-    if (n.batch) {
-      if (f.threads <= 256 && f.each <= 4) launch_k(norm_back_fused_kernel<T, ACT, 256, 4>, grid, f.threads, 0, s, n);
-      else if (f.each <= 4) launch_k(norm_back_fused_kernel<T, ACT, 1024, 4>, grid, f.threads, 0, s, n);
-      else launch_k(norm_back_fused_kernel<T, ACT, 1024, 8>, grid, f.threads, 0, s, n);
-    }
-    if (n.dgamma || n.dbeta) launch_k(norm_back_params_kernel, columns, 1024, 0, s, n, n.batch);
-    return;
+    n.splits = f.splits;
   }
-  const dim3 grid(n.batch * n.splits);
-  if (n.batch) {
+  // part [batch][splits][2][channels], counts [batch][splits], sums [batch][2][groups]
+  const size_t parts = (size_t)n.batch * n.splits;
+  n.counts = n.part + parts * 2 * n.channels;
+  n.sums = n.counts + parts;
+  if (n.batch && !f.groups) {
+    const dim3 grid(n.batch * n.splits);
     launch_k(norm_back_sums_kernel<T, ACT>, grid, GT, 0, s, n);
-    launch_k(norm_back_join_kernel, dim3((n.batch * n.groups + GT / 64 - 1) / (GT / 64)), GT, 0, s, n);
+    launch_k(norm_back_join_kernel, join, GT, 0, s, n);
     launch_k(norm_back_apply_kernel<T, ACT>, grid, GT, 0, s, n);
+  } else if (n.batch) {
+    const dim3 grid((n.batch * f.splits * (n.groups / f.groups) + 7) / 8 * 8);
+    const size_t lds = slab_lds_bytes(kVec<T>, f.threads, (f.groups * n.width + kVec<T> - 1) / kVec<T>, f.groups, true);
+    if (f.splits > 1) {
+      launch_k(norm_back_slab_kernel<T, ACT, 512, 8, true, false>, grid, f.threads, lds, s, n);
+      launch_k(norm_back_join_kernel, join, GT, 0, s, n);
+      launch_k(norm_back_slab_apply_kernel<T, ACT, 512, 8>, grid, f.threads, lds, s, n);
+    } else if (f.each > 4) launch_k(norm_back_slab_kernel<T, ACT, 1024, 8, false, false>, grid, f.threads, lds, s, n);
+    else if (grid.x <= kCUs) launch_k(norm_back_slab_kernel<T, ACT, 1024, 4, false, true>, grid, f.threads, lds, s, n);
+    else launch_k(norm_back_slab_kernel<T, ACT, 1024, 4, false, false>, grid, f.threads, lds, s, n);
   }
   if (n.dgamma || n.dbeta) launch_k(norm_back_params_kernel, columns, 1024, 0, s, n, n.batch * n.splits);
 }
@@ -980,8 +1171,11 @@ int group_norm_splits(int batch, int points, int channels) {
   return n < 1 ? 1 : (int)n;
 }
 
+// For any type and strides: the most shares that one of the ways to run it takes.
 size_t group_norm_workspace(int batch, int points, int channels, int groups, bool backward) {
-  const size_t parts = (size_t)batch * group_norm_splits(batch, points, channels);
+  int splits = group_norm_splits(batch, points, channels);
+  for (int vec = 4; vec <= 8; vec += 4) splits = std::max(splits, slab_shape(points, groups, channels / groups, vec).splits);
+  const size_t parts = (size_t)batch * splits;
   const size_t floats = backward ? parts * (2 * (size_t)channels + 1) + (size_t)batch * 2 * groups : parts * 3 * groups;
   return (floats * 4 + 255) / 256 * 256;
 }
@@ -998,9 +1192,6 @@ void launch_group_norm(const kg_group_norm_args& a, hipStream_t s) {
 
 void launch_group_norm_backward(const kg_group_norm_args& a, hipStream_t s) {
   NormArgs n = norm_args(a);
-  const size_t parts = (size_t)n.batch * n.splits;
-  n.counts = n.part + parts * 2 * n.channels;
-  n.sums = n.counts + parts;
   switch (a.type) {
     case PREC_F32: norm_backward<float>(n, a.act, s); break;
     case PREC_F16: norm_backward<f16>(n, a.act, s); break;

@@ -88,7 +88,9 @@ def _case(learn, b, points, c, groups, dtype, act, mask, seed, affine=True, shif
 
 SHAPES = [(1, 1, 1, 1), (2, 1, 8, 2), (3, 5, 3, 3), (2, 361, 384, 32), (3, 361, 128, 8), (2, 361, 75, 5), (1, 300, 25, 5), (2, 70, 44, 4),
           (5, 33, 1024, 64), (2, 9, 2056, 8), (1, 40, 4100, 1), (1, 13, 2048, 2048), (2, 4096, 16, 2), (1, 9001, 2, 1), (70, 7, 30, 3),
-          (2, 50, 96, 96), (1, 20011, 7, 7)]
+          (2, 50, 96, 96), (1, 20011, 7, 7),
+          # Rows in shares, columns that are not whole, groups wider than a share's workgroup joins.
+          (2, 5000, 96, 4), (1, 12001, 45, 3), (2, 16385, 33, 1), (1, 30000, 20, 4), (2, 700, 500, 1), (2, 700, 1000, 1), (3, 50, 17, 1)]
 
 
 @pytest.mark.parametrize("shape", SHAPES)

@@ -282,30 +282,45 @@ __global__ __launch_bounds__(kWaves * 64) void adamw_kernel(AdamArgs a) {
   else adamw_chunk<BYTES, false>(a, t, h, base);
 }
 
-// A block a wave, four elements a lane.
+// kUnroll blocks a wave, four elements of each a lane, all loads before the first store.
 template <bool BYTES>
-__global__ __launch_bounds__(256) void adamw_moments_kernel(const void* m, const void* v, const unsigned char* m_exp,
-                                                            const unsigned char* v_exp, long long blocks, int type,
-                                                            void* out_m, void* out_root) {
-  const int lane = threadIdx.x & 63;
-  for (long long b = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); b < blocks; b += (long long)gridDim.x * 4) {
-    const long long i = b * kBlock + lane * 4;
-    floatx4 fm, fr;
-    if constexpr (BYTES) {
-      const unsigned mc = *(const u32_any*)((const unsigned char*)m + i), vc = *(const u32_any*)((const unsigned char*)v + i);
-      const float mu = unit_of(m_exp[b], M_BIAS), vu = v_unit_of(v_exp[b]);
-      fm = floatx4{__builtin_amdgcn_cvt_f32_fp8(mc, 0), __builtin_amdgcn_cvt_f32_fp8(mc, 1),
-                   __builtin_amdgcn_cvt_f32_fp8(mc, 2), __builtin_amdgcn_cvt_f32_fp8(mc, 3)} * mu;
+__global__ __launch_bounds__(kWaves * 64) void adamw_moments_kernel(const void* m, const void* v, const unsigned char* m_exp,
+                                                                    const unsigned char* v_exp, long long blocks, int type,
+                                                                    void* out_m, void* out_root) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (long long b0 = ((long long)blockIdx.x * kWaves + wave) * kUnroll; b0 < blocks; b0 += (long long)gridDim.x * kWaves * kUnroll) {
+    unsigned mc[kUnroll], vc[kUnroll], me[kUnroll], ve[kUnroll];
+    floatx4 fm[kUnroll], fr[kUnroll];
 #pragma unroll
-      for (int j = 0; j < 4; j++) fr[j] = decode_v(vc, j, vu);
-    } else {
-      fm = *(const f32x4_any*)((const float*)m + i);
-      fr = *(const f32x4_any*)((const float*)v + i);
-#pragma unroll
-      for (int j = 0; j < 4; j++) fr[j] = sqrtf(fr[j]);
+    for (int u = 0; u < kUnroll; u++) {
+      const long long b = b0 + u < blocks ? b0 + u : blocks - 1, i = b * kBlock + lane * 4;
+      if constexpr (BYTES) {
+        mc[u] = __builtin_nontemporal_load((const u32_any*)((const unsigned char*)m + i));
+        vc[u] = __builtin_nontemporal_load((const u32_any*)((const unsigned char*)v + i));
+        me[u] = m_exp[b];
+        ve[u] = v_exp[b];
+      } else {
+        fm[u] = __builtin_nontemporal_load((const f32x4_any*)((const float*)m + i));
+        fr[u] = __builtin_nontemporal_load((const f32x4_any*)((const float*)v + i));
+      }
     }
-    store4_any<true>(out_m, type, i, blocks * kBlock, fm);
-    store4_any<true>(out_root, type, i, blocks * kBlock, fr);
+#pragma unroll
+    for (int u = 0; u < kUnroll; u++) {
+      if (b0 + u >= blocks) break;
+      if constexpr (BYTES) {
+        const float mu = unit_of(me[u], M_BIAS), vu = v_unit_of(ve[u]);
+        fm[u] = floatx4{__builtin_amdgcn_cvt_f32_fp8(mc[u], 0), __builtin_amdgcn_cvt_f32_fp8(mc[u], 1),
+                        __builtin_amdgcn_cvt_f32_fp8(mc[u], 2), __builtin_amdgcn_cvt_f32_fp8(mc[u], 3)} * mu;
+#pragma unroll
+        for (int j = 0; j < 4; j++) fr[u][j] = decode_v(vc[u], j, vu);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) fr[u][j] = sqrtf(fr[u][j]);
+      }
+      const long long i = (b0 + u) * kBlock + lane * 4;
+      store4_any<true>(out_m, type, i, blocks * kBlock, fm[u]);
+      store4_any<true>(out_root, type, i, blocks * kBlock, fr[u]);
+    }
   }
 }
 
@@ -356,12 +371,12 @@ void launch_adamw(int count, const kg_adamw_tensor* tensors, const kg_adamw_stat
 
 void launch_adamw_moments(long long blocks, const kg_adamw_state& state, int type, void* m, void* root, hipStream_t s) {
   if (blocks <= 0) return;
-  const long long groups = (blocks + 3) / 4;
+  const long long groups = (blocks + kWaves * kUnroll - 1) / (kWaves * kUnroll);
   const dim3 grid((unsigned)(groups < (1 << 20) ? groups : (1 << 20)));
   if (state.state_bits == 8)
-    launch_k(adamw_moments_kernel<true>, grid, 256, 0, s, state.m, state.v, state.m_exp, state.v_exp, blocks, type, m, root);
+    launch_k(adamw_moments_kernel<true>, grid, kWaves * 64, 0, s, state.m, state.v, state.m_exp, state.v_exp, blocks, type, m, root);
   else
-    launch_k(adamw_moments_kernel<false>, grid, 256, 0, s, state.m, state.v, state.m_exp, state.v_exp, blocks, type, m, root);
+    launch_k(adamw_moments_kernel<false>, grid, kWaves * 64, 0, s, state.m, state.v, state.m_exp, state.v_exp, blocks, type, m, root);
   KGX_CHECK_LAUNCH();
 }
 

@@ -61,13 +61,28 @@ __device__ __forceinline__ float row_reduce(float v, float* red) {
   return v;
 }
 
-// log(s) in double for a float s >= 1, from s = 2^k f, f in [0.7, 1.42): log f = 2 atanh(t) = 2 (t + t^3/3 + ...),
+// A row's sum, its waves' added in double: a workgroup's last roundings to float are the whole sum's, and a sequence's
+// log-probability adds up those of all its rows (margins of 512 rows off by 1.0e-7 rms with them, 0.4e-7 without).
+template <int NT>
+__device__ __forceinline__ double row_sum(float v, float* red) {
+  v = wave_reduce<false>(v);
+  if constexpr (NT == 64) return (double)v;
+  lds_barrier();  // (the last reduction's values have been read)
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  lds_barrier();
+  double t = (double)red[0];
+#pragma unroll
+  for (int k = 1; k < NT / 64; k++) t += (double)red[k];
+  return t;
+}
+
+// log(s) in double for s >= 1, from s = 2^k f, f in [0.7, 1.42): log f = 2 atanh(t) = 2 (t + t^3/3 + ...),
 // t = (f - 1) / (f + 1), |t| < 0.172, so that the terms to t^13 leave 1e-12. NaN and infinity stay.
-__device__ __forceinline__ double log_sum(float s) {
+__device__ __forceinline__ double log_sum(double s) {
   int k;
-  float f = frexpf(s, &k);
-  if (f < 0.70710678f) { f *= 2.f; k--; }
-  const double t = ((double)f - 1.0) / ((double)f + 1.0), q = t * t;
+  double f = frexp(s, &k);
+  if (f < 0.70710678) { f *= 2.0; k--; }
+  const double t = (f - 1.0) / (f + 1.0), q = t * t;
   double p = 1.0 / 13;
   p = __builtin_fma(p, q, 1.0 / 11);
   p = __builtin_fma(p, q, 1.0 / 9);
@@ -95,6 +110,7 @@ __device__ __forceinline__ float exp_of(float x, Base2 c) {
 // The running maximum and sum of e^((z - top) s) over a thread's share of a row.
 struct Running {
   float top = -INFINITY, sum = 0.f;
+  double total = 0.0;  // the row's, once joined
   // Takes V values, which become z - top; e: their exponentials. Returns what the sum so far was scaled by, and in `moved`
   // how far the maximum it is relative to went down (old minus new).
   template <int V>
@@ -128,7 +144,7 @@ struct Running {
     const float all = row_reduce<NT, true>(top, red);
     moved = top - all;
     const float keep = top == -INFINITY ? 0.f : exp_of(moved, c);
-    sum = row_reduce<NT, false>(sum * keep, red);
+    total = row_sum<NT>(sum * keep, red);
     top = all;
     return keep;
   }
@@ -170,14 +186,14 @@ struct PolicyFactors {
 // The row's results and factors from its sums, the action's logit (-infinity where it is illegal) and cross = sum e^(z -
 // top) ((z - top) - (r - its top)). Every lane of a wave computes them; `writes`: this one stores the results.
 template <bool FULL>
-__device__ __forceinline__ PolicyFactors policy_row(const PolicyRows& a, int row, bool padding, float za, float top, float sum,
-                                                    float ref_sum, float cross, bool writes) {
+__device__ __forceinline__ PolicyFactors policy_row(const PolicyRows& a, int row, bool padding, float za, float top, double sum,
+                                                    double ref_sum, float cross, bool writes) {
   const double log_s = log_sum(sum);
   const double lp = za == -INFINITY ? -(double)INFINITY : ((double)za - (double)top) * a.scale - log_s;
   PolicyFactors f = {0.f, 0.f, 0.f, 0.f, !padding && !(lp == -(double)INFINITY)};
   float loss = 0.f, logp = padding ? 0.f : -INFINITY, kl = 0.f;
   if (f.part) {
-    const float w = a.weight ? a.weight[row] : 1.f, adv = a.advantage[row], inv = __builtin_amdgcn_rcpf(sum);
+    const float w = a.weight ? a.weight[row] : 1.f, adv = a.advantage[row], inv = __builtin_amdgcn_rcpf((float)sum);
     const double delta = lp - (double)a.old_logp[row];
     const float ratio = exp_of((float)delta, Base2(1.0));
     const bool held = adv > 0.f ? delta > a.log_high : adv < 0.f ? delta < a.log_low : false;
@@ -210,8 +226,8 @@ __device__ __forceinline__ PolicyFactors policy_row(const PolicyRows& a, int row
 
 // The same for a row of NT threads: one wave computes, the others read its factors.
 template <int NT, bool FULL>
-__device__ __forceinline__ PolicyFactors policy_row_shared(const PolicyRows& a, int row, bool padding, float za, float top, float sum,
-                                                           float ref_sum, float cross, PolicyFactors* box) {
+__device__ __forceinline__ PolicyFactors policy_row_shared(const PolicyRows& a, int row, bool padding, float za, float top, double sum,
+                                                           double ref_sum, float cross, PolicyFactors* box) {
   if constexpr (NT <= 64) {
     return policy_row<FULL>(a, row, padding, za, top, sum, ref_sum, cross, (threadIdx.x & 63) == 0);
   } else {
@@ -470,12 +486,13 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void policy_row_kernel(PolicyR
         asm volatile("" : "+v"(sum), "+v"(ref_sum), "+v"(cross));
         __builtin_amdgcn_sched_barrier(0);
       }
-      sum = row_reduce<NT, false>(sum, red);
+      const double total = row_sum<NT>(sum, red);
+      double ref_total = 0.0;
       if constexpr (FULL) {
-        ref_sum = row_reduce<NT, false>(ref_sum, red);
+        ref_total = row_sum<NT>(ref_sum, red);
         cross = row_reduce<NT, false>(cross, red);
       }
-      f = policy_row_shared<NT, FULL>(a, row, false, za, top, sum, ref_sum, cross, &box);
+      f = policy_row_shared<NT, FULL>(a, row, false, za, top, total, ref_total, cross, &box);
       forget<E>(raw);
       if constexpr (FULL) forget<E>(ref);
     } else if (tid == 0) {
@@ -580,7 +597,7 @@ __global__ __launch_bounds__(NT) void policy_long_kernel(PolicyRows a) {
     }
     float za = -INFINITY;
     if (!padding && (!LEGAL || lg[act])) za = (float)z[act];
-    const PolicyFactors f = policy_row_shared<NT, FULL>(a, row, padding, za, run.top, run.sum, ref.sum, cross, &box);
+    const PolicyFactors f = policy_row_shared<NT, FULL>(a, row, padding, za, run.top, run.total, ref.total, cross, &box);
     if (!g) continue;
     const bool part = __builtin_amdgcn_readfirstlane(f.part);
     const int hot_chunk = part ? at.of(act) : -1;
@@ -727,15 +744,15 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void pref_rows_held_kernel(Pre
       sum += t;
       __builtin_amdgcn_sched_barrier(0);
     }
-    sum = row_reduce<NT, false>(sum, red);
+    const double total = row_sum<NT>(sum, red);
     if (tid == 0)
-      a.row[row] = PrefRow{za == -INFINITY ? -(double)INFINITY : (double)za - (double)base - log_sum(sum), base, 1.f / sum};
+      a.row[row] = PrefRow{za == -INFINITY ? -(double)INFINITY : (double)za - (double)base - log_sum(total), base, (float)(1.0 / total)};
   }
 }
 
 // The same for longer rows, E chunks of each thread at a time relative to the running maximum. (Held by 1024 threads in 16
 // chunks each, such a row has a CU to itself, whose loads and exponentials wait for each other: 297 us for 2430 rows of
-// 100003 f16, against TODO here.)
+// 100003 f16, against 116 here.)
 template <typename T, int NT, int E>
 __global__ __launch_bounds__(NT) void pref_rows_long_kernel(PrefRows a) {
   constexpr int V = kVec<T>;
@@ -767,8 +784,8 @@ __global__ __launch_bounds__(NT) void pref_rows_long_kernel(PrefRows a) {
     run.join<NT>(c2, red, moved);
     if (tid == 0) {
       const float za = (float)z[label];
-      a.row[row] = PrefRow{za == -INFINITY ? -(double)INFINITY : (double)za - (double)run.top - log_sum(run.sum), run.top,
-                           1.f / run.sum};
+      a.row[row] = PrefRow{za == -INFINITY ? -(double)INFINITY : (double)za - (double)run.top - log_sum(run.total), run.top,
+                           (float)(1.0 / run.total)};
     }
   }
 }

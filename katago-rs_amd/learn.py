@@ -20,6 +20,7 @@ runtime.
 import collections
 import ctypes
 import math
+import operator
 import struct
 
 import numpy as np
@@ -31,6 +32,8 @@ TYPES = {torch.float32: PRECISION_F32, torch.float16: PRECISION_F16, torch.bfloa
 ACTS = {"identity": 0, "relu": 1, "mish": 2, "silu": 3}
 BLOCK = 256  # KG_ADAMW_BLOCK
 _BYTES = (torch.bool, torch.uint8)
+_DTYPE, _DEVICE = operator.attrgetter("dtype"), torch.Tensor.get_device
+_NUMEL, _CONTIGUOUS, _POINTER = torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.data_ptr
 
 PolicyLoss = collections.namedtuple("PolicyLoss", ["loss", "logp", "kl", "grad"])
 PreferenceLoss = collections.namedtuple("PreferenceLoss", ["loss", "margin", "seq_logp", "grad"])
@@ -300,6 +303,7 @@ class AdamW:
         self.lr, self.betas, self.eps = lr, tuple(betas), eps
         self.step_count = 0
         self._sizes = [p.numel() for p in params]
+        self._elements = np.array(self._sizes, np.int64)
         blocks = [-(-p.numel() // BLOCK) for p in params]
         self.first_block = np.concatenate([[0], np.cumsum(blocks)]).astype(np.int64)
         total = int(self.first_block[-1])
@@ -325,22 +329,26 @@ class AdamW:
         grads = list(grads)
         if len(grads) != len(self.params):
             raise ValueError(f"AdamW needs {len(self.params)} gradients, got {len(grads)}")
-        some = [g for g in grads if g is not None]
-        sizes = self._sizes if len(some) == len(grads) else [n for g, n in zip(grads, self._sizes) if g is not None]
         # (Whole lists at once: a network has hundreds of gradients, and a step's time on the GPU is near this one's.)
-        dev = self.device.index
-        if [g.numel() for g in some] != sizes or not all([g.is_contiguous() for g in some]) or \
-                any([g.get_device() != dev for g in some]) or not all([g.dtype in TYPES for g in some]):
-            raise ValueError("each gradient must be contiguous float32, float16 or bfloat16 of its parameter's size and GPU")
-        if len(some) == len(grads):
-            self._rec["grad"] = [g.data_ptr() for g in grads]
-            self._rec["grad_type"] = [TYPES[g.dtype] for g in grads]
-            self._rec["elements"] = sizes
-        else:
-            self._rec["grad"] = [0 if g is None else g.data_ptr() for g in grads]
-            self._rec["grad_type"] = [0 if g is None else TYPES[g.dtype] for g in grads]
-            self._rec["elements"] = [0 if g is None else g.numel() for g in grads]
+        try:
+            self._check_grads(grads, self._sizes)
+            some, here, sizes = grads, slice(None), self._elements
+        except TypeError:  # (None has no sizes)
+            here = [g is not None for g in grads]
+            some = [g for g in grads if g is not None]
+            sizes = self._elements[here]
+            self._check_grads(some, sizes.tolist())
+            self._rec["grad"] = self._rec["grad_type"] = self._rec["elements"] = 0
+        kinds = list(map(_DTYPE, some))
+        self._rec["grad"][here] = list(map(_POINTER, some))
+        self._rec["grad_type"][here] = TYPES[kinds[0]] if len(set(kinds)) == 1 else [TYPES[k] for k in kinds]
+        self._rec["elements"][here] = sizes
         self.grads = grads
+
+    def _check_grads(self, grads, sizes):
+        if list(map(_NUMEL, grads)) != sizes or not all(map(_CONTIGUOUS, grads)) or \
+                set(map(_DEVICE, grads)) - {self.device.index} or set(map(_DTYPE, grads)) - TYPES.keys():
+            raise ValueError("each gradient must be contiguous float32, float16 or bfloat16 of its parameter's size and GPU")
 
     def _hyper(self, lr, step, grad_scale, seed):
         return _AdamHyper(self.lr if lr is None else lr, *self.betas, self.eps, grad_scale, step,

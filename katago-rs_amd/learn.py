@@ -299,6 +299,9 @@ class AdamW:
             if w is not None and (w.dtype != torch.float32 or w.shape != p.shape or w.device != self.device or
                                   not w.is_contiguous()):
                 raise ValueError(f"master {i} must be contiguous float32 of its parameter's shape and device")
+        places = [t.data_ptr() for t in (*params, *masters) if t is not None and t.numel()]
+        if len(set(places)) != len(places):
+            raise ValueError("each parameter and master must be a tensor of its own")
         self.params, self.masters, self.state_bits = params, masters, state_bits
         self.lr, self.betas, self.eps = lr, tuple(betas), eps
         self.step_count = 0

@@ -15,6 +15,7 @@
 
 #include "kgx_device.h"
 #include "kgx_learn.h"
+#include "kgx_wave.h"
 
 namespace kgx {
 
@@ -455,6 +456,10 @@ __global__ __launch_bounds__(GT) void norm_back_apply_kernel(NormArgs a) {
 
 // ---- Slabs: whole groups over the points of a batch row, or over one of its shares, in a workgroup's registers. ----
 
+// i / n for 0 <= i < 2048 and 1 <= n <= 2048, from (i + 1/2) / n in float: its error, 2^-21 of a quotient below 2048 / n, is less
+// than the half n-th that it lies from a whole number. (The compiler's division takes 30 instructions.)
+__device__ __forceinline__ int part_of(int i, int n) { return (int)(((float)i + 0.5f) * __builtin_amdgcn_rcpf((float)n)); }
+
 // A workgroup's slab: thread (col, lane) takes points p0 + lane + e lanes, e < each (at most E), of the slab's 16-byte column
 // col. A last column that is not whole starts earlier: its first `skip` channels are the column's before, and both threads
 // compute the same for them. Threads and points past the end read the last one's address, so that no load is behind a
@@ -478,8 +483,8 @@ struct Slab {
     threads = blockDim.x;
     width = a.slab_groups * a.width;
     cols = (width + V - 1) / V;
-    lanes = threads / cols;
-    lane = threadIdx.x / cols;
+    lanes = __builtin_amdgcn_readfirstlane(part_of(threads, cols));
+    lane = part_of(threadIdx.x, cols);
     col = threadIdx.x - lane * cols;
     start = min(col * V, width - V);
     skip = col * V - start;
@@ -602,7 +607,7 @@ struct ColumnEntry {
   __device__ __forceinline__ ColumnEntry(const NormArgs& a, const Slab<T, E>& s) {
     mine = (int)threadIdx.x < s.cols * kVec<T>;
     const int c = mine ? s.channel() : 0;
-    group = c / a.width;
+    group = part_of(c, a.width);
     gamma = a.gamma ? a.gamma[s.c0 + c] : 1.f;
     beta = a.beta ? a.beta[s.c0 + c] : 0.f;
   }
@@ -694,9 +699,9 @@ __global__ __launch_bounds__(NT) void norm_slab_kernel(NormArgs a) {
   __syncthreads();
   // Joined over the lanes: R rows of the slab's channels, then over a group's channels and those rows. Each join is
   // exact: the mean first, then M2 = sum M2_i + n_i (mean_i - mean)^2.
-  const int R = min(s.threads / s.width, s.lanes);
+  const int R = min(part_of(s.threads, s.width), s.lanes);
   if (tid < R * s.width) {
-    const int c = tid % s.width, r = tid / s.width;
+    const int r = part_of(tid, s.width), c = tid - r * s.width;
     const float* qm = s_mean + (c % V) * P + c / V;
     const float* q2 = s_m2 + (c % V) * P + c / V;
     float cn = 0.f, cs = 0.f, c2 = 0.f;
@@ -715,23 +720,24 @@ __global__ __launch_bounds__(NT) void norm_slab_kernel(NormArgs a) {
   }
   __syncthreads();
   {
-    const int share = join_share(a.slab_groups, s.threads), sub = tid % share, g = tid / share;
+    const int share = join_share(a.slab_groups, s.threads), sub = tid & (share - 1), g = part_of(tid, share);
     const bool mine = g < a.slab_groups;
     const int items = mine ? a.width * R : 0, first = mine ? g * a.width : 0;
     float cn = 0.f, cs = 0.f, c2 = 0.f;
     for (int i = sub; i < items; i += share) {
-      const int at = (i / a.width) * s.width + first + i % a.width;
+      const int at = part_of(i, a.width) * (s.width - a.width) + first + i;
       cn += r_n[at];
       cs = __builtin_fmaf(r_n[at], r_mean[at], cs);
     }
-    for (int o = share >> 1; o >= 1; o >>= 1) { cn += __shfl_xor(cn, o); cs += __shfl_xor(cs, o); }
+    cn = share_sum(cn, share);
+    cs = share_sum(cs, share);
     const float mean = cn > 0.f ? cs / cn : 0.f;
     for (int i = sub; i < items; i += share) {
-      const int at = (i / a.width) * s.width + first + i % a.width;
+      const int at = part_of(i, a.width) * (s.width - a.width) + first + i;
       const float d = r_mean[at] - mean;
       c2 += r_m2[at] + r_n[at] * d * d;
     }
-    for (int o = share >> 1; o >= 1; o >>= 1) c2 += __shfl_xor(c2, o);
+    c2 = share_sum(c2, share);
     if (mine && sub == 0) {
       if constexpr (PART) {
         float* out = a.part + (size_t)(s.b * a.splits + s.k) * 3 * a.groups + s.c0 / a.width + g;
@@ -764,7 +770,7 @@ __global__ __launch_bounds__(NT) void norm_slab_apply_kernel(NormArgs a) {
   u32x4 raw[E];
   load_slab<T, E>(a, s, a.x, a.ldx, raw);
   const ColumnEntry entry(a, s);
-  const int share = join_share(a.slab_groups, s.threads), sub = tid % share, g = tid / share;
+  const int share = join_share(a.slab_groups, s.threads), sub = tid & (share - 1), g = part_of(tid, share);
   const bool mine = g < a.slab_groups;
   const float* in = a.part + (size_t)s.b * a.splits * 3 * a.groups + s.c0 / a.width + (mine ? g : 0);
   float n = 0.f, sum = 0.f, m2 = 0.f;
@@ -773,14 +779,15 @@ __global__ __launch_bounds__(NT) void norm_slab_apply_kernel(NormArgs a) {
     n += q[0];
     sum = __builtin_fmaf(q[0], q[a.groups], sum);
   }
-  for (int o = share >> 1; o >= 1; o >>= 1) { n += __shfl_xor(n, o); sum += __shfl_xor(sum, o); }
+  n = share_sum(n, share);
+  sum = share_sum(sum, share);
   const float mean = n > 0.f ? sum / n : 0.f;
   for (int i = sub; i < a.splits; i += share) {
     const float* q = in + (size_t)i * 3 * a.groups;
     const float d = q[a.groups] - mean;
     m2 += q[2 * a.groups] + (q[0] > 0.f ? q[0] * d * d : 0.f);
   }
-  for (int o = share >> 1; o >= 1; o >>= 1) m2 += __shfl_xor(m2, o);
+  m2 = share_sum(m2, share);
   if (mine && sub == 0) {
     const float rstd = 1.f / sqrtf((n > 0.f ? m2 / n : 0.f) + a.eps);
     g_mean[g] = mean;
@@ -824,7 +831,7 @@ __device__ __forceinline__ void slab_backward(const NormArgs& a, Slab<T, E>& s, 
   const int all = s.cols * V;
   float *c_k1 = slab_lds, *c_k2 = c_k1 + all;
   if ((int)threadIdx.x < all) {
-    const int g = s.channel() / a.width;
+    const int g = part_of(s.channel(), a.width);
     c_k1[threadIdx.x] = g_1[g];
     c_k2[threadIdx.x] = g_2[g];
   }
@@ -884,9 +891,9 @@ __global__ __launch_bounds__(NT) void norm_back_slab_kernel(NormArgs a) {
   load_slab<T, E>(a, s, a.x, a.ldx, rx);
   load_slab<T, E>(a, s, a.dy, a.lddy, rd);
   back_params<T, ACT, E>(a, s, c);
-  const int own = min(tid, s.width - 1), share = join_share(a.slab_groups, s.threads), sub = tid % share, g = tid / share;
+  const int own = min(tid, s.width - 1), share = join_share(a.slab_groups, s.threads), sub = tid & (share - 1), g = part_of(tid, share);
   const float* rstd = a.rstd + (size_t)s.b * a.groups + s.c0 / a.width;
-  const float own_rstd = rstd[own / a.width], own_gamma = a.gamma ? a.gamma[s.c0 + own] : 1.f, g_rstd = rstd[min(g, a.slab_groups - 1)];
+  const float own_rstd = rstd[part_of(own, a.width)], own_gamma = a.gamma ? a.gamma[s.c0 + own] : 1.f, g_rstd = rstd[min(g, a.slab_groups - 1)];
   if (s.lane < s.lanes && s.col == 0) s_n[s.lane] = (float)__builtin_popcount(s.on);
   lds_barrier();  // (the parameters; x and dy may still be on their way)
   clear_off<E>(rx, s.on);
@@ -922,9 +929,9 @@ __global__ __launch_bounds__(NT) void norm_back_slab_kernel(NormArgs a) {
     }
   }
   __syncthreads();
-  const int R = min(s.threads / s.width, s.lanes);
+  const int R = min(part_of(s.threads, s.width), s.lanes);
   if (tid < R * s.width) {
-    const int ch = tid % s.width, r = tid / s.width, from = (ch % V) * P + ch / V;
+    const int r = part_of(tid, s.width), ch = tid - r * s.width, from = (ch % V) * P + ch / V;
     float tb = 0.f, tg = 0.f;
     for (int l = r; l < s.lanes; l += R) {
       tb += s_b[from + l * s.cols];
@@ -966,11 +973,9 @@ __global__ __launch_bounds__(NT) void norm_back_slab_kernel(NormArgs a) {
       t2 += s_g[g * a.width + i];
     }
     for (int i = sub; i < (mine ? s.lanes : 0); i += share) cn += s_n[i];
-    for (int o = share >> 1; o >= 1; o >>= 1) {
-      t1 += __shfl_xor(t1, o);
-      t2 += __shfl_xor(t2, o);
-      cn += __shfl_xor(cn, o);
-    }
+    t1 = share_sum(t1, share);
+    t2 = share_sum(t2, share);
+    cn = share_sum(cn, share);
     if (mine && sub == 0) {
       const float inv = cn > 0.f ? 1.f / (cn * (float)a.width) : 0.f;
       g_1[g] = g_rstd * (t1 * inv);

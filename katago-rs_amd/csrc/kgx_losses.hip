@@ -11,6 +11,7 @@
 // sequence are differences of sums of thousands. (A comparison of logp - old_logp with log(1 +- clip) needs no exp.)
 #include "kgx_device.h"
 #include "kgx_learn.h"
+#include "kgx_wave.h"
 
 namespace kgx {
 
@@ -26,25 +27,6 @@ typedef unsigned int u32_any __attribute__((aligned(1)));
 typedef unsigned long long u64_any __attribute__((aligned(1)));
 
 template <typename T> constexpr int kVec = 16 / sizeof(T);
-
-// A wave's sum or maximum, in every lane: within each row of 16 lanes by the lanes' crossbar of the vector unit, then the four
-// rows through scalar registers (six exchanges through LDS, before, were most of a narrow row's time).
-template <int CTRL>
-__device__ __forceinline__ float crossed(float v) {
-  return __uint_as_float((unsigned)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), CTRL, 0xf, 0xf, true));
-}
-__device__ __forceinline__ float lane_of(float v, int lane) {
-  return __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(v), lane));
-}
-template <bool MAX>
-__device__ __forceinline__ float wave_reduce(float v) {
-  auto join = [](float a, float b) { return MAX ? fmaxf(a, b) : a + b; };
-  v = join(v, crossed<0xB1>(v));   // lane ^ 1
-  v = join(v, crossed<0x4E>(v));   // lane ^ 2
-  v = join(v, crossed<0x141>(v));  // mirrored within 8
-  v = join(v, crossed<0x140>(v));  // mirrored within 16
-  return join(join(lane_of(v, 0), lane_of(v, 16)), join(lane_of(v, 32), lane_of(v, 48)));
-}
 
 // Reductions over the NT threads of a row: a wave, or the whole workgroup through `red` (16 floats).
 template <int NT, bool MAX>

@@ -469,10 +469,12 @@ struct Slab {
   static constexpr int V = kVec<T>;
   int b, k, c0, p0, each, threads, width, cols, lanes, col, lane, start, skip, last;  // width: the slab's channels
   unsigned in, on;  // bit e: the point exists; and is not masked
-  // Neighbouring slabs (which share cache lines) are on one XCD, workgroup g running on XCD g mod 8. False past the last.
-  __device__ __forceinline__ bool take(const NormArgs& a) {
+  // Neighbouring slabs (which share cache lines) are on one XCD, workgroup g running on XCD g mod 8. last_first: each XCD's
+  // slabs in the other order, for a second reading that begins with what the caches still hold (16 x 4096 points of 512 f32
+  // channels backward: 154 -> 134 us). False past the last.
+  __device__ __forceinline__ bool take(const NormArgs& a, bool last_first = false) {
     const int slabs = a.groups / a.slab_groups, n = a.batch * a.splits * slabs, per = (n + 7) / 8;
-    const int id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+    const int at = blockIdx.x >> 3, id = (int)(blockIdx.x & 7) * per + (last_first ? per - 1 - at : at);
     if (id >= n) return false;
     // (Scalar registers: every address is one of them plus a 32-bit offset.)
     const int row = __builtin_amdgcn_readfirstlane(id / slabs);
@@ -764,7 +766,7 @@ __global__ __launch_bounds__(NT) void norm_slab_kernel(NormArgs a) {
 template <typename T, int ACT, int NT, int E>
 __global__ __launch_bounds__(NT) void norm_slab_apply_kernel(NormArgs a) {
   Slab<T, E> s;
-  if (!s.take(a)) return;
+  if (!s.take(a, true)) return;
   const int tid = threadIdx.x;
   float *g_mean = slab_lds + 3 * kVec<T> * s.cols, *g_rstd = g_mean + a.slab_groups;
   u32x4 raw[E];
@@ -991,7 +993,7 @@ template <typename T, int ACT, int NT, int E>
 __global__ __launch_bounds__(NT) void norm_back_slab_apply_kernel(NormArgs a) {
   constexpr int V = kVec<T>;
   Slab<T, E> s;
-  if (!s.take(a)) return;
+  if (!s.take(a, true)) return;
   const int all = s.cols * V;
   float *c_mean = slab_lds + 3 * all, *g_1 = c_mean + 3 * all, *g_2 = g_1 + a.slab_groups;
   const BackLds c = {c_mean, c_mean + all, c_mean + 2 * all, (double*)(g_2 + a.slab_groups)};

@@ -207,15 +207,15 @@ int kg_adamw_step(int device, void* stream, int count, const kg_adamw_tensor* te
     check_state(*state, op);
     for (int i = 0; i < count; i++) {
       const kg_adamw_tensor& t = tensors[i];
-      const std::string at = "tensor " + std::to_string(i) + ": ";
+      const auto at = [i] { return "tensor " + std::to_string(i) + ": "; };
       check_type(t.param_type, op);
       check_type(t.grad_type, op);
-      if (t.elements < 0 || t.first_block < 0 || t.elements > (1ll << 46) || t.first_block > (1ll << 38)) bad(op, at + "size out of range");
-      if (!std::isfinite(t.weight_decay)) bad(op, at + "weight_decay must be finite");
+      if (t.elements < 0 || t.first_block < 0 || t.elements > (1ll << 46) || t.first_block > (1ll << 38)) bad(op, at() + "size out of range");
+      if (!std::isfinite(t.weight_decay)) bad(op, at() + "weight_decay must be finite");
       if (!t.elements) continue;
-      if (!t.param || !t.grad) bad(op, at + "null argument");
+      if (!t.param || !t.grad) bad(op, at() + "null argument");
       if (!aligned(t.param, size_of(t.param_type)) || !aligned(t.grad, size_of(t.grad_type)) || !aligned(t.master, 4))
-        bad(op, at + "not aligned to its elements");
+        bad(op, at() + "not aligned to its elements");
     }
     OnDevice on(device, op);
     kgx::launch_adamw(count, tensors, *state, values_of(*hyper), values, (hipStream_t)stream);

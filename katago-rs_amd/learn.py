@@ -334,24 +334,26 @@ class AdamW:
             raise ValueError(f"AdamW needs {len(self.params)} gradients, got {len(grads)}")
         # (Whole lists at once: a network has hundreds of gradients, and a step's time on the GPU is near this one's.)
         try:
-            self._check_grads(grads, self._sizes)
+            kinds = self._check_grads(grads, self._sizes)
             some, here, sizes = grads, slice(None), self._elements
         except TypeError:  # (None has no sizes)
             here = [g is not None for g in grads]
             some = [g for g in grads if g is not None]
             sizes = self._elements[here]
-            self._check_grads(some, sizes.tolist())
+            kinds = self._check_grads(some, sizes.tolist())
             self._rec["grad"] = self._rec["grad_type"] = self._rec["elements"] = 0
-        kinds = list(map(_DTYPE, some))
         self._rec["grad"][here] = list(map(_POINTER, some))
-        self._rec["grad_type"][here] = TYPES[kinds[0]] if len(set(kinds)) == 1 else [TYPES[k] for k in kinds]
+        self._rec["grad_type"][here] = kinds
         self._rec["elements"][here] = sizes
         self.grads = grads
 
     def _check_grads(self, grads, sizes):
-        if list(map(_NUMEL, grads)) != sizes or not all(map(_CONTIGUOUS, grads)) or \
-                set(map(_DEVICE, grads)) - {self.device.index} or set(map(_DTYPE, grads)) - TYPES.keys():
+        own = list(map(_NUMEL, grads))
+        types = list(map(_DTYPE, grads))
+        if own != sizes or not all(map(_CONTIGUOUS, grads)) or \
+                set(map(_DEVICE, grads)) - {self.device.index} or set(types) - TYPES.keys():
             raise ValueError("each gradient must be contiguous float32, float16 or bfloat16 of its parameter's size and GPU")
+        return TYPES[types[0]] if len(set(types)) == 1 else [TYPES[t] for t in types]
 
     def _hyper(self, lr, step, grad_scale, seed):
         return _AdamHyper(self.lr if lr is None else lr, *self.betas, self.eps, grad_scale, step,

@@ -343,7 +343,7 @@ int kg_rmsnorm_rows_of(int rows, int channels, int region, int workgroup, int* g
  * graph, and calls on different streams may overlap as long as their buffers differ. The argument structures are read
  * before the call returns; every pointer in them is memory of `device` unless it says otherwise, aligned to its elements.
  * The caller's current device is left as it was. Outputs must not overlap inputs. Element types are KG_PRECISION_F32, _F16
- * and _BF16; all sums and row statistics are float or wider.
+ * and _BF16; all sums and row statistics are float or wider. Rows have at most 2^30 columns.
  * ------------------------------------------------------------------------------------------------------------------ */
 
 /* The clipped policy loss with a KL term of `rows` rows of logits, and its gradient. Row i holds `columns` logits z (362
@@ -473,7 +473,8 @@ int kg_adamw_moments(int device, void* stream, long long blocks, const kg_adamw_
  * Over the points with a nonzero mask (all without one) and the channels of a group, mean and variance:
  *   rstd = 1 / sqrt(variance + eps), y = act((x - mean) rstd gamma + beta), 0 where the mask is 0.
  * Masked points take no part whatever they hold. A row without any point gives mean 0, rstd 1 / sqrt(eps) and zeros.
- * act: KG_ACT_*. The statistics are outputs for the backward pass. */
+ * act: KG_ACT_*. The statistics are outputs for the backward pass. At most 2048 groups; batch points and batch groups are
+ * below 2^31, and a launch of some 2^32 / 1024 slabs of groups is the most that one call makes. */
 #define KG_ACT_IDENTITY 0
 #define KG_ACT_RELU 1
 #define KG_ACT_MISH 2

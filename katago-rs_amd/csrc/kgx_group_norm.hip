@@ -1212,6 +1212,14 @@ size_t group_norm_workspace(int batch, int points, int channels, int groups, boo
   return (floats * 4 + 255) / 256 * 256;
 }
 
+bool group_norm_fits(const kg_group_norm_args& a) {
+  const NormArgs n = norm_args(a);
+  const SlabShape f = slab_shape(n, a.type == KG_PRECISION_F32 ? 4 : 2);
+  const long long workgroups = f.groups ? (long long)n.batch * f.splits * (n.groups / f.groups) + 7 : (long long)n.batch * n.splits,
+                  joins = ((long long)n.batch * n.groups + GT / 64 - 1) / (GT / 64);
+  return std::max(workgroups * (f.groups ? f.threads : GT), joins * GT) < 1ll << 32;
+}
+
 void launch_group_norm(const kg_group_norm_args& a, hipStream_t s) {
   NormArgs n = norm_args(a);
   switch (a.type) {

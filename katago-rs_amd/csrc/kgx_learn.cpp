@@ -158,6 +158,7 @@ void check_norm(const kg_group_norm_args& a, bool backward) {
     need(a.workspace, op, "workspace is null");
     need(aligned(a.workspace, 16), op, "workspace is not aligned to 16 bytes");
   }
+  need(kgx::group_norm_fits(a), op, "batch x groups is out of range");
 }
 
 }  // namespace

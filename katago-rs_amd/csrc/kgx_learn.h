@@ -26,6 +26,7 @@ void launch_adamw_moments(long long blocks, const kg_adamw_state& state, int typ
 // Group norm: how many workgroups share a batch row's points, and the workspace that this asks for.
 int group_norm_splits(int batch, int points, int channels);
 size_t group_norm_workspace(int batch, int points, int channels, int groups, bool backward);
+bool group_norm_fits(const kg_group_norm_args& a);  // its launches' threads fit 32 bits
 void launch_group_norm(const kg_group_norm_args& a, hipStream_t s);
 void launch_group_norm_backward(const kg_group_norm_args& a, hipStream_t s);
 

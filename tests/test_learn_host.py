@@ -77,6 +77,7 @@ def test_preference_loss_refuses(kgx, learn, change, text):
     (dict(batch=1 << 20, points=1 << 20), "out of range"), (dict(type=-1), "type"), (dict(act=4), "activation"),
     (dict(x=None), "x is null"), (dict(ldx=11), "row stride of x"), (dict(mean=None), "mean"), (dict(workspace=None), "workspace"),
     (dict(workspace=4104), "workspace"), (dict(y=4096, dx=4096), "overlap"),
+    (dict(batch=1 << 28, points=1), "batch x groups"), (dict(batch=1 << 25, points=1, channels=3), "batch x groups"),
 ])
 def test_group_norm_refuses(kgx, learn, change, text, backward):
     base = dict(batch=2, points=9, channels=12, groups=3, type=0, act=2, eps=1e-5, x=4096, ldx=12, mask=None, gamma=None,

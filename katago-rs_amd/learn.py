@@ -278,7 +278,8 @@ def group_norm_backward(dy, x, mean, rstd, groups, gamma=None, beta=None, *, mas
 
 class AdamW:
     """AdamW over a list of parameters, one call a step (kg_adamw_step). The parameters (contiguous float32, float16 or
-    bfloat16 tensors of one GPU) and their float32 `masters` (a list, None where a parameter has none) are updated in place.
+    bfloat16 tensors of one GPU) and their float32 `masters` (a list, None where a parameter has none) are updated in place,
+    where they lie now.
     weight_decay is one number or one for each parameter. The moments of all parameters lie in one state (m, v and, in 8 bits,
     m_exp, v_exp), each parameter's from element BLOCK * first_block[i] on; a program saves state() and gives it to load_state."""
 

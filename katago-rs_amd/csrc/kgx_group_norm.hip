@@ -1071,7 +1071,7 @@ struct SlabShape {
 };
 SlabShape slab_shape(int points, int groups, int width, int vec) {
   SlabShape best;
-  if (points < 1) return best;
+  if (points < 1 || width < 1) return best;
   for (int sg = 1; sg <= groups; sg++) {
     if (groups % sg || sg * width < vec) continue;
     const int w = sg * width, cols = (w + vec - 1) / vec;

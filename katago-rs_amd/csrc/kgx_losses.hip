@@ -208,13 +208,13 @@ __device__ __forceinline__ PolicyFactors policy_row(const PolicyRows& a, int row
 
 // The same for a row of NT threads: one wave computes, the others read its factors.
 template <int NT, bool FULL>
-__device__ __forceinline__ PolicyFactors policy_row_shared(const PolicyRows& a, int row, bool padding, float za, float top, double sum,
+__device__ __forceinline__ PolicyFactors policy_row_shared(const PolicyRows& a, int row, float za, float top, double sum,
                                                            double ref_sum, float cross, PolicyFactors* box) {
   if constexpr (NT <= 64) {
-    return policy_row<FULL>(a, row, padding, za, top, sum, ref_sum, cross, (threadIdx.x & 63) == 0);
+    return policy_row<FULL>(a, row, false, za, top, sum, ref_sum, cross, (threadIdx.x & 63) == 0);
   } else {
     if (threadIdx.x < 64) {
-      const PolicyFactors f = policy_row<FULL>(a, row, padding, za, top, sum, ref_sum, cross, threadIdx.x == 0);
+      const PolicyFactors f = policy_row<FULL>(a, row, false, za, top, sum, ref_sum, cross, threadIdx.x == 0);
       if (threadIdx.x == 0) *box = f;
     }
     lds_barrier();
@@ -474,7 +474,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void policy_row_kernel(PolicyR
         ref_total = row_sum<NT>(ref_sum, red);
         cross = row_reduce<NT, false>(cross, red);
       }
-      f = policy_row_shared<NT, FULL>(a, row, false, za, top, total, ref_total, cross, &box);
+      f = policy_row_shared<NT, FULL>(a, row, za, top, total, ref_total, cross, &box);
       forget<E>(raw);
       if constexpr (FULL) forget<E>(ref);
     } else if (tid == 0) {
@@ -534,7 +534,7 @@ __global__ __launch_bounds__(NT) void policy_long_kernel(PolicyRows a) {
     const int act = a.action[row];
     const bool padding = (unsigned)act >= (unsigned)a.columns;
     Running run, ref;
-    float cross = 0.f;
+    PolicyFactors f = {0.f, 0.f, 0.f, 0.f, 0};
     // The words of E chunks of the row (and of the reference's) from chunk c0 on, with -infinity where nothing is.
     auto piece = [&](int c0, u32x4(&raw)[E], u32x4(&raw_r)[FULL ? E : 1]) {
       load_row<T, NT, E>(z, tid, at, raw, c0);
@@ -544,17 +544,18 @@ __global__ __launch_bounds__(NT) void policy_long_kernel(PolicyRows a) {
       if constexpr (FULL) remove_past<T, NT, E>(tid, at, raw_r, c0);
     };
     if (!padding) {
+      float cross = 0.f;
       for (int c0 = 0; !at.none(c0); c0 += NT * E) {
         u32x4 raw[E], raw_r[FULL ? E : 1];
         piece(c0, raw, raw_r);
-        float f[E * V], e[E * V], moved;
+        float fz[E * V], e[E * V], moved;
 #pragma unroll
         for (int k = 0; k < E; k++) {
 #pragma unroll
-          for (int j = 0; j < V; j++) f[k * V + j] = !at.none(c0 + k * NT) ? element<T>(raw[k], j) : -INFINITY;
+          for (int j = 0; j < V; j++) fz[k * V + j] = !at.none(c0 + k * NT) ? element<T>(raw[k], j) : -INFINITY;
         }
         const float before = run.sum;
-        const float keep = run.add<E * V>(f, c2, e, moved);
+        const float keep = run.add<E * V>(fz, c2, e, moved);
         if constexpr (FULL) {
           float fr[E * V], er[E * V], r_moved;
 #pragma unroll
@@ -565,7 +566,7 @@ __global__ __launch_bounds__(NT) void policy_long_kernel(PolicyRows a) {
           ref.add<E * V>(fr, c2, er, r_moved);
           float x = 0.f;
 #pragma unroll
-          for (int j = 0; j < E * V; j++) x += e[j] == 0.f ? 0.f : e[j] * (f[j] - fr[j]);
+          for (int j = 0; j < E * V; j++) x += e[j] == 0.f ? 0.f : e[j] * (fz[j] - fr[j]);
           cross = keep == 0.f ? x : __builtin_fmaf(__builtin_fmaf(before, moved - r_moved, cross), keep, x);
         }
       }
@@ -576,10 +577,11 @@ __global__ __launch_bounds__(NT) void policy_long_kernel(PolicyRows a) {
         ref.join<NT>(c2, red, r_moved);
         cross = row_reduce<NT, false>(keep == 0.f ? 0.f : __builtin_fmaf(before, moved - r_moved, cross) * keep, red);
       }
+      const float za = !LEGAL || lg[act] ? (float)z[act] : -INFINITY;
+      f = policy_row_shared<NT, FULL>(a, row, za, run.top, run.total, ref.total, cross, &box);
+    } else if (tid == 0) {
+      a.loss[row] = a.logp[row] = a.kl[row] = 0.f;
     }
-    float za = -INFINITY;
-    if (!padding && (!LEGAL || lg[act])) za = (float)z[act];
-    const PolicyFactors f = policy_row_shared<NT, FULL>(a, row, padding, za, run.top, run.total, ref.total, cross, &box);
     if (!g) continue;
     const bool part = __builtin_amdgcn_readfirstlane(f.part);
     const int hot_chunk = part ? at.of(act) : -1;

@@ -380,7 +380,7 @@ class AdamW:
 
     def values(self, *, lr=None, step=None, grad_scale=1.0, seed=None):
         """The scalars of a step (the next one by default) as a uint8 tensor on the host, to be copied to a captured step's
-        `values`."""
+        `values`. Replays are not counted: a program that replays gives `step`."""
         out = AdamValues()
         number = self.step_count + 1 if step is None else step
         _check(lib().kg_adamw_values(ctypes.byref(self._hyper(lr, number, grad_scale, seed)), ctypes.byref(out)))

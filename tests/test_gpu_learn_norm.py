@@ -205,3 +205,20 @@ def test_group_norm_refuses_on_the_gpu(learn):
         learn.group_norm(x, 3, torch.ones(12, device="cuda").half())
     with pytest.raises(ValueError, match="mean"):
         learn.group_norm_backward(x, x.clone(), torch.zeros(2, 4, device="cuda"), torch.zeros(2, 3, device="cuda"), 3)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(40, 361, 45, 3), (6, 9000, 27, 3), (64, 81, 250, 2)])
+def test_group_norm_again_is_the_same(learn, shape, dtype):
+    """Widths whose last column of 16 bytes is not whole: two threads compute its first channels, and both store them."""
+    b, p, c, groups = shape
+    g = torch.Generator(device="cuda").manual_seed(9)
+    x, dy = (torch.randn(b, p, c, generator=g, device="cuda").to(dtype) for _ in range(2))
+    gm, bt = (torch.randn(c, generator=g, device="cuda") for _ in range(2))
+    for act in ("mish", "silu"):
+        first = None
+        for _ in range(8):
+            y, mean, rstd = learn.group_norm(x, groups, gm, bt, act=act)
+            got = [y, mean, rstd, *learn.group_norm_backward(dy, x, mean, rstd, groups, gm, bt, act=act)]
+            first = first or got
+            assert all(torch.equal(a, b) for a, b in zip(got, first))

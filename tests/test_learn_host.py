@@ -133,6 +133,7 @@ def test_workspaces(kgx):
     for b, p, c, g in ((1, 1, 1, 1), (32, 361, 384, 32), (3, 16384, 1024, 64), (70000, 1, 4, 2)):
         assert L.kg_group_norm_workspace(b, p, c, g, 0) >= b * g * 12
         assert L.kg_group_norm_workspace(b, p, c, g, 1) >= b * (8 * c + 8 * g + 4)
+    assert L.kg_group_norm_workspace(2, 5, 3, 2 ** 31 - 1, 1) >= 0  # (at once, also for what no call takes)
 
 
 def test_python_calls_refuse_what_they_cannot_take(learn):

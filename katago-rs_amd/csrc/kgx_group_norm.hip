@@ -75,7 +75,8 @@ struct NormArgs {
   float *mean, *rstd, *dgamma, *dbeta;
   float* part;     // forward: [batch][splits][3][groups] count, mean, M2; backward: [batch][splits][2][channels] sums
   float* counts;   // backward: [batch][splits] points
-  float* sums;     // backward: [batch][splits][2][groups] sums of da gamma and da gamma xh; by rows [batch][2][groups] means
+  float* sums;     // backward: [batch][splits][2][groups] sums of da gamma and da gamma xh
+  float* means;    // backward by rows: [batch][2][groups]
   int batch, points, channels, groups, width, splits;  // width: channels of a group
   int slab_groups, each;  // slabs: their groups, the points a thread takes
   int past;               // y or dx is stored past the caches
@@ -325,7 +326,7 @@ __device__ __forceinline__ float back_dx(float da, float xc, float mul, float k1
   return __builtin_fmaf(da, mul, __builtin_fmaf(-xc, k2, -k1));
 }
 
-// Backward, first launch: sums of da and da xh over the workgroup's points, per channel.
+// Backward, first launch: sums of da and da xh over the workgroup's points, per channel, and with gamma per group.
 template <typename T, int ACT>
 __global__ __launch_bounds__(GT) void norm_back_sums_kernel(NormArgs a) {
   constexpr int V = kVec<T>;
@@ -383,6 +384,23 @@ __global__ __launch_bounds__(GT) void norm_back_sums_kernel(NormArgs a) {
     }
     __syncthreads();
   }
+  // (The channels' sums that the workgroup has just written.)
+  for (int g = tid >> 6; g < a.groups; g += GT / 64) {
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll 4
+    for (int c = g * a.width + (tid & 63); c < (g + 1) * a.width; c += 64) {
+      const float gm = a.gamma ? a.gamma[c] : 1.f;
+      s1 = __builtin_fmaf(gm, out[c], s1);
+      s2 = __builtin_fmaf(gm, out[a.channels + c], s2);
+    }
+    s1 = share_sum(s1, 64);
+    s2 = share_sum(s2, 64);
+    if ((tid & 63) == 0) {
+      float* to = a.sums + (size_t)blockIdx.x * 2 * a.groups + g;
+      to[0] = s1;
+      to[a.groups] = s2;
+    }
+  }
 }
 
 // Second launch: a wave a group of a batch row, its sums divided by its elements.
@@ -392,24 +410,18 @@ __global__ __launch_bounds__(GT) void norm_back_join_kernel(NormArgs a) {
   const int b = id / a.groups, g = id % a.groups;
   float n = 0.f, s1 = 0.f, s2 = 0.f;
   for (int k = lane; k < a.splits; k += 64) n += a.counts[(size_t)b * a.splits + k];
-#pragma unroll 4
-  for (int i = lane; i < a.width * a.splits; i += 64) {
-    const int c = g * a.width + i % a.width, k = i / a.width;
-    const float* q = a.part + ((size_t)b * a.splits + k) * 2 * a.channels + c;
-    const float gm = a.gamma ? a.gamma[c] : 1.f;
-    s1 = __builtin_fmaf(gm, q[0], s1);
-    s2 = __builtin_fmaf(gm, q[a.channels], s2);
+  for (int k = lane; k < a.splits; k += 64) {
+    const float* q = a.sums + ((size_t)b * a.splits + k) * 2 * a.groups + g;
+    s1 += q[0];
+    s2 += q[a.groups];
   }
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    n += __shfl_xor(n, o);
-    s1 += __shfl_xor(s1, o);
-    s2 += __shfl_xor(s2, o);
-  }
+  n = share_sum(n, 64);
+  s1 = share_sum(s1, 64);
+  s2 = share_sum(s2, 64);
   if (lane == 0) {
     const float inv = n > 0.f ? 1.f / (n * (float)a.width) : 0.f;
-    a.sums[(size_t)b * 2 * a.groups + g] = s1 * inv;
-    a.sums[(size_t)b * 2 * a.groups + a.groups + g] = s2 * inv;
+    a.means[(size_t)b * 2 * a.groups + g] = s1 * inv;
+    a.means[(size_t)b * 2 * a.groups + a.groups + g] = s2 * inv;
   }
 }
 
@@ -432,8 +444,8 @@ __global__ __launch_bounds__(GT) void norm_back_apply_kernel(NormArgs a) {
     for (int j = 0; j < V; j++) {
       const int g = min(c0 + j, a.channels - 1) / a.width;
       const float rstd = a.rstd[(size_t)b * a.groups + g];
-      k1[j] = rstd * a.sums[(size_t)b * 2 * a.groups + g];
-      k2[j] = rstd * rstd * a.sums[(size_t)b * 2 * a.groups + a.groups + g];
+      k1[j] = rstd * a.means[(size_t)b * 2 * a.groups + g];
+      k2[j] = rstd * rstd * a.means[(size_t)b * 2 * a.groups + a.groups + g];
     }
     const T* x = (const T*)a.x + (size_t)b * a.points * a.ldx + c0;
     const T* dy = (const T*)a.dy + (size_t)b * a.points * a.lddy + c0;
@@ -1161,10 +1173,11 @@ void norm_backward_act(NormArgs& n, hipStream_t s) {
     n.each = f.each;
     n.splits = f.splits;
   }
-  // part [batch][splits][2][channels], counts [batch][splits], sums [batch][splits][2][groups] (by rows: [batch][2][groups])
+  // part [batch][splits][2][channels], counts [batch][splits], sums [batch][splits][2][groups], means [batch][2][groups]
   const size_t parts = (size_t)n.batch * n.splits;
   n.counts = n.part + parts * 2 * n.channels;
   n.sums = n.counts + parts;
+  n.means = n.sums + parts * 2 * n.groups;
   if (n.batch && !f.groups) {
     const dim3 grid(n.batch * n.splits);
     launch_k(norm_back_sums_kernel<T, ACT>, grid, GT, 0, s, n);
@@ -1196,7 +1209,9 @@ void norm_backward(NormArgs& n, int act, hipStream_t s) {
 }  // namespace
 
 int group_norm_splits(int batch, int points, int channels) {
-  const long long want = ((long long)points * channels + kSplitTarget - 1) / kSplitTarget;
+  // (A row of fewer channels takes a thread all the same: 36 x 11761 points of one channel took 53 us forward and 96
+  // backward by its elements alone, 16 and 38 so.)
+  const long long want = ((long long)points * std::max(channels, 8) + kSplitTarget - 1) / kSplitTarget;
   const long long most = batch > 0 ? (2048 + batch - 1) / batch : 1;
   long long n = want < most ? want : most;
   if (n > points) n = points;
@@ -1208,7 +1223,7 @@ size_t group_norm_workspace(int batch, int points, int channels, int groups, boo
   int splits = group_norm_splits(batch, points, channels);
   for (int vec = 4; vec <= 8; vec += 4) splits = std::max(splits, slab_shape(points, groups, channels / groups, vec).splits);
   const size_t parts = (size_t)batch * splits;
-  const size_t floats = parts * (backward ? 2 * ((size_t)channels + groups) + 1 : 3 * (size_t)groups);
+  const size_t floats = parts * (backward ? 2 * ((size_t)channels + groups) + 1 : 3 * (size_t)groups) + (backward ? (size_t)batch * 2 * groups : 0);
   return (floats * 4 + 255) / 256 * 256;
 }
 

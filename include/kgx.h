@@ -379,8 +379,11 @@ typedef struct {
   float* kl;                   /* [rows] */
   void* grad;                  /* [rows] rows of ld_grad (columns past `columns` stay as they are); or NULL */
   long long ld_grad;
+  void* workspace;             /* kg_policy_loss_workspace(rows, columns) bytes, 16-byte aligned, this call's own until it
+                                  has run; NULL where that is 0 (all but few long rows) */
 } kg_policy_loss_args;
 int kg_policy_loss(int device, void* stream, const kg_policy_loss_args* args);
+size_t kg_policy_loss_workspace(int rows, int columns);
 
 /* The preference loss of `pairs` pairs of lines of moves (or token sequences), and its gradient. The sequences lie packed in
  * `rows` rows of logits: sequence q is rows [offsets[q], offsets[q + 1]), pair i prefers sequence 2 i to 2 i + 1. A row

@@ -40,7 +40,7 @@ EXPORTS = [
     "kg_conv_geometry", "kg_conv_tile_of", "kg_conv_weight_load", "kg_conv_weight_chunk", "kg_float_tile_of", "kg_small_tile_of",
     "kg_junction_tile_of", "kg_gpool_tile_of", "kg_l2_touch_line", "kg_rmsnorm_rows_of",
     "kg_featurize", "kg_featurize_rows", "kg_evaluate_positions",
-    "kg_policy_loss", "kg_preference_loss", "kg_preference_loss_workspace", "kg_adamw_step", "kg_adamw_values",
+    "kg_policy_loss", "kg_policy_loss_workspace", "kg_preference_loss", "kg_preference_loss_workspace", "kg_adamw_step", "kg_adamw_values",
     "kg_adamw_moments", "kg_group_norm", "kg_group_norm_backward", "kg_group_norm_workspace",
 ]
 # Completion callback of kg_get_output_async: (user, status).
@@ -226,6 +226,8 @@ def lib():
         # The learning operators (learn.py gives their structures).
         L.kg_policy_loss.argtypes = [ci, vp, vp]
         L.kg_preference_loss.argtypes = [ci, vp, vp]
+        L.kg_policy_loss_workspace.argtypes = [ci, ci]
+        L.kg_policy_loss_workspace.restype = ctypes.c_size_t
         L.kg_preference_loss_workspace.argtypes = [ci]
         L.kg_preference_loss_workspace.restype = ctypes.c_size_t
         L.kg_adamw_step.argtypes = [ci, vp, ci, vp, vp, vp, vp]

@@ -75,6 +75,10 @@ void check_policy(const kg_policy_loss_args& a) {
   if (a.legal) need(a.ld_legal >= (a.rows > 1 ? a.columns : 0), op, "the row stride of legal is less than its row");
   need(a.action && a.old_logp && a.advantage && a.loss && a.logp && a.kl, op, "null argument");
   need(a.grad != a.logits && (!a.grad || a.grad != a.ref_logits), op, "grad must not overlap an input");
+  if (kgx::policy_loss_workspace(a.rows, a.columns)) {
+    need(a.workspace, op, "workspace is null");
+    need(aligned(a.workspace, 16), op, "workspace is not aligned to 16 bytes");
+  }
 }
 
 void check_preference(const kg_preference_loss_args& a) {
@@ -174,6 +178,8 @@ int kg_policy_loss(int device, void* stream, const kg_policy_loss_args* args) {
     kgx::launch_policy_loss(*args, (hipStream_t)stream);
   });
 }
+
+size_t kg_policy_loss_workspace(int rows, int columns) { return kgx::policy_loss_workspace(rows, columns); }
 
 size_t kg_preference_loss_workspace(int rows) {
   return rows > 0 ? ((size_t)rows * (sizeof(kgx::PrefRow) + sizeof(float)) + 255) / 256 * 256 : 0;

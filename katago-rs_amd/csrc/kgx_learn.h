@@ -8,6 +8,7 @@
 
 namespace kgx {
 
+size_t policy_loss_workspace(int rows, int columns);
 void launch_policy_loss(const kg_policy_loss_args& a, hipStream_t s);
 
 // The preference loss's per-row and per-pair results between its kernels, in one workspace: row t's log-probability of its

@@ -9,6 +9,9 @@
 //
 // A row's few scalars are computed in double: logp decides on which side of the clip the row is, and the losses of a
 // sequence are differences of sums of thousands. (A comparison of logp - old_logp with log(1 +- clip) needs no exp.)
+#include <algorithm>
+#include <climits>
+
 #include "kgx_device.h"
 #include "kgx_learn.h"
 #include "kgx_wave.h"
@@ -144,6 +147,11 @@ __device__ __forceinline__ int wave_row() {
 // stay where the next operator finds them.
 constexpr long long kPastBytes = 64ll << 20;
 
+// The sums over a part of a row (see PolicyRows), relative to the part's maxima.
+struct PolicyPart {
+  double sum, ref_sum;
+  float top, ref_top, cross, none;
+};
 struct PolicyRows {
   const void* logits;
   const unsigned char* legal;
@@ -153,7 +161,8 @@ struct PolicyRows {
   const int* action;
   const float *old_logp, *advantage, *weight, *ref_logp;
   float *loss, *logp, *kl;
-  int rows, columns, past;
+  PolicyPart* parts;  // rows cut into `split` parts of `span` chunks (1: not cut)
+  int rows, columns, past, split, span;
   double scale, low, high, log_low, log_high;  // clip_low, clip_high; log(1 - clip_low), log(1 + clip_high)
   float kl_coef;
 };
@@ -517,15 +526,21 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void policy_row_kernel(PolicyR
 // Longer rows: E chunks of each thread at a time relative to the running maxima, and again for the gradient, whose second
 // reading comes from the caches. (Held by 1024 threads in 16 chunks each, a row has a CU to itself, whose loads,
 // exponentials and stores wait for each other.)
-template <typename T, int NT, int E, bool FULL, bool LEGAL>
+// Few such rows are cut into parts for as many workgroups: a launch for the parts' sums (PARTS), and one that joins them and writes
+// the gradient (JOIN). One row of 125123 f16 with legality and a full KL took TODO us on one CU, now 10.
+enum { WHOLE, PARTS, JOIN };
+template <typename T, int NT, int E, bool FULL, bool LEGAL, int STAGE>
 __global__ __launch_bounds__(NT) void policy_long_kernel(PolicyRows a) {
   constexpr int V = kVec<T>;
   __shared__ float red[16];
   __shared__ PolicyFactors box;
+  __shared__ float tops[2];
   const int tid = threadIdx.x;
   const float s = (float)a.scale;
   const Base2 c2(a.scale);
-  for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
+  for (int id = blockIdx.x; id < a.rows * (STAGE == WHOLE ? 1 : a.split); id += gridDim.x) {
+    const int row = STAGE == WHOLE ? id : id / a.split, part = STAGE == WHOLE ? 0 : id - row * a.split;
+    const int begin = part * a.span, end = STAGE == WHOLE ? INT_MAX : begin + a.span;  // its chunks
     const T* z = (const T*)a.logits + (size_t)row * a.ld;
     const T* r = FULL ? (const T*)a.ref + (size_t)row * a.ld_ref : nullptr;
     const unsigned char* lg = LEGAL ? a.legal + (size_t)row * a.ld_legal : nullptr;
@@ -543,9 +558,9 @@ __global__ __launch_bounds__(NT) void policy_long_kernel(PolicyRows a) {
       remove_past<T, NT, E>(tid, at, raw, c0);
       if constexpr (FULL) remove_past<T, NT, E>(tid, at, raw_r, c0);
     };
-    if (!padding) {
+    if (!padding && STAGE != JOIN) {
       float cross = 0.f;
-      for (int c0 = 0; !at.none(c0); c0 += NT * E) {
+      for (int c0 = begin; c0 < end && !at.none(c0); c0 += NT * E) {
         u32x4 raw[E], raw_r[FULL ? E : 1];
         piece(c0, raw, raw_r);
         float fz[E * V], e[E * V], moved;
@@ -577,23 +592,58 @@ __global__ __launch_bounds__(NT) void policy_long_kernel(PolicyRows a) {
         ref.join<NT>(c2, red, r_moved);
         cross = row_reduce<NT, false>(keep == 0.f ? 0.f : __builtin_fmaf(before, moved - r_moved, cross) * keep, red);
       }
-      const float za = !LEGAL || lg[act] ? (float)z[act] : -INFINITY;
-      f = policy_row_shared<NT, FULL>(a, row, za, run.top, run.total, ref.total, cross, &box);
-    } else if (tid == 0) {
+      if constexpr (STAGE == PARTS) {
+        if (tid == 0) a.parts[id] = PolicyPart{run.total, ref.total, run.top, ref.top, cross, 0.f};
+      } else {
+        const float za = !LEGAL || lg[act] ? (float)z[act] : -INFINITY;
+        f = policy_row_shared<NT, FULL>(a, row, za, run.top, run.total, ref.total, cross, &box);
+      }
+    } else if (STAGE == JOIN && !padding) {
+      lds_barrier();  // (the last part's factors have been read)
+      if (tid < 64) {
+        PolicyPart q = {0.0, 0.0, -INFINITY, -INFINITY, 0.f, 0.f};
+        if (tid < a.split) q = a.parts[row * a.split + tid];
+        const float top = wave_reduce<true>(q.top), ref_top = FULL ? wave_reduce<true>(q.ref_top) : 0.f;
+        const float moved = q.top - top, keep = q.top == -INFINITY ? 0.f : exp_of(moved, c2);
+        double total = q.sum * (double)keep, ref_total = 0.0;
+        float cross = 0.f;
+        if constexpr (FULL) {
+          const float r_moved = q.ref_top - ref_top;
+          ref_total = q.ref_sum * (double)(q.ref_top == -INFINITY ? 0.f : exp_of(r_moved, c2));
+          cross = wave_reduce<false>(keep == 0.f ? 0.f : __builtin_fmaf((float)q.sum, moved - r_moved, q.cross) * keep);
+        }
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) {
+          total += __shfl_xor(total, o);
+          if constexpr (FULL) ref_total += __shfl_xor(ref_total, o);
+        }
+        const float za = !LEGAL || lg[act] ? (float)z[act] : -INFINITY;
+        const PolicyFactors mine = policy_row<FULL>(a, row, false, za, top, total, ref_total, cross, tid == 0 && part == 0);
+        if (tid == 0) {
+          box = mine;
+          tops[0] = top;
+          tops[1] = ref_top;
+        }
+      }
+      lds_barrier();
+      f = box;
+      run.top = tops[0];
+      ref.top = tops[1];
+    } else if (tid == 0 && part == 0) {
       a.loss[row] = a.logp[row] = a.kl[row] = 0.f;
     }
-    if (!g) continue;
-    const bool part = __builtin_amdgcn_readfirstlane(f.part);
-    const int hot_chunk = part ? at.of(act) : -1;
-    for (int c0 = 0; !at.none(c0); c0 += NT * E) {
+    if (STAGE == PARTS || !g) continue;
+    const bool takes = __builtin_amdgcn_readfirstlane(f.part);
+    const int hot_chunk = takes ? at.of(act) : -1;
+    for (int c0 = begin; c0 < end && !at.none(c0); c0 += NT * E) {
       u32x4 raw[E], raw_r[FULL ? E : 1];
-      if (part) piece(c0, raw, raw_r);
+      if (takes) piece(c0, raw, raw_r);
 #pragma unroll
       for (int k = 0; k < E; k++) {
         if (at.none(c0 + k * NT)) break;
         const int c = fresh(tid) + c0 + k * NT;
         float gf[V] = {};
-        if (part) {
+        if (takes) {
 #pragma unroll
           for (int j = 0; j < V; j++) {
             const float x = element<T>(raw[k], j) - run.top, ex = __builtin_amdgcn_exp2f(x * c2.hi);
@@ -639,8 +689,22 @@ RowShape row_shape(int columns, const void* p, long long ld, int rows) {
   return {512, 8};
 }
 
+// How many parts a row may be cut into, two workgroups a CU in all: what the workspace holds.
+int most_parts(int rows, int columns) { return rows < 1 || rows > 256 || columns <= 16384 ? 1 : std::min(64, 512 / rows); }
+
+// The parts that a call takes, whole pieces of `piece` chunks each.
+template <typename T>
+PolicyRows in_parts(PolicyRows p, int piece) {
+  const int chunks = (p.columns + kVec<T> - 1) / kVec<T> + Chunks<T>::line(p.columns) / 16, pieces = (chunks + piece - 1) / piece;
+  const int most = std::min(most_parts(p.rows, p.columns), pieces), each = (pieces + most - 1) / most;
+  p.span = each * piece;
+  p.split = (pieces + each - 1) / each;
+  return p;
+}
+
 template <typename T, bool FULL, bool LEGAL>
 void policy_rows(const PolicyRows& p, hipStream_t s) {
+  const PolicyRows cut = in_parts<T>(p, 512 * (FULL ? 2 : 4));
   const RowShape r = p.grad ? row_shape<T>(p.columns, p.grad, p.ld_grad, p.rows) : row_shape<T>(p.columns, p.logits, p.ld, p.rows);
   const dim3 waves(row_grid(p.rows, 4)), groups(row_grid(p.rows, 1));
   if (r.threads == 64 && r.each == 2) launch_k(policy_row_kernel<T, 64, 2, FULL, LEGAL>, waves, 256, 0, s, p);
@@ -651,8 +715,12 @@ void policy_rows(const PolicyRows& p, hipStream_t s) {
   // (Float rows over 160 KB on 1024 threads: with four workgroups of 512 a CU, more rows are under way than the caches hold
   // for the second reading: 614 against 477 us with gradient at 2700 x 100000, 431 against 442 at 8192 x 32768. 16-bit rows, half
   // as long, stay on 512: 274 against 292 us.)
-  else if (sizeof(T) == 4 && p.columns > 40960) launch_k(policy_long_kernel<T, 1024, 2, FULL, LEGAL>, groups, 1024, 0, s, p);
-  else launch_k(policy_long_kernel<T, 512, FULL ? 2 : 4, FULL, LEGAL>, groups, 512, 0, s, p);
+  else if (cut.split > 1) {
+    const dim3 parts(p.rows * cut.split);
+    launch_k(policy_long_kernel<T, 512, FULL ? 2 : 4, FULL, LEGAL, PARTS>, parts, 512, 0, s, cut);
+    launch_k(policy_long_kernel<T, 512, FULL ? 2 : 4, FULL, LEGAL, JOIN>, parts, 512, 0, s, cut);
+  } else if (sizeof(T) == 4 && p.columns > 40960) launch_k(policy_long_kernel<T, 1024, 2, FULL, LEGAL, WHOLE>, groups, 1024, 0, s, p);
+  else launch_k(policy_long_kernel<T, 512, FULL ? 2 : 4, FULL, LEGAL, WHOLE>, groups, 512, 0, s, p);
 }
 
 template <typename T>
@@ -923,6 +991,11 @@ bool gradient_past(int rows, int columns, int type) { return (long long)rows * c
 
 }  // namespace
 
+size_t policy_loss_workspace(int rows, int columns) {
+  const int parts = most_parts(rows, columns);
+  return parts > 1 ? (size_t)rows * parts * sizeof(PolicyPart) : 0;
+}
+
 void launch_policy_loss(const kg_policy_loss_args& a, hipStream_t s) {
   PolicyRows p;
   p.logits = a.logits; p.ld = a.ld;
@@ -934,6 +1007,9 @@ void launch_policy_loss(const kg_policy_loss_args& a, hipStream_t s) {
   p.rows = a.rows; p.columns = a.columns;
   p.past = gradient_past(a.rows, a.columns, a.type);
   p.scale = a.logit_scale;
+  p.parts = (PolicyPart*)a.workspace;
+  p.split = 1;
+  p.span = 0;
   p.low = a.clip_low; p.high = a.clip_high;
   p.log_low = log1p(-a.clip_low); p.log_high = log1p(a.clip_high);
   p.kl_coef = (float)a.kl_coef;

@@ -43,7 +43,7 @@ _vp, _ci, _ll, _cd = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_
 
 # The argument structures of include/kgx.h, packed at their natural alignment: a third of a ctypes structure's time, and a small
 # batch's call is its host time.
-_POLICY_ARGS = struct.Struct("@3iPqPqPPPPPqPddddPPPPq0q")
+_POLICY_ARGS = struct.Struct("@3iPqPqPPPPPqPddddPPPPqP0q")
 _PREFERENCE_ARGS = struct.Struct("@3iPqPiPPPddiPPPPqP0q")
 _NORM_ARGS = struct.Struct("@6idPqPPPPPPPqPqPqPP0q")
 
@@ -135,13 +135,17 @@ def policy_loss(logits, actions, old_logp, advantage, *, legal=None, weight=None
         g, ld_g = grad.data_ptr(), v
     loss, logp, kl = torch.empty((3, n), dtype=torch.float32, device=logits.device).unbind()
     o = loss.data_ptr()
+    L = _library()
+    # (Few long rows: 16384 columns are the least that a workspace is for.)
+    bytes_ = L.kg_policy_loss_workspace(n, v) if v > 16384 else 0
+    work = torch.empty(bytes_, dtype=torch.uint8, device=logits.device).data_ptr() if bytes_ else 0
     args = _POLICY_ARGS.pack(n, v, TYPES[logits.dtype], ptr, ld, lg, ld_lg, _vector(actions, n, torch.int32, "actions", dev),
                              _vector(old_logp, n, torch.float32, "old_logp", dev),
                              _vector(advantage, n, torch.float32, "advantage", dev),
                              _vector(weight, n, torch.float32, "weight", dev), ref, ld_ref,
                              _vector(ref_logp, n, torch.float32, "ref_logp", dev), logit_scale, clip[0], clip[1], kl_coef, o,
-                             o + 4 * n, o + 8 * n, g, ld_g)
-    if _library().kg_policy_loss(dev, _stream(dev), args):
+                             o + 4 * n, o + 8 * n, g, ld_g, work)
+    if L.kg_policy_loss(dev, _stream(dev), args):
         _check(1)
     return PolicyLoss(loss, logp, kl, grad)
 

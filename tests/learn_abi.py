@@ -10,7 +10,7 @@ class PolicyArgs(ctypes.Structure):
                 ("ld_legal", _ll), ("action", _vp), ("old_logp", _vp), ("advantage", _vp), ("weight", _vp),
                 ("ref_logits", _vp), ("ld_ref", _ll), ("ref_logp", _vp), ("logit_scale", _cd), ("clip_low", _cd),
                 ("clip_high", _cd), ("kl_coef", _cd), ("loss", _vp), ("logp", _vp), ("kl", _vp), ("grad", _vp),
-                ("ld_grad", _ll)]
+                ("ld_grad", _ll), ("workspace", _vp)]
 
 
 class PreferenceArgs(ctypes.Structure):

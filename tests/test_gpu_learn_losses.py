@@ -106,6 +106,43 @@ def test_policy_loss_widths(learn, v, dtype):
         _policy_case(learn, 5 if v < 5000 else 2, v, dtype, kl, legal, 100 * v + i, ld=v + i, shift=i)
 
 
+@pytest.mark.parametrize("v,dtype,kl,legal", [(16500, torch.float32, "full", True), (41001, torch.float32, "estimate", False),
+                                              (33001, torch.bfloat16, "full", False), (33001, torch.float16, "none", True)])
+def test_policy_loss_many_long_rows(learn, v, dtype, kl, legal):
+    """More long rows than are cut into parts, and one fewer than that."""
+    for n in (257, 256):
+        _policy_case(learn, n, v, dtype, kl, legal, n + v)
+
+
+def test_policy_loss_few_long_rows_captured(learn):
+    """Rows cut into parts, two captured calls with a workspace each, replayed in turn."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    n, v = 3, 70001
+    zs = [torch.randn(n, v, generator=g, device="cuda").bfloat16() for _ in range(3)]
+    refl = torch.randn(n, v, generator=g, device="cuda").bfloat16()
+    act = torch.tensor([5, -1, 70000], dtype=torch.int32, device="cuda")
+    old, adv = torch.full((n,), -11.0, device="cuda"), torch.tensor([1.0, 2.0, -1.0], device="cuda")
+
+    def call(z):
+        return list(learn.policy_loss(z, act, old, adv, kl_coef=0.2, ref_logits=refl))
+
+    want = [[t.clone() for t in call(z)] for z in zs]
+    graphs = []
+    for _ in range(2):
+        buf = zs[0].clone()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = call(buf)
+        graphs.append((gr, buf, out))
+    for k in range(3):
+        for j, (gr, buf, _) in enumerate(graphs):
+            buf.copy_(zs[(k + j) % 3])
+            gr.replay()
+        torch.cuda.synchronize()
+        for j, (_, _, out) in enumerate(graphs):
+            assert all(torch.equal(a, b) for a, b in zip(out, want[(k + j) % 3]))
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_policy_loss_rows_temperature_and_strided_gradient(learn, dtype):
     for n in (1, 3, 4, 61):

@@ -32,6 +32,8 @@ def _policy_args(learn, **change):
     (dict(clip_low=1.0), "clip"), (dict(clip_low=-0.1), "clip"), (dict(clip_high=float("inf")), "clip"),
     (dict(kl_coef=float("nan")), "kl_coef"), (dict(ref_logits=4096, ld_ref=9, ref_logp=4096), "not both"),
     (dict(ref_logits=4096, ld_ref=3), "row stride of ref_logits"), (dict(grad=4096), "overlap"), (dict(ld_grad=1), "row stride of grad"),
+    (dict(columns=20000, ld=20000, ld_grad=20000), "workspace is null"),
+    (dict(columns=20000, ld=20000, ld_grad=20000, workspace=4104), "workspace is not aligned"),
 ])
 def test_policy_loss_refuses(kgx, learn, change, text):
     assert kgx.lib().kg_policy_loss(0, None, ctypes.byref(_policy_args(learn, **change))) == 1
@@ -127,6 +129,8 @@ def test_adamw_values(kgx, learn):
 
 def test_workspaces(kgx):
     L = kgx.lib()
+    assert L.kg_policy_loss_workspace(-1, 100000) == L.kg_policy_loss_workspace(300, 100000) == L.kg_policy_loss_workspace(4, 362) == 0
+    assert L.kg_policy_loss_workspace(1, 100000) >= 64 * 32 and L.kg_policy_loss_workspace(200, 17000) >= 200 * 2 * 32
     assert L.kg_preference_loss_workspace(0) == 0 and L.kg_preference_loss_workspace(-3) == 0
     assert L.kg_preference_loss_workspace(1000) >= 1000 * 20
     assert L.kg_group_norm_workspace(-1, 5, 8, 2, 0) == 0 and L.kg_group_norm_workspace(2, 5, 0, 2, 1) == 0

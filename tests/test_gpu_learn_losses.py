@@ -110,7 +110,7 @@ def test_policy_loss_widths(learn, v, dtype):
                                               (33001, torch.bfloat16, "full", False), (33001, torch.float16, "none", True)])
 def test_policy_loss_many_long_rows(learn, v, dtype, kl, legal):
     """More long rows than are cut into parts, and one fewer than that."""
-    for n in (257, 256):
+    for n in (385, 384):
         _policy_case(learn, n, v, dtype, kl, legal, n + v)
 
 

@@ -129,7 +129,7 @@ def test_adamw_values(kgx, learn):
 
 def test_workspaces(kgx):
     L = kgx.lib()
-    assert L.kg_policy_loss_workspace(-1, 100000) == L.kg_policy_loss_workspace(300, 100000) == L.kg_policy_loss_workspace(4, 362) == 0
+    assert L.kg_policy_loss_workspace(-1, 100000) == L.kg_policy_loss_workspace(400, 100000) == L.kg_policy_loss_workspace(4, 362) == 0
     assert L.kg_policy_loss_workspace(1, 100000) >= 64 * 32 and L.kg_policy_loss_workspace(200, 17000) >= 200 * 2 * 32
     assert L.kg_preference_loss_workspace(0) == 0 and L.kg_preference_loss_workspace(-3) == 0
     assert L.kg_preference_loss_workspace(1000) >= 1000 * 20

@@ -343,7 +343,7 @@ int kg_rmsnorm_rows_of(int rows, int channels, int region, int workgroup, int* g
  * graph, and calls on different streams may overlap as long as their buffers differ. The argument structures are read
  * before the call returns; every pointer in them is memory of `device` unless it says otherwise, aligned to its elements.
  * The caller's current device is left as it was. Outputs must not overlap inputs. Element types are KG_PRECISION_F32, _F16
- * and _BF16; all sums and row statistics are float or wider. Rows have at most 2^30 columns.
+ * and _BF16; all sums and row statistics are float or wider. The losses take at most 2^30 rows of 2^30 columns.
  * ------------------------------------------------------------------------------------------------------------------ */
 
 /* The clipped policy loss with a KL term of `rows` rows of logits, and its gradient. Row i holds `columns` logits z (362
@@ -380,7 +380,8 @@ typedef struct {
   void* grad;                  /* [rows] rows of ld_grad (columns past `columns` stay as they are); or NULL */
   long long ld_grad;
   void* workspace;             /* kg_policy_loss_workspace(rows, columns) bytes, 16-byte aligned, this call's own until it
-                                  has run; NULL where that is 0 (all but few long rows) */
+                                  has run; NULL where that is 0 (all but few long rows, which are cut into parts: their sums are
+                                  added in another order than those of the same rows among many) */
 } kg_policy_loss_args;
 int kg_policy_loss(int device, void* stream, const kg_policy_loss_args* args);
 size_t kg_policy_loss_workspace(int rows, int columns);

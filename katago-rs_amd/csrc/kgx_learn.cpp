@@ -57,11 +57,12 @@ void check_rows(const void* p, long long rows, long long width, long long ld, in
   if (!aligned(p, size_of(type))) bad(op, std::string(name) + " is not aligned to its elements");
 }
 
+constexpr int kMaxRows = 1 << 30;     // a workgroup's step over them stays below 2^31
 constexpr int kMaxColumns = 1 << 30;  // a row's element indices have 31 bits, past its end too
 
 void check_policy(const kg_policy_loss_args& a) {
   const char* op = "policy loss";
-  need(a.rows >= 0 && a.columns >= 1 && a.columns <= kMaxColumns, op, "rows must be at least 0 and columns in [1, 2^30]");
+  need(a.rows >= 0 && a.rows <= kMaxRows && a.columns >= 1 && a.columns <= kMaxColumns, op, "rows must be in [0, 2^30] and columns in [1, 2^30]");
   check_type(a.type, op);
   need(std::isfinite(a.logit_scale) && a.logit_scale > 0, op, "logit_scale must be positive");
   need(finite_at_least(a.clip_low, 0) && a.clip_low < 1 && finite_at_least(a.clip_high, 0), op,
@@ -83,8 +84,8 @@ void check_policy(const kg_policy_loss_args& a) {
 
 void check_preference(const kg_preference_loss_args& a) {
   const char* op = "preference loss";
-  need(a.rows >= 0 && a.columns >= 1 && a.columns <= kMaxColumns && a.pairs >= 0, op,
-       "rows and pairs must be at least 0 and columns in [1, 2^30]");
+  need(a.rows >= 0 && a.rows <= kMaxRows && a.columns >= 1 && a.columns <= kMaxColumns && a.pairs >= 0, op,
+       "rows must be in [0, 2^30], columns in [1, 2^30] and pairs at least 0");
   need(a.pairs <= std::numeric_limits<int>::max() / 2 - 1, op, "too many pairs");
   check_type(a.type, op);
   need(std::isfinite(a.beta) && a.beta > 0, op, "beta must be positive");
@@ -181,9 +182,7 @@ int kg_policy_loss(int device, void* stream, const kg_policy_loss_args* args) {
 
 size_t kg_policy_loss_workspace(int rows, int columns) { return kgx::policy_loss_workspace(rows, columns); }
 
-size_t kg_preference_loss_workspace(int rows) {
-  return rows > 0 ? ((size_t)rows * (sizeof(kgx::PrefRow) + sizeof(float)) + 255) / 256 * 256 : 0;
-}
+size_t kg_preference_loss_workspace(int rows) { return kgx::preference_loss_workspace(rows); }
 
 int kg_preference_loss(int device, void* stream, const kg_preference_loss_args* args) {
   return guarded([&] {

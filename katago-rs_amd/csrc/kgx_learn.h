@@ -17,6 +17,7 @@ struct PrefRow {
   double logp;
   float top, inv_sum;
 };
+size_t preference_loss_workspace(int rows);
 void launch_preference_loss(const kg_preference_loss_args& a, hipStream_t s);
 
 // The AdamW step over `count` tensors, and the moments as numbers.

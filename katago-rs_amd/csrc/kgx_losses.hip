@@ -693,19 +693,23 @@ RowShape row_shape(int columns, const void* p, long long ld, int rows) {
 // KL 88 us whole, 63 in parts; 512 rows 133 and 114, but 27 and 34 of 40001 without a reference.)
 int most_parts(int rows, int columns) { return rows < 1 || rows > 384 || columns <= 16384 ? 1 : std::min(64, 1024 / rows); }
 
-// The parts that a call takes, whole pieces of `piece` chunks each.
+// The parts that a call takes, of whole pieces of `piece` chunks each.
+struct RowParts {
+  int split, span;
+};
 template <typename T>
-PolicyRows in_parts(PolicyRows p, int piece) {
-  const int chunks = (p.columns + kVec<T> - 1) / kVec<T> + Chunks<T>::line(p.columns) / 16, pieces = (chunks + piece - 1) / piece;
-  const int most = std::min(most_parts(p.rows, p.columns), pieces), each = (pieces + most - 1) / most;
-  p.span = each * piece;
-  p.split = (pieces + each - 1) / each;
-  return p;
+RowParts row_parts(int rows, int columns, int piece) {
+  const int chunks = (columns + kVec<T> - 1) / kVec<T> + Chunks<T>::line(columns) / 16, pieces = (chunks + piece - 1) / piece;
+  const int most = std::min(most_parts(rows, columns), pieces), each = (pieces + most - 1) / most;
+  return {(pieces + each - 1) / each, each * piece};
 }
 
 template <typename T, bool FULL, bool LEGAL>
 void policy_rows(const PolicyRows& p, hipStream_t s) {
-  const PolicyRows cut = in_parts<T>(p, 512 * (FULL ? 2 : 4));
+  PolicyRows cut = p;
+  const RowParts parts = row_parts<T>(p.rows, p.columns, 512 * (FULL ? 2 : 4));
+  cut.split = parts.split;
+  cut.span = parts.span;
   const RowShape r = p.grad ? row_shape<T>(p.columns, p.grad, p.ld_grad, p.rows) : row_shape<T>(p.columns, p.logits, p.ld, p.rows);
   const dim3 waves(row_grid(p.rows, 4)), groups(row_grid(p.rows, 1));
   if (r.threads == 64 && r.each == 2) launch_k(policy_row_kernel<T, 64, 2, FULL, LEGAL>, waves, 256, 0, s, p);
@@ -717,9 +721,9 @@ void policy_rows(const PolicyRows& p, hipStream_t s) {
   // for the second reading: 614 against 477 us with gradient at 2700 x 100000, 431 against 442 at 8192 x 32768. 16-bit rows, half
   // as long, stay on 512: 274 against 292 us.)
   else if (cut.split > 1) {
-    const dim3 parts(p.rows * cut.split);
-    launch_k(policy_long_kernel<T, 512, FULL ? 2 : 4, FULL, LEGAL, PARTS>, parts, 512, 0, s, cut);
-    launch_k(policy_long_kernel<T, 512, FULL ? 2 : 4, FULL, LEGAL, JOIN>, parts, 512, 0, s, cut);
+    const dim3 grid(p.rows * cut.split);
+    launch_k(policy_long_kernel<T, 512, FULL ? 2 : 4, FULL, LEGAL, PARTS>, grid, 512, 0, s, cut);
+    launch_k(policy_long_kernel<T, 512, FULL ? 2 : 4, FULL, LEGAL, JOIN>, grid, 512, 0, s, cut);
   } else if (sizeof(T) == 4 && p.columns > 40960) launch_k(policy_long_kernel<T, 1024, 2, FULL, LEGAL, WHOLE>, groups, 1024, 0, s, p);
   else launch_k(policy_long_kernel<T, 512, FULL ? 2 : 4, FULL, LEGAL, WHOLE>, groups, 512, 0, s, p);
 }
@@ -735,6 +739,11 @@ void policy_typed(const PolicyRows& p, hipStream_t s) {
   }
 }
 
+// The sum over a part of a row, relative to the part's maximum.
+struct PrefPart {
+  double sum;
+  float top, none;
+};
 struct PrefRows {
   const void* logits;
   void* grad;
@@ -743,6 +752,8 @@ struct PrefRows {
   const float *ref_logp, *weight;
   PrefRow* row;
   float* coef;
+  PrefPart* parts;  // rows cut into `split` parts of `span` chunks (1: not cut)
+  int split, span;
   float *loss, *margin, *seq_logp;
   int rows, columns, past, pairs, average;
   double beta, smooth;
@@ -805,22 +816,25 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void pref_rows_held_kernel(Pre
 
 // The same for longer rows, E chunks of each thread at a time relative to the running maximum. (Held by 1024 threads in 16
 // chunks each, such a row has a CU to itself, whose loads and exponentials wait for each other: 297 us for 2430 rows of
-// 100003 f16, against 116 here.)
-template <typename T, int NT, int E>
+// 100003 f16, against 116 here.) PARTS: few such rows in parts, with the label's logit in logp's place until pref_pairs_kernel
+// joins them.
+template <typename T, int NT, int E, bool PARTS>
 __global__ __launch_bounds__(NT) void pref_rows_long_kernel(PrefRows a) {
   constexpr int V = kVec<T>;
   __shared__ float red[16];
   const int tid = threadIdx.x;
   const int first = a.offsets[0], last = a.offsets[2 * a.pairs];
   const Base2 c2(1.0);
-  for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
+  for (int id = blockIdx.x; id < a.rows * (PARTS ? a.split : 1); id += gridDim.x) {
+    const int row = PARTS ? id / a.split : id, part = PARTS ? id - row * a.split : 0;
+    const int begin = part * a.span, end = PARTS ? begin + a.span : INT_MAX;  // its chunks
     const int label = a.label[row];
-    if (tid == 0) a.coef[row] = 0.f;
+    if (tid == 0 && part == 0) a.coef[row] = 0.f;
     if (row < first || row >= last || (unsigned)label >= (unsigned)a.columns) continue;
     const T* z = (const T*)a.logits + (size_t)row * a.ld;
     const Chunks<T> at(a.columns, z);
     Running run;
-    for (int c0 = 0; !at.none(c0); c0 += NT * E) {
+    for (int c0 = begin; c0 < end && !at.none(c0); c0 += NT * E) {
       u32x4 raw[E];
       load_row<T, NT, E>(z, tid, at, raw, c0);
       remove_past<T, NT, E>(tid, at, raw, c0);
@@ -837,6 +851,11 @@ __global__ __launch_bounds__(NT) void pref_rows_long_kernel(PrefRows a) {
     run.join<NT>(c2, red, moved);
     if (tid == 0) {
       const float za = (float)z[label];
+      if constexpr (PARTS) {
+        a.parts[id] = PrefPart{run.total, run.top, 0.f};
+        if (part == 0) a.row[row].logp = (double)za;
+        continue;
+      }
       a.row[row] = PrefRow{za == -INFINITY ? -(double)INFINITY : (double)za - (double)run.top - log_sum(run.total), run.top,
                            (float)(1.0 / run.total)};
     }
@@ -844,6 +863,20 @@ __global__ __launch_bounds__(NT) void pref_rows_long_kernel(PrefRows a) {
 }
 
 constexpr int PT = 512;  // threads of a pair's workgroup
+// Preference rows cut into parts: 2 rows of 125123 f16 31 -> 14 us, 64 of 100003 bf16 32 -> 20, but 256 of them 37.5 -> 39.
+constexpr int kPrefPartRows = 128;
+
+// A row's results from its parts.
+__device__ __forceinline__ PrefRow joined(const PrefRows& a, int row) {
+  const PrefPart* q = a.parts + row * a.split;
+  const Base2 c2(1.0);
+  const double za = a.row[row].logp;
+  float top = -INFINITY;
+  for (int k = 0; k < a.split; k++) top = fmaxf(top, q[k].top);
+  double sum = 0.0;
+  for (int k = 0; k < a.split; k++) sum += q[k].sum * (double)(q[k].top == -INFINITY ? 0.f : exp_of(q[k].top - top, c2));
+  return PrefRow{za == -(double)INFINITY ? za : za - (double)top - log_sum(sum), top, (float)(1.0 / sum)};
+}
 
 // One workgroup a pair: the sequences' sums in a fixed order, the loss, and the factor of each counted row's gradient.
 __global__ __launch_bounds__(PT) void pref_pairs_kernel(PrefRows a) {
@@ -861,6 +894,7 @@ __global__ __launch_bounds__(PT) void pref_pairs_kernel(PrefRows a) {
       for (int t = at[q] + tid; t < at[q + 1]; t += PT) {
         // (Every row's place is the workspace's own: read whether it counts or not, so that the loads run ahead.)
         const bool counted = (unsigned)a.label[t] < (unsigned)a.columns;
+        if (counted && a.split > 1) a.row[t] = joined(a, t);
         const double lp = a.row[t].logp;
         sum[q] += counted ? lp : 0.0;
         count[q] += counted;
@@ -914,7 +948,8 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void pref_grad_kernel(PrefRows
   const int tid = threadIdx.x % NT;
   // (Cut to the rows, so that each row comes once.)
   const int last = min(max(a.offsets[2 * a.pairs], 0), a.rows), first = min(max(a.offsets[0], 0), last);
-  for (int r = blockIdx.x * PER + wave_row<NT>(); r < a.rows; r += gridDim.x * PER) {
+  for (int id = blockIdx.x * PER + wave_row<NT>(); id < a.rows * a.split; id += gridDim.x * PER) {
+    const int r = id / a.split, begin = (id - r * a.split) * a.span, end = a.split > 1 ? begin + a.span : INT_MAX;
     const int row = r < last - first ? last - 1 - r : r - (last - first) < first ? r - (last - first) : r;
     const int label = a.label[row];
     const bool counted = row >= first && row < last && (unsigned)label < (unsigned)a.columns;
@@ -928,7 +963,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void pref_grad_kernel(PrefRows
       f = -hot * a.row[row].inv_sum;
     }
     const int hot_chunk = counted ? at.of(label) : -1;
-    for (int c0 = 0; !at.none(c0); c0 += NT * E) {
+    for (int c0 = begin; c0 < end && !at.none(c0); c0 += NT * E) {
       u32x4 raw[E];
       if (counted) load_row<T, NT, E>(z, tid, at, raw, c0);
 #pragma unroll
@@ -967,7 +1002,7 @@ __global__ __launch_bounds__(256) void pref_grad_short_kernel(PrefRows a) {
 }
 
 template <typename T>
-void pref_typed(const PrefRows& p, hipStream_t s) {
+void pref_typed(PrefRows p, hipStream_t s) {
   const dim3 waves(row_grid(p.rows, 4)), groups(row_grid(p.rows, 1));
   const bool tiny = p.columns < kVec<T>;  // rows shorter than a chunk
   if (p.rows > 0) {
@@ -977,14 +1012,22 @@ void pref_typed(const PrefRows& p, hipStream_t s) {
     else if (r.threads == 256) launch_k(pref_rows_held_kernel<T, 256, 8>, groups, 256, 0, s, p);
     else if (r.threads == 512) launch_k(pref_rows_held_kernel<T, 512, 8>, groups, 512, 0, s, p);
     else if (tiny) launch_k(pref_rows_short_kernel<T>, waves, 256, 0, s, p);
-    else launch_k(pref_rows_long_kernel<T, 512, 4>, groups, 512, 0, s, p);
+    else {
+      if (p.rows <= kPrefPartRows) {
+        const RowParts cut = row_parts<T>(p.rows, p.columns, 512 * 4);
+        p.split = cut.split;
+        p.span = cut.span;
+      }
+      if (p.split > 1) launch_k(pref_rows_long_kernel<T, 512, 4, true>, dim3(p.rows * p.split), 512, 0, s, p);
+      else launch_k(pref_rows_long_kernel<T, 512, 4, false>, groups, 512, 0, s, p);
+    }
   }
   if (p.pairs > 0) launch_k(pref_pairs_kernel, dim3(p.pairs < 65536 ? p.pairs : 65536), PT, 0, s, p);
   if (p.rows > 0 && p.grad) {
     if (tiny) launch_k(pref_grad_short_kernel<T>, dim3(row_grid(p.rows, 32)), 256, 0, s, p);
     else if (p.columns <= 512 * kVec<T>) launch_k(pref_grad_kernel<T, 64, 4>, waves, 256, 0, s, p);
     else if (p.columns <= 2048 * kVec<T>) launch_k(pref_grad_kernel<T, 256, 4>, groups, 256, 0, s, p);
-    else launch_k(pref_grad_kernel<T, 512, 4>, groups, 512, 0, s, p);
+    else launch_k(pref_grad_kernel<T, 512, 4>, dim3(row_grid(p.rows * p.split, 1)), 512, 0, s, p);
   }
 }
 
@@ -1022,6 +1065,14 @@ void launch_policy_loss(const kg_policy_loss_args& a, hipStream_t s) {
   KGX_CHECK_LAUNCH();
 }
 
+// The parts' place in the workspace, behind the rows' results and factors.
+size_t pref_parts_at(int rows) { return ((size_t)rows * (sizeof(PrefRow) + sizeof(float)) + 15) / 16 * 16; }
+size_t preference_loss_workspace(int rows) {
+  if (rows < 1) return 0;
+  const int parts = rows <= kPrefPartRows ? most_parts(rows, INT_MAX) : 1;
+  return (pref_parts_at(rows) + (parts > 1 ? (size_t)rows * parts * sizeof(PrefPart) : 0) + 255) / 256 * 256;
+}
+
 void launch_preference_loss(const kg_preference_loss_args& a, hipStream_t s) {
   PrefRows p;
   p.logits = a.logits; p.ld = a.ld;
@@ -1029,6 +1080,9 @@ void launch_preference_loss(const kg_preference_loss_args& a, hipStream_t s) {
   p.label = a.label; p.offsets = a.offsets; p.ref_logp = a.ref_logp; p.weight = a.weight;
   p.row = (PrefRow*)a.workspace;
   p.coef = (float*)(p.row + a.rows);
+  p.parts = (PrefPart*)((char*)a.workspace + pref_parts_at(a.rows));
+  p.split = 1;
+  p.span = 0;
   p.loss = a.loss; p.margin = a.margin; p.seq_logp = a.seq_logp;
   p.rows = a.rows; p.columns = a.columns; p.pairs = a.pairs; p.average = a.average;
   p.past = gradient_past(a.rows, a.columns, a.type);

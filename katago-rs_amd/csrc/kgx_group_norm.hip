@@ -1083,7 +1083,7 @@ __global__ __launch_bounds__(1024) void norm_back_params_kernel(NormArgs a, int 
 struct SlabShape {
   int groups = 0, threads = 0, each = 0, splits = 1;
 };
-SlabShape slab_shape(int points, int groups, int width, int vec) {
+SlabShape slab_shape(int points, int groups, int width, int vec, int batch) {
   SlabShape best;
   if (points < 1 || width < 1) return best;
   for (int sg = 1; sg <= groups; sg++) {
@@ -1096,6 +1096,14 @@ SlabShape slab_shape(int points, int groups, int width, int vec) {
     // 768 threads, where 1024 threads left a third of the work to empty points).
     best = {sg, std::max(round_up((points + each - 1) / each * cols, 64), round_up(w, 64)), each, 1};
     if (w >= 4 * vec) break;
+  }
+  // Where there are more workgroups than CUs, four points a thread rather than one or two: smaller workgroups, more of them at once
+  // on a CU. 143 x 194 points of 864 bf16 channels in 24 groups 110 -> 28 us and backward 108 -> 33; 512 boards of 361 x 128 f32 in 8
+  // groups 59 -> 40 and 78 -> 57. (Three points stay: 128 boards of 361 x 384 bf16 with mish backward 45 us, 59 with four.)
+  if (best.groups && best.each < 3 && (long long)batch * (groups / best.groups) > kCUs) {
+    const int w = best.groups * width, cols = (w + vec - 1) / vec;
+    best.each = std::min(4, points);
+    best.threads = std::max(round_up((points + best.each - 1) / best.each * cols, 64), round_up(w, 64));
   }
   if (best.groups) return best;
   for (int sg = 1; sg <= groups; sg++) {
@@ -1111,7 +1119,7 @@ SlabShape slab_shape(int points, int groups, int width, int vec) {
 }
 // The same for a call: byte offsets within a share have 31 bits.
 SlabShape slab_shape(const NormArgs& n, int size) {
-  const SlabShape f = slab_shape(n.points, n.groups, n.width, 16 / size);
+  const SlabShape f = slab_shape(n.points, n.groups, n.width, 16 / size, n.batch);
   const long long ld = std::max(std::max(n.ldx, n.ldy), std::max(n.lddy, n.lddx));
   const long long share = f.splits == 1 ? n.points : 8 * 1024;
   return share * ld < (1ll << 31) / size ? f : SlabShape();
@@ -1223,7 +1231,7 @@ int group_norm_splits(int batch, int points, int channels) {
 // For any type and strides: the most shares that one of the ways to run it takes.
 size_t group_norm_workspace(int batch, int points, int channels, int groups, bool backward) {
   int splits = group_norm_splits(batch, points, channels);
-  for (int vec = 4; vec <= 8; vec += 4) splits = std::max(splits, slab_shape(points, groups, channels / groups, vec).splits);
+  for (int vec = 4; vec <= 8; vec += 4) splits = std::max(splits, slab_shape(points, groups, channels / groups, vec, batch).splits);
   const size_t parts = (size_t)batch * splits;
   const size_t floats = parts * (backward ? 2 * ((size_t)channels + groups) + 1 : 3 * (size_t)groups) + (backward ? (size_t)batch * 2 * groups : 0);
   return (floats * 4 + 255) / 256 * 256;

@@ -90,7 +90,9 @@ SHAPES = [(1, 1, 1, 1), (2, 1, 8, 2), (3, 5, 3, 3), (2, 361, 384, 32), (3, 361, 
           (5, 33, 1024, 64), (2, 9, 2056, 8), (1, 40, 4100, 1), (1, 13, 2048, 2048), (2, 4096, 16, 2), (1, 9001, 2, 1), (70, 7, 30, 3),
           (2, 50, 96, 96), (1, 20011, 7, 7),
           # Rows in shares, columns that are not whole, groups wider than a share's workgroup joins.
-          (2, 5000, 96, 4), (1, 12001, 45, 3), (2, 16385, 33, 1), (1, 30000, 20, 4), (2, 700, 500, 1), (2, 700, 1000, 1), (3, 50, 17, 1)]
+          (2, 5000, 96, 4), (1, 12001, 45, 3), (2, 16385, 33, 1), (1, 30000, 20, 4), (2, 700, 500, 1), (2, 700, 1000, 1), (3, 50, 17, 1),
+          # More workgroups than CUs: four points a thread.
+          (40, 37, 189, 21), (300, 3, 33, 1), (270, 1, 40, 2)]
 
 
 @pytest.mark.parametrize("shape", SHAPES)

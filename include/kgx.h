@@ -371,7 +371,7 @@ typedef struct {
   const void* ref_logits;      /* [rows] rows of ld_ref, under the same legality and scale; or NULL */
   long long ld_ref;
   const float* ref_logp;       /* [rows] or NULL (not with ref_logits) */
-  double logit_scale;          /* 1 / temperature, > 0 */
+  double logit_scale;          /* 1 / temperature, in [2^-64, 2^64] */
   double clip_low, clip_high;  /* >= 0, clip_low < 1 */
   double kl_coef;
   float* loss;                 /* [rows] */

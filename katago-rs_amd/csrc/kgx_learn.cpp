@@ -64,7 +64,7 @@ void check_policy(const kg_policy_loss_args& a) {
   const char* op = "policy loss";
   need(a.rows >= 0 && a.rows <= kMaxRows && a.columns >= 1 && a.columns <= kMaxColumns, op, "rows must be in [0, 2^30] and columns in [1, 2^30]");
   check_type(a.type, op);
-  need(std::isfinite(a.logit_scale) && a.logit_scale > 0, op, "logit_scale must be positive");
+  need(a.logit_scale >= 0x1p-64 && a.logit_scale <= 0x1p64, op, "logit_scale must be positive, in [2^-64, 2^64]");
   need(finite_at_least(a.clip_low, 0) && a.clip_low < 1 && finite_at_least(a.clip_high, 0), op,
        "clip_low must be in [0, 1) and clip_high at least 0");
   need(std::isfinite(a.kl_coef), op, "kl_coef must be finite");

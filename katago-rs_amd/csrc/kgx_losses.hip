@@ -78,16 +78,22 @@ __device__ __forceinline__ double log_sum(double s) {
   return __builtin_fma((double)k, 0.69314718055994530942, 2.0 * t * p);
 }
 
-// s log2 e in two floats: the first alone is off by up to 2^-25, relative, the same way in every term of a row. A sequence's
+// s log2 e in two floats: the first alone is off by up to 2^-23, relative, the same way in every term of a row. A sequence's
 // log-probability sums that error over its rows, and the margin is a small difference of such sums (0.15 of 5000 in a case of
-// 500 tokens: the margin was off by 7e-6, with both parts by 4e-7).
+// 500 tokens: the margin was off by 7e-6, with both parts by 4e-7). The first is the largest float below the product, so that the
+// second is positive: both products of -infinity, which stands in every place that takes no part, are then -infinity, and never
+// infinity less infinity. (s is in [2^-64, 2^64]: neither part is subnormal.) The gradients, which no sum takes further, make do
+// with the first part: off by up to 2^-23 X of a probability that lies X octaves below the row's largest.
 struct Base2 {
   float hi, lo;
   __device__ __forceinline__ explicit Base2(double s) {
-    hi = (float)(s * 1.44269504088896340736);
-    lo = (float)(s * 1.44269504088896340736 - (double)hi);
+    const double all = s * 1.44269504088896340736;
+    hi = (float)all;
+    if ((double)hi >= all) hi = __uint_as_float(__float_as_uint(hi) - 1);
+    lo = (float)(all - (double)hi);
   }
 };
+// (0 below 2^-126: the hardware's exponential gives no subnormal numbers.)
 __device__ __forceinline__ float exp_of(float x, Base2 c) {
   return __builtin_amdgcn_exp2f(__builtin_fmaf(x, c.hi, x * c.lo));
 }

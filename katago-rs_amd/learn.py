@@ -110,6 +110,12 @@ def _vector(t, n, dtype, name, device):
     return t.data_ptr()
 
 
+def _workspace(size, device):
+    """A call's workspace, None for 0 bytes. The caller holds it until the library has been called: memory that goes back to the
+    allocator before that is another thread's to take, with kernels of its own between this call's."""
+    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+
+
 def policy_loss(logits, actions, old_logp, advantage, *, legal=None, weight=None, logit_scale=1.0, clip=(0.2, 0.2),
                 kl_coef=0.0, ref_logits=None, ref_logp=None, want_grad=True, grad=None):
     """The clipped policy loss of each row with its KL term, and the gradient of their sum (kg_policy_loss).
@@ -138,13 +144,13 @@ def policy_loss(logits, actions, old_logp, advantage, *, legal=None, weight=None
     L = _library()
     # (Few long rows: 16384 columns are the least that a workspace is for.)
     bytes_ = L.kg_policy_loss_workspace(n, v) if v > 16384 else 0
-    work = torch.empty(bytes_, dtype=torch.uint8, device=logits.device).data_ptr() if bytes_ else 0
+    work = _workspace(bytes_, logits.device)
     args = _POLICY_ARGS.pack(n, v, TYPES[logits.dtype], ptr, ld, lg, ld_lg, _vector(actions, n, torch.int32, "actions", dev),
                              _vector(old_logp, n, torch.float32, "old_logp", dev),
                              _vector(advantage, n, torch.float32, "advantage", dev),
                              _vector(weight, n, torch.float32, "weight", dev), ref, ld_ref,
                              _vector(ref_logp, n, torch.float32, "ref_logp", dev), logit_scale, clip[0], clip[1], kl_coef, o,
-                             o + 4 * n, o + 8 * n, g, ld_g, work)
+                             o + 4 * n, o + 8 * n, g, ld_g, work.data_ptr() if work is not None else 0)
     if L.kg_policy_loss(dev, _stream(dev), args):
         _check(1)
     return PolicyLoss(loss, logp, kl, grad)
@@ -242,12 +248,11 @@ def group_norm(x, groups, gamma=None, beta=None, *, mask=None, eps=1e-5, act="id
         yp, ldy = _like(y, x, "y")
     L = _library()
     stats = torch.empty((2, b, max(g, 0)), dtype=torch.float32, device=x.device)
-    bytes_ = L.kg_group_norm_workspace(b, p, c, g, 0)
-    work = torch.empty(bytes_, dtype=torch.uint8, device=x.device).data_ptr() if bytes_ else 0
+    work = _workspace(L.kg_group_norm_workspace(b, p, c, g, 0), x.device)
     mean, rstd = stats.unbind()
     o = stats.data_ptr()
-    args = _NORM_ARGS.pack(b, p, c, g, TYPES[x.dtype], ACTS[act], eps, ptr, ld, mk, gm, bt, o, o + 4 * b * g, work, yp, ldy, 0, 0,
-                           0, 0, 0, 0)
+    args = _NORM_ARGS.pack(b, p, c, g, TYPES[x.dtype], ACTS[act], eps, ptr, ld, mk, gm, bt, o, o + 4 * b * g,
+                           work.data_ptr() if work is not None else 0, yp, ldy, 0, 0, 0, 0, 0, 0)
     if L.kg_group_norm(dev, _stream(dev), args):
         _check(1)
     return y, mean, rstd
@@ -268,13 +273,12 @@ def group_norm_backward(dy, x, mean, rstd, groups, gamma=None, beta=None, *, mas
         if t.dtype is not torch.float32 or t.shape != (b, g) or t.get_device() != dev or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous float32 of shape ({b}, {g}) on GPU {dev}")
     L = _library()
-    bytes_ = L.kg_group_norm_workspace(b, p, c, g, 1)
-    work = torch.empty(bytes_, dtype=torch.uint8, device=x.device).data_ptr() if bytes_ else 0
+    work = _workspace(L.kg_group_norm_workspace(b, p, c, g, 1), x.device)
     out = torch.empty((2, c), dtype=torch.float32, device=x.device)
     dgamma, dbeta = out.unbind()
     o = out.data_ptr()
     args = _NORM_ARGS.pack(b, p, c, g, TYPES[x.dtype], ACTS[act], 0.0, ptr, ld, mk, gm, bt, mean.data_ptr(), rstd.data_ptr(),
-                           work, 0, 0, dyp, lddy, dxp, lddx, o, o + 4 * c)
+                           work.data_ptr() if work is not None else 0, 0, 0, dyp, lddy, dxp, lddx, o, o + 4 * c)
     if L.kg_group_norm_backward(dev, _stream(dev), args):
         _check(1)
     return dx, dgamma, dbeta

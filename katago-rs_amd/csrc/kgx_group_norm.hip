@@ -102,8 +102,11 @@ struct Cover {
 };
 
 // Forward, first launch: count, mean and sum of squared deviations of every group over the workgroup's points. A thread
-// sums each of its channels relative to the first value that it meets (no cancellation for a mean far from 0); the
-// parts are joined pairwise exactly: M2 = sum M2_i + n_i (mean_i - mean)^2.
+// takes kPiece points at a time relative to the mean of its points so far (of the first piece: to its first value), s1 and s2 their sum
+// and sum of squares: M2 grows by s2 - s1^2 / n. A mean far from 0 does not cancel, and one value far from the rest only within
+// a piece (relative to the first value throughout, 3906 points with such a first one left 7 % of an error). The parts are joined
+// pairwise exactly: M2 = sum M2_i + n_i (mean_i - mean)^2.
+constexpr int kPiece = 16;
 template <typename T>
 __global__ __launch_bounds__(GT) void norm_stats_kernel(NormArgs a) {
   constexpr int V = kVec<T>;
@@ -117,35 +120,47 @@ __global__ __launch_bounds__(GT) void norm_stats_kernel(NormArgs a) {
   for (int first = 0; first < total; first += GT) {
     const Cover w(total, first);
     const int c0 = (first + w.col) * V, left = a.channels - c0;
-    float pivot[V], s1[V], s2[V], n = 0.f;
+    float mean[V], m2[V], n = 0.f;
 #pragma unroll
-    for (int j = 0; j < V; j++) pivot[j] = s1[j] = s2[j] = 0.f;
+    for (int j = 0; j < V; j++) mean[j] = m2[j] = 0.f;
     if (w.lane < w.lanes) {
       const T* x = (const T*)a.x + (size_t)b * a.points * a.ldx + c0;
-      for (int p = p0 + w.lane; p < p1; p += w.lanes) {
-        if (a.mask && a.mask[(size_t)b * a.points + p] == 0.f) continue;
-        float f[V];
-        load_vec<T>(x + (size_t)p * a.ldx, left, f);
-        if (n == 0.f) {
+      for (int p = p0 + w.lane; p < p1;) {
+        float s1[V], s2[V];
+        const float before = n;
 #pragma unroll
-          for (int j = 0; j < V; j++) pivot[j] = f[j];
+        for (int j = 0; j < V; j++) s1[j] = s2[j] = 0.f;
+        for (int i = 0; i < kPiece && p < p1; i++, p += w.lanes) {
+          if (a.mask && a.mask[(size_t)b * a.points + p] == 0.f) continue;
+          float f[V];
+          load_vec<T>(x + (size_t)p * a.ldx, left, f);
+          if (n == 0.f) {
+#pragma unroll
+            for (int j = 0; j < V; j++) mean[j] = f[j];
+          }
+          n += 1.f;
+#pragma unroll
+          for (int j = 0; j < V; j++) {
+            const float d = f[j] - mean[j];
+            s1[j] += d;
+            s2[j] = __builtin_fmaf(d, d, s2[j]);
+          }
         }
-        n += 1.f;
+        if (n == before) continue;
+        const float inv = 1.f / n;
 #pragma unroll
         for (int j = 0; j < V; j++) {
-          const float d = f[j] - pivot[j];
-          s1[j] += d;
-          s2[j] = __builtin_fmaf(d, d, s2[j]);
+          const float up = s1[j] * inv;
+          m2[j] += fmaxf(__builtin_fmaf(-s1[j], up, s2[j]), 0.f);
+          mean[j] += up;
         }
       }
     }
-    const float inv = n > 0.f ? 1.f / n : 0.f;
     s_n[tid] = n;
 #pragma unroll
     for (int j = 0; j < V; j++) {
-      const float mean = s1[j] * inv;
-      s_mean[j * GT + tid] = pivot[j] + mean;
-      s_m2[j * GT + tid] = fmaxf(__builtin_fmaf(-s1[j], mean, s2[j]), 0.f);
+      s_mean[j * GT + tid] = mean[j];
+      s_m2[j * GT + tid] = m2[j];
     }
     __syncthreads();
     // Groups with channels in this column block: 256 / share groups at a time, `share` threads each.

@@ -143,13 +143,28 @@ __device__ __forceinline__ int exp_of(unsigned top, unsigned carry, int least) {
 }
 
 // The correctly rounded root: the hardware's (an ulp), or the neighbour below or above it by the sign of what their product with
-// it leaves of v. 0, infinity and NaN keep the hardware's: every comparison fails. (Without the scaling of arguments below
-// 2^-96, whose roots are nothing beside any eps: seven of nineteen operations.)
+// it leaves of v. 0, infinity and NaN keep the hardware's: every comparison fails. Below 2^-96 what they leave underflows, and the
+// hardware takes subnormal numbers for 0: those are scaled by 2^64 first, their roots by 2^-32. (Few steps have one, so the four of
+// a lane are tested together, for scaling each argument would be seven of nineteen operations.)
 __device__ __forceinline__ float root_of(float v) {
   const float s = __builtin_amdgcn_sqrtf(v);
   const float below = __uint_as_float(__float_as_uint(s) - 1), above = __uint_as_float(__float_as_uint(s) + 1);
   float r = __builtin_fmaf(-below, s, v) <= 0.f ? below : s;
   return __builtin_fmaf(-above, s, v) > 0.f ? above : r;
+}
+__device__ __forceinline__ floatx4 roots_of(const floatx4& v) {
+  floatx4 r;
+  unsigned least = ~0u;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    r[j] = root_of(v[j]);
+    least = min(least, __float_as_uint(v[j]) - 1);  // (0 needs no scaling)
+  }
+  if (least < __float_as_uint(0x1p-96f) - 1) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) r[j] = v[j] < 0x1p-96f ? root_of(v[j] * 0x1p64f) * 0x1p-32f : r[j];
+  }
+  return r;
 }
 
 constexpr int M_BIAS = 135, M_LEAST = 9, V_BIAS = 138, V_LEAST = 12;
@@ -237,7 +252,6 @@ __device__ __forceinline__ void adamw_chunk(const AdamArgs& a, const AdamTensor&
         v[u][j] = r * r;
       }
     }
-    floatx4 root;
     unsigned mtop = 0, vtop = 0;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -245,7 +259,10 @@ __device__ __forceinline__ void adamw_chunk(const AdamArgs& a, const AdamTensor&
       m[u][j] = m[u][j] * h.beta1 + gj * h.beta1_rest;
       v[u][j] = v[u][j] * h.beta2 + gj * gj * h.beta2_rest;
       if (!WHOLE && i + j >= t.elements) m[u][j] = v[u][j] = 0.f;
-      root[j] = root_of(v[u][j]);
+    }
+    const floatx4 root = roots_of(v[u]);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
       // (The quotient by the hardware's reciprocal: an ulp of the update, where the parameter keeps an ulp of itself.)
       p[u][j] = p[u][j] * decay - h.step_size * m[u][j] * __builtin_amdgcn_rcpf(root[j] * h.root_scale + h.eps);
       mtop = max(mtop, __float_as_uint(m[u][j]) & 0x7fffffffu);

@@ -446,7 +446,7 @@ typedef struct {
   int param_type, grad_type;
 } kg_adamw_tensor;
 typedef struct {
-  double lr, beta1, beta2, eps;
+  double lr, beta1, beta2, eps;  /* all finite as floats, also lr / (1 - beta1^step); betas in [0, 1), eps >= 2^-126 */
   double grad_scale;
   long long step;          /* from 1 */
   unsigned seed;           /* state_bits 8 */
@@ -487,7 +487,7 @@ typedef struct {
   int batch, points, channels, groups;
   int type;                /* of x, y, dy and dx */
   int act;
-  double eps;              /* > 0 */
+  double eps;              /* >= 2^-126 */
   const void* x;
   long long ldx;
   const float* mask;       /* [batch][points] or NULL */

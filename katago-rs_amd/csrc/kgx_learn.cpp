@@ -48,6 +48,9 @@ void check_type(int type, const char* op) {
 bool aligned(const void* p, size_t to) { return ((uintptr_t)p) % to == 0; }
 size_t size_of(int type) { return type == KG_PRECISION_F32 ? 4 : 2; }
 bool finite_at_least(double v, double least) { return std::isfinite(v) && v >= least; }
+bool finite_float(double v) { return std::isfinite((float)v); }
+// An eps whose reciprocal, and the square of whose root's, are finite floats.
+bool usable_eps(double v) { return v >= (double)std::numeric_limits<float>::min() && finite_float(v); }
 
 // A matrix of `rows` rows of `width` elements, `ld` apart.
 void check_rows(const void* p, long long rows, long long width, long long ld, int type, const char* op, const char* name) {
@@ -67,7 +70,7 @@ void check_policy(const kg_policy_loss_args& a) {
   need(a.logit_scale >= 0x1p-64 && a.logit_scale <= 0x1p64, op, "logit_scale must be positive, in [2^-64, 2^64]");
   need(finite_at_least(a.clip_low, 0) && a.clip_low < 1 && finite_at_least(a.clip_high, 0), op,
        "clip_low must be in [0, 1) and clip_high at least 0");
-  need(std::isfinite(a.kl_coef), op, "kl_coef must be finite");
+  need(finite_float(a.kl_coef), op, "kl_coef must be finite in float");
   need(!(a.ref_logits && a.ref_logp), op, "give ref_logits or ref_logp, not both");
   if (!a.rows) return;
   check_rows(a.logits, a.rows, a.columns, a.ld, a.type, op, "logits");
@@ -109,13 +112,16 @@ void check_state(const kg_adamw_state& s, const char* op) {
   else need(aligned(s.m, 4) && aligned(s.v, 4), op, "the moments are not aligned to their elements");
 }
 
+double step_size(const kg_adamw_hyper& h) { return h.lr / (1.0 - std::pow(h.beta1, (double)h.step)); }
+
 void check_hyper(const kg_adamw_hyper& h) {
   const char* op = "AdamW";
-  need(std::isfinite(h.lr), op, "lr must be finite");
+  need(finite_float(h.lr), op, "lr must be finite in float");
   need(h.beta1 >= 0 && h.beta1 < 1 && h.beta2 >= 0 && h.beta2 < 1, op, "beta1 and beta2 must be in [0, 1)");
-  need(std::isfinite(h.eps) && h.eps > 0 && (float)h.eps > 0, op, "eps must be positive");
-  need(std::isfinite(h.grad_scale), op, "grad_scale must be finite");
+  need(usable_eps(h.eps), op, "eps must be positive, at least 2^-126");
+  need(finite_float(h.grad_scale), op, "grad_scale must be finite in float");
   need(h.step >= 1, op, "step counts from 1");
+  need(finite_float(step_size(h)), op, "lr / (1 - beta1^step) must be finite in float");
 }
 
 kg_adamw_values_t values_of(const kg_adamw_hyper& h) {
@@ -128,7 +134,7 @@ kg_adamw_values_t values_of(const kg_adamw_hyper& h) {
   v.beta2_rest = (float)(1.0 - h.beta2);
   v.eps = (float)h.eps;
   v.grad_scale = (float)h.grad_scale;
-  v.step_size = (float)(h.lr / (1.0 - std::pow(h.beta1, t)));
+  v.step_size = (float)step_size(h);
   v.root_scale = (float)(1.0 / std::sqrt(1.0 - std::pow(h.beta2, t)));
   v.seed = h.seed;
   return v;
@@ -146,7 +152,7 @@ void check_norm(const kg_group_norm_args& a, bool backward) {
   check_type(a.type, op);
   need(a.act >= KG_ACT_IDENTITY && a.act <= KG_ACT_SILU, op, "unknown activation");
   const long long rows = (long long)a.batch * a.points;
-  if (!backward) need(std::isfinite(a.eps) && (float)a.eps > 0, op, "eps must be positive");
+  if (!backward) need(usable_eps(a.eps), op, "eps must be positive, at least 2^-126");
   if (a.batch) need(a.mean && a.rstd, op, "mean or rstd is null");
   if (rows) {
     check_rows(a.x, rows, a.channels, a.ldx, a.type, op, "x");
@@ -217,7 +223,7 @@ int kg_adamw_step(int device, void* stream, int count, const kg_adamw_tensor* te
       check_type(t.param_type, op);
       check_type(t.grad_type, op);
       if (t.elements < 0 || t.first_block < 0 || t.elements > (1ll << 46) || t.first_block > (1ll << 38)) bad(op, at() + "size out of range");
-      if (!std::isfinite(t.weight_decay)) bad(op, at() + "weight_decay must be finite");
+      if (!finite_float(t.weight_decay)) bad(op, at() + "weight_decay must be finite in float");
       if (!t.elements) continue;
       if (!t.param || !t.grad) bad(op, at() + "null argument");
       if (!aligned(t.param, size_of(t.param_type)) || !aligned(t.grad, size_of(t.grad_type)) || !aligned(t.master, 4))

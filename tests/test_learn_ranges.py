@@ -1,0 +1,47 @@
+"""Scalars that the learning operators' kernels hold in float: what overflows there, and an eps whose reciprocal does, is refused on the
+host. (AdamW of a zero gradient is 0 / (0 + eps), 0 times an infinite reciprocal otherwise; group norm's backward pass squares rstd.)"""
+
+import ctypes
+import importlib
+
+import pytest
+
+import learn_abi as abi
+
+
+@pytest.fixture(scope="module")
+def learn():
+    return importlib.import_module("katago-rs_amd.learn")
+
+
+@pytest.mark.parametrize("change,text", [
+    ({}, None), (dict(eps=2.0 ** -126), None), (dict(eps=2.0 ** -127), "eps"), (dict(eps=1e-40), "eps"), (dict(lr=1e39), "lr"),
+    (dict(lr=-1e300), "lr"), (dict(lr=1e38, beta1=0.999), "lr"), (dict(grad_scale=1e39), "grad_scale")])
+def test_adamw_scalars(kgx, learn, change, text):
+    h = learn._AdamHyper(**{**dict(lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, step=1, seed=0), **change})
+    state, L = learn._AdamState(32, 4096, 4096, None, None), kgx.lib()
+    for rc in (L.kg_adamw_values(ctypes.byref(h), ctypes.byref(learn.AdamValues())),
+               L.kg_adamw_step(0, None, 0, None, ctypes.byref(state), ctypes.byref(h), None)):
+        assert rc == (text is not None) and (text is None or text in L.kg_last_error().decode())
+
+
+def test_adamw_weight_decay(kgx, learn):
+    good = dict(param=4096, grad=4096, master=None, elements=0, first_block=0, weight_decay=0.1, param_type=0, grad_type=0)
+    h, state, L = learn._AdamHyper(1e-3, 0.9, 0.999, 1e-8, 1.0, 1, 0), learn._AdamState(32, 4096, 4096, None, None), kgx.lib()
+    tensor = learn._AdamTensor(**{**good, "weight_decay": 1e39})
+    assert L.kg_adamw_step(0, None, 1, ctypes.byref(tensor), ctypes.byref(state), ctypes.byref(h), None) == 1
+    assert "weight_decay" in L.kg_last_error().decode()
+
+
+@pytest.mark.parametrize("kl_coef", [1e39, -1e200])
+def test_policy_loss_kl_coef(kgx, kl_coef):
+    args = abi.PolicyArgs(rows=0, columns=9, logit_scale=1.0, kl_coef=kl_coef)
+    assert kgx.lib().kg_policy_loss(0, None, ctypes.byref(args)) == 1
+    assert "kl_coef" in kgx.lib().kg_last_error().decode()
+
+
+def test_group_norm_eps(kgx):
+    for eps, refused in ((2.0 ** -126, 0), (2.0 ** -127, 1), (1e-44, 1)):
+        args = abi.NormArgs(batch=0, points=9, channels=12, groups=3, eps=eps)
+        assert kgx.lib().kg_group_norm(0, None, ctypes.byref(args)) == refused
+        assert not refused or "eps" in kgx.lib().kg_last_error().decode()

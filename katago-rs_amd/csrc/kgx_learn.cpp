@@ -215,6 +215,7 @@ int kg_adamw_step(int device, void* stream, int count, const kg_adamw_tensor* te
     need(count >= 0, op, "count must be at least 0");
     need((tensors || !count) && state && hyper, op, "null argument");
     check_hyper(*hyper);
+    need(aligned(values, 4), op, "values is not aligned to its floats");
     if (!count) return;
     check_state(*state, op);
     for (int i = 0; i < count; i++) {

@@ -67,3 +67,12 @@ def test_tiny_gradients_with_a_tiny_eps(learn, bits):
     v = 1e-3 * grad.double() ** 2
     bound = 16 * U + 0.5 * 2.0 ** -150 / v
     assert (bound < 0.01).all() and ((p.cpu().double() + 1).abs() <= bound + 1e-30 / grad.double()).all()
+
+
+def test_step_values_off_their_alignment(learn):
+    p = torch.zeros(8, device="cuda")
+    opt = learn.AdamW([p], lr=1e-2)
+    room = torch.zeros(64, dtype=torch.uint8, device="cuda")
+    with pytest.raises(importlib.import_module("katago-rs_amd").KgError, match="values"):
+        opt.step([torch.ones_like(p)], values=room[1:41])
+    assert opt.step_count == 0 and not p.any()

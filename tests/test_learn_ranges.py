@@ -45,3 +45,11 @@ def test_group_norm_eps(kgx):
         args = abi.NormArgs(batch=0, points=9, channels=12, groups=3, eps=eps)
         assert kgx.lib().kg_group_norm(0, None, ctypes.byref(args)) == refused
         assert not refused or "eps" in kgx.lib().kg_last_error().decode()
+
+
+@pytest.mark.parametrize("count,values", [(0, 4098), (1, 4097), (1, 4098)])
+def test_adamw_values_off_their_alignment(kgx, learn, count, values):
+    h, state, L = learn._AdamHyper(1e-3, 0.9, 0.999, 1e-8, 1.0, 1, 0), learn._AdamState(32, 4096, 4096, None, None), kgx.lib()
+    tensor = learn._AdamTensor(param=4096, grad=4096, elements=0)
+    assert L.kg_adamw_step(0, None, count, ctypes.byref(tensor), ctypes.byref(state), ctypes.byref(h), values) == 1
+    assert "values" in L.kg_last_error().decode()

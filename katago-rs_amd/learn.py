@@ -43,10 +43,14 @@ _vp, _ci, _ll, _cd = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_
 
 
 # The argument structures of include/kgx.h, packed at their natural alignment: a third of a ctypes structure's time, and a small
-# batch's call is its host time.
+# batch's call is its host time. (A size past 31 bits does not pack: _out_of_range.)
 _POLICY_ARGS = struct.Struct("@3iPqPqPPPPPqPddddPPPPqP0q")
 _PREFERENCE_ARGS = struct.Struct("@3iPqPiPPPddiPPPPqP0q")
 _NORM_ARGS = struct.Struct("@6idPqPPPPPPPqPqPqPP0q")
+
+
+def _out_of_range(op, error):
+    return ValueError(f"{op}: a size or number is out of range ({error})")
 
 
 class _AdamTensor(ctypes.Structure):
@@ -150,12 +154,15 @@ def policy_loss(logits, actions, old_logp, advantage, *, legal=None, weight=None
     # (Few long rows: 16384 columns are the least that a workspace is for.)
     bytes_ = L.kg_policy_loss_workspace(n, v) if v > 16384 else 0
     work = _workspace(bytes_, logits.device)
-    args = _POLICY_ARGS.pack(n, v, TYPES[logits.dtype], ptr, ld, lg, ld_lg, _vector(actions, n, torch.int32, "actions", dev),
-                             _vector(old_logp, n, torch.float32, "old_logp", dev),
-                             _vector(advantage, n, torch.float32, "advantage", dev),
-                             _vector(weight, n, torch.float32, "weight", dev), ref, ld_ref,
-                             _vector(ref_logp, n, torch.float32, "ref_logp", dev), logit_scale, clip[0], clip[1], kl_coef, o,
-                             o + 4 * n, o + 8 * n, g, ld_g, work.data_ptr() if work is not None else 0)
+    try:
+        args = _POLICY_ARGS.pack(n, v, TYPES[logits.dtype], ptr, ld, lg, ld_lg, _vector(actions, n, torch.int32, "actions", dev),
+                                 _vector(old_logp, n, torch.float32, "old_logp", dev),
+                                 _vector(advantage, n, torch.float32, "advantage", dev),
+                                 _vector(weight, n, torch.float32, "weight", dev), ref, ld_ref,
+                                 _vector(ref_logp, n, torch.float32, "ref_logp", dev), logit_scale, clip[0], clip[1], kl_coef, o,
+                                 o + 4 * n, o + 8 * n, g, ld_g, work.data_ptr() if work is not None else 0)
+    except struct.error as e:
+        raise _out_of_range("policy_loss", e) from None
     if L.kg_policy_loss(dev, _stream(dev), args):
         _check(1)
     if given is not None:
@@ -190,11 +197,14 @@ def preference_loss(logits, labels, offsets, ref_logp, *, beta=0.1, label_smooth
     out = torch.empty(room // 4 + L.kg_preference_loss_workspace(t) // 4, dtype=torch.float32, device=logits.device)
     loss, margin, seq_logp, _ = out.split_with_sizes((p, p, 2 * p, out.numel() - 4 * p))
     o = out.data_ptr()
-    args = _PREFERENCE_ARGS.pack(t, v, TYPES[logits.dtype], ptr, ld, _vector(labels, t, torch.int32, "labels", dev), p,
-                                 _vector(offsets, 2 * p + 1, torch.int32, "offsets", dev),
-                                 _vector(ref_logp, 2 * p, torch.float32, "ref_logp", dev),
-                                 _vector(weight, p, torch.float32, "weight", dev), beta, label_smoothing, bool(average), o,
-                                 o + 4 * p, o + 8 * p, g, ld_g, o + room)
+    try:
+        args = _PREFERENCE_ARGS.pack(t, v, TYPES[logits.dtype], ptr, ld, _vector(labels, t, torch.int32, "labels", dev), p,
+                                     _vector(offsets, 2 * p + 1, torch.int32, "offsets", dev),
+                                     _vector(ref_logp, 2 * p, torch.float32, "ref_logp", dev),
+                                     _vector(weight, p, torch.float32, "weight", dev), beta, label_smoothing, bool(average), o,
+                                     o + 4 * p, o + 8 * p, g, ld_g, o + room)
+    except struct.error as e:
+        raise _out_of_range("preference_loss", e) from None
     if L.kg_preference_loss(dev, _stream(dev), args):
         _check(1)
     if given is not None:
@@ -258,12 +268,15 @@ def group_norm(x, groups, gamma=None, beta=None, *, mask=None, eps=1e-5, act="id
     else:
         yp, ldy = _like(y, x, "y")
     L = _library()
-    stats = torch.empty((2, b, max(g, 0)), dtype=torch.float32, device=x.device)
+    stats = torch.empty((2, b, max(min(g, c), 0)), dtype=torch.float32, device=x.device)
     work = _workspace(L.kg_group_norm_workspace(b, p, c, g, 0), x.device)
     mean, rstd = stats.unbind()
     o = stats.data_ptr()
-    args = _NORM_ARGS.pack(b, p, c, g, TYPES[x.dtype], ACTS[act], eps, ptr, ld, mk, gm, bt, o, o + 4 * b * g,
-                           work.data_ptr() if work is not None else 0, yp, ldy, 0, 0, 0, 0, 0, 0)
+    try:
+        args = _NORM_ARGS.pack(b, p, c, g, TYPES[x.dtype], ACTS[act], eps, ptr, ld, mk, gm, bt, o, o + 4 * b * g,
+                               work.data_ptr() if work is not None else 0, yp, ldy, 0, 0, 0, 0, 0, 0)
+    except struct.error as e:
+        raise _out_of_range("group_norm", e) from None
     if L.kg_group_norm(dev, _stream(dev), args):
         _check(1)
     if given is not None:
@@ -291,8 +304,11 @@ def group_norm_backward(dy, x, mean, rstd, groups, gamma=None, beta=None, *, mas
     out = torch.empty((2, c), dtype=torch.float32, device=x.device)
     dgamma, dbeta = out.unbind()
     o = out.data_ptr()
-    args = _NORM_ARGS.pack(b, p, c, g, TYPES[x.dtype], ACTS[act], 0.0, ptr, ld, mk, gm, bt, mean.data_ptr(), rstd.data_ptr(),
-                           work.data_ptr() if work is not None else 0, 0, 0, dyp, lddy, dxp, lddx, o, o + 4 * c)
+    try:
+        args = _NORM_ARGS.pack(b, p, c, g, TYPES[x.dtype], ACTS[act], 0.0, ptr, ld, mk, gm, bt, mean.data_ptr(), rstd.data_ptr(),
+                               work.data_ptr() if work is not None else 0, 0, 0, dyp, lddy, dxp, lddx, o, o + 4 * c)
+    except struct.error as e:
+        raise _out_of_range("group_norm_backward", e) from None
     if L.kg_group_norm_backward(dev, _stream(dev), args):
         _check(1)
     if given is not None:

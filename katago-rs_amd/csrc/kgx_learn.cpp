@@ -250,7 +250,7 @@ int kg_adamw_moments(int device, void* stream, long long blocks, const kg_adamw_
 }
 
 size_t kg_group_norm_workspace(int batch, int points, int channels, int groups, int backward) {
-  if (batch < 0 || points < 0 || channels < 1 || groups < 1) return 0;
+  if (batch < 0 || points < 0 || channels < 1 || groups < 1 || groups > kMaxNormGroups) return 0;  // (no call takes those)
   return kgx::group_norm_workspace(batch, points, channels, groups, backward != 0);
 }
 

@@ -1,6 +1,7 @@
 """Sizes past 31 bits are refused with the errors that the calls name (ValueError or KgError), and at once."""
 
 import importlib
+import time
 
 import pytest
 import torch
@@ -54,3 +55,13 @@ def test_groups(kgx, learn, monkeypatch):
                           (2 ** 40, ValueError)):
         with pytest.raises(error, match="group"):
             learn.group_norm(x, groups)
+
+
+def test_group_norm_workspace_of_any_sizes(kgx):
+    """At once, and 0 for groups that no call takes."""
+    L, start = kgx.lib(), time.monotonic()
+    for groups in (2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 19, 2049):
+        assert L.kg_group_norm_workspace(1, 361, 2 ** 31 - 1, groups, 0) == 0
+        assert L.kg_group_norm_workspace(1, 361, 2 ** 31 - 1, groups, 1) == 0
+    assert L.kg_group_norm_workspace(1, 361, 2048, 2048, 0) >= 2048 * 12
+    assert time.monotonic() - start < 1

@@ -355,8 +355,9 @@ int kg_rmsnorm_rows_of(int rows, int channels, int region, int workgroup, int* g
  * and grad[i] is the gradient of loss[i] with respect to row i's logits (scale weight to scale both). Illegal columns take
  * no part whatever they hold, and their gradient is 0. A row whose action is outside [0, columns) is padding: loss, logp, kl
  * and gradient 0. A row whose action is illegal or has the logit -infinity, or that has no legal column, takes no part
- * either: logp -infinity, the rest 0. At the clip's border the ratio counts as unclipped. NaN in a legal column makes the
- * row's results NaN. */
+ * either: logp -infinity, the rest 0. At the clip's border the ratio counts as unclipped. An advantage of 0 takes no
+ * part however large the ratio; an infinite kl makes loss and gradient infinite or NaN, with a kl_coef of 0 too. NaN in a legal
+ * column makes the row's results NaN. */
 typedef struct {
   int rows, columns;
   int type;                    /* of logits, ref_logits and grad */

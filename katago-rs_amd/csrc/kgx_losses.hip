@@ -193,7 +193,8 @@ __device__ __forceinline__ PolicyFactors policy_row(const PolicyRows& a, int row
     const float w = a.weight ? a.weight[row] : 1.f, adv = a.advantage[row], inv = __builtin_amdgcn_rcpf((float)sum);
     const double delta = lp - (double)a.old_logp[row];
     const float ratio = exp_of((float)delta, Base2(1.0));
-    const bool held = adv > 0.f ? delta > a.log_high : adv < 0.f ? delta < a.log_low : false;
+    // (No advantage: 0 on either side, and on the held one whatever the ratio. NaN is on neither.)
+    const bool held = adv >= 0.f ? delta > a.log_high : adv < 0.f ? delta < a.log_low : false;
     const float bounded = fminf(fmaxf(ratio, (float)(1.0 - a.low)), (float)(1.0 + a.high));
     float c = held ? 0.f : -ratio * adv;
     if constexpr (FULL) {

@@ -477,7 +477,8 @@ int kg_adamw_moments(int device, void* stream, long long blocks, const kg_adamw_
  * elements, row stride ldx, batch stride points ldx; group q is channels [q channels / groups, (q + 1) channels / groups).
  * Over the points with a nonzero mask (all without one) and the channels of a group, mean and variance:
  *   rstd = 1 / sqrt(variance + eps), y = act((x - mean) rstd gamma + beta), 0 where the mask is 0.
- * Masked points take no part whatever they hold. A row without any point gives mean 0, rstd 1 / sqrt(eps) and zeros.
+ * Masked points take no part whatever they hold; NaN or infinity at another point makes its group's rstd, y and dx NaN. A row without
+ * any point gives mean 0, rstd 1 / sqrt(eps) and zeros.
  * act: KG_ACT_*. The statistics are outputs for the backward pass. At most 2048 groups; batch points and batch groups are
  * below 2^31, and a launch of some 2^32 / 1024 slabs of groups is the most that one call makes. */
 #define KG_ACT_IDENTITY 0

@@ -83,6 +83,13 @@ struct NormArgs {
   float eps;
 };
 
+// act_f, but for ReLU of NaN, which act_f makes 0: a norm with a value that is no finite number shows it in every activation.
+template <int ACT>
+__device__ __forceinline__ float norm_act(float v) {
+  if constexpr (ACT == ACT_RELU) return v < 0.f ? 0.f : v;
+  else return act_f<ACT>(v);
+}
+
 // The points [p0, p1) of split k.
 __device__ __forceinline__ void split_range(const NormArgs& a, int k, int& p0, int& p1) {
   p0 = (int)((long long)a.points * k / a.splits);
@@ -266,7 +273,7 @@ __global__ __launch_bounds__(GT) void norm_apply_kernel(NormArgs a) {
       } else {
         load_vec<T>(x + (size_t)p * a.ldx, left, f);
 #pragma unroll
-        for (int j = 0; j < V; j++) f[j] = act_f<ACT>(__builtin_fmaf(f[j] - mean[j], mul[j], add[j]));
+        for (int j = 0; j < V; j++) f[j] = norm_act<ACT>(__builtin_fmaf(f[j] - mean[j], mul[j], add[j]));
       }
       store_vec<T>(y + (size_t)p * a.ldy, left, f);
     }
@@ -679,7 +686,7 @@ __device__ __forceinline__ void slab_forward(const NormArgs& a, Slab<T, E>& s, c
     if (e >= s.each) break;
     float f[V];
 #pragma unroll
-    for (int j = 0; j < V; j++) f[j] = act_f<ACT>(__builtin_fmaf(element<T>(raw[e], j) - mean[j], mul[j], add[j]));
+    for (int j = 0; j < V; j++) f[j] = norm_act<ACT>(__builtin_fmaf(element<T>(raw[e], j) - mean[j], mul[j], add[j]));
     u32x4 w;
 #pragma unroll
     for (int k = 0; k < 4; k++) {

@@ -35,3 +35,21 @@ def test_no_advantage_no_part(learn, v):
     r = learn.policy_loss(z, act, old, zero)
     assert torch.isnan(r.loss).all() and torch.isnan(r.grad).all()
     assert torch.isnan(learn.policy_loss(refl, act, old, zero * torch.nan).grad).all()
+
+
+@pytest.mark.parametrize("shape", [(2, 37, 24, 3), (2, 5000, 96, 4), (2, 9, 2056, 8), (1, 901, 3, 3)])
+@pytest.mark.parametrize("act", ["identity", "relu", "mish", "silu"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_no_number_is_seen(learn, shape, act, bad):
+    """A value that is no finite number at a point that counts makes its group's results NaN, in y and dx too, and no other's."""
+    b, p, c, groups = shape
+    g = torch.Generator().manual_seed(p)
+    x, dy = torch.randn(b, p, c, generator=g).cuda(), torch.randn(b, p, c, generator=g).cuda()
+    x[0, p // 2, c - 1] = bad
+    y, mean, rstd = learn.group_norm(x, groups, act=act)
+    dx, dgamma, _ = learn.group_norm_backward(dy, x, mean, rstd, groups, act=act)
+    w = c // groups
+    for t in (y, dx):
+        assert torch.isnan(t[0, :, c - w:]).all() and torch.isfinite(t[0, :, :c - w]).all() and torch.isfinite(t[1:]).all()
+    assert torch.isnan(rstd[0, -1]) and torch.isfinite(rstd[0, :-1]).all() and torch.isfinite(rstd[1:]).all()
+    assert torch.isnan(dgamma[c - w:]).all() and torch.isfinite(dgamma[:c - w]).all()

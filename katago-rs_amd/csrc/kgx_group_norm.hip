@@ -282,7 +282,8 @@ __global__ __launch_bounds__(GT) void norm_apply_kernel(NormArgs a) {
 
 // d act(a) / d a. Mish: with e = exp(a) and n = e (e + 2), tanh(softplus) = n / (n + 2) and 1 - tanh^2 = 4 (e + 1)^2 /
 // (n + 2)^2, so the derivative n / (n + 2) + 4 a e (e + 1) / (n + 2)^2 has no cancellation but its own sign's. From a = 20 on
-// it is 1 in float, as it is at 20: the argument is held there, with no branch.
+// it is 1 in float, as it is at 20: the argument is held there, with no branch. The exponentials are the fast ones, off by some U |a|
+// (U = 2^-24) of terms that fall as a e^-|a|: a few U of the slope, as the reciprocals' ulp.
 template <int ACT>
 __device__ __forceinline__ float act_slope(float v) {
   if constexpr (ACT == ACT_RELU) {

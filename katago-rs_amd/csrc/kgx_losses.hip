@@ -62,7 +62,8 @@ __device__ __forceinline__ double row_sum(float v, float* red) {
 }
 
 // log(s) in double for s >= 1, from s = 2^k f, f in [0.7, 1.42): log f = 2 atanh(t) = 2 (t + t^3/3 + ...),
-// t = (f - 1) / (f + 1), |t| < 0.172, so that the terms to t^13 leave 1e-12. NaN and infinity stay.
+// t = (f - 1) / (f + 1), |t| < 0.172, so that the terms to t^13 leave 1e-12. NaN stays; s is finite
+// (a sum of at most 2^30 terms up to 1).
 __device__ __forceinline__ double log_sum(double s) {
   int k;
   double f = frexp(s, &k);
@@ -190,6 +191,7 @@ __device__ __forceinline__ PolicyFactors policy_row(const PolicyRows& a, int row
   PolicyFactors f = {0.f, 0.f, 0.f, 0.f, !padding && !(lp == -(double)INFINITY)};
   float loss = 0.f, logp = padding ? 0.f : -INFINITY, kl = 0.f;
   if (f.part) {
+    // (1 / sum by the hardware's reciprocal: an ulp of the row's probabilities, whose exponentials are off by more.)
     const float w = a.weight ? a.weight[row] : 1.f, adv = a.advantage[row], inv = __builtin_amdgcn_rcpf((float)sum);
     const double delta = lp - (double)a.old_logp[row];
     const float ratio = exp_of((float)delta, Base2(1.0));

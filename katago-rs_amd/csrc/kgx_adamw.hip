@@ -1,7 +1,7 @@
 // The AdamW step over many tensors at once (kg_adamw_step), with moments in 32 or in 8 bits, and the moments as numbers.
 //
 // Bound by memory: 28 bytes an element in float, 16 with 16-bit parameters and gradients, float masters and 8-bit moments. A step
-// of 29 M float elements in 310 tensors takes 144 us (5.6 TB/s), one of 240 M bf16 with masters and 8 bits 700 (5.5 TB/s).
+// of 29 M float elements in 310 tensors takes 144 us (5.6 TB/s), one of 240 M bf16 with masters and 8 bits 710 (5.4 TB/s).
 // One launch covers up to kTensors tensors, whose descriptions travel as kernel arguments: nothing has to be uploaded, and a
 // captured launch carries them. Each workgroup takes kChunk consecutive elements of one tensor.
 //

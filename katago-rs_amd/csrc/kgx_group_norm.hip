@@ -1122,7 +1122,8 @@ SlabShape slab_shape(int points, int groups, int width, int vec, int batch) {
   }
   // Where there are more workgroups than CUs, four points a thread rather than one or two: smaller workgroups, more of them at once
   // on a CU. 143 x 194 points of 864 bf16 channels in 24 groups 110 -> 28 us and backward 108 -> 33; 512 boards of 361 x 128 f32 in 8
-  // groups 59 -> 40 and 78 -> 57. (Three points stay: 128 boards of 361 x 384 bf16 with mish backward 45 us, 59 with four.)
+  // groups 59 -> 40 and 78 -> 57. (Three points stay, for both directions: 128 boards of 361 x 384 bf16 with mish backward 45 us, 59 with
+  // four; forward with four is not measured.)
   if (best.groups && best.each < 3 && (long long)batch * (groups / best.groups) > kCUs) {
     const int w = best.groups * width, cols = (w + vec - 1) / vec;
     best.each = std::min(4, points);

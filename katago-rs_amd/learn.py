@@ -9,7 +9,7 @@
 The calls run on torch's current stream of the tensors' device and do not wait. They take part in no autograd graph: gradients
 are returned. What they write into a caller's tensor raises its version counter as torch's own in-place operations do (a replayed
 graph raises none, as with those). There is no other compute path, and a call that the library refuses raises KgError; a tensor of another shape,
-type or device than the call needs raises ValueError. A network's own policy rows come from Handle.policy_rows:
+type or device than the call needs, or a size past 31 bits, raises ValueError. A network's own policy rows come from Handle.policy_rows:
 
     rows = torch.as_tensor(handle.policy_rows(n), device="cuda")   # [n, 362], inside the raw rows
     r = learn.policy_loss(rows, actions, old_logp, advantage, legal=legal, kl_coef=0.1, ref_logits=before)

@@ -419,6 +419,44 @@ typedef struct {
 int kg_preference_loss(int device, void* stream, const kg_preference_loss_args* args);
 size_t kg_preference_loss_workspace(int rows);
 
+/* The distillation loss of `rows` rows of a student's logits against a teacher of whom each row holds `k` top logits, and its
+ * gradient. Row i's entries are columns c = top_index[i][j] with the teacher's logits t = top_logits[i][j]. An entry counts
+ * where c is in [0, columns), legal, and named by no entry before it. Over the legal columns, with p = softmax(logit_scale z):
+ *   q_j  = exp(logit_scale t_j) / their sum over the entries that count, or with teacher_lse exp(logit_scale t_j - teacher_lse),
+ *          which leaves rest = max(0, 1 - sum q) to the legal columns without such an entry, whose p together is R,
+ *   loss = weight (sum q_j log(q_j / p_c) + rest log(rest / R)),
+ * and grad[i] is the gradient of loss[i] with respect to row i's logits: weight logit_scale (m p - q) in a listed column and
+ * weight logit_scale p (m - rest / R) in the others, m = sum q + rest. (With a temperature T: logit_scale 1 / T, and
+ * weight T^2 to keep the gradients' size.) Where no other column has mass, rest is 0. Illegal columns take no part whatever they
+ * hold, and their gradient is 0. A row without an entry that counts (padding: every index -1), or whose legal columns are all
+ * -infinity, or all of whose teacher's logits are (without teacher_lse), takes no part: loss and gradient 0. A listed column with the logit
+ * -infinity and q above 0 makes the loss infinite. NaN in a legal column or an entry that counts makes the row's loss NaN, and its gradient
+ * wherever p is not 0. */
+#define KG_DISTILL_MAX_K 1024
+typedef struct {
+  int rows, columns, k;        /* k in [1, KG_DISTILL_MAX_K] */
+  int type;                    /* of logits and grad */
+  int top_type;                /* of top_logits */
+  const void* logits;          /* [rows] rows of ld elements */
+  long long ld;
+  const unsigned char* legal;  /* [rows] rows of ld_legal bytes, nonzero where legal; NULL: every column */
+  long long ld_legal;
+  const int* top_index;        /* [rows] rows of ld_index, k each */
+  long long ld_index;
+  const void* top_logits;      /* [rows] rows of ld_top, k each */
+  long long ld_top;
+  const float* teacher_lse;    /* [rows] log of the sum of exp(logit_scale t) over all the teacher's columns; or NULL */
+  const float* weight;         /* [rows] or NULL: 1 */
+  double logit_scale;          /* 1 / temperature, in [2^-64, 2^64] */
+  float* loss;                 /* [rows] */
+  void* grad;                  /* [rows] rows of ld_grad (columns past `columns` stay as they are); or NULL */
+  long long ld_grad;
+  void* workspace;             /* kg_distill_loss_workspace(rows, columns) bytes, 16-byte aligned, this call's own until it has run;
+                                  NULL where that is 0 */
+} kg_distill_loss_args;
+int kg_distill_loss(int device, void* stream, const kg_distill_loss_args* args);
+size_t kg_distill_loss_workspace(int rows, int columns);
+
 /* One AdamW step over `count` tensors at once (decoupled weight decay), in float:
  *   g = grad_scale grad; m = beta1 m + (1 - beta1) g; v = beta2 v + (1 - beta2) g^2;
  *   p = p (1 - lr weight_decay) - (lr / (1 - beta1^step)) m / (sqrt(v) / sqrt(1 - beta2^step) + eps).
@@ -513,6 +551,66 @@ int kg_group_norm(int device, void* stream, const kg_group_norm_args* args);
 /* The gradients of a loss whose gradient with respect to y is dy (eps and y are not used). */
 int kg_group_norm_backward(int device, void* stream, const kg_group_norm_args* args);
 size_t kg_group_norm_workspace(int batch, int points, int channels, int groups, int backward);
+
+/* Layer norm over the `channels` of each of `rows` rows, and RMS norm (`rms`: mean 0, variance the mean of the squares):
+ *   rstd = 1 / sqrt(variance + eps), y = (x - mean) rstd gamma + beta.
+ * The statistics are outputs for the backward pass. NaN or infinity in a row makes that row NaN, and with it dgamma and dbeta's channels. At
+ * most 2^30 rows of 2^30 channels. */
+typedef struct {
+  int rows, channels;
+  int type;                /* of x, y, dy and dx */
+  int rms;
+  double eps;              /* >= 2^-126 */
+  const void* x;           /* rows of ldx elements */
+  long long ldx;
+  const float* gamma;      /* [channels] or NULL: 1 */
+  const float* beta;       /* [channels] or NULL: 0 */
+  float* mean;             /* [rows]: written by kg_layer_norm, read by kg_layer_norm_backward; with rms unused, may be NULL */
+  float* rstd;             /* [rows] */
+  void* workspace;         /* kg_layer_norm_backward: kg_layer_norm_workspace bytes, 16-byte aligned, this call's own until it has run */
+  /* kg_layer_norm */
+  void* y;                 /* rows of ldy */
+  long long ldy;
+  /* kg_layer_norm_backward */
+  const void* dy;          /* rows of lddy */
+  long long lddy;
+  void* dx;                /* rows of lddx */
+  long long lddx;
+  float* dgamma;           /* [channels], sums over the rows; or NULL */
+  float* dbeta;            /* [channels]; or NULL */
+} kg_layer_norm_args;
+int kg_layer_norm(int device, void* stream, const kg_layer_norm_args* args);
+/* The gradients of a loss whose gradient with respect to y is dy (eps, beta and y are not used). */
+int kg_layer_norm_backward(int device, void* stream, const kg_layer_norm_args* args);
+size_t kg_layer_norm_workspace(int rows, int channels);
+
+/* The rows of a table that `count` tokens name, y[i] = scale table[tokens[i]], and the table's gradient,
+ *   grad[v] = scale sum of dy[i] over the tokens i with tokens[i] = v, added up in their order,
+ * 0 where there is none. A token outside [0, vocab) is padding: its row of y is 0, and its dy is not read. `accumulate`: the sums are
+ * added to what grad holds, and rows that no token names are left as they are (a table that is the head's weight too). At most 2^30
+ * tokens, rows and channels. */
+typedef struct {
+  int count, vocab, channels;
+  int type;                /* of table, y and dy */
+  const int* tokens;       /* [count] */
+  double scale;            /* finite as a float */
+  /* kg_embedding */
+  const void* table;       /* [vocab] rows of ld_table elements */
+  long long ld_table;
+  void* y;                 /* [count] rows of ld_y */
+  long long ld_y;
+  /* kg_embedding_backward */
+  const void* dy;          /* [count] rows of ld_dy */
+  long long ld_dy;
+  int grad_type;           /* `type` or KG_PRECISION_F32 */
+  int accumulate;
+  void* grad;              /* [vocab] rows of ld_grad */
+  long long ld_grad;
+  void* workspace;         /* kg_embedding_backward_workspace bytes, 16-byte aligned, this call's own until it has run; NULL where that is 0 */
+} kg_embedding_args;
+int kg_embedding(int device, void* stream, const kg_embedding_args* args);
+int kg_embedding_backward(int device, void* stream, const kg_embedding_args* args);
+size_t kg_embedding_backward_workspace(int count, int vocab, int channels);
 
 #ifdef __cplusplus
 }

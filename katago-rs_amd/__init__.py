@@ -237,6 +237,17 @@ def lib():
         L.kg_group_norm_backward.argtypes = [ci, vp, vp]
         L.kg_group_norm_workspace.argtypes = [ci] * 5
         L.kg_group_norm_workspace.restype = ctypes.c_size_t
+        L.kg_distill_loss.argtypes = [ci, vp, vp]
+        L.kg_distill_loss_workspace.argtypes = [ci, ci]
+        L.kg_distill_loss_workspace.restype = ctypes.c_size_t
+        L.kg_layer_norm.argtypes = [ci, vp, vp]
+        L.kg_layer_norm_backward.argtypes = [ci, vp, vp]
+        L.kg_layer_norm_workspace.argtypes = [ci, ci]
+        L.kg_layer_norm_workspace.restype = ctypes.c_size_t
+        L.kg_embedding.argtypes = [ci, vp, vp]
+        L.kg_embedding_backward.argtypes = [ci, vp, vp]
+        L.kg_embedding_backward_workspace.argtypes = [ci, ci, ci]
+        L.kg_embedding_backward_workspace.restype = ctypes.c_size_t
         _ = cf
         _lib = L
     return _lib

@@ -105,6 +105,27 @@ void check_preference(const kg_preference_loss_args& a) {
   if (a.pairs) need(a.ref_logp && a.loss && a.margin && a.seq_logp, op, "null argument");
 }
 
+void check_distill(const kg_distill_loss_args& a) {
+  const char* op = "distillation loss";
+  need(a.rows >= 0 && a.rows <= kMaxRows && a.columns >= 1 && a.columns <= kMaxColumns, op, "rows must be in [0, 2^30] and columns in [1, 2^30]");
+  need(a.k >= 1 && a.k <= KG_DISTILL_MAX_K, op, "k must be in [1, 1024]");
+  check_type(a.type, op);
+  check_type(a.top_type, op);
+  need(a.logit_scale >= 0x1p-64 && a.logit_scale <= 0x1p64, op, "logit_scale must be positive, in [2^-64, 2^64]");
+  if (!a.rows) return;
+  check_rows(a.logits, a.rows, a.columns, a.ld, a.type, op, "logits");
+  check_rows(a.top_index, a.rows, a.k, a.ld_index, KG_PRECISION_F32, op, "top_index");  // (4 bytes too)
+  check_rows(a.top_logits, a.rows, a.k, a.ld_top, a.top_type, op, "top_logits");
+  if (a.grad) check_rows(a.grad, a.rows, a.columns, a.ld_grad, a.type, op, "grad");
+  if (a.legal) need(a.ld_legal >= (a.rows > 1 ? a.columns : 0), op, "the row stride of legal is less than its row");
+  need(a.loss, op, "null argument");
+  need(!a.grad || (a.grad != a.logits && a.grad != a.top_logits), op, "grad must not overlap an input");
+  if (kgx::distill_loss_workspace(a.rows, a.columns)) {
+    need(a.workspace, op, "workspace is null");
+    need(aligned(a.workspace, 16), op, "workspace is not aligned to 16 bytes");
+  }
+}
+
 void check_state(const kg_adamw_state& s, const char* op) {
   need(s.state_bits == 8 || s.state_bits == 32, op, "state_bits must be 8 or 32");
   need(s.m && s.v, op, "the moments are null");
@@ -170,6 +191,51 @@ void check_norm(const kg_group_norm_args& a, bool backward) {
     need(aligned(a.workspace, 16), op, "workspace is not aligned to 16 bytes");
   }
   need(kgx::group_norm_fits(a), op, "batch x groups is out of range");
+}
+
+void check_layer_norm(const kg_layer_norm_args& a, bool backward) {
+  const char* op = backward ? "layer norm backward" : "layer norm";
+  need(a.rows >= 0 && a.rows <= kMaxRows && a.channels >= 1 && a.channels <= kMaxColumns, op,
+       "rows must be in [0, 2^30] and channels in [1, 2^30]");
+  check_type(a.type, op);
+  if (!backward) need(usable_eps(a.eps), op, "eps must be positive, at least 2^-126");
+  if (!a.rows) return;
+  need((a.mean || a.rms) && a.rstd, op, "mean or rstd is null");
+  check_rows(a.x, a.rows, a.channels, a.ldx, a.type, op, "x");
+  if (backward) {
+    check_rows(a.dy, a.rows, a.channels, a.lddy, a.type, op, "dy");
+    check_rows(a.dx, a.rows, a.channels, a.lddx, a.type, op, "dx");
+    need(a.dx != a.x && a.dx != a.dy, op, "dx must not overlap an input");
+    need(a.workspace, op, "workspace is null");
+    need(aligned(a.workspace, 16), op, "workspace is not aligned to 16 bytes");
+  } else {
+    check_rows(a.y, a.rows, a.channels, a.ldy, a.type, op, "y");
+    need(a.y != a.x, op, "y must not overlap x");
+  }
+}
+
+void check_embedding(const kg_embedding_args& a, bool backward) {
+  const char* op = backward ? "embedding backward" : "embedding";
+  need(a.count >= 0 && a.count <= kMaxRows && a.vocab >= 1 && a.vocab <= kMaxRows && a.channels >= 1 && a.channels <= kMaxColumns, op,
+       "count must be in [0, 2^30], vocab and channels in [1, 2^30]");
+  check_type(a.type, op);
+  need(finite_float(a.scale), op, "scale must be finite in float");
+  if (backward) {
+    need(a.grad_type == a.type || a.grad_type == KG_PRECISION_F32, op, "grad_type must be the type of dy or float");
+    if (a.count || !a.accumulate) check_rows(a.grad, a.vocab, a.channels, a.ld_grad, a.grad_type, op, "grad");
+  }
+  if (!a.count) return;
+  need(a.tokens && aligned(a.tokens, 4), op, "tokens is null or not aligned to its elements");
+  if (backward) {
+    check_rows(a.dy, a.count, a.channels, a.ld_dy, a.type, op, "dy");
+    need(a.grad != a.dy, op, "grad must not overlap an input");
+    need(a.workspace, op, "workspace is null");
+    need(aligned(a.workspace, 16), op, "workspace is not aligned to 16 bytes");
+  } else {
+    check_rows(a.table, a.vocab, a.channels, a.ld_table, a.type, op, "table");
+    check_rows(a.y, a.count, a.channels, a.ld_y, a.type, op, "y");
+    need(a.y != a.table, op, "y must not overlap the table");
+  }
 }
 
 }  // namespace
@@ -270,6 +336,64 @@ int kg_group_norm_backward(int device, void* stream, const kg_group_norm_args* a
     check_norm(*args, true);
     OnDevice on(device, "group norm backward");
     kgx::launch_group_norm_backward(*args, (hipStream_t)stream);
+  });
+}
+
+size_t kg_distill_loss_workspace(int rows, int columns) { return kgx::distill_loss_workspace(rows, columns); }
+
+int kg_distill_loss(int device, void* stream, const kg_distill_loss_args* args) {
+  return guarded([&] {
+    need(args, "distillation loss", "null argument");
+    check_distill(*args);
+    if (!args->rows) return;
+    OnDevice on(device, "distillation loss");
+    kgx::launch_distill_loss(*args, (hipStream_t)stream);
+  });
+}
+
+size_t kg_layer_norm_workspace(int rows, int channels) { return kgx::layer_norm_workspace(rows, channels); }
+
+int kg_layer_norm(int device, void* stream, const kg_layer_norm_args* args) {
+  return guarded([&] {
+    need(args, "layer norm", "null argument");
+    check_layer_norm(*args, false);
+    if (!args->rows) return;
+    OnDevice on(device, "layer norm");
+    kgx::launch_layer_norm(*args, (hipStream_t)stream);
+  });
+}
+
+int kg_layer_norm_backward(int device, void* stream, const kg_layer_norm_args* args) {
+  return guarded([&] {
+    need(args, "layer norm backward", "null argument");
+    check_layer_norm(*args, true);
+    OnDevice on(device, "layer norm backward");
+    kgx::launch_layer_norm_backward(*args, (hipStream_t)stream);
+  });
+}
+
+size_t kg_embedding_backward_workspace(int count, int vocab, int channels) {
+  if (count < 1 || vocab < 1 || channels < 1) return 0;
+  return kgx::embedding_backward_workspace(count, vocab, channels);
+}
+
+int kg_embedding(int device, void* stream, const kg_embedding_args* args) {
+  return guarded([&] {
+    need(args, "embedding", "null argument");
+    check_embedding(*args, false);
+    if (!args->count) return;
+    OnDevice on(device, "embedding");
+    kgx::launch_embedding(*args, (hipStream_t)stream);
+  });
+}
+
+int kg_embedding_backward(int device, void* stream, const kg_embedding_args* args) {
+  return guarded([&] {
+    need(args, "embedding backward", "null argument");
+    check_embedding(*args, true);
+    if (!args->count && args->accumulate) return;
+    OnDevice on(device, "embedding backward");
+    kgx::launch_embedding_backward(*args, (hipStream_t)stream);
   });
 }
 

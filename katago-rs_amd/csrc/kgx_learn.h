@@ -32,4 +32,17 @@ bool group_norm_fits(const kg_group_norm_args& a);  // its launches' threads fit
 void launch_group_norm(const kg_group_norm_args& a, hipStream_t s);
 void launch_group_norm_backward(const kg_group_norm_args& a, hipStream_t s);
 
+size_t distill_loss_workspace(int rows, int columns);
+void launch_distill_loss(const kg_distill_loss_args& a, hipStream_t s);
+
+// Layer norm: the backward pass's sums over parts of the rows.
+size_t layer_norm_workspace(int rows, int channels);
+void launch_layer_norm(const kg_layer_norm_args& a, hipStream_t s);
+void launch_layer_norm_backward(const kg_layer_norm_args& a, hipStream_t s);
+
+// The embedding's backward pass: the tokens sorted, and the sums of runs over several ranges of them.
+size_t embedding_backward_workspace(int count, int vocab, int channels);
+void launch_embedding(const kg_embedding_args& a, hipStream_t s);
+void launch_embedding_backward(const kg_embedding_args& a, hipStream_t s);
+
 }  // namespace kgx

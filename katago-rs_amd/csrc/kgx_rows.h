@@ -5,6 +5,7 @@
 #include <climits>
 
 #include "kgx_device.h"
+#include "kgx_vec.h"
 #include "kgx_wave.h"
 
 namespace kgx {
@@ -17,8 +18,6 @@ template <typename T> struct AnyWords { typedef u32x4_any2 type; };
 template <> struct AnyWords<float> { typedef u32x4_any4 type; };
 typedef unsigned int u32_any __attribute__((aligned(1)));
 typedef unsigned long long u64_any __attribute__((aligned(1)));
-
-template <typename T> inline constexpr int kVec = 16 / sizeof(T);
 
 // Reductions over the NT threads of a row: a wave, or the whole workgroup through `red` (16 floats).
 template <int NT, bool MAX>

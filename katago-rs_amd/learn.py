@@ -3,8 +3,11 @@
 - `policy_loss`: the clipped policy loss with a KL term on rows of logits (a network's policy rows with their legal moves,
   or tokens), and its gradient;
 - `preference_loss`: pairs of lines of moves or token sequences, the better against the worse, and its gradient;
+- `distill_loss`: rows of logits against a teacher's top logits, and its gradient;
 - `AdamW`: one step over many tensors at once, moments in 32 or in 8 bits;
-- `group_norm` and `group_norm_backward`: group norm with an activation on channels-last rows under the board mask.
+- `group_norm` and `group_norm_backward`: group norm with an activation on channels-last rows under the board mask;
+- `layer_norm` and `layer_norm_backward`: layer norm and RMS norm over a row's channels;
+- `embedding` and `embedding_backward`: the rows of a table that tokens name.
 
 The calls run on torch's current stream of the tensors' device and do not wait. They take part in no autograd graph: gradients
 are returned. What they write into a caller's tensor raises its version counter as torch's own in-place operations do (a replayed
@@ -38,6 +41,7 @@ _NUMEL, _CONTIGUOUS, _POINTER = torch.Tensor.numel, torch.Tensor.is_contiguous, 
 
 PolicyLoss = collections.namedtuple("PolicyLoss", ["loss", "logp", "kl", "grad"])
 PreferenceLoss = collections.namedtuple("PreferenceLoss", ["loss", "margin", "seq_logp", "grad"])
+DistillLoss = collections.namedtuple("DistillLoss", ["loss", "grad"])
 
 _vp, _ci, _ll, _cd = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_double
 
@@ -47,6 +51,9 @@ _vp, _ci, _ll, _cd = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_
 _POLICY_ARGS = struct.Struct("@3iPqPqPPPPPqPddddPPPPqP0q")
 _PREFERENCE_ARGS = struct.Struct("@3iPqPiPPPddiPPPPqP0q")
 _NORM_ARGS = struct.Struct("@6idPqPPPPPPPqPqPqPP0q")
+_DISTILL_ARGS = struct.Struct("@5iPqPqPqPqPPdPPqP0q")
+_LAYER_ARGS = struct.Struct("@4idPqPPPPPPqPqPqPP0q")
+_EMBED_ARGS = struct.Struct("@4iPdPqPqPq2iPqP0q")
 
 
 def _out_of_range(op, error):
@@ -212,6 +219,55 @@ def preference_loss(logits, labels, offsets, ref_logp, *, beta=0.1, label_smooth
     return PreferenceLoss(loss, margin, seq_logp, grad)
 
 
+def distill_loss(logits, top_index, top_logits, *, legal=None, weight=None, logit_scale=1.0, teacher_lse=None, want_grad=True,
+                 grad=None):
+    """The distillation loss of each row against a teacher's top logits, and the gradient of their sum (kg_distill_loss).
+
+    logits [n, v] (rows may be strided); top_index [n, k] int32, the columns of the teacher's top logits, outside [0, v) where a row has
+    fewer (every one: padding); top_logits [n, k] float32, float16 or bfloat16; legal [n, v] bool or uint8; weight [n] float32;
+    logit_scale, 1 / temperature, is of both sides. The teacher's probabilities are those of its top logits among each other, or with
+    teacher_lse [n] float32 (the log of the sum of exp(logit_scale t) over all its columns) its true ones, whose rest is held
+    against the student's whole rest. Returns loss [n] float32 and grad [n, v] of the logits' type (into `grad` when given; None
+    without want_grad)."""
+    ptr, ld = _rows(logits, "logits")
+    n, v = logits.shape
+    dev = logits.get_device()
+    lg = ld_lg = g = ld_g = 0
+    if legal is not None:
+        if legal.shape != (n, v) or legal.dtype not in _BYTES or legal.get_device() != dev or (legal.stride(1) != 1 and v > 1):
+            raise ValueError(f"legal must be [{n}, {v}] bool or uint8 on GPU {dev} with contiguous columns")
+        lg, ld_lg = legal.data_ptr(), legal.stride(0)
+    top, ld_top = _rows(top_logits, "top_logits")
+    k = top_logits.shape[1]
+    if top_logits.shape[0] != n or top_logits.get_device() != dev:
+        raise ValueError(f"top_logits must be [{n}, k] on GPU {dev}")
+    if top_index.dtype is not torch.int32 or top_index.shape != (n, k) or top_index.get_device() != dev or \
+            (top_index.stride(1) != 1 and k > 1):
+        raise ValueError(f"top_index must be [{n}, {k}] int32 on GPU {dev} with contiguous columns")
+    given = grad
+    if grad is not None:
+        g, ld_g = _rows(grad, "grad", logits)
+    elif want_grad:
+        grad = torch.empty((n, v), dtype=logits.dtype, device=logits.device)
+        g, ld_g = grad.data_ptr(), v
+    loss = torch.empty(n, dtype=torch.float32, device=logits.device)
+    L = _library()
+    # (Few long rows: 16384 columns are the least that a workspace is for.)
+    work = _workspace(L.kg_distill_loss_workspace(n, v) if v > 16384 else 0, logits.device)
+    try:
+        args = _DISTILL_ARGS.pack(n, v, k, TYPES[logits.dtype], TYPES[top_logits.dtype], ptr, ld, lg, ld_lg, top_index.data_ptr(),
+                                  top_index.stride(0), top, ld_top, _vector(teacher_lse, n, torch.float32, "teacher_lse", dev),
+                                  _vector(weight, n, torch.float32, "weight", dev), logit_scale, loss.data_ptr(), g, ld_g,
+                                  work.data_ptr() if work is not None else 0)
+    except struct.error as e:
+        raise _out_of_range("distill_loss", e) from None
+    if L.kg_distill_loss(dev, _stream(dev), args):
+        _check(1)
+    if given is not None:
+        _written(given)
+    return DistillLoss(loss, grad)
+
+
 def _points(t, name):
     """(pointer, row stride) of [batch, ..., channels] whose points lie evenly spaced."""
     shape = t.shape
@@ -314,6 +370,145 @@ def group_norm_backward(dy, x, mean, rstd, groups, gamma=None, beta=None, *, mas
     if given is not None:
         _written(given)
     return dx, dgamma, dbeta
+
+
+def layer_norm(x, gamma=None, beta=None, *, eps=1e-5, rms=False, y=None):
+    """Layer norm of x [batch, ..., channels] over its channels, or RMS norm (kg_layer_norm); gamma and beta [channels] float32.
+    Returns y (into `y` when given), and mean and rstd [batch, ...] float32; mean is None with rms."""
+    ptr, ld = _points(x, "x")
+    shape, dev = x.shape, x.get_device()
+    c = shape[-1]
+    n = shape[0] if len(shape) == 2 else math.prod(shape[:-1])
+    gm, bt = _vector(gamma, c, torch.float32, "gamma", dev), _vector(beta, c, torch.float32, "beta", dev)
+    given = y
+    if y is None:
+        y = torch.empty(shape, dtype=x.dtype, device=x.device)
+        yp, ldy = y.data_ptr(), c
+    else:
+        yp, ldy = _like(y, x, "y")
+    L = _library()
+    rows = shape[:-1]
+    if rms:
+        mean, rstd = None, torch.empty(rows, dtype=torch.float32, device=x.device)
+        mp, rp = 0, rstd.data_ptr()
+    else:
+        mean, rstd = torch.empty((2, *rows), dtype=torch.float32, device=x.device).unbind()
+        mp = mean.data_ptr()
+        rp = mp + 4 * n
+    try:
+        args = _LAYER_ARGS.pack(n, c, TYPES[x.dtype], bool(rms), eps, ptr, ld, gm, bt, mp, rp, 0, yp, ldy, 0, 0, 0, 0, 0, 0)
+    except struct.error as e:
+        raise _out_of_range("layer_norm", e) from None
+    if L.kg_layer_norm(dev, _stream(dev), args):
+        _check(1)
+    if given is not None:
+        _written(given)
+    return y, mean, rstd
+
+
+def layer_norm_backward(dy, x, mean, rstd, gamma=None, *, dx=None):
+    """The gradients (dx, dgamma, dbeta) of a loss whose gradient with respect to layer_norm's y is dy, from its mean (None: RMS norm)
+    and rstd (kg_layer_norm_backward); dx into `dx` when given."""
+    ptr, ld = _points(x, "x")
+    shape, dev = x.shape, x.get_device()
+    c = shape[-1]
+    n = shape[0] if len(shape) == 2 else math.prod(shape[:-1])
+    gm = _vector(gamma, c, torch.float32, "gamma", dev)
+    dyp, lddy = _like(dy, x, "dy")
+    given = dx
+    if dx is None:
+        dx = torch.empty(shape, dtype=x.dtype, device=x.device)
+        dxp, lddx = dx.data_ptr(), c
+    else:
+        dxp, lddx = _like(dx, x, "dx")
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        if t is None and name == "mean":
+            continue
+        if t.dtype is not torch.float32 or t.shape != shape[:-1] or t.get_device() != dev or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous float32 of shape {tuple(shape[:-1])} on GPU {dev}")
+    L = _library()
+    work = _workspace(L.kg_layer_norm_workspace(n, c), x.device)
+    out = torch.empty((2, c), dtype=torch.float32, device=x.device)
+    dgamma, dbeta = out.unbind()
+    o = out.data_ptr()
+    try:
+        args = _LAYER_ARGS.pack(n, c, TYPES[x.dtype], mean is None, 0.0, ptr, ld, gm, 0, 0 if mean is None else mean.data_ptr(),
+                                rstd.data_ptr(), work.data_ptr() if work is not None else 0, 0, 0, dyp, lddy, dxp, lddx, o, o + 4 * c)
+    except struct.error as e:
+        raise _out_of_range("layer_norm_backward", e) from None
+    if L.kg_layer_norm_backward(dev, _stream(dev), args):
+        _check(1)
+    if given is not None:
+        _written(given)
+    return dx, dgamma, dbeta
+
+
+def _tokens(tokens, device):
+    if tokens.dtype is not torch.int32 or tokens.get_device() != device or not tokens.is_contiguous() or not tokens.dim():
+        raise ValueError(f"tokens must be contiguous int32 of at least one dimension on GPU {device}")
+    return tokens.data_ptr(), tokens.numel()
+
+
+def embedding(tokens, table, *, scale=1.0, y=None):
+    """scale times the rows of table [vocab, channels] (rows may be strided) that tokens [...] int32 name, 0 for tokens outside
+    the table (kg_embedding). Returns y [..., channels] of the table's type (into `y` when given)."""
+    ptr, ld = _rows(table, "table")
+    vocab, c = table.shape
+    dev = table.get_device()
+    tp, n = _tokens(tokens, dev)
+    shape = (*tokens.shape, c)
+    given = y
+    if y is None:
+        y = torch.empty(shape, dtype=table.dtype, device=table.device)
+        yp, ldy = y.data_ptr(), c
+    else:
+        if y.shape != shape or y.dtype is not table.dtype or y.get_device() != dev:
+            raise ValueError(f"y must be {shape} of the table's type on GPU {dev}")
+        yp, ldy = _points(y, "y")
+    try:
+        args = _EMBED_ARGS.pack(n, vocab, c, TYPES[table.dtype], tp, scale, ptr, ld, yp, ldy, 0, 0, 0, 0, 0, 0, 0)
+    except struct.error as e:
+        raise _out_of_range("embedding", e) from None
+    L = _library()
+    if L.kg_embedding(dev, _stream(dev), args):
+        _check(1)
+    if given is not None:
+        _written(given)
+    return y
+
+
+def embedding_backward(dy, tokens, vocab, *, scale=1.0, grad=None, dtype=None, accumulate=False):
+    """The gradient [vocab, channels] of embedding's table from that of its y, dy [..., channels] (kg_embedding_backward), of dy's type
+    or float32 (`dtype`, dy's by default). Into `grad` when given (rows may be strided); with accumulate it is added to what grad
+    holds, and rows that no token names stay as they are."""
+    ptr, ld = _points(dy, "dy")
+    dev, c = dy.get_device(), dy.shape[-1]
+    tp, n = _tokens(tokens, dev)
+    if dy.shape[:-1] != tokens.shape:
+        raise ValueError(f"dy must be {(*tokens.shape, 'channels')}")
+    vocab = operator.index(vocab)
+    given = grad
+    if grad is None:
+        if accumulate:
+            raise ValueError("accumulate needs grad")
+        if not 1 <= vocab <= 1 << 30:
+            raise ValueError("vocab must be in [1, 2^30]")
+        grad = torch.empty((vocab, c), dtype=dtype or dy.dtype, device=dy.device)
+    elif grad.shape != (vocab, c) or grad.get_device() != dev or (dtype is not None and grad.dtype is not dtype):
+        raise ValueError(f"grad must be [{vocab}, {c}] on GPU {dev}" + (f" of {dtype}" if dtype else ""))
+    gp, ldg = _rows(grad, "grad")
+    L = _library()
+    work = _workspace(L.kg_embedding_backward_workspace(n, vocab, c) if n <= 1 << 30 else 0, dy.device)
+    try:
+        args = _EMBED_ARGS.pack(n, vocab, c, TYPES[dy.dtype], tp, scale, 0, 0, 0, 0, ptr, ld, TYPES[grad.dtype], bool(accumulate), gp, ldg,
+                                work.data_ptr() if work is not None else 0)
+    except struct.error as e:
+        raise _out_of_range("embedding_backward", e) from None
+    if L.kg_embedding_backward(dev, _stream(dev), args):
+        _check(1)
+    if given is not None:
+        _written(given)
+    return grad
 
 
 class AdamW:

@@ -16,7 +16,8 @@ namespace kgx {
 namespace {
 
 constexpr int LT = 256;        // threads of a workgroup
-constexpr int kMostParts = 512;  // of the rows, for the sums over them
+constexpr int kMostParts = 1024;  // of the rows, for the sums over them
+constexpr int kGrid = 2048;       // workgroups that take the rows in turn
 
 struct LayerArgs {
   const void *x, *dy;
@@ -25,8 +26,8 @@ struct LayerArgs {
   const float *gamma, *beta;
   float *mean, *rstd, *dgamma, *dbeta;
   float* parts;  // [parts][2][channels] sums of dy h and dy over a part's rows
-  int rows, channels, rms, split;
-  double eps;
+  int rows, channels, rms, past, split;
+  double eps, inverse;  // inverse: 1 / channels
 };
 
 // (NaN stays NaN: a comparison, not fmax.)
@@ -35,10 +36,254 @@ __device__ __forceinline__ float root_of(double variance, double eps) { return (
 // The deviations' mean where it says something of the row's mean. Below 2^-22 of their size it is their own rounding: values on a
 // coarse grid less a mean off that grid are rounded the same way all over a binade (2047 rows of 10007 f16 whose mean was 0.01 of
 // their size: the means were off by 4e-6 with it, by 8e-8 without).
-__device__ __forceinline__ double correction(double off, double square, int channels) {
-  const double m = off / channels, size = square / channels;
-  return m * m > 0x1p-44 * size ? m : 0.0;
+__device__ __forceinline__ double correction(double off, double squares) { return off * off > 0x1p-44 * squares ? off : 0.0; }
+
+// ---- Rows that fit the registers of their lanes: one read. ----
+
+// L lanes a row: neighbours of one wave (several rows a wave below 64), or a workgroup. Lane i holds chunks i, i + L, ... of 16
+// bytes; what lies past the row's end is 0 in the words.
+template <typename T, int L, int E>
+struct Row {
+  static constexpr int V = kVec<T>, THREADS = L <= 64 ? LT : L, ROWS = THREADS / L;  // of a workgroup
+  typedef typename AnyWords<T>::type words_t;
+  static __device__ __forceinline__ int lane() { return threadIdx.x % L; }
+  static __device__ __forceinline__ void load(const T* row, int channels, bool in, u32x4 (&raw)[E]) {
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const int c = (lane() + e * L) * V, left = in ? channels - c : 0;
+      raw[e] = u32x4{0, 0, 0, 0};
+      if (left >= V) {
+        raw[e] = *(const words_t*)(row + c);
+      } else if (left > 0) {
+        unsigned w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < V - 1; j++)
+          if (j < left) {
+            if constexpr (sizeof(T) == 4) w[j] = ((const unsigned*)row)[c + j];
+            else w[j >> 1] |= (unsigned)((const unsigned short*)row)[c + j] << (j & 1 ? 16 : 0);
+          }
+        raw[e] = u32x4{w[0], w[1], w[2], w[3]};
+      }
+    }
+  }
+  static __device__ __forceinline__ void store(T* row, int channels, int e, bool past, const float (&f)[V]) {
+    const int c = (lane() + e * L) * V, left = channels - c;
+    if (left >= V) {
+      const words_t w = words_of<T>(f);
+      if (past) {
+        asm volatile("");  // (or the two stores become one, a plain one)
+        __builtin_nontemporal_store(w, (words_t*)(row + c));
+        asm volatile("");
+      } else {
+        *(words_t*)(row + c) = w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < V - 1; j++)
+        if (j < left) row[c + j] = to_t<T>(f[j]);
+    }
+  }
+  // A lane's share of a vector of the channels, `none` where there is no vector.
+  static __device__ __forceinline__ void vector(const float* p, int channels, float none, float (&f)[E][V]) {
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const int c = (lane() + e * L) * V;
+      if (p && c + V <= channels) {
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+          const f32x4_any w = *(const f32x4_any*)(p + c + j);
+#pragma unroll
+          for (int k = 0; k < 4; k++) f[e][j + k] = w[k];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; j++) f[e][j] = p && c + j < channels ? p[c + j] : none;
+      }
+    }
+  }
+  // Sums over the row, in each of its lanes. red: of the workgroup, another one from call to call in turns of two or more.
+  template <int N>
+  static __device__ __forceinline__ void sum(float (&v)[N], float (*red)[N]) {
+#pragma unroll
+    for (int k = 0; k < N; k++) v[k] = share_sum(v[k], L < 64 ? L : 64);
+    if constexpr (L > 64) {
+      if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int k = 0; k < N; k++) red[threadIdx.x >> 6][k] = v[k];
+      lds_barrier();
+#pragma unroll
+      for (int k = 0; k < N; k++) {
+        float t[L / 64];
+#pragma unroll
+        for (int w = 0; w < L / 64; w++) t[w] = red[w][k];
+#pragma unroll
+        for (int o = L / 128; o >= 1; o >>= 1)
+#pragma unroll
+          for (int w = 0; w < o; w++) t[w] += t[w + o];
+        v[k] = t[0];
+      }
+    }
+  }
+};
+
+template <typename T, int L, int E>
+__global__ __launch_bounds__((Row<T, L, E>::THREADS)) void layer_norm_held_kernel(LayerArgs a) {
+  using R = Row<T, L, E>;
+  constexpr int V = R::V;
+  __shared__ float red[2][16][1], red2[2][16][2];
+  float gamma[E][V], beta[E][V];
+  R::vector(a.gamma, a.channels, 1.f, gamma);
+  R::vector(a.beta, a.channels, 0.f, beta);
+  int turn = 0;
+  for (int first = blockIdx.x * R::ROWS; first < a.rows; first += gridDim.x * R::ROWS) {
+    const int row = first + threadIdx.x / L;
+    const bool in = row < a.rows;
+    u32x4 raw[E];
+    R::load((const T*)a.x + (size_t)row * a.ldx, a.channels, in, raw);
+    float mean = 0.f;
+    if (!a.rms) {
+      float s[1] = {0.f};
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        float t = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; j++) t += element<T>(raw[e], j);
+        s[0] += t;
+      }
+      R::sum(s, red[turn]);
+      mean = (float)((double)s[0] * a.inverse);
+    }
+    float q[2] = {0.f, 0.f};  // of the deviations, and of their squares
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const int left = a.channels - (R::lane() + e * L) * V;
+      float t = 0.f, u = 0.f;
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        const float d = j < left ? element<T>(raw[e], j) - mean : 0.f;
+        t += d;
+        u = __builtin_fmaf(d, d, u);
+      }
+      q[0] += t;
+      q[1] += u;
+    }
+    R::sum(q, red2[turn]);
+    turn ^= 1;
+    const double squares = (double)q[1] * a.inverse, m = a.rms ? 0.0 : correction((double)q[0] * a.inverse, squares);
+    const float rstd = root_of(squares - m * m, a.eps), shift = (float)m;
+    if (!in) continue;
+    T* y = (T*)a.y + (size_t)row * a.ldy;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      float f[V];
+#pragma unroll
+      for (int j = 0; j < V; j++) f[j] = __builtin_fmaf(((element<T>(raw[e], j) - mean) - shift) * rstd, gamma[e][j], beta[e][j]);
+      R::store(y, a.channels, e, a.past, f);
+    }
+    if (R::lane() == 0) {
+      if (!a.rms) a.mean[row] = (float)((double)mean + m);
+      a.rstd[row] = rstd;
+    }
+  }
 }
+
+// The rows of a workgroup one after another, with the channels' sums of dy h and dy in registers: a part for each workgroup.
+template <typename T, int L, int E>
+__global__ __launch_bounds__((Row<T, L, E>::THREADS)) void layer_norm_back_held_kernel(LayerArgs a) {
+  using R = Row<T, L, E>;
+  constexpr int V = R::V, SPAN = L * E * V;  // elements that a row's lanes hold
+  __shared__ float red[2][16][2];
+  __shared__ float joined[L <= 64 ? 2 * SPAN : 1];
+  float gamma[E][V], s1[E][V] = {}, s2[E][V] = {};
+  R::vector(a.gamma, a.channels, 1.f, gamma);
+  int turn = 0;
+  for (int first = blockIdx.x * R::ROWS; first < a.rows; first += gridDim.x * R::ROWS) {
+    const int row = first + threadIdx.x / L;
+    const bool in = row < a.rows;
+    u32x4 x[E], dy[E];
+    R::load((const T*)a.x + (size_t)row * a.ldx, a.channels, in, x);
+    R::load((const T*)a.dy + (size_t)row * a.lddy, a.channels, in, dy);
+    const float mean = a.rms || !in ? 0.f : a.mean[row], rstd = in ? a.rstd[row] : 0.f;
+    float q[2] = {0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      float t = 0.f, u = 0.f;
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        // (Past the row's end dy is 0.)
+        const float g = element<T>(dy[e], j), d = g * gamma[e][j], h = (element<T>(x[e], j) - mean) * rstd;
+        t += d;
+        u = __builtin_fmaf(d, h, u);
+        s1[e][j] = __builtin_fmaf(g, h, s1[e][j]);
+        s2[e][j] += g;
+      }
+      q[0] += t;
+      q[1] += u;
+    }
+    R::sum(q, red[turn]);
+    turn ^= 1;
+    if (!in) continue;
+    const float m1 = a.rms ? 0.f : (float)((double)q[0] * a.inverse), m2 = (float)((double)q[1] * a.inverse);
+    T* dx = (T*)a.dx + (size_t)row * a.lddx;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      float f[V];
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        const float d = element<T>(dy[e], j) * gamma[e][j], h = (element<T>(x[e], j) - mean) * rstd;
+        f[j] = rstd * __builtin_fmaf(-h, m2, d - m1);
+      }
+      R::store(dx, a.channels, e, a.past, f);
+    }
+  }
+  if (!a.dgamma && !a.dbeta) return;
+  float* part = a.parts + (size_t)blockIdx.x * 2 * a.channels;
+  if constexpr (L <= 64) {
+    // The rows that a wave held side by side, then its waves in turn.
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+#pragma unroll
+        for (int o = L; o < 64; o <<= 1) {
+          s1[e][j] += __shfl_xor(s1[e][j], o);
+          s2[e][j] += __shfl_xor(s2[e][j], o);
+        }
+      }
+    }
+    for (int w = 0; w < LT / 64; w++) {
+      if (threadIdx.x >> 6 == w && (threadIdx.x & 63) < L) {
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+#pragma unroll
+          for (int j = 0; j < V; j++) {
+            float* at = joined + (R::lane() + e * L) * V + j;
+            at[0] = (w ? at[0] : 0.f) + s1[e][j];
+            at[SPAN] = (w ? at[SPAN] : 0.f) + s2[e][j];
+          }
+        }
+      }
+      lds_barrier();
+    }
+    for (int c = threadIdx.x; c < a.channels; c += LT) {
+      part[c] = joined[c];
+      part[a.channels + c] = joined[SPAN + c];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const int c = (R::lane() + e * L) * V;
+#pragma unroll
+      for (int j = 0; j < V; j++)
+        if (c + j < a.channels) {
+          part[c + j] = s1[e][j];
+          part[a.channels + c + j] = s2[e][j];
+        }
+    }
+  }
+}
+
+// ---- Any row. ----
 
 // A workgroup a row, whatever its width.
 template <typename T>
@@ -52,7 +297,7 @@ __global__ __launch_bounds__(LT) void layer_norm_kernel(LayerArgs a) {
     if (!a.rms) {
       float sum = 0.f;
       for (int c = tid; c < a.channels; c += LT) sum += (float)x[c];
-      mean = (float)(row_sum<LT>(sum, red) / a.channels);
+      mean = (float)(row_sum<LT>(sum, red) * a.inverse);
     }
     float off = 0.f, square = 0.f;
     for (int c = tid; c < a.channels; c += LT) {
@@ -60,9 +305,9 @@ __global__ __launch_bounds__(LT) void layer_norm_kernel(LayerArgs a) {
       off += d;
       square = __builtin_fmaf(d, d, square);
     }
-    const double squares = row_sum<LT>(square, red);
-    const double m = a.rms ? 0.0 : correction(row_sum<LT>(off, red), squares, a.channels);
-    const float rstd = root_of(squares / a.channels - m * m, a.eps), shift = (float)m;
+    const double squares = row_sum<LT>(square, red) * a.inverse;
+    const double m = a.rms ? 0.0 : correction(row_sum<LT>(off, red) * a.inverse, squares);
+    const float rstd = root_of(squares - m * m, a.eps), shift = (float)m;
     for (int c = tid; c < a.channels; c += LT) {
       const float h = (((float)x[c] - mean) - shift) * rstd;
       y[c] = to_t<T>(__builtin_fmaf(h, a.gamma ? a.gamma[c] : 1.f, a.beta ? a.beta[c] : 0.f));
@@ -89,7 +334,7 @@ __global__ __launch_bounds__(LT) void layer_norm_back_kernel(LayerArgs a) {
       s1 += d;
       s2 = __builtin_fmaf(d, ((float)x[c] - mean) * rstd, s2);
     }
-    const float m1 = a.rms ? 0.f : (float)(row_sum<LT>(s1, red) / a.channels), m2 = (float)(row_sum<LT>(s2, red) / a.channels);
+    const float m1 = a.rms ? 0.f : (float)(row_sum<LT>(s1, red) * a.inverse), m2 = (float)(row_sum<LT>(s2, red) * a.inverse);
     for (int c = tid; c < a.channels; c += LT) {
       const float d = (float)dy[c] * (a.gamma ? a.gamma[c] : 1.f), h = ((float)x[c] - mean) * rstd;
       dx[c] = to_t<T>(rstd * __builtin_fmaf(-h, m2, d - m1));
@@ -114,17 +359,57 @@ __global__ __launch_bounds__(LT) void layer_norm_sums_kernel(LayerArgs a) {
   }
 }
 
-// The parts' sums joined in double.
-__global__ __launch_bounds__(LT) void layer_norm_params_kernel(LayerArgs a) {
-  for (long long i = (long long)blockIdx.x * LT + threadIdx.x; i < 2ll * a.channels; i += (long long)gridDim.x * LT) {
-    double s = 0.0;
-    for (int p = 0; p < a.split; p++) s += (double)a.parts[(size_t)p * 2 * a.channels + i];
-    float* out = i < a.channels ? a.dgamma : a.dbeta;
-    if (out) out[i < a.channels ? i : i - a.channels] = (float)s;
+// The parts' sums joined in double: a workgroup takes 64 of the sums, PG groups of 16 threads the parts in turn.
+constexpr int PT = 1024, PG = PT / 16;
+__global__ __launch_bounds__(PT) void layer_norm_params_kernel(LayerArgs a) {
+  __shared__ double joined[PG][65];
+  const int lane = threadIdx.x & 15, group = threadIdx.x >> 4;
+  for (long long first = blockIdx.x * 64ll; first < 2ll * a.channels; first += gridDim.x * 64ll) {
+    double s[4] = {0.0, 0.0, 0.0, 0.0};
+    const long long at = first + lane * 4;
+#pragma unroll 4
+    for (int p = group; p < a.split; p += PG) {
+      float f[4];
+      load_vec<float>(a.parts + (size_t)p * 2 * a.channels + at, (int)max(min(2ll * a.channels - at, 4ll), 0ll), f);
+#pragma unroll
+      for (int j = 0; j < 4; j++) s[j] += (double)f[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; j++) joined[group][lane * 4 + j] = s[j];
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      double t = 0.0;
+#pragma unroll 8
+      for (int g = 0; g < PG; g++) t += joined[g][threadIdx.x];
+      const long long i = first + threadIdx.x;
+      float* out = i < a.channels ? a.dgamma : a.dbeta;
+      if (out && i < 2ll * a.channels) out[i < a.channels ? i : i - a.channels] = (float)t;
+    }
   }
 }
 
-int parts_of(int rows) { return std::min(std::max(rows / 8, 1), kMostParts); }
+// ---- Launches. ----
+
+// How a row lies: L lanes with E chunks each; lanes 0 where no variant holds it.
+struct Shape {
+  int lanes = 0, each = 0;
+};
+// (Narrow rows share a wave, so that its lanes are busy and their sums take fewer steps.)
+Shape shape_of(int channels, int vec, bool backward) {
+  const int chunks = (channels + vec - 1) / vec;
+  if (chunks <= 8) return {8, 1};
+  if (chunks <= 64) return {16, (chunks + 15) / 16};
+  if (chunks <= 256) return {64, (chunks + 63) / 64};
+  if (chunks <= 512) return {256, 2};
+  if (chunks <= 1024) return {512, 2};
+  if (chunks <= 2048) return {1024, 2};
+  if (chunks <= 4096 && !backward) return {1024, 4};
+  return {};
+}
+
+// Workgroups of the backward pass, each with a part of the sums: at least eight rows each once there is one for each CU.
+int parts_of(int rows, int per) { return (int)std::min((rows + (long long)per - 1) / per, (long long)std::min(std::max(256, rows / 8), kMostParts)); }
 
 LayerArgs args_of(const kg_layer_norm_args& a) {
   LayerArgs p;
@@ -137,45 +422,74 @@ LayerArgs args_of(const kg_layer_norm_args& a) {
   p.dgamma = a.dgamma; p.dbeta = a.dbeta;
   p.parts = (float*)a.workspace;
   p.rows = a.rows; p.channels = a.channels; p.rms = a.rms != 0;
-  p.split = parts_of(a.rows);
+  p.past = gradient_past(a.rows, a.channels, a.type);
+  p.split = 0;
   p.eps = a.eps;
+  p.inverse = 1.0 / a.channels;
   return p;
 }
 
+template <typename T, int L, int E>
+void held(LayerArgs p, bool backward, hipStream_t s) {
+  constexpr int per = Row<T, L, E>::ROWS;
+  if (backward) {
+    p.split = parts_of(p.rows, per);
+    launch_k(layer_norm_back_held_kernel<T, L, E>, dim3(p.split), Row<T, L, E>::THREADS, 0, s, p);
+  } else {
+    launch_k(layer_norm_held_kernel<T, L, E>, dim3(std::min(row_grid(p.rows, per), kGrid)), Row<T, L, E>::THREADS, 0, s, p);
+  }
+}
+
+// Returns the parts that the sums over the rows are in.
 template <typename T>
-void backward_typed(const LayerArgs& p, hipStream_t s) {
-  launch_k(layer_norm_back_kernel<T>, dim3(row_grid(p.rows, 1)), LT, 0, s, p);
-  if (p.dgamma || p.dbeta)
-    launch_k(layer_norm_sums_kernel<T>, dim3(std::min((p.channels + LT - 1) / LT, 1024), p.split), LT, 0, s, p);
+int rows_typed(LayerArgs p, bool backward, hipStream_t s) {
+  const Shape r = shape_of(p.channels, kVec<T>, backward);
+  p.split = parts_of(p.rows, r.lanes == 0 || r.lanes > 64 ? 1 : LT / r.lanes);
+  if (r.lanes == 8) held<T, 8, 1>(p, backward, s);
+  else if (r.lanes == 16 && r.each == 1) held<T, 16, 1>(p, backward, s);
+  else if (r.lanes == 16 && r.each == 2) held<T, 16, 2>(p, backward, s);
+  else if (r.lanes == 16 && r.each == 3) held<T, 16, 3>(p, backward, s);
+  else if (r.lanes == 16) held<T, 16, 4>(p, backward, s);
+  else if (r.lanes == 64 && r.each == 2) held<T, 64, 2>(p, backward, s);
+  else if (r.lanes == 64 && r.each == 3) held<T, 64, 3>(p, backward, s);
+  else if (r.lanes == 64) held<T, 64, 4>(p, backward, s);
+  else if (r.lanes == 256) held<T, 256, 2>(p, backward, s);
+  else if (r.lanes == 512) held<T, 512, 2>(p, backward, s);
+  else if (r.lanes == 1024 && r.each == 2) held<T, 1024, 2>(p, backward, s);
+  else if (r.lanes == 1024) launch_k(layer_norm_held_kernel<T, 1024, 4>, dim3(std::min(row_grid(p.rows, 1), kGrid)), 1024, 0, s, p);
+  else if (!backward) launch_k(layer_norm_kernel<T>, dim3(row_grid(p.rows, 1)), LT, 0, s, p);
+  else {
+    launch_k(layer_norm_back_kernel<T>, dim3(row_grid(p.rows, 1)), LT, 0, s, p);
+    if (p.dgamma || p.dbeta)
+      launch_k(layer_norm_sums_kernel<T>, dim3(std::min((p.channels + LT - 1) / LT, 1024), p.split), LT, 0, s, p);
+  }
+  return p.split;
+}
+
+int rows_of(const LayerArgs& p, int type, bool backward, hipStream_t s) {
+  switch (type) {
+    case PREC_F32: return rows_typed<float>(p, backward, s);
+    case PREC_F16: return rows_typed<f16>(p, backward, s);
+    default: return rows_typed<bf16>(p, backward, s);
+  }
 }
 
 }  // namespace
 
 size_t layer_norm_workspace(int rows, int channels) {
   if (rows < 1 || channels < 1) return 0;
-  return (size_t)parts_of(rows) * 2 * channels * sizeof(float);
+  return (size_t)parts_of(rows, 1) * 2 * channels * sizeof(float);
 }
 
 void launch_layer_norm(const kg_layer_norm_args& a, hipStream_t s) {
-  const LayerArgs p = args_of(a);
-  const dim3 grid(row_grid(p.rows, 1));
-  switch (a.type) {
-    case PREC_F32: launch_k(layer_norm_kernel<float>, grid, LT, 0, s, p); break;
-    case PREC_F16: launch_k(layer_norm_kernel<f16>, grid, LT, 0, s, p); break;
-    default: launch_k(layer_norm_kernel<bf16>, grid, LT, 0, s, p); break;
-  }
+  rows_of(args_of(a), a.type, false, s);
   KGX_CHECK_LAUNCH();
 }
 
 void launch_layer_norm_backward(const kg_layer_norm_args& a, hipStream_t s) {
   LayerArgs p = args_of(a);
-  if (!p.rows) p.split = 0;  // (the sums over no rows are 0)
-  else switch (a.type) {
-    case PREC_F32: backward_typed<float>(p, s); break;
-    case PREC_F16: backward_typed<f16>(p, s); break;
-    default: backward_typed<bf16>(p, s); break;
-  }
-  if (p.dgamma || p.dbeta) launch_k(layer_norm_params_kernel, dim3((int)std::min((2ll * p.channels + LT - 1) / LT, 65536ll)), LT, 0, s, p);
+  if (p.rows) p.split = rows_of(p, a.type, true, s);  // (the sums over no rows are 0)
+  if (p.dgamma || p.dbeta) launch_k(layer_norm_params_kernel, dim3((int)std::min((2ll * p.channels + 63) / 64, 65536ll)), PT, 0, s, p);
   KGX_CHECK_LAUNCH();
 }
 

@@ -9,7 +9,7 @@
 
 #include "kgx_device.h"
 #include "kgx_learn.h"
-#include "kgx_vec.h"
+#include "kgx_rows.h"
 
 namespace kgx {
 
@@ -19,22 +19,34 @@ constexpr int ET = 256;       // threads of a workgroup
 constexpr int ST = 1024;      // of the sort's
 constexpr int kDigit = 9;     // bits of a digit, at most
 constexpr int kMostBlocks = 64;  // of tokens, in the sort
+constexpr long long kFewColumns = 1 << 20;  // two threads for each that the card holds
 constexpr int FR = 16;        // rows that a wave looks for at once
 
-template <typename T>
+// A thread a column of 16 bytes of EACH rows, whose loads are under way together.
+template <typename T, int EACH>
 __global__ __launch_bounds__(ET) void embedding_kernel(const int* tokens, const T* table, T* y, long long ld, long long ld_y, int count,
-                                                       int vocab, int channels, int chunks, float scale) {
+                                                       int vocab, int channels, int chunks, float scale, int past) {
   constexpr int V = kVec<T>;
-  const long long all = (long long)count * chunks;
+  const int groups = (count + EACH - 1) / EACH;
+  const long long all = (long long)groups * chunks;
   for (long long id = (long long)blockIdx.x * ET + threadIdx.x; id < all; id += (long long)gridDim.x * ET) {
-    const int i = (int)(id / chunks), c = (int)(id - (long long)i * chunks) * V, token = tokens[i];
-    float f[V] = {};
-    if ((unsigned)token < (unsigned)vocab) {
-      load_vec<T>(table + (size_t)token * ld + c, channels - c, f);
+    const int group = (int)(id / chunks), c = (int)(id - (long long)group * chunks) * V, i0 = group * EACH;
+    float f[EACH][V] = {};
+    int token[EACH];
 #pragma unroll
-      for (int j = 0; j < V; j++) f[j] *= scale;
+    for (int k = 0; k < EACH; k++) token[k] = i0 + k < count ? tokens[i0 + k] : -1;
+#pragma unroll
+    for (int k = 0; k < EACH; k++)
+      if ((unsigned)token[k] < (unsigned)vocab) load_vec<T>(table + (size_t)token[k] * ld + c, channels - c, f[k]);
+#pragma unroll
+    for (int k = 0; k < EACH; k++) {
+      if (i0 + k >= count) break;
+#pragma unroll
+      for (int j = 0; j < V; j++) f[k][j] *= scale;
+      T* to = y + (size_t)(i0 + k) * ld_y + c;
+      if (past && c + V <= channels) store_past<T>(to, f[k]);
+      else store_vec<T>(to, channels - c, f[k]);
     }
-    store_vec<T>(y + (size_t)i * ld_y + c, channels - c, f);
   }
 }
 
@@ -43,11 +55,33 @@ __global__ __launch_bounds__(ET) void embedding_kernel(const int* tokens, const 
 // Tokens outside the table are behind all others.
 __device__ __forceinline__ unsigned key_of(int token, int vocab) { return min((unsigned)token, (unsigned)vocab); }
 
+// 0 in every row, by the workgroups behind those that sort, while these wait for memory: where most rows are not named, that is less
+// than finding them afterwards takes (100003 rows of 512 f16, 5003 tokens: @ us, @ otherwise).
+struct FillArgs {
+  void* grad;
+  long long ld;    // bytes
+  long long bytes;
+  int rows, groups;  // groups: workgroups that sort
+};
+__device__ __forceinline__ bool fills(const FillArgs& f) {
+  if ((int)blockIdx.x < f.groups) return false;
+  const int wave = (blockIdx.x - f.groups) * (ST / 64) + (threadIdx.x >> 6), waves = (gridDim.x - f.groups) * (ST / 64);
+  for (int row = wave; row < f.rows; row += waves) {
+    char* p = (char*)f.grad + (size_t)row * f.ld;
+    for (long long c = (threadIdx.x & 63) * 16; c < f.bytes; c += 1024) {
+      if (c + 16 <= f.bytes) *(u32x4_any2*)(p + c) = u32x4{0, 0, 0, 0};
+      else for (long long k = c; k < f.bytes; k += 2) *(unsigned short*)(p + k) = 0;
+    }
+  }
+  return true;
+}
+
 // Few tokens: each one's place is the number of tokens before it, counted. RI tokens a workgroup, whose threads share the tokens
 // that they are compared with, 64 ways: 5003 tokens in 5 us, where two launches for each digit take 20.
 constexpr int kRanked = 8192, RI = 16;
 __global__ __launch_bounds__(ST) void sort_rank_kernel(const int* __restrict__ tokens, unsigned* __restrict__ keys, int* __restrict__ places,
-                                                       int count, int vocab) {
+                                                       int count, int vocab, FillArgs fill) {
+  if (fills(fill)) return;
   __shared__ __align__(16) unsigned all[kRanked];
   __shared__ int part[ST / 64][RI];
   const int tid = threadIdx.x, w = tid >> 6, item = tid & (RI - 1), share = (w << 2) | (tid & 63) / RI;
@@ -56,12 +90,14 @@ __global__ __launch_bounds__(ST) void sort_rank_kernel(const int* __restrict__ t
   __syncthreads();
   const int i = blockIdx.x * RI + item;
   const unsigned key = all[min(i, room - 1)];
-  // A token before this one counts where its key is no larger, one behind where it is less: the shares cross from the ones to the others
-  // at i.
+  // A token before this one counts where its key is no larger, one behind where it is less. Those of the workgroup's own RI are both.
+  const int i0 = blockIdx.x * RI;
   int n = 0;
   for (int j = share * 4; j < room; j += 256) {
     const uint4 k = *(const uint4*)(all + j);
-    n += (k.x < key + (j < i)) + (k.y < key + (j + 1 < i)) + (k.z < key + (j + 2 < i)) + (k.w < key + (j + 3 < i));
+    const unsigned limit = key + (j < i0);
+    n += (k.x < limit) + (k.y < limit) + (k.z < limit) + (k.w < limit);
+    if (j >= i0 && j < i0 + RI) n += (k.x == key && j < i) + (k.y == key && j + 1 < i) + (k.z == key && j + 2 < i) + (k.w == key && j + 3 < i);
   }
   for (int o = RI; o < 64; o <<= 1) n += __shfl_xor(n, o);
   if ((tid & 63) < RI) part[w][item] = n;
@@ -74,33 +110,34 @@ __global__ __launch_bounds__(ST) void sort_rank_kernel(const int* __restrict__ t
   }
 }
 
-// More: by digits from the lowest, two launches for the first and one for each other: a launch that moves the tokens by a digit counts
-// the next digit at their new places.
+// More: by digits from the lowest, two launches for each. (Counting the next digit at the tokens' new places in the launch that moves
+// them, by atomics, took 10 us more of it, and the launch that it saves takes 5.)
 struct SortArgs {
   const int* tokens;
   const unsigned* keys;  // sorted by lower digits, with their places; the first pass reads the tokens themselves
   const int* places;
   unsigned* keys_out;
   int* places_out;
-  int *counts, *next_counts;  // [blocks][2^bits] of this digit and, but for the last, the next one
-  int count, vocab, blocks, each, shift, bits, rest;  // each: tokens of a block, a multiple of ST; rest: counts behind these, to be cleared
+  int* counts;  // [blocks][2^bits]
+  int count, vocab, blocks, each, shift, bits;  // each: tokens of a block, a multiple of ST
 };
 
-__global__ __launch_bounds__(ST) void sort_count_kernel(SortArgs a) {
+template <bool FIRST>
+__global__ __launch_bounds__(ST) void sort_count_kernel(SortArgs a, FillArgs fill) {
+  if (FIRST && fills(fill)) return;
   __shared__ int n[1 << kDigit];
   const int digits = 1 << a.bits, tid = threadIdx.x, b = blockIdx.x;
   for (int d = tid; d < digits; d += ST) n[d] = 0;
-  for (int k = b * ST + tid; k < a.rest; k += a.blocks * ST) a.next_counts[k] = 0;
   __syncthreads();
   for (int r = 0; r < a.each; r += ST) {
     const long long i = (long long)b * a.each + r + tid;
-    if (i < a.count) atomicAdd(&n[key_of(a.tokens[i], a.vocab) & (digits - 1)], 1);
+    if (i < a.count) atomicAdd(&n[(FIRST ? key_of(a.tokens[i], a.vocab) : a.keys[i]) >> a.shift & (digits - 1)], 1);
   }
   __syncthreads();
   for (int d = tid; d < digits; d += ST) a.counts[b * digits + d] = n[d];
 }
 
-template <bool FIRST, bool LAST>
+template <bool FIRST>
 __global__ __launch_bounds__(ST) void sort_move_kernel(SortArgs a) {
   constexpr int WAVES = ST / 64;
   __shared__ int to[WAVES][1 << kDigit];  // where a wave's next token of a digit goes
@@ -157,7 +194,6 @@ __global__ __launch_bounds__(ST) void sort_move_kernel(SortArgs a) {
       a.keys_out[at] = key;
       a.places_out[at] = FIRST ? (int)i : a.places[i];
       if (same >> lane == 1) to[w][d] = at + 1;  // (the last of its digit; the reads above came before, in one wave's order)
-      if (!LAST) atomicAdd(&a.next_counts[at / a.each * digits + (key >> (a.shift + a.bits) & (digits - 1))], 1);
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -172,7 +208,7 @@ struct SumArgs {
   void* grad;
   float* parts;  // [ranges][2][channels]: the sum of a run from before the range, and of one that goes on behind it
   long long ld, ld_grad;
-  int count, vocab, channels, ranges, each, slabs, sum_groups, accumulate;  // slabs: of a row's columns; sum_groups: workgroups that sum
+  int count, vocab, channels, ranges, each, slabs, sum_groups, accumulate, filled;  // slabs: of a row's columns; sum_groups: workgroups that sum
   float scale;
 };
 
@@ -196,17 +232,19 @@ __device__ __forceinline__ void put(G* p, int left, const float (&sum)[N], float
   }
 }
 
-// The first sorted place whose key is at least `key`.
+// The first sorted place whose key is at least `key`, by seven probes at a time: each step waits for memory.
 __device__ __forceinline__ int lower_bound(const unsigned* keys, int count, unsigned key) {
-  int lo = 0, n = count;
-  while (n > 0) {
-    const int half = n >> 1;
-    if (keys[lo + half] < key) {
-      lo += half + 1;
-      n -= half + 1;
-    } else {
-      n = half;
+  int lo = 0, hi = count;
+  while (lo < hi) {
+    const int step = (hi - lo + 7) / 8;
+    int below = 0;
+#pragma unroll
+    for (int t = 1; t < 8; t++) {
+      const int at = lo + t * step - 1;
+      below += at < hi && keys[min(at, hi - 1)] < key;
     }
+    lo += below * step;
+    if (below < 7) hi = min(hi, lo + step - 1);
   }
   return lo;
 }
@@ -306,40 +344,49 @@ __global__ __launch_bounds__(ET) void embedding_sums_kernel(SumArgs a) {
   if (run < a.vocab) end_run(next == run);
 }
 
-// Runs over several ranges: a workgroup for 256 channels of each range that such a run begins in, its waves for the ranges in turn.
-constexpr int JT = 512;
+// Runs over several ranges: a workgroup for up to JS slabs of 256 channels of each range that such a run begins in. Its waves are
+// `wide` slabs side by side, and share the ranges where there are fewer.
+constexpr int JT = 512, JS = JT / 64;
 template <typename G>
-__global__ __launch_bounds__(JT) void embedding_join_kernel(SumArgs a, int slabs) {
-  __shared__ double joined[JT / 64][64][4];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const long long all = (long long)(a.ranges - 1) * slabs;
+__global__ __launch_bounds__(JT) void embedding_join_kernel(SumArgs a, int blocks, int wide) {
+  __shared__ float4 joined[JS][64];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slab = w & (wide - 1), step = JS / wide;
+  const long long all = (long long)(a.ranges - 1) * blocks;
   for (long long id = blockIdx.x; id < all; id += gridDim.x) {
-    const int range = (int)(id / slabs), c = (int)(id - (long long)range * slabs) * 256 + lane * 4;
+    const int range = (int)(id / blocks), c = ((int)(id - (long long)range * blocks) * JS + slab) * 256 + lane * 4;
     const int first = range * a.each, last = first + a.each;  // (one more range follows)
-    const unsigned key = a.keys[last];
-    if (key >= (unsigned)a.vocab || a.keys[last - 1] != key) continue;
-    if (a.keys[first] == key && first > 0 && a.keys[first - 1] == key) continue;  // begins before
-    const int ends = (lower_bound(a.keys, a.count, key + 1) - 1) / a.each;        // the range of its last token
+    const unsigned key = a.keys[last], at_first = a.keys[first], at_last = a.keys[last - 1], ahead = first > 0 ? a.keys[first - 1] : ~0u;
+    if (key >= (unsigned)a.vocab || at_last != key) continue;
+    if (at_first == key && ahead == key) continue;  // begins before
+    int ends = range + 1;  // the last range with its tokens: 64 ranges' first keys at a time
+    for (int r = range + 2; r < a.ranges; r += 64) {
+      const unsigned long long others = __ballot(r + lane >= a.ranges || a.keys[min(r + lane, a.ranges - 1) * a.each] != key);
+      ends = r + (others ? __ffsll(others) - 1 : 64) - 1;
+      if (others) break;
+    }
     double sum[4] = {0.0, 0.0, 0.0, 0.0};
+    const int left = max(a.channels - c, 0);
 #pragma unroll 4
-    for (int r = range + w; r <= ends; r += JT / 64) {
+    for (int r = range + w / wide; r <= ends; r += step) {
       float f[4];
-      load_vec<float>(a.parts + ((size_t)r * 2 + (r == range)) * a.channels + c, max(a.channels - c, 0), f);
+      load_vec<float>(a.parts + ((size_t)r * 2 + (r == range)) * a.channels + c, left, f);
 #pragma unroll
       for (int j = 0; j < 4; j++) sum[j] += (double)f[j];
     }
-#pragma unroll
-    for (int j = 0; j < 4; j++) joined[w][lane][j] = sum[j];
+    // (A share's sum is rounded to float here; at most JS of them make the row's.)
+    joined[w][lane] = float4{(float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]};
     __syncthreads();
-    if (w == 0) {
-      float f[4];
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        double t = 0.0;
-        for (int k = 0; k < JT / 64; k++) t += joined[k][lane][j];
-        f[j] = (float)t;
+    if (w < wide) {
+      for (int j = 0; j < 4; j++) sum[j] = 0.0;
+      for (int k = w; k < JS; k += wide) {
+        const float4 f = joined[k][lane];
+        sum[0] += f.x;
+        sum[1] += f.y;
+        sum[2] += f.z;
+        sum[3] += f.w;
       }
-      put<G, 4>((G*)a.grad + (size_t)key * a.ld_grad + c, max(a.channels - c, 0), f, a.scale, a.accumulate);
+      const float f[4] = {(float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]};
+      put<G, 4>((G*)a.grad + (size_t)key * a.ld_grad + c, left, f, a.scale, a.accumulate);
     }
     __syncthreads();
   }
@@ -372,45 +419,48 @@ Plan plan_of(int count, int vocab, int channels) {
   const size_t copies = p.passes > 1 ? 2 : 1;
   p.keys = room(copies * count * 4);
   p.places = room(copies * count * 4);
-  p.counts = room((size_t)p.passes * p.blocks * (4 << p.bits));
+  p.counts = room((size_t)p.blocks * (4 << p.bits));
   p.parts = room((size_t)p.ranges * 2 * channels * 4);
   return p;
 }
 
 inline int grid_of(long long threads) { return (int)std::min((threads + ET - 1) / ET, 1ll << 20); }
 
-void sort_tokens(const kg_embedding_args& a, const Plan& plan, SumArgs& p, hipStream_t s) {
+// filled: whether the launch has set every row to 0.
+void sort_tokens(const kg_embedding_args& a, const Plan& plan, SumArgs& p, bool filled, hipStream_t s) {
   char* w = (char*)a.workspace;
   unsigned* keys = (unsigned*)(w + plan.keys);
   int* places = (int*)(w + plan.places);
-  int* counts = (int*)(w + plan.counts);
   p.keys = keys;
   p.places = places;
+  FillArgs fill = {};
+  fill.groups = plan.passes ? plan.blocks : (a.count + RI - 1) / RI;
+  int more = 0;
+  if (filled) {
+    const int size = a.grad_type == PREC_F32 ? 4 : 2;
+    fill.grad = a.grad; fill.ld = a.ld_grad * size;
+    fill.rows = a.vocab; fill.bytes = (long long)a.channels * size;
+    more = std::min((a.vocab + ST / 64 - 1) / (ST / 64), 512);
+  }
   if (!plan.passes) {
-    launch_k(sort_rank_kernel, dim3((a.count + RI - 1) / RI), ST, 0, s, a.tokens, keys, places, a.count, a.vocab);
+    launch_k(sort_rank_kernel, dim3(fill.groups + more), ST, 0, s, a.tokens, keys, places, a.count, a.vocab, fill);
     return;
   }
-  const int of_pass = plan.blocks << plan.bits;
   SortArgs t = {};
   t.tokens = a.tokens;
+  t.counts = (int*)(w + plan.counts);
   t.count = a.count; t.vocab = a.vocab; t.blocks = plan.blocks; t.each = plan.each_block; t.bits = plan.bits;
   for (int k = 0; k < plan.passes; k++) {
     const dim3 grid(t.blocks);
-    const bool last = k == plan.passes - 1;
     t.shift = k * plan.bits;
     t.keys_out = keys + (size_t)(k & 1) * a.count;
     t.places_out = places + (size_t)(k & 1) * a.count;
-    t.counts = counts + (size_t)k * of_pass;
-    t.next_counts = t.counts + of_pass;
     if (k == 0) {
-      t.rest = (plan.passes - 1) * of_pass;
-      launch_k(sort_count_kernel, grid, ST, 0, s, t);
-      if (last) launch_k(sort_move_kernel<true, true>, grid, ST, 0, s, t);
-      else launch_k(sort_move_kernel<true, false>, grid, ST, 0, s, t);
-    } else if (last) {
-      launch_k(sort_move_kernel<false, true>, grid, ST, 0, s, t);
+      launch_k(sort_count_kernel<true>, dim3(t.blocks + more), ST, 0, s, t, fill);
+      launch_k(sort_move_kernel<true>, grid, ST, 0, s, t);
     } else {
-      launch_k(sort_move_kernel<false, false>, grid, ST, 0, s, t);
+      launch_k(sort_count_kernel<false>, grid, ST, 0, s, t, fill);
+      launch_k(sort_move_kernel<false>, grid, ST, 0, s, t);
     }
     p.keys = t.keys = t.keys_out;
     p.places = t.places = t.places_out;
@@ -422,11 +472,12 @@ void sums(SumArgs p, hipStream_t s) {
   const int chunks = (p.channels + kVec<T> - 1) / kVec<T>;
   p.slabs = (chunks + L - 1) / L;
   p.sum_groups = (int)(((long long)p.ranges * p.slabs + ET / L - 1) / (ET / L));
-  const int fill = p.accumulate ? 0 : (int)std::min(((long long)p.vocab + FR * ET / 64 - 1) / (FR * ET / 64), 8192ll);
+  const int fill = p.accumulate || p.filled ? 0 : (int)std::min(((long long)p.vocab + FR * ET / 64 - 1) / (FR * ET / 64), 8192ll);
   launch_k(embedding_sums_kernel<T, G, L>, dim3(p.sum_groups + fill), ET, 0, s, p);
   if (p.ranges > 1) {
-    const int slabs = (p.channels + 255) / 256;
-    launch_k(embedding_join_kernel<G>, dim3((int)std::min((long long)(p.ranges - 1) * slabs, 1ll << 20)), JT, 0, s, p, slabs);
+    const int blocks = (p.channels + 256 * JS - 1) / (256 * JS);
+    const int wide = p.channels <= 256 ? 1 : p.channels <= 512 ? 2 : p.channels <= 1024 ? 4 : JS;
+    launch_k(embedding_join_kernel<G>, dim3((int)std::min((long long)(p.ranges - 1) * blocks, 1ll << 20)), JT, 0, s, p, blocks, wide);
   }
 }
 template <typename T, typename G>
@@ -446,8 +497,14 @@ void launch_embedding(const kg_embedding_args& a, hipStream_t s) {
   const auto go = [&](auto zero) {
     using T = decltype(zero);
     const int chunks = (a.channels + kVec<T> - 1) / kVec<T>;
-    launch_k(embedding_kernel<T>, dim3(grid_of((long long)a.count * chunks)), ET, 0, s, a.tokens, (const T*)a.table, (T*)a.y, a.ld_table,
-             a.ld_y, a.count, a.vocab, a.channels, chunks, scale);
+    const long long columns = (long long)a.count * chunks;
+    const int past = columns * 16 > kPastBytes;
+    if (columns < kFewColumns)
+      launch_k(embedding_kernel<T, 1>, dim3(grid_of(columns)), ET, 0, s, a.tokens, (const T*)a.table, (T*)a.y, a.ld_table, a.ld_y, a.count,
+               a.vocab, a.channels, chunks, scale, past);
+    else
+      launch_k(embedding_kernel<T, 4>, dim3(grid_of((a.count + 3ll) / 4 * chunks)), ET, 0, s, a.tokens, (const T*)a.table, (T*)a.y,
+               a.ld_table, a.ld_y, a.count, a.vocab, a.channels, chunks, scale, past);
   };
   switch (a.type) {
     case PREC_F32: go(0.f); break;
@@ -468,7 +525,8 @@ void launch_embedding_backward(const kg_embedding_args& a, hipStream_t s) {
     p.parts = (float*)((char*)a.workspace + plan.parts);
     p.ranges = plan.ranges;
     p.each = plan.each;
-    sort_tokens(a, plan, p, s);
+    p.filled = !p.accumulate && a.count <= a.vocab / 4;
+    sort_tokens(a, plan, p, p.filled, s);
   }
   if (a.grad_type == a.type) {
     switch (a.type) {

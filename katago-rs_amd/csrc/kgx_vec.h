@@ -40,5 +40,15 @@ __device__ __forceinline__ void store_vec(T* p, int left, const float (&f)[kVec<
       if (j < left) p[j] = t[j];
   }
 }
+// A whole vector past the caches.
+template <typename T>
+__device__ __forceinline__ void store_past(T* p, const float (&f)[kVec<T>]) {
+  T t[kVec<T>];
+#pragma unroll
+  for (int j = 0; j < kVec<T>; j++) t[j] = to_t<T>(f[j]);
+  asm volatile("");  // (or this and a plain store in another branch become one, a plain one)
+  __builtin_nontemporal_store(__builtin_bit_cast(typename RowVec<T>::type, t), (typename RowVec<T>::type*)p);
+  asm volatile("");
+}
 
 }  // namespace kgx

@@ -451,11 +451,11 @@ typedef struct {
   float* loss;                 /* [rows] */
   void* grad;                  /* [rows] rows of ld_grad (columns past `columns` stay as they are); or NULL */
   long long ld_grad;
-  void* workspace;             /* kg_distill_loss_workspace(rows, columns) bytes, 16-byte aligned, this call's own until it has run;
+  void* workspace;             /* kg_distill_loss_workspace(rows, columns, k) bytes, 16-byte aligned, this call's own until it has run;
                                   NULL where that is 0 */
 } kg_distill_loss_args;
 int kg_distill_loss(int device, void* stream, const kg_distill_loss_args* args);
-size_t kg_distill_loss_workspace(int rows, int columns);
+size_t kg_distill_loss_workspace(int rows, int columns, int k);
 
 /* One AdamW step over `count` tensors at once (decoupled weight decay), in float:
  *   g = grad_scale grad; m = beta1 m + (1 - beta1) g; v = beta2 v + (1 - beta2) g^2;

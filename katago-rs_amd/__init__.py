@@ -238,7 +238,7 @@ def lib():
         L.kg_group_norm_workspace.argtypes = [ci] * 5
         L.kg_group_norm_workspace.restype = ctypes.c_size_t
         L.kg_distill_loss.argtypes = [ci, vp, vp]
-        L.kg_distill_loss_workspace.argtypes = [ci, ci]
+        L.kg_distill_loss_workspace.argtypes = [ci, ci, ci]
         L.kg_distill_loss_workspace.restype = ctypes.c_size_t
         L.kg_layer_norm.argtypes = [ci, vp, vp]
         L.kg_layer_norm_backward.argtypes = [ci, vp, vp]

@@ -18,6 +18,11 @@ namespace kgx {
 
 namespace {
 
+struct Known;
+struct Others {  // a row's columns that are not listed: their maximum, and the sum of e^((z - top) s)
+  double total;
+  float top;
+};
 struct DistillRows {
   const void* logits;
   const unsigned char* legal;
@@ -27,24 +32,37 @@ struct DistillRows {
   long long ld, ld_legal, ld_grad, ld_index, ld_top;
   const float *lse, *weight;
   float* loss;
-  int rows, columns, k, top_type, past;
+  int rows, columns, k, top_type, past, list_bytes;  // list_bytes: of a wave's lists
   double scale;
+  // Of rows that take a workgroup, by a launch before: what a wave knows of their entries (see Known).
+  Known* known;
+  Others* others;
+  double *share, *q;  // [rows][k]
+  int* column;        // [rows][k], -1 where an entry does not count
 };
 
-// A row's listed columns in LDS: the lists (link: column, or -1 where it does not count, and 1 + the next entry; heads: 1 + the
-// first), the student's logits and the teacher's; later z holds the entries' gradients.
-struct Listed {
+// A row's listed columns in LDS: the lists (link: column, or -1 where it does not count, and 1 + the next entry, see also placed(); heads:
+// 1 + the first), and the entries' gradients.
+struct Lists {
   int* heads;
   int2* link;
-  float *z, *t;
+  float* hot;
   int k;
-  __device__ __forceinline__ Listed(char* lds, int slots, int k_) : k(k_) {
+  __device__ __forceinline__ Lists(char* lds, int k_) : k(k_) {
     link = (int2*)lds;
-    z = (float*)(link + k);
-    t = z + k;
-    heads = (int*)(t + k);
+    hot = (float*)(link + k);
+    heads = (int*)(hot + k);
   }
-  static size_t bytes(int slots, int k) { return (size_t)k * 16 + (size_t)slots * 4; }
+  static size_t bytes(int slots, int k) { return ((size_t)k * 12 + (size_t)slots * 4 + 15) / 16 * 16; }
+};
+// Those with what a wave learns of the entries: the student's share e^(s (z - their maximum)) and the teacher's q.
+struct Listed : Lists {
+  double *share, *q;
+  __device__ __forceinline__ Listed(char* lds, int k_) : Lists(lds + (size_t)k_ * 16, k_) {
+    share = (double*)lds;
+    q = share + k;
+  }
+  static size_t bytes(int slots, int k) { return (size_t)k * 16 + Lists::bytes(slots, k); }
 };
 
 // LDS written before is read after: a wave's accesses are in order by themselves.
@@ -68,38 +86,54 @@ __device__ __forceinline__ float top_value(const DistillRows& a, int row, int i)
   }
 }
 
-// Fills the lists of a row; slot: a column's head.
-template <typename T, int NT, int SLOTS, typename Slot>
-__device__ __forceinline__ void list_row(const DistillRows& a, int row, const T* z, const unsigned char* legal, const Listed& l,
+// A thread's entry of a row, asked for before the row itself: what is asked for later arrives later.
+struct Entry {
+  int c = -1;
+  float t = -INFINITY;
+  __device__ __forceinline__ Entry() {}
+  __device__ __forceinline__ Entry(const DistillRows& a, int row, int i) {
+    if (i < a.k) {
+      c = a.index[(size_t)row * a.ld_index + i];
+      t = top_value(a, row, i);
+      if ((unsigned)c >= (unsigned)a.columns) c = -1;
+    }
+  }
+};
+
+// Fills the lists of a row, whose heads are 0, with NT threads; slot: a column's head; mine: this thread's first entry. The logits of
+// both sides are left, as floats, in share and q.
+template <typename T, int NT, typename Slot>
+__device__ __forceinline__ void list_row(const DistillRows& a, int row, const T* z, const unsigned char* legal, const Listed& l, const Entry& mine,
                                          const Slot& slot) {
   const int tid = threadIdx.x % NT;
-#pragma unroll
-  for (int i = 0; i < SLOTS / NT; i++) l.heads[tid + i * NT] = 0;
-  row_sync<NT>();
+  const auto entry = [&](int i) { return i < NT ? mine : Entry(a, row, i); };
+#pragma unroll 1
   for (int i = tid; i < l.k; i += NT) {
-    int c = a.index[(size_t)row * a.ld_index + i], next = 0;
-    if ((unsigned)c >= (unsigned)a.columns || (legal && !legal[c])) c = -1;
-    const float t = top_value(a, row, i);
-    if (c >= 0) next = atomicExch(&l.heads[slot(c)], i + 1);
-    l.link[i] = int2{c, next};
-    l.z[i] = c >= 0 ? (float)z[c] : -INFINITY;
-    l.t[i] = c >= 0 ? t : -INFINITY;
+    const int c = entry(i).c;
+    l.link[i] = int2{c, c >= 0 ? atomicExch(&l.heads[slot(c)], i + 1) : 0};
   }
   row_sync<NT>();
-  // Of entries that name one column the first counts.
+  // Of entries that name one column the first counts. An illegal column's entries do not.
   unsigned gone = 0;
+#pragma unroll 1
   for (int i = tid, b = 0; i < l.k; i += NT, b++) {
-    const int c = l.link[i].x;
-    if (c < 0) continue;
-    for (int h = l.heads[slot(c)]; h; h = l.link[h - 1].y)
-      if (h - 1 < i && l.link[h - 1].x == c) gone |= 1u << b;
+    const Entry own = entry(i);
+    float v = -INFINITY;
+    bool counts = own.c >= 0;
+    if (counts) {
+      v = (float)z[own.c];
+      if (legal) counts = legal[own.c] != 0;
+      for (int h = l.heads[slot(own.c)]; h; h = l.link[h - 1].y)
+        if (h - 1 < i && l.link[h - 1].x == own.c) counts = false;
+      if (!counts) gone |= 1u << b;
+    }
+    *(float*)(l.share + i) = counts ? v : -INFINITY;
+    *(float*)(l.q + i) = counts ? own.t : -INFINITY;
   }
   row_sync<NT>();
+#pragma unroll 1
   for (int i = tid, b = 0; i < l.k; i += NT, b++)
-    if (gone >> b & 1) {
-      l.link[i].x = -1;
-      l.z[i] = l.t[i] = -INFINITY;
-    }
+    if (gone >> b & 1) l.link[i].x = -1;
   row_sync<NT>();
 }
 
@@ -109,73 +143,117 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
-// What the others' gradient takes: grad_j = each e^((z_j - top) s). part: the row takes part.
+// What a wave knows of a row from its entries alone, in double: what is left of a loss between near distributions are differences of
+// logarithms. The student's sum is of e^(s (z - top)), cross = sum q (log q - s (z - top)), mass = sum q.
+struct Known {
+  double sum, mass, cross, rest;
+  float top;
+  bool any;  // an entry counts, and the teacher has mass
+};
+__device__ __forceinline__ Known know(const DistillRows& a, int row, const Listed& l) {
+  const int lane = threadIdx.x & 63;
+  const double s = a.scale;
+  Known n;
+  n.top = -INFINITY;
+  float t_top = -INFINITY;
+  bool any = false;
+#pragma unroll 1
+  for (int i = lane; i < l.k; i += 64) {
+    n.top = fmaxf(n.top, *(const float*)(l.share + i));
+    t_top = fmaxf(t_top, *(const float*)(l.q + i));
+    any |= l.link[i].x >= 0;
+  }
+  n.any = __ballot(any) != 0;
+  n.top = wave_reduce<true>(n.top);
+  t_top = wave_reduce<true>(t_top);
+  // (Nothing but -infinity: keep the differences from infinity less infinity.)
+  const double z0 = n.top == -INFINITY ? 0.0 : (double)n.top * s, t0 = t_top == -INFINITY ? 0.0 : (double)t_top * s;
+  double sum = 0.0, t_sum = 0.0, weighed = 0.0;
+#pragma unroll 1
+  for (int i = lane; i < l.k; i += 64) {
+    const double z = (double)*(const float*)(l.share + i) * s - z0, t = (double)*(const float*)(l.q + i) * s - (a.lse ? (double)a.lse[row] : t0);
+    const double e = exp(z), q = l.link[i].x < 0 ? 0.0 : exp(t);
+    sum += e;
+    t_sum += q;
+    weighed += q == 0.0 ? 0.0 : q * (t - z);
+    l.share[i] = e;
+    l.q[i] = q;
+  }
+  n.sum = wave_sum(sum);
+  t_sum = wave_sum(t_sum);
+  weighed = wave_sum(weighed);
+  n.rest = 0.0;
+  if (a.lse) {
+    n.mass = t_sum;
+    n.cross = weighed;
+    if (t_sum < 1.0) n.rest = 1.0 - t_sum;
+  } else {
+    // q is each one's share of their sum (a NaN among them is everyone's).
+    const double inverse = 1.0 / t_sum;
+    n.any = n.any && !(t_sum == 0.0);
+    n.mass = 1.0 + 0.0 * t_sum;
+    n.cross = weighed * inverse - log_sum(t_sum);
+#pragma unroll 1
+    for (int i = lane; i < l.k; i += 64) l.q[i] *= inverse;
+  }
+  return n;
+}
+
+// 1 / x of a normal x, to double's precision but for its last bits; NaN stays.
+__device__ __forceinline__ double reciprocal(double x) {
+  double r = __builtin_amdgcn_rcp(x);
+  r = __builtin_fma(__builtin_fma(-x, r, 1.0), r, r);
+  return __builtin_fma(__builtin_fma(-x, r, 1.0), r, r);
+}
+
+// What the others' gradient takes: grad_j = each e^((z_j - top) s), and a listed column's: ws (to share - q). part: the row takes part.
 struct DistillFactors {
+  double ws, to;
   float each;
   int part;
 };
 
-// The row's loss, the listed columns' gradients (into l.z) and the others' factor, from the others' maximum and their sum of
-// e^((z - top) s), 0 where there are none. One wave computes it, in double: what is left of a loss between near distributions
-// are differences of logarithms.
-__device__ __forceinline__ DistillFactors distill_row(const DistillRows& a, int row, const Listed& l, float top, double total, bool writes) {
-  const int lane = threadIdx.x & 63;
-  const double s = a.scale, none = -(double)INFINITY;
-  float z_max = -INFINITY, t_max = -INFINITY;
-  bool any = false;
-  for (int i = lane; i < l.k; i += 64) {
-    z_max = fmaxf(z_max, l.z[i]);
-    t_max = fmaxf(t_max, l.t[i]);
-    any |= l.link[i].x >= 0;
-  }
-  any = __ballot(any) != 0;
-  z_max = wave_reduce<true>(z_max);
-  t_max = wave_reduce<true>(t_max);
+// e^(the others' maximum's distance from the listed columns'), below 1 whichever is larger. FAST: to a float's ulp, by the hardware's
+// exponential, for gradients: few registers beside a row's.
+template <bool FAST>
+__device__ __forceinline__ double lead_of(const DistillRows& a, const Known& n, float top) {
+  const double x = -fabs(((double)top - (double)n.top) * a.scale);
+  if (!FAST) return exp(x);
+  const double y = x * 1.44269504088896340736;
+  const float high = (float)y;
+  // (Infinitely far: no rest.)
+  const float rest = high > -1000.f ? (float)(y - (double)high) * 0.693147181f : 0.f;
+  return (double)__builtin_fmaf(__builtin_amdgcn_exp2f(high), rest, __builtin_amdgcn_exp2f(high));
+}
+// The factors from the others' maximum and their sum of e^((z - top) s), 0 where there are none.
+__device__ __forceinline__ DistillFactors distill_row(const DistillRows& a, int row, const Known& n, float top, double lead, double total,
+                                                      double& all) {
   // (A sum that is NaN takes part, and makes everything NaN.)
-  const bool others = !(total == 0.0);
-  const double lo = others ? (double)top * s + log_sum(total) : none;
-  double z_top = fmax((double)z_max * s, lo), t_top = (double)t_max * s;
-  if (z_top == none) z_top = 0.0;
-  if (t_top == none) t_top = 0.0;
-  double z_sum = 0.0, t_sum = 0.0;
-  for (int i = lane; i < l.k; i += 64) {
-    z_sum += exp((double)l.z[i] * s - z_top);
-    if (!a.lse) t_sum += exp((double)l.t[i] * s - t_top);
-  }
-  z_sum = wave_sum(z_sum) + (others ? exp(lo - z_top) : 0.0);
-  t_sum = wave_sum(t_sum);
-  const double lse = z_top + log_sum(z_sum);
-  const double t_lse = a.lse ? (double)a.lse[row] : t_top + log_sum(t_sum);
-  DistillFactors f = {0.f, any && !(z_sum == 0.0) && (a.lse || !(t_sum == 0.0))};
-  double loss = 0.0, mass = 0.0;
+  const bool others = !(total == 0.0), listed = n.top != -INFINITY, ahead = others && (!listed || top >= n.top);
+  const double mine = !ahead ? 1.0 : listed ? lead : 0.0, theirs = !others ? 0.0 : ahead ? 1.0 : lead;  // of the larger maximum
+  all = n.sum * mine + (others ? total * theirs : 0.0);
+  DistillFactors f = {0.0, 0.0, 0.f, n.any && !(all == 0.0)};
   if (f.part) {
-    for (int i = lane; i < l.k; i += 64) {
-      const double x = (double)l.t[i] * s - t_lse, q = l.link[i].x < 0 ? 0.0 : exp(x);
-      mass += q;
-      loss += q == 0.0 ? 0.0 : q * (x - ((double)l.z[i] * s - lse));
-    }
-    mass = wave_sum(mass);
-    loss = wave_sum(loss);
-    double rest = 0.0;
-    if (a.lse) {
-      if (others && mass < 1.0) {
-        rest = 1.0 - mass;
-        loss += rest * (log_sum(rest) - (lo - lse));
-      }
-      mass += rest;
-    } else {
-      mass = 1.0 + 0.0 * t_lse;  // (a NaN among the teacher's is everyone's)
-    }
-    const double w = a.weight ? (double)a.weight[row] : 1.0, ws = w * s;
-    loss *= w;
-    if (others) f.each = (float)(ws * (mass * exp(lo - lse) - rest) / total);
-    for (int i = lane; i < l.k; i += 64) {
-      const double x = (double)l.t[i] * s - t_lse, q = l.link[i].x < 0 ? 0.0 : exp(x);
-      l.z[i] = (float)(ws * (mass * exp((double)l.z[i] * s - lse) - q));
-    }
+    f.ws = (a.weight ? (double)a.weight[row] : 1.0) * a.scale;
+    const double inverse = reciprocal(all), rest = others ? n.rest : 0.0, mass = n.mass + rest;
+    if (others) f.each = (float)(f.ws * (mass * (theirs * inverse) - (rest > 0.0 ? rest * reciprocal(total) : 0.0)));
+    f.to = mass * (mine * inverse);
   }
-  if (writes) a.loss[row] = (float)loss;
   return f;
+}
+__device__ __forceinline__ float hot_of(DistillFactors f, double share, double q) { return (float)(f.ws * (f.to * share - q)); }
+// The row's loss.
+__device__ __forceinline__ float loss_of(const DistillRows& a, int row, const Known& n, float top, double total, double all, bool part) {
+  double loss = 0.0;
+  if (part) {
+    const bool others = !(total == 0.0), listed = n.top != -INFINITY;
+    const double s = a.scale, above = others && (!listed || top >= n.top) ? (double)top * s : (double)n.top * s;
+    const double lse = above + log_sum(all);
+    loss = n.cross + n.mass * (lse - (listed ? (double)n.top * s : 0.0));
+    if (others && n.rest > 0.0) loss += n.rest * (log_sum(n.rest) - ((double)top * s + log_sum(total) - lse));
+    loss *= a.weight ? (double)a.weight[row] : 1.0;
+  }
+  return (float)loss;
 }
 
 // Rows shorter than 16 bytes: a wave a row, a lane a column.
@@ -183,44 +261,339 @@ template <typename T>
 __global__ __launch_bounds__(64) void distill_short_kernel(DistillRows a) {
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x;
-  const Listed l(lds, 64, a.k);
+  const Listed l(lds, a.k);
   const Base2 c2(a.scale);
   for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* z = (const T*)a.logits + (size_t)row * a.ld;
     const unsigned char* legal = a.legal ? a.legal + (size_t)row * a.ld_legal : nullptr;
     row_sync<64>();  // (the last row's lists have been read)
-    list_row<T, 64, 64>(a, row, z, legal, l, [](int c) { return c; });
+    l.heads[lane] = 0;
+    row_sync<64>();
+    list_row<T, 64>(a, row, z, legal, l, Entry(a, row, lane), [](int c) { return c; });
     int mine = -1;  // the entry that lists this lane's column
     for (int h = l.heads[lane]; h; h = l.link[h - 1].y)
       if (l.link[h - 1].x >= 0) mine = h - 1;
+    const Known known = know(a, row, l);
     const bool in = lane < a.columns && (!legal || legal[lane]) && mine < 0;
-    const float v = in ? (float)z[lane] : -INFINITY;
-    float top = wave_reduce<true>(v);
+    const float v = in ? (float)z[lane] : -INFINITY, top = wave_reduce<true>(v);
     const float e = exp_of(v - (top == -INFINITY ? 0.f : top), c2);
-    const float sum = wave_reduce<false>(e);
-    const DistillFactors f = distill_row(a, row, l, top, (double)sum, lane == 0);
-    row_sync<64>();
+    const double total = (double)wave_reduce<false>(e);
+    double all;
+    const DistillFactors f = distill_row(a, row, known, top, lead_of<false>(a, known, top), total, all);
+    const float loss = loss_of(a, row, known, top, total, all, f.part);
+    if (lane == 0) a.loss[row] = loss;
     if (a.grad && lane < a.columns)
-      ((T*)a.grad)[(size_t)row * a.ld_grad + lane] = to_t<T>(!f.part ? 0.f : mine >= 0 ? l.z[mine] : in ? e * f.each : 0.f);
+      ((T*)a.grad)[(size_t)row * a.ld_grad + lane] = to_t<T>(!f.part ? 0.f : mine >= 0 ? hot_of(f, l.share[mine], l.q[mine]) : e == 0.f ? 0.f : e * f.each);
   }
+}
+
+// w with element j (known at run time) replaced: the element's bits are in each place of `bits` that it can have in a word.
+template <typename T>
+__device__ __forceinline__ u32x4 replaced(const u32x4& w, int j, unsigned bits) {
+  const int k = sizeof(T) == 4 ? j : j >> 1;
+  const unsigned mask = sizeof(T) == 4 ? ~0u : j & 1 ? 0xffff0000u : 0xffffu, put = bits & mask;
+  return u32x4{k == 0 ? (w[0] & ~mask) | put : w[0], k == 1 ? (w[1] & ~mask) | put : w[1], k == 2 ? (w[2] & ~mask) | put : w[2],
+               k == 3 ? (w[3] & ~mask) | put : w[3]};
+}
+template <typename T>
+__device__ __forceinline__ unsigned bits_of(float v) {
+  if constexpr (sizeof(T) == 4) return __float_as_uint(v);
+  else return __builtin_bit_cast(unsigned short, to_t<T>(v)) * 0x10001u;
+}
+
+// An entry's link once its row's chunks are laid: its chunk (-1 where it does not count), and 1 + the next entry with its element of the
+// chunk above. A chunk's walk then asks for nothing else.
+template <typename T>
+__device__ __forceinline__ int2 placed(const Chunks<T>& at, int column, int next) {
+  if (column < 0) return int2{-1, next};
+  const int c = at.of(column);
+  return int2{c, next | (column - at.start(c)) << 16};
+}
+template <typename T>
+__device__ __forceinline__ void place_row(const Lists& l, const Chunks<T>& at) {
+#pragma unroll 1
+  for (int i = threadIdx.x & 63; i < l.k; i += 64) l.link[i] = placed<T>(at, l.link[i].x, l.link[i].y);
+  row_sync<64>();
 }
 
 // -infinity in the place of listed columns, of the E chunks of a thread from chunk c0 on.
 template <typename T, int NT, int E>
-__device__ __forceinline__ void remove_listed(const Listed& l, int tid, const Chunks<T>& at, u32x4 (&raw)[E], int c0) {
+__device__ __forceinline__ void remove_listed(const Lists& l, int tid, const Chunks<T>& at, u32x4 (&raw)[E], int c0) {
+  int head[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) head[e] = l.heads[tid + e * NT];
 #pragma unroll
   for (int e = 0; e < E; e++) {
     if (at.none(c0 + e * NT)) break;
     const int c = tid + c0 + e * NT;
-    for (int h = l.heads[tid + e * NT]; h; ) {
+    for (int h = head[e]; h; ) {
       const int2 entry = l.link[h - 1];
-      if (entry.x >= 0 && at.of(entry.x) == c) {
-        const int j0 = entry.x - at.start(c);
-#pragma unroll
-        for (int j = 0; j < kVec<T>; j++) remove<T>(raw[e], j, j == j0);
-      }
-      h = entry.y;
+      if (entry.x == c) raw[e] = replaced<T>(raw[e], entry.y >> 16, bits_of<T>(-INFINITY));
+      h = entry.y & 0xffff;
     }
+  }
+}
+
+// Stores the gradients f of chunk c, of head `slot`, with those of its listed columns.
+template <typename T, int SLOTS>
+__device__ __forceinline__ void store_listed(T* row, const Lists& l, int slot, int c, bool whole, int past, const Chunks<T>& at,
+                                             const float (&f)[kVec<T>]) {
+  typedef typename AnyWords<T>::type words_t;
+  u32x4 w = words_of<T>(f);
+  for (int h = l.heads[slot]; h; ) {
+    const int2 entry = l.link[h - 1];
+    if (entry.x == c) w = replaced<T>(w, entry.y >> 16, bits_of<T>(l.hot[h - 1]));
+    h = entry.y & 0xffff;
+  }
+  const int first = whole ? 0 : at.first(c), limit = whole ? kVec<T> : at.limit(c);
+  T* p = row + at.start(c);
+  if (whole || (first == 0 && limit == kVec<T>)) {
+    if (past) {
+      asm volatile("");  // (or the two stores become one, a plain one)
+      __builtin_nontemporal_store((words_t)w, (words_t*)p);
+      asm volatile("");
+    } else {
+      *(words_t*)p = w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kVec<T>; j++)
+      if (j >= first && j < limit) {
+        if constexpr (sizeof(T) == 4) ((unsigned*)p)[j] = w[j];
+        else ((unsigned short*)p)[j] = (unsigned short)(w[j >> 1] >> (j & 1 ? 16 : 0));
+      }
+  }
+}
+
+// The maximum of a thread's chunks, their sum of e^((z - top) s) and their gradients, of rows that stay in registers.
+template <typename T, int NT, int E>
+__device__ __forceinline__ float own_top(const Chunks<T>& at, const u32x4 (&raw)[E]) {
+  float top = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    if (at.none(e * NT)) break;
+#pragma unroll
+    for (int j = 0; j < kVec<T>; j++) top = fmaxf(top, element<T>(raw[e], j));
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  return top;
+}
+template <typename T, int NT, int E>
+__device__ __forceinline__ float own_sum(const Chunks<T>& at, u32x4 (&raw)[E], float base, Base2 c2) {
+  forget<E>(raw);
+  float sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    if (at.none(e * NT)) break;
+    float t = 0.f;
+#pragma unroll
+    for (int j = 0; j < kVec<T>; j++) t += exp_of(element<T>(raw[e], j) - base, c2);
+    sum += t;
+    asm volatile("" : "+v"(sum));  // (here, and not behind the sum's reduction)
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  return sum;
+}
+template <typename T, int NT, int E>
+__device__ __forceinline__ void own_gradient(T* g, int tid, const Chunks<T>& at, u32x4 (&raw)[E], const Lists& l, float base, Base2 c2,
+                                             float each, int takes, int past) {
+  forget<E>(raw);
+  const bool part = __builtin_amdgcn_readfirstlane(takes);
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    if (at.none(e * NT)) break;
+    const int c = fresh(tid) + e * NT;
+    float gf[kVec<T>] = {};
+    if (part) {
+      // (A column without mass has no gradient, whatever the factor. A listed one's place is filled below.)
+#pragma unroll
+      for (int j = 0; j < kVec<T>; j++) {
+        const float ex = __builtin_amdgcn_exp2f((element<T>(raw[e], j) - base) * c2.hi);
+        gf[j] = ex == 0.f ? 0.f : ex * each;
+      }
+      store_listed<T, NT * E>(g, l, tid + e * NT, c, at.whole(e * NT, NT), past, at, gf);
+    } else {
+      store_gradient<T>(g, c, at.whole(e * NT, NT), past, at, gf);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// Rows of up to 64 E chunks: a wave a row, one read.
+template <typename T, int E>
+__global__ __launch_bounds__(256) void distill_wave_kernel(DistillRows a) {
+  extern __shared__ __align__(16) char lds[];
+  const int tid = threadIdx.x & 63;
+  const Listed l(lds + wave_row<64>() * a.list_bytes, a.k);
+  const Base2 c2(a.scale);
+  for (int row = blockIdx.x * 4 + wave_row<64>(); row < a.rows; row += gridDim.x * 4) {
+    const T* z = (const T*)a.logits + (size_t)row * a.ld;
+    const unsigned char* legal = a.legal ? a.legal + (size_t)row * a.ld_legal : nullptr;
+    T* g = a.grad ? (T*)a.grad + (size_t)row * a.ld_grad : nullptr;
+    const Chunks<T> at(a.columns, g ? g : z);
+    u32x4 raw[E], unused[1];
+    const Entry mine(a, row, tid);
+    load_row<T, 64, E>(z, tid, at, raw);
+    row_sync<64>();  // (the last row's lists have been read)
+#pragma unroll
+    for (int e = 0; e < E; e++) l.heads[tid + e * 64] = 0;
+    row_sync<64>();
+    list_row<T, 64>(a, row, z, legal, l, mine, [&](int c) { return at.of(c); });
+    const Known known = know(a, row, l);
+    place_row<T>(l, at);
+    if (legal) remove_illegal<T, 64, E, false>(legal, tid, at, raw, unused);
+    remove_past<T, 64, E>(tid, at, raw);
+    remove_listed<T, 64, E>(l, tid, at, raw, 0);
+    const float top = wave_reduce<true>(own_top<T, 64, E>(at, raw)), base = top == -INFINITY ? 0.f : top;
+    const double total = (double)wave_reduce<false>(own_sum<T, 64, E>(at, raw, base, c2));
+    double all;
+    const DistillFactors f = distill_row(a, row, known, top, lead_of<false>(a, known, top), total, all);
+#pragma unroll 1
+    for (int i = tid; i < l.k; i += 64) l.hot[i] = hot_of(f, l.share[i], l.q[i]);
+    row_sync<64>();
+    if (g) own_gradient<T, 64, E>(g, tid, at, raw, l, base, c2, f.each, f.part, a.past);
+    const float loss = loss_of(a, row, known, top, total, all, f.part);
+    if (tid == 0) a.loss[row] = loss;
+  }
+}
+
+// What the workgroups of longer rows need of the entries, by a wave a row. (Its double arithmetic and its dependent loads in the row's own
+// launch, at 4093 x 32768 bf16: 240 us, and 175 by a wave of its own beside the row's; apart @.)
+constexpr int kSlots = 256;
+template <typename T>
+__global__ __launch_bounds__(64) void distill_known_kernel(DistillRows a) {
+  extern __shared__ __align__(16) char lds[];
+  const int lane = threadIdx.x;
+  const Listed l(lds, a.k);
+  for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const Entry mine(a, row, lane);
+    row_sync<64>();  // (the last row's lists have been read)
+#pragma unroll
+    for (int i = 0; i < kSlots / 64; i++) l.heads[lane + i * 64] = 0;
+    row_sync<64>();
+    list_row<T, 64>(a, row, (const T*)a.logits + (size_t)row * a.ld, a.legal ? a.legal + (size_t)row * a.ld_legal : nullptr, l, mine,
+                    [](int c) { return c % kSlots; });
+    const Known known = know(a, row, l);
+    if (lane == 0) a.known[row] = known;
+    for (int i = lane; i < a.k; i += 64) {
+      const size_t at = (size_t)row * a.k + i;
+      a.column[at] = l.link[i].x;
+      a.share[at] = l.share[i];
+      a.q[at] = l.q[i];
+    }
+  }
+}
+
+// What a row's workgroup has of its entries in LDS, copied there by NT threads that ask for theirs before they ask for the row, as what is
+// asked for first arrives first. Two barriers around begin(): the last row's are read, and these are there.
+struct Copied : Listed {
+  Known* known;
+  __device__ __forceinline__ Copied(char* lds, int k_) : Listed(lds + sizeof(Known), k_) { known = (Known*)lds; }
+  static size_t bytes(int slots, int k) { return sizeof(Known) + Listed::bytes(slots, k); }
+};
+template <int NT>
+struct Asked {
+  int c;
+  double share, q;
+  unsigned known;
+  __device__ __forceinline__ Asked(const DistillRows& a, int row) {
+    const int i = threadIdx.x;
+    const size_t at = (size_t)row * a.k + min(i, a.k - 1);
+    c = a.column[at];
+    share = a.share[at];
+    q = a.q[at];
+    known = ((const unsigned*)(a.known + row))[min(i, (int)(sizeof(Known) / 4) - 1)];
+  }
+  __device__ __forceinline__ void begin(const DistillRows& a, int row, const Copied& l) const {
+    const int tid = threadIdx.x;
+    if (tid < (int)(sizeof(Known) / 4)) ((unsigned*)l.known)[tid] = known;
+#pragma unroll 1
+    for (int i = tid; i < l.k; i += NT) {
+      const size_t at = (size_t)row * a.k + i;
+      l.share[i] = i == tid ? share : a.share[at];
+      l.q[i] = i == tid ? q : a.q[at];
+      l.link[i].x = i == tid ? c : a.column[at];
+    }
+  }
+};
+// The row's lists, whose heads are 0, from the columns that count: there behind a barrier.
+template <typename T, int NT, int SLOTS>
+__device__ __forceinline__ void link_row(const Copied& l, const Chunks<T>& at) {
+#pragma unroll 1
+  for (int i = threadIdx.x; i < l.k; i += NT) {
+    const int c = l.link[i].x;
+    l.link[i] = placed<T>(at, c, c >= 0 ? atomicExch(&l.heads[at.of(c) % SLOTS], i + 1) : 0);
+  }
+}
+template <int NT>
+__device__ __forceinline__ void hot_row(const Copied& l, const DistillFactors& f) {
+#pragma unroll 1
+  for (int i = threadIdx.x; i < l.k; i += NT) l.hot[i] = hot_of(f, l.share[i], l.q[i]);
+}
+
+// Longer rows that fit the registers of NT threads: a workgroup a row, one read.
+template <typename T, int NT, int E>
+__global__ __launch_bounds__(NT, 6) void distill_row_kernel(DistillRows a) {
+  constexpr int WAVES = NT / 64;
+  extern __shared__ __align__(16) char lds[];
+  __shared__ float tops[WAVES], sums[WAVES];
+  __shared__ DistillFactors box;
+  const int tid = threadIdx.x;
+  const Copied l(lds, a.k);
+  const Base2 c2(a.scale);
+  for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* z = (const T*)a.logits + (size_t)row * a.ld;
+    const unsigned char* legal = a.legal ? a.legal + (size_t)row * a.ld_legal : nullptr;
+    T* g = a.grad ? (T*)a.grad + (size_t)row * a.ld_grad : nullptr;
+    const Chunks<T> at(a.columns, g ? g : z);
+    u32x4 raw[E], unused[1];
+    const Asked<NT> asked(a, row);
+    load_row<T, NT, E>(z, tid, at, raw);
+    lds_barrier();
+    asked.begin(a, row, l);
+#pragma unroll
+    for (int e = 0; e < E; e++) l.heads[tid + e * NT] = 0;
+    lds_barrier();
+    link_row<T, NT, NT * E>(l, at);
+    if (legal) remove_illegal<T, NT, E, false>(legal, tid, at, raw, unused);
+    remove_past<T, NT, E>(tid, at, raw);
+    lds_barrier();
+    remove_listed<T, NT, E>(l, tid, at, raw, 0);
+    float top = wave_reduce<true>(own_top<T, NT, E>(at, raw));
+    if ((tid & 63) == 0) tops[tid >> 6] = top;
+    lds_barrier();
+#pragma unroll
+    for (int k = 0; k < WAVES; k++) top = fmaxf(top, tops[k]);
+    const float base = top == -INFINITY ? 0.f : top, sum = wave_reduce<false>(own_sum<T, NT, E>(at, raw, base, c2));
+    if ((tid & 63) == 0) sums[tid >> 6] = sum;
+    lds_barrier();
+    if (tid < 64) {
+      const Known known = *l.known;
+      double total = 0.0, all;
+#pragma unroll
+      for (int k = 0; k < WAVES; k++) total += (double)sums[k];
+      const DistillFactors f = distill_row(a, row, known, top, lead_of<true>(a, known, top), total, all);
+      if (tid == 0) {
+        box = f;
+        a.others[row] = Others{total, top};
+      }
+    }
+    lds_barrier();
+    hot_row<NT>(l, box);
+    lds_barrier();
+    if (g) own_gradient<T, NT, E>(g, tid, at, raw, l, base, c2, box.each, box.part, a.past);
+  }
+}
+
+// The losses from what the two launches before found, a thread a row. (At the end of a row's own launch its constants alone, which the
+// compiler keeps over the loop of rows, cost 50 registers a thread.)
+__global__ __launch_bounds__(256) void distill_loss_kernel(DistillRows a) {
+  for (int row = blockIdx.x * 256 + threadIdx.x; row < a.rows; row += gridDim.x * 256) {
+    const Known known = a.known[row];
+    const Others others = a.others[row];
+    double all;
+    const DistillFactors f = distill_row(a, row, known, others.top, lead_of<false>(a, known, others.top), others.total, all);
+    a.loss[row] = loss_of(a, row, known, others.top, others.total, all, f.part);
   }
 }
 
@@ -232,15 +605,21 @@ __global__ __launch_bounds__(NT) void distill_long_kernel(DistillRows a) {
   __shared__ float red[16];
   __shared__ DistillFactors box;
   const int tid = threadIdx.x;
-  const Listed l(lds, SLOTS, a.k);
+  const Copied l(lds, a.k);
   const Base2 c2(a.scale);
   for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* z = (const T*)a.logits + (size_t)row * a.ld;
     const unsigned char* legal = a.legal ? a.legal + (size_t)row * a.ld_legal : nullptr;
     T* g = a.grad ? (T*)a.grad + (size_t)row * a.ld_grad : nullptr;
     const Chunks<T> at(a.columns, g ? g : z);
-    lds_barrier();  // (the last row's lists and factors have been read)
-    list_row<T, NT, SLOTS>(a, row, z, legal, l, [&](int c) { return at.of(c) % SLOTS; });
+    const Asked<NT> asked(a, row);
+    lds_barrier();
+    asked.begin(a, row, l);
+#pragma unroll
+    for (int e = 0; e < E; e++) l.heads[tid + e * NT] = 0;
+    lds_barrier();
+    link_row<T, NT, SLOTS>(l, at);
+    lds_barrier();
     auto piece = [&](int c0, u32x4(&raw)[E]) {
       u32x4 unused[1];
       load_row<T, NT, E>(z, tid, at, raw, c0);
@@ -264,14 +643,20 @@ __global__ __launch_bounds__(NT) void distill_long_kernel(DistillRows a) {
     float moved;
     run.join<NT>(c2, red, moved);
     if (tid < 64) {
-      const DistillFactors mine = distill_row(a, row, l, run.top, run.total, tid == 0);
-      if (tid == 0) box = mine;
+      const Known known = *l.known;
+      double all;
+      const DistillFactors f = distill_row(a, row, known, run.top, lead_of<true>(a, known, run.top), run.total, all);
+      if (tid == 0) {
+        box = f;
+        a.others[row] = Others{run.total, run.top};
+      }
     }
     lds_barrier();
     if (!g) continue;
-    const DistillFactors f = box;
-    const bool part = __builtin_amdgcn_readfirstlane(f.part);
-    const float top = run.top == -INFINITY ? 0.f : run.top;
+    hot_row<NT>(l, box);
+    lds_barrier();
+    const bool part = __builtin_amdgcn_readfirstlane(box.part);
+    const float each = box.each, top = run.top == -INFINITY ? 0.f : run.top;
     for (int c0 = 0; !at.none(c0); c0 += NT * E) {
       u32x4 raw[E];
       if (part) piece(c0, raw);
@@ -285,34 +670,62 @@ __global__ __launch_bounds__(NT) void distill_long_kernel(DistillRows a) {
 #pragma unroll
           for (int j = 0; j < V; j++) {
             const float ex = __builtin_amdgcn_exp2f((element<T>(raw[e], j) - top) * c2.hi);
-            gf[j] = ex == 0.f ? 0.f : ex * f.each;
+            gf[j] = ex == 0.f ? 0.f : ex * each;
           }
-          for (int h = l.heads[tid + e * NT]; h; ) {
-            const int2 entry = l.link[h - 1];
-            if (entry.x >= 0 && at.of(entry.x) == c) {
-              const int j0 = entry.x - at.start(c);
-#pragma unroll
-              for (int j = 0; j < V; j++) gf[j] = j == j0 ? l.z[h - 1] : gf[j];
-            }
-            h = entry.y;
-          }
+          store_listed<T, SLOTS>(g, l, tid + e * NT, c, at.whole(c0 + e * NT, NT), a.past, at, gf);
+        } else {
+          store_gradient<T>(g, c, at.whole(c0 + e * NT, NT), a.past, at, gf);
         }
-        store_gradient<T>(g, c, at.whole(c0 + e * NT, NT), a.past, at, gf);
       }
     }
   }
 }
 
+// Rows that a wave takes alone, whatever their type: they need no workspace.
+constexpr int kWaveColumns = 448, kWaveEntries = 256;
+
 template <typename T>
-void distill_typed(const DistillRows& p, hipStream_t s) {
+void distill_typed(DistillRows p, hipStream_t s) {
   const dim3 groups(row_grid(p.rows, 1));
-  if (p.columns < kVec<T>) launch_k(distill_short_kernel<T>, groups, 64, Listed::bytes(64, p.k), s, p);
-  else launch_k(distill_long_kernel<T, 256, 4>, groups, 256, Listed::bytes(1024, p.k), s, p);
+  if (p.columns < kVec<T>) return launch_k(distill_short_kernel<T>, groups, 64, Listed::bytes(64, p.k), s, p);
+  const RowShape r = p.grad ? row_shape<T>(p.columns, p.grad, p.ld_grad, p.rows) : row_shape<T>(p.columns, p.logits, p.ld, p.rows);
+  if (r.threads == 64 && r.each == 2 && p.k <= kWaveEntries) {
+    p.list_bytes = (int)Listed::bytes(64 * 2, p.k);
+    return launch_k(distill_wave_kernel<T, 2>, dim3(row_grid(p.rows, 4)), 256, p.list_bytes * 4, s, p);
+  }
+  launch_k(distill_known_kernel<T>, groups, 64, Listed::bytes(kSlots, p.k), s, p);
+  if (r.threads == 64) launch_k(distill_row_kernel<T, 256, 2>, groups, 256, Copied::bytes(256 * 2, p.k), s, p);
+  else if (r.threads == 256) launch_k(distill_row_kernel<T, 256, 8>, groups, 256, Copied::bytes(256 * 8, p.k), s, p);
+  else if (r.threads == 512) launch_k(distill_row_kernel<T, 512, 8>, groups, 512, Copied::bytes(512 * 8, p.k), s, p);
+  else launch_k(distill_long_kernel<T, 256, 4>, groups, 256, Copied::bytes(256 * 4, p.k), s, p);
+  launch_k(distill_loss_kernel, dim3(row_grid(p.rows, 256)), 256, 0, s, p);
+}
+
+// Where what is known of the entries lies in the workspace.
+struct Plan {
+  size_t known, others, share, q, column, bytes;
+};
+Plan plan_of(int rows, int columns, int k) {
+  Plan p = {};
+  const auto room = [&](size_t n) {
+    const size_t at = p.bytes;
+    p.bytes += (n + 255) / 256 * 256;
+    return at;
+  };
+  p.known = room((size_t)rows * sizeof(Known));
+  p.others = room((size_t)rows * sizeof(Others));
+  p.share = room((size_t)rows * k * 8);
+  p.q = room((size_t)rows * k * 8);
+  p.column = room((size_t)rows * k * 4);
+  return p;
 }
 
 }  // namespace
 
-size_t distill_loss_workspace(int rows, int columns) { return 0; }
+size_t distill_loss_workspace(int rows, int columns, int k) {
+  if (rows < 1 || k < 1 || (columns <= kWaveColumns && k <= kWaveEntries)) return 0;
+  return plan_of(rows, columns, k).bytes;
+}
 
 void launch_distill_loss(const kg_distill_loss_args& a, hipStream_t s) {
   DistillRows p;
@@ -326,6 +739,13 @@ void launch_distill_loss(const kg_distill_loss_args& a, hipStream_t s) {
   p.rows = a.rows; p.columns = a.columns; p.k = a.k; p.top_type = a.top_type;
   p.past = gradient_past(a.rows, a.columns, a.type);
   p.scale = a.logit_scale;
+  const Plan plan = plan_of(a.rows, a.columns, a.k);
+  char* w = (char*)a.workspace;
+  p.known = (Known*)(w + plan.known);
+  p.others = (Others*)(w + plan.others);
+  p.share = (double*)(w + plan.share);
+  p.q = (double*)(w + plan.q);
+  p.column = (int*)(w + plan.column);
   switch (a.type) {
     case PREC_F32: distill_typed<float>(p, s); break;
     case PREC_F16: distill_typed<f16>(p, s); break;

@@ -120,7 +120,7 @@ void check_distill(const kg_distill_loss_args& a) {
   if (a.legal) need(a.ld_legal >= (a.rows > 1 ? a.columns : 0), op, "the row stride of legal is less than its row");
   need(a.loss, op, "null argument");
   need(!a.grad || (a.grad != a.logits && a.grad != a.top_logits), op, "grad must not overlap an input");
-  if (kgx::distill_loss_workspace(a.rows, a.columns)) {
+  if (kgx::distill_loss_workspace(a.rows, a.columns, a.k)) {
     need(a.workspace, op, "workspace is null");
     need(aligned(a.workspace, 16), op, "workspace is not aligned to 16 bytes");
   }
@@ -339,7 +339,7 @@ int kg_group_norm_backward(int device, void* stream, const kg_group_norm_args* a
   });
 }
 
-size_t kg_distill_loss_workspace(int rows, int columns) { return kgx::distill_loss_workspace(rows, columns); }
+size_t kg_distill_loss_workspace(int rows, int columns, int k) { return kgx::distill_loss_workspace(rows, columns, k); }
 
 int kg_distill_loss(int device, void* stream, const kg_distill_loss_args* args) {
   return guarded([&] {

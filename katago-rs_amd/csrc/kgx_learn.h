@@ -32,7 +32,7 @@ bool group_norm_fits(const kg_group_norm_args& a);  // its launches' threads fit
 void launch_group_norm(const kg_group_norm_args& a, hipStream_t s);
 void launch_group_norm_backward(const kg_group_norm_args& a, hipStream_t s);
 
-size_t distill_loss_workspace(int rows, int columns);
+size_t distill_loss_workspace(int rows, int columns, int k);
 void launch_distill_loss(const kg_distill_loss_args& a, hipStream_t s);
 
 // Layer norm: the backward pass's sums over parts of the rows.

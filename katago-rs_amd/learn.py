@@ -252,8 +252,8 @@ def distill_loss(logits, top_index, top_logits, *, legal=None, weight=None, logi
         g, ld_g = grad.data_ptr(), v
     loss = torch.empty(n, dtype=torch.float32, device=logits.device)
     L = _library()
-    # (Few long rows: 16384 columns are the least that a workspace is for.)
-    work = _workspace(L.kg_distill_loss_workspace(n, v) if v > 16384 else 0, logits.device)
+    # (A board's rows need none: up to 448 columns with up to 256 entries.)
+    work = _workspace(L.kg_distill_loss_workspace(n, v, k) if v > 448 or k > 256 else 0, logits.device)
     try:
         args = _DISTILL_ARGS.pack(n, v, k, TYPES[logits.dtype], TYPES[top_logits.dtype], ptr, ld, lg, ld_lg, top_index.data_ptr(),
                                   top_index.stride(0), top, ld_top, _vector(teacher_lse, n, torch.float32, "teacher_lse", dev),

@@ -27,6 +27,7 @@ DISTILL = dict(rows=4, columns=9, k=3, type=0, top_type=1, logits=4096, ld=9, le
     (dict(ld_top=2), "row stride of top_logits"), (dict(legal=4096, ld_legal=8), "legal"), (dict(loss=None), "null argument"),
     (dict(logit_scale=0.0), "logit_scale"), (dict(logit_scale=float("nan")), "logit_scale"), (dict(logit_scale=2.0 ** 65), "logit_scale"),
     (dict(grad=4096), "overlap"), (dict(ld_grad=1), "row stride of grad"),
+    (dict(columns=2000, ld=2000, ld_grad=2000), "workspace is null"), (dict(columns=2000, ld=2000, ld_grad=2000, workspace=4104), "workspace is not aligned"),
 ])
 def test_distill_loss_refuses(kgx, change, text):
     assert kgx.lib().kg_distill_loss(0, None, ctypes.byref(abi.DistillArgs(**{**DISTILL, **change}))) == 1
@@ -103,7 +104,8 @@ def test_packed_arguments_lie_as_the_structures_do(learn, name):
 
 def test_workspaces(kgx):
     L = kgx.lib()
-    assert L.kg_distill_loss_workspace(-1, 100000) == L.kg_distill_loss_workspace(4, 362) == 0
+    assert L.kg_distill_loss_workspace(-1, 100000, 5) == L.kg_distill_loss_workspace(4, 362, 24) == L.kg_distill_loss_workspace(4, 5000, -1) == 0
+    assert L.kg_distill_loss_workspace(1, 362, 1024) >= 20 * 1024 and L.kg_distill_loss_workspace(2 ** 30, 2 ** 30, 1024) >= 20 * 2 ** 40
     assert L.kg_layer_norm_workspace(0, 5) == L.kg_layer_norm_workspace(-2, 5) == L.kg_layer_norm_workspace(5, -1) == 0
     assert L.kg_layer_norm_workspace(1, 1) >= 8 and L.kg_layer_norm_workspace(100000, 1024) >= 8192
     assert L.kg_embedding_backward_workspace(0, 5, 5) == L.kg_embedding_backward_workspace(5, 0, 5) == 0

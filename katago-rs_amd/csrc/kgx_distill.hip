@@ -36,7 +36,8 @@ struct DistillRows {
   double scale;
   // Of rows that take a workgroup, by a launch before: what a wave knows of their entries (see Known).
   Known* known;
-  Others* others;
+  Others *others, *parts;  // parts: of rows cut into `split` parts of `span` chunks
+  int split, span;
   double *share, *q;  // [rows][k]
   int* column;        // [rows][k], -1 where an entry does not count
 };
@@ -585,29 +586,51 @@ __global__ __launch_bounds__(NT, 6) void distill_row_kernel(DistillRows a) {
   }
 }
 
-// The losses from what the two launches before found, a thread a row. (At the end of a row's own launch its constants alone, which the
+// A row's loss from what the launches before found, by one thread. (At the end of a row's own launch its constants alone, which the
 // compiler keeps over the loop of rows, cost 50 registers a thread.)
-__global__ __launch_bounds__(256) void distill_loss_kernel(DistillRows a) {
-  for (int row = blockIdx.x * 256 + threadIdx.x; row < a.rows; row += gridDim.x * 256) {
-    const Known known = a.known[row];
-    const Others others = a.others[row];
-    double all;
-    const DistillFactors f = distill_row(a, row, known, others.top, lead_of<false>(a, known, others.top), others.total, all);
-    a.loss[row] = loss_of(a, row, known, others.top, others.total, all, f.part);
+__device__ __forceinline__ void loss_row(const DistillRows& a, int row, const Others& others) {
+  const Known known = a.known[row];
+  double all;
+  const DistillFactors f = distill_row(a, row, known, others.top, lead_of<false>(a, known, others.top), others.total, all);
+  a.loss[row] = loss_of(a, row, known, others.top, others.total, all, f.part);
+}
+__global__ __launch_bounds__(64) void distill_loss_kernel(DistillRows a) {
+  for (int row = blockIdx.x * 64 + threadIdx.x; row < a.rows; row += gridDim.x * 64) loss_row(a, row, a.others[row]);
+}
+// The same from the rows' parts.
+__device__ __forceinline__ void losses_of_parts(const DistillRows& a, int first, int step, Base2 c2) {
+  for (int row = first; row < a.rows; row += step) {
+    const Others* parts = a.parts + (size_t)row * a.split;
+    Others others = {0.0, -INFINITY};
+    for (int k = 0; k < a.split; k++) others.top = fmaxf(others.top, parts[k].top);
+    for (int k = 0; k < a.split; k++)
+      others.total += parts[k].top == -INFINITY ? parts[k].total : parts[k].total * (double)exp_of(parts[k].top - others.top, c2);
+    loss_row(a, row, others);
   }
 }
 
-// Any row of at least 16 bytes: E chunks of each thread at a time relative to the running maximum, and again for the gradient.
-template <typename T, int NT, int E>
+// Longer rows: E chunks of each thread at a time relative to the running maximum, and again for the gradient, whose second reading comes
+// from the caches. Few such rows are cut into parts for as many workgroups: a launch for the parts' sums (PARTS), and one that joins
+// them and writes the gradient (JOIN): 301 rows of 100003 f16 @ us whole, @ in parts.
+enum { WHOLE, PARTS, JOIN };
+template <typename T, int NT, int E, int STAGE>
 __global__ __launch_bounds__(NT) void distill_long_kernel(DistillRows a) {
   constexpr int V = kVec<T>, SLOTS = NT * E;
   extern __shared__ __align__(16) char lds[];
   __shared__ float red[16];
   __shared__ DistillFactors box;
+  __shared__ float base;
   const int tid = threadIdx.x;
   const Copied l(lds, a.k);
   const Base2 c2(a.scale);
-  for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
+  // (The launch that joins has a workgroup more, for the losses.)
+  if (STAGE == JOIN && blockIdx.x + 1 == gridDim.x) {
+    losses_of_parts(a, tid, NT, c2);
+    return;
+  }
+  for (int id = blockIdx.x; id < a.rows * (STAGE == WHOLE ? 1 : a.split); id += gridDim.x - (STAGE == JOIN)) {
+    const int row = STAGE == WHOLE ? id : id / a.split, part = STAGE == WHOLE ? 0 : id - row * a.split;
+    const int begin = part * a.span, end = STAGE == WHOLE ? INT_MAX : begin + a.span;  // its chunks, whole pieces of SLOTS
     const T* z = (const T*)a.logits + (size_t)row * a.ld;
     const unsigned char* legal = a.legal ? a.legal + (size_t)row * a.ld_legal : nullptr;
     T* g = a.grad ? (T*)a.grad + (size_t)row * a.ld_grad : nullptr;
@@ -627,45 +650,58 @@ __global__ __launch_bounds__(NT) void distill_long_kernel(DistillRows a) {
       remove_past<T, NT, E>(tid, at, raw, c0);
     };
     Running run;
-    for (int c0 = 0; !at.none(c0); c0 += NT * E) {
-      u32x4 raw[E];
-      piece(c0, raw);
-      remove_listed<T, NT, E>(l, tid, at, raw, c0);
-      float f[E * V];
+    if (STAGE != JOIN) {
+      for (int c0 = begin; c0 < end && !at.none(c0); c0 += SLOTS) {
+        u32x4 raw[E];
+        piece(c0, raw);
+        remove_listed<T, NT, E>(l, tid, at, raw, c0);
+        float f[E * V];
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        const bool in = !at.none(c0 + e * NT);
+        for (int e = 0; e < E; e++) {
+          const bool in = !at.none(c0 + e * NT);
 #pragma unroll
-        for (int j = 0; j < V; j++) f[e * V + j] = in ? element<T>(raw[e], j) : -INFINITY;
+          for (int j = 0; j < V; j++) f[e * V + j] = in ? element<T>(raw[e], j) : -INFINITY;
+        }
+        run.add<E * V>(f, c2);
       }
-      run.add<E * V>(f, c2);
+      float moved;
+      run.join<NT>(c2, red, moved);
     }
-    float moved;
-    run.join<NT>(c2, red, moved);
+    if (STAGE == PARTS) {
+      if (tid == 0) a.parts[id] = Others{run.total, run.top};
+      continue;
+    }
     if (tid < 64) {
+      if (STAGE == JOIN) {
+        Others q = {0.0, -INFINITY};
+        if (tid < a.split) q = a.parts[row * a.split + tid];
+        run.top = wave_reduce<true>(q.top);
+        run.total = wave_sum(q.top == -INFINITY ? q.total : q.total * (double)exp_of(q.top - run.top, c2));
+      }
       const Known known = *l.known;
       double all;
       const DistillFactors f = distill_row(a, row, known, run.top, lead_of<true>(a, known, run.top), run.total, all);
       if (tid == 0) {
         box = f;
-        a.others[row] = Others{run.total, run.top};
+        base = run.top == -INFINITY ? 0.f : run.top;
+        if (STAGE == WHOLE) a.others[row] = Others{run.total, run.top};
       }
     }
     lds_barrier();
     if (!g) continue;
     hot_row<NT>(l, box);
     lds_barrier();
-    const bool part = __builtin_amdgcn_readfirstlane(box.part);
-    const float each = box.each, top = run.top == -INFINITY ? 0.f : run.top;
-    for (int c0 = 0; !at.none(c0); c0 += NT * E) {
+    const bool takes = __builtin_amdgcn_readfirstlane(box.part);
+    const float each = box.each, top = base;
+    for (int c0 = begin; c0 < end && !at.none(c0); c0 += SLOTS) {
       u32x4 raw[E];
-      if (part) piece(c0, raw);
+      if (takes) piece(c0, raw);
 #pragma unroll
       for (int e = 0; e < E; e++) {
         if (at.none(c0 + e * NT)) break;
-        const int c = tid + c0 + e * NT;
+        const int c = fresh(tid) + c0 + e * NT;
         float gf[V] = {};
-        if (part) {
+        if (takes) {
           // (A column without mass has no gradient, whatever the factor. A listed one's place is filled below.)
 #pragma unroll
           for (int j = 0; j < V; j++) {
@@ -697,13 +733,23 @@ void distill_typed(DistillRows p, hipStream_t s) {
   if (r.threads == 64) launch_k(distill_row_kernel<T, 256, 2>, groups, 256, Copied::bytes(256 * 2, p.k), s, p);
   else if (r.threads == 256) launch_k(distill_row_kernel<T, 256, 8>, groups, 256, Copied::bytes(256 * 8, p.k), s, p);
   else if (r.threads == 512) launch_k(distill_row_kernel<T, 512, 8>, groups, 512, Copied::bytes(512 * 8, p.k), s, p);
-  else launch_k(distill_long_kernel<T, 256, 4>, groups, 256, Copied::bytes(256 * 4, p.k), s, p);
-  launch_k(distill_loss_kernel, dim3(row_grid(p.rows, 256)), 256, 0, s, p);
+  else {
+    const RowParts cut = row_parts<T>(p.rows, p.columns, 512 * 4);
+    p.split = cut.split;
+    p.span = cut.span;
+    const size_t lds = Copied::bytes(512 * 4, p.k);
+    if (p.split > 1) {
+      launch_k(distill_long_kernel<T, 512, 4, PARTS>, dim3(p.rows * p.split), 512, lds, s, p);
+      return launch_k(distill_long_kernel<T, 512, 4, JOIN>, dim3(p.rows * p.split + 1), 512, lds, s, p);
+    }
+    launch_k(distill_long_kernel<T, 512, 4, WHOLE>, groups, 512, lds, s, p);
+  }
+  launch_k(distill_loss_kernel, dim3(row_grid(p.rows, 64)), 64, 0, s, p);
 }
 
 // Where what is known of the entries lies in the workspace.
 struct Plan {
-  size_t known, others, share, q, column, bytes;
+  size_t known, others, parts, share, q, column, bytes;
 };
 Plan plan_of(int rows, int columns, int k) {
   Plan p = {};
@@ -714,6 +760,7 @@ Plan plan_of(int rows, int columns, int k) {
   };
   p.known = room((size_t)rows * sizeof(Known));
   p.others = room((size_t)rows * sizeof(Others));
+  p.parts = room((size_t)rows * most_parts(rows, columns) * sizeof(Others));
   p.share = room((size_t)rows * k * 8);
   p.q = room((size_t)rows * k * 8);
   p.column = room((size_t)rows * k * 4);
@@ -743,6 +790,9 @@ void launch_distill_loss(const kg_distill_loss_args& a, hipStream_t s) {
   char* w = (char*)a.workspace;
   p.known = (Known*)(w + plan.known);
   p.others = (Others*)(w + plan.others);
+  p.parts = (Others*)(w + plan.parts);
+  p.split = 1;
+  p.span = 0;
   p.share = (double*)(w + plan.share);
   p.q = (double*)(w + plan.q);
   p.column = (int*)(w + plan.column);

@@ -187,6 +187,96 @@ __global__ __launch_bounds__((Row<T, L, E>::THREADS)) void layer_norm_held_kerne
   }
 }
 
+// Forward, a workgroup a row: its chunks lie along the lines of y (see Chunks), so that rows of odd strides are stored in whole ones, and
+// gamma and beta are read where they are used, which leaves a CU's registers to four rows and more: 2047 rows of 10007 f16 take
+// @ us (94 with chunks from the row's start and gamma and beta in registers, one row a CU).
+template <typename T, int NT, int E>
+__global__ __launch_bounds__(NT) void layer_norm_wide_kernel(LayerArgs a) {
+  constexpr int V = kVec<T>;
+  __shared__ float red[2][16][1], red2[2][16][2];
+  typedef Row<T, NT, E> R;
+  const int tid = threadIdx.x;
+  int turn = 0;
+  for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* x = (const T*)a.x + (size_t)row * a.ldx;
+    T* y = (T*)a.y + (size_t)row * a.ldy;
+    const Chunks<T> at(a.channels, y);
+    u32x4 raw[E];
+    load_row<T, NT, E>(x, tid, at, raw);
+    float mean = 0.f;
+    if (!a.rms) {
+      float s[1] = {0.f};
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        if (at.none(e * NT)) break;
+        const int c = tid + e * NT, first = at.first(c), limit = at.limit(c);
+        float t = 0.f;
+        if (at.whole(e * NT, NT)) {
+#pragma unroll
+          for (int j = 0; j < V; j++) t += element<T>(raw[e], j);
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; j++) t += j >= first && j < limit ? element<T>(raw[e], j) : 0.f;
+        }
+        s[0] += t;
+      }
+      R::sum(s, red[turn]);
+      mean = (float)((double)s[0] * a.inverse);
+    }
+    forget<E>(raw);
+    float q[2] = {0.f, 0.f};  // of the deviations, and of their squares
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      if (at.none(e * NT)) break;
+      const int c = tid + e * NT, first = at.first(c), limit = at.limit(c);
+      const bool whole = at.whole(e * NT, NT);
+      float t = 0.f, u = 0.f;
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        const float d = whole || (j >= first && j < limit) ? element<T>(raw[e], j) - mean : 0.f;
+        t += d;
+        u = __builtin_fmaf(d, d, u);
+      }
+      q[0] += t;
+      q[1] += u;
+    }
+    R::sum(q, red2[turn]);
+    turn ^= 1;
+    const double squares = (double)q[1] * a.inverse, m = a.rms ? 0.0 : correction((double)q[0] * a.inverse, squares);
+    const float rstd = root_of(squares - m * m, a.eps), shift = (float)m;
+    forget<E>(raw);
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      if (at.none(e * NT)) break;
+      const int c = fresh(tid) + e * NT, start = at.start(c);
+      float f[V];
+#pragma unroll
+      for (int j = 0; j < V; j++) f[j] = ((element<T>(raw[e], j) - mean) - shift) * rstd;
+      if (a.gamma) {
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+          const f32x4_any w = *(const f32x4_any*)(a.gamma + start + j);
+#pragma unroll
+          for (int k = 0; k < 4; k++) f[j + k] *= w[k];
+        }
+      }
+      if (a.beta) {
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+          const f32x4_any w = *(const f32x4_any*)(a.beta + start + j);
+#pragma unroll
+          for (int k = 0; k < 4; k++) f[j + k] += w[k];
+        }
+      }
+      store_gradient<T>(y, c, at.whole(e * NT, NT), a.past, at, f);
+    }
+    if (tid == 0) {
+      if (!a.rms) a.mean[row] = (float)((double)mean + m);
+      a.rstd[row] = rstd;
+    }
+  }
+}
+
 // The rows of a workgroup one after another, with the channels' sums of dy h and dy in registers: a part for each workgroup.
 template <typename T, int L, int E>
 __global__ __launch_bounds__((Row<T, L, E>::THREADS)) void layer_norm_back_held_kernel(LayerArgs a) {
@@ -396,15 +486,32 @@ struct Shape {
   int lanes = 0, each = 0;
 };
 // (Narrow rows share a wave, so that its lanes are busy and their sums take fewer steps.)
-Shape shape_of(int channels, int vec, bool backward) {
-  const int chunks = (channels + vec - 1) / vec;
+Shape wave_shape(int chunks) {
   if (chunks <= 8) return {8, 1};
   if (chunks <= 64) return {16, (chunks + 15) / 16};
   if (chunks <= 256) return {64, (chunks + 63) / 64};
+  return {};
+}
+// Of the forward pass, whose chunks may begin up to a line before the row.
+template <typename T>
+Shape forward_shape(const LayerArgs& p) {
+  const int line = Chunks<T>::line(p.channels);
+  const bool aligned = (uintptr_t)p.y % line == 0 && (p.rows == 1 || p.ldy * (long long)sizeof(T) % line == 0);
+  const int least = (int)(((long long)p.channels + kVec<T> - 1) / kVec<T>), chunks = least + (aligned ? 0 : line / 16);
+  if (least <= 256) return wave_shape(least);
+  if (chunks <= 512) return {256, 2};
+  if (chunks <= 1024) return {256, 4};
+  if (chunks <= 1536) return {512, 3};
+  if (chunks <= 2048) return {512, 4};
+  if (chunks <= 4096) return {1024, 4};
+  return {};
+}
+Shape backward_shape(int channels, int vec) {
+  const int chunks = (int)(((long long)channels + vec - 1) / vec);
+  if (chunks <= 256) return wave_shape(chunks);
   if (chunks <= 512) return {256, 2};
   if (chunks <= 1024) return {512, 2};
   if (chunks <= 2048) return {1024, 2};
-  if (chunks <= 4096 && !backward) return {1024, 4};
   return {};
 }
 
@@ -430,48 +537,52 @@ LayerArgs args_of(const kg_layer_norm_args& a) {
 }
 
 template <typename T, int L, int E>
-void held(LayerArgs p, bool backward, hipStream_t s) {
-  constexpr int per = Row<T, L, E>::ROWS;
-  if (backward) {
-    p.split = parts_of(p.rows, per);
-    launch_k(layer_norm_back_held_kernel<T, L, E>, dim3(p.split), Row<T, L, E>::THREADS, 0, s, p);
-  } else {
-    launch_k(layer_norm_held_kernel<T, L, E>, dim3(std::min(row_grid(p.rows, per), kGrid)), Row<T, L, E>::THREADS, 0, s, p);
-  }
+void held(const LayerArgs& p, bool backward, hipStream_t s) {
+  constexpr int threads = Row<T, L, E>::THREADS;
+  if (backward) launch_k(layer_norm_back_held_kernel<T, L, E>, dim3(p.split), threads, 0, s, p);
+  else if constexpr (L <= 64) launch_k(layer_norm_held_kernel<T, L, E>, dim3(std::min(row_grid(p.rows, Row<T, L, E>::ROWS), kGrid)), threads, 0, s, p);
 }
-
-// Returns the parts that the sums over the rows are in.
+// A row of at most 256 chunks.
 template <typename T>
-int rows_typed(LayerArgs p, bool backward, hipStream_t s) {
-  const Shape r = shape_of(p.channels, kVec<T>, backward);
-  p.split = parts_of(p.rows, r.lanes == 0 || r.lanes > 64 ? 1 : LT / r.lanes);
+void waves(const LayerArgs& p, Shape r, bool backward, hipStream_t s) {
   if (r.lanes == 8) held<T, 8, 1>(p, backward, s);
   else if (r.lanes == 16 && r.each == 1) held<T, 16, 1>(p, backward, s);
   else if (r.lanes == 16 && r.each == 2) held<T, 16, 2>(p, backward, s);
   else if (r.lanes == 16 && r.each == 3) held<T, 16, 3>(p, backward, s);
   else if (r.lanes == 16) held<T, 16, 4>(p, backward, s);
-  else if (r.lanes == 64 && r.each == 2) held<T, 64, 2>(p, backward, s);
-  else if (r.lanes == 64 && r.each == 3) held<T, 64, 3>(p, backward, s);
-  else if (r.lanes == 64) held<T, 64, 4>(p, backward, s);
-  else if (r.lanes == 256) held<T, 256, 2>(p, backward, s);
-  else if (r.lanes == 512) held<T, 512, 2>(p, backward, s);
-  else if (r.lanes == 1024 && r.each == 2) held<T, 1024, 2>(p, backward, s);
-  else if (r.lanes == 1024) launch_k(layer_norm_held_kernel<T, 1024, 4>, dim3(std::min(row_grid(p.rows, 1), kGrid)), 1024, 0, s, p);
-  else if (!backward) launch_k(layer_norm_kernel<T>, dim3(row_grid(p.rows, 1)), LT, 0, s, p);
+  else if (r.each == 2) held<T, 64, 2>(p, backward, s);
+  else if (r.each == 3) held<T, 64, 3>(p, backward, s);
+  else held<T, 64, 4>(p, backward, s);
+}
+
+template <typename T>
+void forward_typed(const LayerArgs& p, hipStream_t s) {
+  const Shape r = forward_shape<T>(p);
+  const dim3 grid(row_grid(p.rows, 1));
+  if (r.lanes && r.lanes <= 64) waves<T>(p, r, false, s);
+  else if (r.lanes == 256 && r.each == 2) launch_k(layer_norm_wide_kernel<T, 256, 2>, grid, 256, 0, s, p);
+  else if (r.lanes == 256) launch_k(layer_norm_wide_kernel<T, 256, 4>, grid, 256, 0, s, p);
+  else if (r.lanes == 512 && r.each == 3) launch_k(layer_norm_wide_kernel<T, 512, 3>, grid, 512, 0, s, p);
+  else if (r.lanes == 512) launch_k(layer_norm_wide_kernel<T, 512, 4>, grid, 512, 0, s, p);
+  else if (r.lanes == 1024) launch_k(layer_norm_wide_kernel<T, 1024, 4>, grid, 1024, 0, s, p);
+  else launch_k(layer_norm_kernel<T>, grid, LT, 0, s, p);
+}
+
+// Returns the parts that the sums over the rows are in.
+template <typename T>
+int backward_typed(LayerArgs p, hipStream_t s) {
+  const Shape r = backward_shape(p.channels, kVec<T>);
+  p.split = parts_of(p.rows, r.lanes == 0 || r.lanes > 64 ? 1 : LT / r.lanes);
+  if (r.lanes && r.lanes <= 64) waves<T>(p, r, true, s);
+  else if (r.lanes == 256) held<T, 256, 2>(p, true, s);
+  else if (r.lanes == 512) held<T, 512, 2>(p, true, s);
+  else if (r.lanes == 1024) held<T, 1024, 2>(p, true, s);
   else {
     launch_k(layer_norm_back_kernel<T>, dim3(row_grid(p.rows, 1)), LT, 0, s, p);
     if (p.dgamma || p.dbeta)
       launch_k(layer_norm_sums_kernel<T>, dim3(std::min((p.channels + LT - 1) / LT, 1024), p.split), LT, 0, s, p);
   }
   return p.split;
-}
-
-int rows_of(const LayerArgs& p, int type, bool backward, hipStream_t s) {
-  switch (type) {
-    case PREC_F32: return rows_typed<float>(p, backward, s);
-    case PREC_F16: return rows_typed<f16>(p, backward, s);
-    default: return rows_typed<bf16>(p, backward, s);
-  }
 }
 
 }  // namespace
@@ -482,13 +593,24 @@ size_t layer_norm_workspace(int rows, int channels) {
 }
 
 void launch_layer_norm(const kg_layer_norm_args& a, hipStream_t s) {
-  rows_of(args_of(a), a.type, false, s);
+  const LayerArgs p = args_of(a);
+  switch (a.type) {
+    case PREC_F32: forward_typed<float>(p, s); break;
+    case PREC_F16: forward_typed<f16>(p, s); break;
+    default: forward_typed<bf16>(p, s); break;
+  }
   KGX_CHECK_LAUNCH();
 }
 
 void launch_layer_norm_backward(const kg_layer_norm_args& a, hipStream_t s) {
   LayerArgs p = args_of(a);
-  if (p.rows) p.split = rows_of(p, a.type, true, s);  // (the sums over no rows are 0)
+  if (p.rows) {  // (the sums over no rows are 0)
+    switch (a.type) {
+      case PREC_F32: p.split = backward_typed<float>(p, s); break;
+      case PREC_F16: p.split = backward_typed<f16>(p, s); break;
+      default: p.split = backward_typed<bf16>(p, s); break;
+    }
+  }
   if (p.dgamma || p.dbeta) launch_k(layer_norm_params_kernel, dim3((int)std::min((2ll * p.channels + 63) / 64, 65536ll)), PT, 0, s, p);
   KGX_CHECK_LAUNCH();
 }

@@ -26,6 +26,7 @@ struct LayerArgs {
   const float *gamma, *beta;
   float *mean, *rstd, *dgamma, *dbeta;
   float* parts;  // [parts][2][channels] sums of dy h and dy over a part's rows
+  struct RowMeans* means;  // [rows], of wide rows
   int rows, channels, rms, past, split;
   double eps, inverse;  // inverse: 1 / channels
 };
@@ -277,16 +278,15 @@ __global__ __launch_bounds__(NT) void layer_norm_wide_kernel(LayerArgs a) {
   }
 }
 
-// The rows of a workgroup one after another, with the channels' sums of dy h and dy in registers: a part for each workgroup.
+// Backward, the rows of a workgroup one after another, with the channels' sums of dy h and dy in registers: a part for each workgroup.
+// Here for rows of a wave and less.
 template <typename T, int L, int E>
-__global__ __launch_bounds__((Row<T, L, E>::THREADS)) void layer_norm_back_held_kernel(LayerArgs a) {
+__global__ __launch_bounds__(LT) void layer_norm_back_held_kernel(LayerArgs a) {
   using R = Row<T, L, E>;
   constexpr int V = R::V, SPAN = L * E * V;  // elements that a row's lanes hold
-  __shared__ float red[2][16][2];
-  __shared__ float joined[L <= 64 ? 2 * SPAN : 1];
+  __shared__ float joined[2 * SPAN];
   float gamma[E][V], s1[E][V] = {}, s2[E][V] = {};
   R::vector(a.gamma, a.channels, 1.f, gamma);
-  int turn = 0;
   for (int first = blockIdx.x * R::ROWS; first < a.rows; first += gridDim.x * R::ROWS) {
     const int row = first + threadIdx.x / L;
     const bool in = row < a.rows;
@@ -310,8 +310,7 @@ __global__ __launch_bounds__((Row<T, L, E>::THREADS)) void layer_norm_back_held_
       q[0] += t;
       q[1] += u;
     }
-    R::sum(q, red[turn]);
-    turn ^= 1;
+    R::sum(q, (float(*)[2])nullptr);
     if (!in) continue;
     const float m1 = a.rms ? 0.f : (float)((double)q[0] * a.inverse), m2 = (float)((double)q[1] * a.inverse);
     T* dx = (T*)a.dx + (size_t)row * a.lddx;
@@ -328,48 +327,117 @@ __global__ __launch_bounds__((Row<T, L, E>::THREADS)) void layer_norm_back_held_
   }
   if (!a.dgamma && !a.dbeta) return;
   float* part = a.parts + (size_t)blockIdx.x * 2 * a.channels;
-  if constexpr (L <= 64) {
-    // The rows that a wave held side by side, then its waves in turn.
+  // The rows that a wave held side by side, then its waves in turn.
 #pragma unroll
-    for (int e = 0; e < E; e++) {
+  for (int e = 0; e < E; e++) {
 #pragma unroll
-      for (int j = 0; j < V; j++) {
+    for (int j = 0; j < V; j++) {
 #pragma unroll
-        for (int o = L; o < 64; o <<= 1) {
-          s1[e][j] += __shfl_xor(s1[e][j], o);
-          s2[e][j] += __shfl_xor(s2[e][j], o);
+      for (int o = L; o < 64; o <<= 1) {
+        s1[e][j] += __shfl_xor(s1[e][j], o);
+        s2[e][j] += __shfl_xor(s2[e][j], o);
+      }
+    }
+  }
+  for (int w = 0; w < LT / 64; w++) {
+    if (threadIdx.x >> 6 == w && (threadIdx.x & 63) < L) {
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          float* at = joined + (R::lane() + e * L) * V + j;
+          at[0] = (w ? at[0] : 0.f) + s1[e][j];
+          at[SPAN] = (w ? at[SPAN] : 0.f) + s2[e][j];
         }
       }
     }
-    for (int w = 0; w < LT / 64; w++) {
-      if (threadIdx.x >> 6 == w && (threadIdx.x & 63) < L) {
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-#pragma unroll
-          for (int j = 0; j < V; j++) {
-            float* at = joined + (R::lane() + e * L) * V + j;
-            at[0] = (w ? at[0] : 0.f) + s1[e][j];
-            at[SPAN] = (w ? at[SPAN] : 0.f) + s2[e][j];
-          }
-        }
-      }
-      lds_barrier();
-    }
-    for (int c = threadIdx.x; c < a.channels; c += LT) {
-      part[c] = joined[c];
-      part[a.channels + c] = joined[SPAN + c];
-    }
-  } else {
+    lds_barrier();
+  }
+  for (int c = threadIdx.x; c < a.channels; c += LT) {
+    part[c] = joined[c];
+    part[a.channels + c] = joined[SPAN + c];
+  }
+}
+
+// The same for a workgroup a row. gamma lies in LDS, and the next row's words are asked for before this one's sums, as few workgroups
+// fit a CU beside the channels' sums (3051 rows of 16384 bf16: @ us, 205 with gamma in registers, some of which went to memory).
+template <typename T, int NT, int E>
+__global__ __launch_bounds__(NT) void layer_norm_back_wide_kernel(LayerArgs a) {
+  using R = Row<T, NT, E>;
+  constexpr int V = R::V;
+  extern __shared__ __align__(16) float gamma[];  // [chunks][V], 1 past the channels
+  __shared__ float red[2][16][2];
+  float s1[E][V] = {}, s2[E][V] = {};
+  for (int c = threadIdx.x; c < NT * E * V; c += NT) gamma[c] = a.gamma && c < a.channels ? a.gamma[c] : 1.f;
+  const auto vec4 = [&](int e, int j) { return *(const floatx4*)(gamma + (threadIdx.x + e * NT) * V + j); };
+  int turn = 0;
+  u32x4 x[E], dy[E], next_x[E], next_dy[E];
+  const auto ask = [&](int row, u32x4(&to_x)[E], u32x4(&to_dy)[E]) {
+    R::load((const T*)a.x + (size_t)row * a.ldx, a.channels, row < a.rows, to_x);
+    R::load((const T*)a.dy + (size_t)row * a.lddy, a.channels, row < a.rows, to_dy);
+  };
+  ask(blockIdx.x, x, dy);
+  __syncthreads();
+  for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const float mean = a.rms ? 0.f : a.mean[row], rstd = a.rstd[row];
+    ask(row + gridDim.x, next_x, next_dy);
+    float q[2] = {0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      const int c = (R::lane() + e * L) * V;
+      float t = 0.f, u = 0.f;
 #pragma unroll
-      for (int j = 0; j < V; j++)
-        if (c + j < a.channels) {
-          part[c + j] = s1[e][j];
-          part[a.channels + c + j] = s2[e][j];
+      for (int j4 = 0; j4 < V; j4 += 4) {
+        const floatx4 w = vec4(e, j4);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int j = j4 + k;
+          const float g = element<T>(dy[e], j), d = g * w[k], h = (element<T>(x[e], j) - mean) * rstd;
+          t += d;
+          u = __builtin_fmaf(d, h, u);
+          s1[e][j] = __builtin_fmaf(g, h, s1[e][j]);
+          s2[e][j] += g;
         }
+      }
+      q[0] += t;
+      q[1] += u;
+      __builtin_amdgcn_sched_barrier(0);
     }
+    R::sum(q, red[turn]);
+    turn ^= 1;
+    const float m1 = a.rms ? 0.f : (float)((double)q[0] * a.inverse), m2 = (float)((double)q[1] * a.inverse);
+    T* dx = (T*)a.dx + (size_t)row * a.lddx;
+    forget<E>(x);
+    forget<E>(dy);
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      float f[V];
+#pragma unroll
+      for (int j4 = 0; j4 < V; j4 += 4) {
+        const floatx4 w = vec4(e, j4);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int j = j4 + k;
+          const float d = element<T>(dy[e], j) * w[k], h = (element<T>(x[e], j) - mean) * rstd;
+          f[j] = rstd * __builtin_fmaf(-h, m2, d - m1);
+        }
+      }
+      R::store(dx, a.channels, e, a.past, f);
+      x[e] = next_x[e];
+      dy[e] = next_dy[e];
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  if (!a.dgamma && !a.dbeta) return;
+  float* part = a.parts + (size_t)blockIdx.x * 2 * a.channels;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const int c = (R::lane() + e * NT) * V;
+#pragma unroll
+    for (int j = 0; j < V; j++)
+      if (c + j < a.channels) {
+        part[c + j] = s1[e][j];
+        part[a.channels + c + j] = s2[e][j];
+      }
   }
 }
 
@@ -409,43 +477,106 @@ __global__ __launch_bounds__(LT) void layer_norm_kernel(LayerArgs a) {
   }
 }
 
+// Backward, any row: a launch for the rows' two means, by a workgroup a row, and one by slabs of the channels, whose waves take a slab of 64
+// chunks over the rows in turn with the channels' sums in few registers. x and dy are read twice, in two streams without a wait between
+// a row's loads and its stores.
+struct RowMeans {
+  float mean, rstd, m1, m2;
+};
 template <typename T>
-__global__ __launch_bounds__(LT) void layer_norm_back_kernel(LayerArgs a) {
-  __shared__ float red[16];
+__global__ __launch_bounds__(LT) void layer_norm_back_means_kernel(LayerArgs a) {
+  constexpr int V = kVec<T>, E = 4;
+  __shared__ float red[2][16][2];
   const int tid = threadIdx.x;
+  int turn = 0;
   for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = (const T*)a.x + (size_t)row * a.ldx;
     const T* dy = (const T*)a.dy + (size_t)row * a.lddy;
-    T* dx = (T*)a.dx + (size_t)row * a.lddx;
     const float mean = a.rms ? 0.f : a.mean[row], rstd = a.rstd[row];
-    float s1 = 0.f, s2 = 0.f;
-    for (int c = tid; c < a.channels; c += LT) {
-      const float d = (float)dy[c] * (a.gamma ? a.gamma[c] : 1.f);
-      s1 += d;
-      s2 = __builtin_fmaf(d, ((float)x[c] - mean) * rstd, s2);
+    float q[2] = {0.f, 0.f};
+    for (int c0 = 0; c0 < a.channels; c0 += LT * E * V) {
+      float fx[E][V], fy[E][V];
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const int c = c0 + (tid + e * LT) * V, left = max(a.channels - c, 0);
+        load_vec<T>(x + c, left, fx[e]);
+        load_vec<T>(dy + c, left, fy[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const int c = c0 + (tid + e * LT) * V, left = max(a.channels - c, 0);
+        float t = 0.f, u = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+          float w[4] = {1.f, 1.f, 1.f, 1.f};
+          if (a.gamma) load_vec<float>(a.gamma + c + j, left - j, w);
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const float d = fy[e][j + k] * w[k];
+            t += d;
+            u = __builtin_fmaf(d, j + k < left ? (fx[e][j + k] - mean) * rstd : 0.f, u);
+          }
+        }
+        q[0] += t;
+        q[1] += u;
+      }
     }
-    const float m1 = a.rms ? 0.f : (float)(row_sum<LT>(s1, red) * a.inverse), m2 = (float)(row_sum<LT>(s2, red) * a.inverse);
-    for (int c = tid; c < a.channels; c += LT) {
-      const float d = (float)dy[c] * (a.gamma ? a.gamma[c] : 1.f), h = ((float)x[c] - mean) * rstd;
-      dx[c] = to_t<T>(rstd * __builtin_fmaf(-h, m2, d - m1));
-    }
+    Row<T, LT, 1>::sum(q, red[turn]);
+    turn ^= 1;
+    if (tid == 0) a.means[row] = RowMeans{mean, rstd, a.rms ? 0.f : (float)((double)q[0] * a.inverse), (float)((double)q[1] * a.inverse)};
   }
 }
 
-// The sums over a part of the rows, a thread a channel.
+constexpr int SW = LT / 64;  // waves of a slab's workgroup
 template <typename T>
-__global__ __launch_bounds__(LT) void layer_norm_sums_kernel(LayerArgs a) {
-  const int per = (a.rows + a.split - 1) / a.split, part = blockIdx.y, first = part * per, last = min(first + per, a.rows);
-  for (int c = blockIdx.x * LT + threadIdx.x; c < a.channels; c += gridDim.x * LT) {
-    float s1 = 0.f, s2 = 0.f;
-    for (int row = first; row < last; row++) {
-      const float d = (float)((const T*)a.dy)[(size_t)row * a.lddy + c];
-      const float h = ((float)((const T*)a.x)[(size_t)row * a.ldx + c] - (a.rms ? 0.f : a.mean[row])) * a.rstd[row];
-      s1 = __builtin_fmaf(d, h, s1);
-      s2 += d;
+__global__ __launch_bounds__(LT) void layer_norm_back_slab_kernel(LayerArgs a, int slabs) {
+  constexpr int V = kVec<T>, AT_ONCE = 4;
+  __shared__ float joined[SW][2][64 * V];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int part = blockIdx.x / slabs, c = ((blockIdx.x - part * slabs) * 64 + lane) * V, left = max(a.channels - c, 0);
+  const int per = (a.rows + a.split - 1) / a.split, first = part * per, last = min(first + per, a.rows);
+  float gamma[V], s1[V] = {}, s2[V] = {};
+#pragma unroll
+  for (int j = 0; j < V; j++) gamma[j] = a.gamma && j < left ? a.gamma[c + j] : 1.f;
+  for (int row = first + w; row < last; row += SW * AT_ONCE) {
+    float x[AT_ONCE][V], dy[AT_ONCE][V];
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; k++) {
+      const int r = min(row + k * SW, last - 1);
+      load_vec<T>((const T*)a.x + (size_t)r * a.ldx + c, left, x[k]);
+      load_vec<T>((const T*)a.dy + (size_t)r * a.lddy + c, left, dy[k]);
     }
-    a.parts[(size_t)part * 2 * a.channels + c] = s1;
-    a.parts[((size_t)part * 2 + 1) * a.channels + c] = s2;
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; k++) {
+      const int r = row + k * SW;
+      if (r >= last) break;
+      const RowMeans n = a.means[r];
+      float f[V];
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        const float g = dy[k][j], h = (x[k][j] - n.mean) * n.rstd;
+        s1[j] = __builtin_fmaf(g, h, s1[j]);
+        s2[j] += g;
+        f[j] = n.rstd * __builtin_fmaf(-h, n.m2, g * gamma[j] - n.m1);
+      }
+      T* to = (T*)a.dx + (size_t)r * a.lddx + c;
+      if (a.past && left >= V) store_past<T>(to, f);
+      else store_vec<T>(to, left, f);
+    }
+  }
+  if (!a.dgamma && !a.dbeta) return;
+#pragma unroll
+  for (int j = 0; j < V; j++) {
+    joined[w][0][lane * V + j] = s1[j];
+    joined[w][1][lane * V + j] = s2[j];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * 64 * V; i += LT) {
+    const int side = i >= 64 * V, at = i - side * 64 * V, column = (blockIdx.x - part * slabs) * 64 * V + at;
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < SW; k++) t += joined[k][side][at];
+    if (column < a.channels) a.parts[((size_t)part * 2 + side) * a.channels + column] = t;
   }
 }
 
@@ -485,20 +616,16 @@ __global__ __launch_bounds__(PT) void layer_norm_params_kernel(LayerArgs a) {
 struct Shape {
   int lanes = 0, each = 0;
 };
-// (Narrow rows share a wave, so that its lanes are busy and their sums take fewer steps.)
-Shape wave_shape(int chunks) {
-  if (chunks <= 8) return {8, 1};
-  if (chunks <= 64) return {16, (chunks + 15) / 16};
-  if (chunks <= 256) return {64, (chunks + 63) / 64};
-  return {};
-}
-// Of the forward pass, whose chunks may begin up to a line before the row.
+// Forward, whose wide rows' chunks may begin up to a line before the row. (Narrow rows share a wave, so that its lanes are busy and their
+// sums take fewer steps.)
 template <typename T>
 Shape forward_shape(const LayerArgs& p) {
   const int line = Chunks<T>::line(p.channels);
   const bool aligned = (uintptr_t)p.y % line == 0 && (p.rows == 1 || p.ldy * (long long)sizeof(T) % line == 0);
   const int least = (int)(((long long)p.channels + kVec<T> - 1) / kVec<T>), chunks = least + (aligned ? 0 : line / 16);
-  if (least <= 256) return wave_shape(least);
+  if (least <= 8) return {8, 1};
+  if (least <= 64) return {16, (least + 15) / 16};
+  if (least <= 256) return {64, (least + 63) / 64};
   if (chunks <= 512) return {256, 2};
   if (chunks <= 1024) return {256, 4};
   if (chunks <= 1536) return {512, 3};
@@ -506,17 +633,31 @@ Shape forward_shape(const LayerArgs& p) {
   if (chunks <= 4096) return {1024, 4};
   return {};
 }
+// Backward: few chunks a thread, whose sums of dy h and dy take four registers an element of 16 bits and more (97656 rows of 512 bf16
+// by 16 lanes with four chunks: 64 us, by 64 with one 49). Wider rows go by slabs (see layer_norm_back_slab_kernel): held, a row and its
+// channels' sums leave a CU one workgroup (3051 rows of 16384 bf16: 152 us, by slabs @; 6103 of 8192 bf16 109 and @, but 3051 of
+// 8192 f32 60 and @).
 Shape backward_shape(int channels, int vec) {
   const int chunks = (int)(((long long)channels + vec - 1) / vec);
-  if (chunks <= 256) return wave_shape(chunks);
+  if (chunks <= 8) return {8, 1};
+  if (chunks <= 16) return {16, 1};
+  if (chunks <= 32) return {32, 1};
+  if (chunks <= 64) return {64, 1};
+  if (chunks <= 128) return {64, 2};
+  if (chunks <= 256) return {256, 1};
   if (chunks <= 512) return {256, 2};
-  if (chunks <= 1024) return {512, 2};
-  if (chunks <= 2048) return {1024, 2};
+  if (vec == 4 && chunks <= 1024) return {512, 2};
+  if (vec == 4 && chunks <= 2048) return {1024, 2};
   return {};
 }
 
+// (Rows that may go by slabs, whatever their type, have their means in front of the parts.)
+size_t means_bytes(int rows, int channels) { return channels > 512 * 8 ? ((size_t)rows * sizeof(RowMeans) + 255) / 256 * 256 : 0; }
 // Workgroups of the backward pass, each with a part of the sums: at least eight rows each once there is one for each CU.
 int parts_of(int rows, int per) { return (int)std::min((rows + (long long)per - 1) / per, (long long)std::min(std::max(256, rows / 8), kMostParts)); }
+
+// The same by slabs: some 2048 workgroups in all, of 16 rows and more.
+int slab_parts(int rows, int slabs) { return std::max(1, std::min({rows / 16, 2048 / slabs, 256})); }
 
 LayerArgs args_of(const kg_layer_norm_args& a) {
   LayerArgs p;
@@ -527,7 +668,8 @@ LayerArgs args_of(const kg_layer_norm_args& a) {
   p.gamma = a.gamma; p.beta = a.beta;
   p.mean = a.mean; p.rstd = a.rstd;
   p.dgamma = a.dgamma; p.dbeta = a.dbeta;
-  p.parts = (float*)a.workspace;
+  p.parts = (float*)((char*)a.workspace + means_bytes(a.rows, a.channels));
+  p.means = (RowMeans*)a.workspace;
   p.rows = a.rows; p.channels = a.channels; p.rms = a.rms != 0;
   p.past = gradient_past(a.rows, a.channels, a.type);
   p.split = 0;
@@ -537,29 +679,21 @@ LayerArgs args_of(const kg_layer_norm_args& a) {
 }
 
 template <typename T, int L, int E>
-void held(const LayerArgs& p, bool backward, hipStream_t s) {
-  constexpr int threads = Row<T, L, E>::THREADS;
-  if (backward) launch_k(layer_norm_back_held_kernel<T, L, E>, dim3(p.split), threads, 0, s, p);
-  else if constexpr (L <= 64) launch_k(layer_norm_held_kernel<T, L, E>, dim3(std::min(row_grid(p.rows, Row<T, L, E>::ROWS), kGrid)), threads, 0, s, p);
+void forward_held(const LayerArgs& p, hipStream_t s) {
+  launch_k(layer_norm_held_kernel<T, L, E>, dim3(std::min(row_grid(p.rows, Row<T, L, E>::ROWS), kGrid)), LT, 0, s, p);
 }
-// A row of at most 256 chunks.
-template <typename T>
-void waves(const LayerArgs& p, Shape r, bool backward, hipStream_t s) {
-  if (r.lanes == 8) held<T, 8, 1>(p, backward, s);
-  else if (r.lanes == 16 && r.each == 1) held<T, 16, 1>(p, backward, s);
-  else if (r.lanes == 16 && r.each == 2) held<T, 16, 2>(p, backward, s);
-  else if (r.lanes == 16 && r.each == 3) held<T, 16, 3>(p, backward, s);
-  else if (r.lanes == 16) held<T, 16, 4>(p, backward, s);
-  else if (r.each == 2) held<T, 64, 2>(p, backward, s);
-  else if (r.each == 3) held<T, 64, 3>(p, backward, s);
-  else held<T, 64, 4>(p, backward, s);
-}
-
 template <typename T>
 void forward_typed(const LayerArgs& p, hipStream_t s) {
   const Shape r = forward_shape<T>(p);
   const dim3 grid(row_grid(p.rows, 1));
-  if (r.lanes && r.lanes <= 64) waves<T>(p, r, false, s);
+  if (r.lanes == 8) forward_held<T, 8, 1>(p, s);
+  else if (r.lanes == 16 && r.each == 1) forward_held<T, 16, 1>(p, s);
+  else if (r.lanes == 16 && r.each == 2) forward_held<T, 16, 2>(p, s);
+  else if (r.lanes == 16 && r.each == 3) forward_held<T, 16, 3>(p, s);
+  else if (r.lanes == 16) forward_held<T, 16, 4>(p, s);
+  else if (r.lanes == 64 && r.each == 2) forward_held<T, 64, 2>(p, s);
+  else if (r.lanes == 64 && r.each == 3) forward_held<T, 64, 3>(p, s);
+  else if (r.lanes == 64) forward_held<T, 64, 4>(p, s);
   else if (r.lanes == 256 && r.each == 2) launch_k(layer_norm_wide_kernel<T, 256, 2>, grid, 256, 0, s, p);
   else if (r.lanes == 256) launch_k(layer_norm_wide_kernel<T, 256, 4>, grid, 256, 0, s, p);
   else if (r.lanes == 512 && r.each == 3) launch_k(layer_norm_wide_kernel<T, 512, 3>, grid, 512, 0, s, p);
@@ -568,19 +702,34 @@ void forward_typed(const LayerArgs& p, hipStream_t s) {
   else launch_k(layer_norm_kernel<T>, grid, LT, 0, s, p);
 }
 
+template <typename T, int NT, int E>
+void backward_wide(const LayerArgs& p, hipStream_t s) {
+  launch_k(layer_norm_back_wide_kernel<T, NT, E>, dim3(p.split), NT, (size_t)NT * E * kVec<T> * 4, s, p);
+}
+
 // Returns the parts that the sums over the rows are in.
 template <typename T>
 int backward_typed(LayerArgs p, hipStream_t s) {
   const Shape r = backward_shape(p.channels, kVec<T>);
   p.split = parts_of(p.rows, r.lanes == 0 || r.lanes > 64 ? 1 : LT / r.lanes);
-  if (r.lanes && r.lanes <= 64) waves<T>(p, r, true, s);
-  else if (r.lanes == 256) held<T, 256, 2>(p, true, s);
-  else if (r.lanes == 512) held<T, 512, 2>(p, true, s);
-  else if (r.lanes == 1024) held<T, 1024, 2>(p, true, s);
-  else {
-    launch_k(layer_norm_back_kernel<T>, dim3(row_grid(p.rows, 1)), LT, 0, s, p);
-    if (p.dgamma || p.dbeta)
-      launch_k(layer_norm_sums_kernel<T>, dim3(std::min((p.channels + LT - 1) / LT, 1024), p.split), LT, 0, s, p);
+  const dim3 grid(p.split);
+  if (r.lanes == 8) launch_k(layer_norm_back_held_kernel<T, 8, 1>, grid, LT, 0, s, p);
+  else if (r.lanes == 16) launch_k(layer_norm_back_held_kernel<T, 16, 1>, grid, LT, 0, s, p);
+  else if (r.lanes == 32) launch_k(layer_norm_back_held_kernel<T, 32, 1>, grid, LT, 0, s, p);
+  else if (r.lanes == 64 && r.each == 1) launch_k(layer_norm_back_held_kernel<T, 64, 1>, grid, LT, 0, s, p);
+  else if (r.lanes == 64) launch_k(layer_norm_back_held_kernel<T, 64, 2>, grid, LT, 0, s, p);
+  else if (r.lanes == 256 && r.each == 1) backward_wide<T, 256, 1>(p, s);
+  else if (r.lanes == 256) backward_wide<T, 256, 2>(p, s);
+  else if (r.lanes) {
+    if constexpr (sizeof(T) == 4) {
+      if (r.lanes == 512) backward_wide<T, 512, 2>(p, s);
+      else backward_wide<T, 1024, 2>(p, s);
+    }
+  } else {
+    const int slabs = (int)(((long long)p.channels + 64 * kVec<T> - 1) / (64 * kVec<T>));
+    p.split = slab_parts(p.rows, slabs);
+    launch_k(layer_norm_back_means_kernel<T>, dim3(row_grid(p.rows, 1)), LT, 0, s, p);
+    launch_k(layer_norm_back_slab_kernel<T>, dim3(p.split * slabs), LT, 0, s, p, slabs);
   }
   return p.split;
 }
@@ -589,7 +738,7 @@ int backward_typed(LayerArgs p, hipStream_t s) {
 
 size_t layer_norm_workspace(int rows, int channels) {
   if (rows < 1 || channels < 1) return 0;
-  return (size_t)parts_of(rows, 1) * 2 * channels * sizeof(float);
+  return means_bytes(rows, channels) + (size_t)parts_of(rows, 1) * 2 * channels * sizeof(float);
 }
 
 void launch_layer_norm(const kg_layer_norm_args& a, hipStream_t s) {

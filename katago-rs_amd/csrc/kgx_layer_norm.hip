@@ -42,54 +42,63 @@ __device__ __forceinline__ double correction(double off, double squares) { retur
 // ---- Rows that fit the registers of their lanes: one read. ----
 
 // L lanes a row: neighbours of one wave (several rows a wave below 64), or a workgroup. Lane i holds chunks i, i + L, ... of 16
-// bytes; what lies past the row's end is 0 in the words.
+// bytes. A chunk that reaches over the row's end is its last 16 bytes instead, so that no lane takes single elements: what it has of the
+// chunk before counts there alone (first), and is stored twice, with the same values. Rows shorter than a chunk are taken by elements,
+// 0 in the words behind them.
 template <typename T, int L, int E>
 struct Row {
   static constexpr int V = kVec<T>, THREADS = L <= 64 ? LT : L, ROWS = THREADS / L;  // of a workgroup
   typedef typename AnyWords<T>::type words_t;
   static __device__ __forceinline__ int lane() { return threadIdx.x % L; }
+  static __device__ __forceinline__ int column(int e) { return (lane() + e * L) * V; }
+  static __device__ __forceinline__ int start(int channels, int e) { return max(min(column(e), channels - V), 0); }
+  // Of a lane's chunk, elements [first, limit) count; every one where whole (the same for all lanes).
+  static __device__ __forceinline__ int first(int channels, int e) { return column(e) - start(channels, e); }
+  static __device__ __forceinline__ int limit(int channels) { return min(channels, V); }
+  static __device__ __forceinline__ bool whole(int channels, int e) { return (e + 1) * L * V <= channels; }
   static __device__ __forceinline__ void load(const T* row, int channels, bool in, u32x4 (&raw)[E]) {
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      const int c = (lane() + e * L) * V, left = in ? channels - c : 0;
       raw[e] = u32x4{0, 0, 0, 0};
-      if (left >= V) {
-        raw[e] = *(const words_t*)(row + c);
-      } else if (left > 0) {
+      if (!in) continue;
+      if (channels >= V) {
+        raw[e] = *(const words_t*)(row + start(channels, e));
+      } else {
         unsigned w[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < V - 1; j++)
-          if (j < left) {
-            if constexpr (sizeof(T) == 4) w[j] = ((const unsigned*)row)[c + j];
-            else w[j >> 1] |= (unsigned)((const unsigned short*)row)[c + j] << (j & 1 ? 16 : 0);
+          if (j < channels) {
+            if constexpr (sizeof(T) == 4) w[j] = ((const unsigned*)row)[j];
+            else w[j >> 1] |= (unsigned)((const unsigned short*)row)[j] << (j & 1 ? 16 : 0);
           }
         raw[e] = u32x4{w[0], w[1], w[2], w[3]};
       }
     }
   }
   static __device__ __forceinline__ void store(T* row, int channels, int e, bool past, const float (&f)[V]) {
-    const int c = (lane() + e * L) * V, left = channels - c;
-    if (left >= V) {
+    if (column(e) >= channels) return;
+    T* p = row + start(channels, e);
+    if (channels >= V) {
       const words_t w = words_of<T>(f);
       if (past) {
         asm volatile("");  // (or the two stores become one, a plain one)
-        __builtin_nontemporal_store(w, (words_t*)(row + c));
+        __builtin_nontemporal_store(w, (words_t*)p);
         asm volatile("");
       } else {
-        *(words_t*)(row + c) = w;
+        *(words_t*)p = w;
       }
     } else {
 #pragma unroll
       for (int j = 0; j < V - 1; j++)
-        if (j < left) row[c + j] = to_t<T>(f[j]);
+        if (j < channels) p[j] = to_t<T>(f[j]);
     }
   }
   // A lane's share of a vector of the channels, `none` where there is no vector.
   static __device__ __forceinline__ void vector(const float* p, int channels, float none, float (&f)[E][V]) {
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      const int c = (lane() + e * L) * V;
-      if (p && c + V <= channels) {
+      const int c = start(channels, e);
+      if (p && channels >= V) {
 #pragma unroll
         for (int j = 0; j < V; j += 4) {
           const f32x4_any w = *(const f32x4_any*)(p + c + j);
@@ -98,7 +107,7 @@ struct Row {
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < V; j++) f[e][j] = p && c + j < channels ? p[c + j] : none;
+        for (int j = 0; j < V; j++) f[e][j] = p && j < channels ? p[j] : none;
       }
     }
   }
@@ -146,9 +155,11 @@ __global__ __launch_bounds__((Row<T, L, E>::THREADS)) void layer_norm_held_kerne
       float s[1] = {0.f};
 #pragma unroll
       for (int e = 0; e < E; e++) {
+        const bool whole = R::whole(a.channels, e);
+        const int least = R::first(a.channels, e), limit = R::limit(a.channels);
         float t = 0.f;
 #pragma unroll
-        for (int j = 0; j < V; j++) t += element<T>(raw[e], j);
+        for (int j = 0; j < V; j++) t += whole || (j >= least && j < limit) ? element<T>(raw[e], j) : 0.f;
         s[0] += t;
       }
       R::sum(s, red[turn]);
@@ -157,11 +168,12 @@ __global__ __launch_bounds__((Row<T, L, E>::THREADS)) void layer_norm_held_kerne
     float q[2] = {0.f, 0.f};  // of the deviations, and of their squares
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      const int left = a.channels - (R::lane() + e * L) * V;
+      const bool whole = R::whole(a.channels, e);
+      const int least = R::first(a.channels, e), limit = R::limit(a.channels);
       float t = 0.f, u = 0.f;
 #pragma unroll
       for (int j = 0; j < V; j++) {
-        const float d = j < left ? element<T>(raw[e], j) - mean : 0.f;
+        const float d = whole || (j >= least && j < limit) ? element<T>(raw[e], j) - mean : 0.f;
         t += d;
         u = __builtin_fmaf(d, d, u);
       }
@@ -297,11 +309,13 @@ __global__ __launch_bounds__(LT) void layer_norm_back_held_kernel(LayerArgs a) {
     float q[2] = {0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < E; e++) {
+      const bool whole = R::whole(a.channels, e);
+      const int least = R::first(a.channels, e);
       float t = 0.f, u = 0.f;
 #pragma unroll
       for (int j = 0; j < V; j++) {
-        // (Past the row's end dy is 0.)
-        const float g = element<T>(dy[e], j), d = g * gamma[e][j], h = (element<T>(x[e], j) - mean) * rstd;
+        // (Behind a short row's end dy is 0.)
+        const float g = whole || j >= least ? element<T>(dy[e], j) : 0.f, d = g * gamma[e][j], h = (element<T>(x[e], j) - mean) * rstd;
         t += d;
         u = __builtin_fmaf(d, h, u);
         s1[e][j] = __builtin_fmaf(g, h, s1[e][j]);
@@ -314,6 +328,10 @@ __global__ __launch_bounds__(LT) void layer_norm_back_held_kernel(LayerArgs a) {
     if (!in) continue;
     const float m1 = a.rms ? 0.f : (float)((double)q[0] * a.inverse), m2 = (float)((double)q[1] * a.inverse);
     T* dx = (T*)a.dx + (size_t)row * a.lddx;
+    if constexpr (E > 1) {
+      forget<E>(x);
+      forget<E>(dy);
+    }
 #pragma unroll
     for (int e = 0; e < E; e++) {
       float f[V];
@@ -345,7 +363,8 @@ __global__ __launch_bounds__(LT) void layer_norm_back_held_kernel(LayerArgs a) {
       for (int e = 0; e < E; e++) {
 #pragma unroll
         for (int j = 0; j < V; j++) {
-          float* at = joined + (R::lane() + e * L) * V + j;
+          if (j < R::first(a.channels, e)) continue;
+          float* at = joined + R::start(a.channels, e) + j;
           at[0] = (w ? at[0] : 0.f) + s1[e][j];
           at[SPAN] = (w ? at[SPAN] : 0.f) + s2[e][j];
         }
@@ -365,10 +384,12 @@ template <typename T, int NT, int E>
 __global__ __launch_bounds__(NT) void layer_norm_back_wide_kernel(LayerArgs a) {
   using R = Row<T, NT, E>;
   constexpr int V = R::V;
-  extern __shared__ __align__(16) float gamma[];  // [chunks][V], 1 past the channels
+  extern __shared__ __align__(16) float gamma[];  // [chunks][V], as the threads hold them
   __shared__ float red[2][16][2];
   float s1[E][V] = {}, s2[E][V] = {};
-  for (int c = threadIdx.x; c < NT * E * V; c += NT) gamma[c] = a.gamma && c < a.channels ? a.gamma[c] : 1.f;
+#pragma unroll
+  for (int e = 0; e < E; e++)
+    for (int j = 0; j < V; j++) gamma[(threadIdx.x + e * NT) * V + j] = a.gamma ? a.gamma[R::start(a.channels, e) + j] : 1.f;
   const auto vec4 = [&](int e, int j) { return *(const floatx4*)(gamma + (threadIdx.x + e * NT) * V + j); };
   int turn = 0;
   u32x4 x[E], dy[E], next_x[E], next_dy[E];
@@ -384,6 +405,8 @@ __global__ __launch_bounds__(NT) void layer_norm_back_wide_kernel(LayerArgs a) {
     float q[2] = {0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < E; e++) {
+      const bool whole = R::whole(a.channels, e);
+      const int least = R::first(a.channels, e);
       float t = 0.f, u = 0.f;
 #pragma unroll
       for (int j4 = 0; j4 < V; j4 += 4) {
@@ -391,7 +414,7 @@ __global__ __launch_bounds__(NT) void layer_norm_back_wide_kernel(LayerArgs a) {
 #pragma unroll
         for (int k = 0; k < 4; k++) {
           const int j = j4 + k;
-          const float g = element<T>(dy[e], j), d = g * w[k], h = (element<T>(x[e], j) - mean) * rstd;
+          const float g = whole || j >= least ? element<T>(dy[e], j) : 0.f, d = g * w[k], h = (element<T>(x[e], j) - mean) * rstd;
           t += d;
           u = __builtin_fmaf(d, h, u);
           s1[e][j] = __builtin_fmaf(g, h, s1[e][j]);
@@ -431,10 +454,10 @@ __global__ __launch_bounds__(NT) void layer_norm_back_wide_kernel(LayerArgs a) {
   float* part = a.parts + (size_t)blockIdx.x * 2 * a.channels;
 #pragma unroll
   for (int e = 0; e < E; e++) {
-    const int c = (R::lane() + e * NT) * V;
+    const int c = R::start(a.channels, e);
 #pragma unroll
     for (int j = 0; j < V; j++)
-      if (c + j < a.channels) {
+      if (j >= R::first(a.channels, e)) {
         part[c + j] = s1[e][j];
         part[a.channels + c + j] = s2[e][j];
       }
@@ -498,23 +521,23 @@ __global__ __launch_bounds__(LT) void layer_norm_back_means_kernel(LayerArgs a) 
       float fx[E][V], fy[E][V];
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        const int c = c0 + (tid + e * LT) * V, left = max(a.channels - c, 0);
-        load_vec<T>(x + c, left, fx[e]);
-        load_vec<T>(dy + c, left, fy[e]);
+        const int c = min(c0 + (tid + e * LT) * V, a.channels - V);
+        load_vec<T>(x + c, V, fx[e]);
+        load_vec<T>(dy + c, V, fy[e]);
       }
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        const int c = c0 + (tid + e * LT) * V, left = max(a.channels - c, 0);
+        const int c = min(c0 + (tid + e * LT) * V, a.channels - V), least = c0 + (tid + e * LT) * V - c;  // (see Row)
         float t = 0.f, u = 0.f;
 #pragma unroll
         for (int j = 0; j < V; j += 4) {
           float w[4] = {1.f, 1.f, 1.f, 1.f};
-          if (a.gamma) load_vec<float>(a.gamma + c + j, left - j, w);
+          if (a.gamma) load_vec<float>(a.gamma + c + j, 4, w);
 #pragma unroll
           for (int k = 0; k < 4; k++) {
-            const float d = fy[e][j + k] * w[k];
+            const float d = j + k >= least ? fy[e][j + k] * w[k] : 0.f;
             t += d;
-            u = __builtin_fmaf(d, j + k < left ? (fx[e][j + k] - mean) * rstd : 0.f, u);
+            u = __builtin_fmaf(d, (fx[e][j + k] - mean) * rstd, u);
           }
         }
         q[0] += t;
@@ -533,18 +556,19 @@ __global__ __launch_bounds__(LT) void layer_norm_back_slab_kernel(LayerArgs a, i
   constexpr int V = kVec<T>, AT_ONCE = 4;
   __shared__ float joined[SW][2][64 * V];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int part = blockIdx.x / slabs, c = ((blockIdx.x - part * slabs) * 64 + lane) * V, left = max(a.channels - c, 0);
+  const int part = blockIdx.x / slabs, column = ((blockIdx.x - part * slabs) * 64 + lane) * V;
+  const int c = min(column, a.channels - V), least = column - c;  // (see Row)
   const int per = (a.rows + a.split - 1) / a.split, first = part * per, last = min(first + per, a.rows);
   float gamma[V], s1[V] = {}, s2[V] = {};
 #pragma unroll
-  for (int j = 0; j < V; j++) gamma[j] = a.gamma && j < left ? a.gamma[c + j] : 1.f;
+  for (int j = 0; j < V; j++) gamma[j] = a.gamma ? a.gamma[c + j] : 1.f;
   for (int row = first + w; row < last; row += SW * AT_ONCE) {
     float x[AT_ONCE][V], dy[AT_ONCE][V];
 #pragma unroll
     for (int k = 0; k < AT_ONCE; k++) {
       const int r = min(row + k * SW, last - 1);
-      load_vec<T>((const T*)a.x + (size_t)r * a.ldx + c, left, x[k]);
-      load_vec<T>((const T*)a.dy + (size_t)r * a.lddy + c, left, dy[k]);
+      load_vec<T>((const T*)a.x + (size_t)r * a.ldx + c, V, x[k]);
+      load_vec<T>((const T*)a.dy + (size_t)r * a.lddy + c, V, dy[k]);
     }
 #pragma unroll
     for (int k = 0; k < AT_ONCE; k++) {
@@ -560,8 +584,9 @@ __global__ __launch_bounds__(LT) void layer_norm_back_slab_kernel(LayerArgs a, i
         f[j] = n.rstd * __builtin_fmaf(-h, n.m2, g * gamma[j] - n.m1);
       }
       T* to = (T*)a.dx + (size_t)r * a.lddx + c;
-      if (a.past && left >= V) store_past<T>(to, f);
-      else store_vec<T>(to, left, f);
+      if (least >= V) continue;
+      if (a.past) store_past<T>(to, f);
+      else store_vec<T>(to, V, f);
     }
   }
   if (!a.dgamma && !a.dbeta) return;
@@ -572,11 +597,12 @@ __global__ __launch_bounds__(LT) void layer_norm_back_slab_kernel(LayerArgs a, i
   }
   __syncthreads();
   for (int i = threadIdx.x; i < 2 * 64 * V; i += LT) {
-    const int side = i >= 64 * V, at = i - side * 64 * V, column = (blockIdx.x - part * slabs) * 64 * V + at;
+    const int side = i >= 64 * V, at = i - side * 64 * V, wanted = (blockIdx.x - part * slabs) * 64 * V + at / V * V;
+    const int from = min(wanted, a.channels - V);
     float t = 0.f;
 #pragma unroll
     for (int k = 0; k < SW; k++) t += joined[k][side][at];
-    if (column < a.channels) a.parts[((size_t)part * 2 + side) * a.channels + column] = t;
+    if (at % V >= wanted - from) a.parts[((size_t)part * 2 + side) * a.channels + from + at % V] = t;
   }
 }
 

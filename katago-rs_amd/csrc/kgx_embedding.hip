@@ -18,34 +18,42 @@ namespace {
 constexpr int ET = 256;       // threads of a workgroup
 constexpr int ST = 1024;      // of the sort's
 constexpr int kDigit = 9;     // bits of a digit, at most
-constexpr int kMostBlocks = 64;  // of tokens, in the sort
+constexpr int kMostBlocks = 128;  // of tokens, in the sort
 constexpr long long kFewColumns = 1 << 20;  // two threads for each that the card holds
 constexpr int FR = 16;        // rows that a wave looks for at once
 
-// A thread a column of 16 bytes of EACH rows, whose loads are under way together.
-template <typename T, int EACH>
+// Rows go by vectors of V elements: 16 bytes, the last of a row overlapping the one before (both have the same values of what they share),
+// or single elements where the row is shorter.
+template <typename T, int V>
+__device__ __forceinline__ void load_columns(const T* p, float (&f)[V]) {
+  if constexpr (V == 1) f[0] = (float)p[0];
+  else load_vec<T>(p, V, f);
+}
+
+// A thread a vector of EACH rows, whose loads are under way together.
+template <typename T, int V, int EACH>
 __global__ __launch_bounds__(ET) void embedding_kernel(const int* tokens, const T* table, T* y, long long ld, long long ld_y, int count,
                                                        int vocab, int channels, int chunks, float scale, int past) {
-  constexpr int V = kVec<T>;
   const int groups = (count + EACH - 1) / EACH;
   const long long all = (long long)groups * chunks;
   for (long long id = (long long)blockIdx.x * ET + threadIdx.x; id < all; id += (long long)gridDim.x * ET) {
-    const int group = (int)(id / chunks), c = (int)(id - (long long)group * chunks) * V, i0 = group * EACH;
+    const int group = (int)(id / chunks), c = min((int)(id - (long long)group * chunks) * V, channels - V), i0 = group * EACH;
     float f[EACH][V] = {};
     int token[EACH];
 #pragma unroll
     for (int k = 0; k < EACH; k++) token[k] = i0 + k < count ? tokens[i0 + k] : -1;
 #pragma unroll
     for (int k = 0; k < EACH; k++)
-      if ((unsigned)token[k] < (unsigned)vocab) load_vec<T>(table + (size_t)token[k] * ld + c, channels - c, f[k]);
+      if ((unsigned)token[k] < (unsigned)vocab) load_columns<T, V>(table + (size_t)token[k] * ld + c, f[k]);
 #pragma unroll
     for (int k = 0; k < EACH; k++) {
       if (i0 + k >= count) break;
 #pragma unroll
       for (int j = 0; j < V; j++) f[k][j] *= scale;
       T* to = y + (size_t)(i0 + k) * ld_y + c;
-      if (past && c + V <= channels) store_past<T>(to, f[k]);
-      else store_vec<T>(to, channels - c, f[k]);
+      if constexpr (V == 1) *to = to_t<T>(f[k][0]);
+      else if (past) store_past<T>(to, f[k]);
+      else store_vec<T>(to, V, f[k]);
     }
   }
 }
@@ -268,80 +276,114 @@ __device__ __forceinline__ void fill_rows(const SumArgs& a, int wave, int waves)
   }
 }
 
-// L lanes take a slab of L columns of 16 bytes over a range, eight tokens' loads at a time. The workgroups behind fill.
-template <typename T, typename G, int L>
+// A workgroup for L vectors of V elements over a range: L lanes take a share of its tokens each, eight tokens' loads at a time. A run that
+// reaches over the ends of a share is added up in LDS; only one that reaches over the range's ends is left to the second launch. The
+// workgroups behind fill.
+template <typename T, typename G, int V, int L>
 __global__ __launch_bounds__(ET) void embedding_sums_kernel(SumArgs a) {
-  constexpr int V = kVec<T>, AT_ONCE = 8;
+  constexpr int AT_ONCE = 8, SHARES = ET / L;
   if ((int)blockIdx.x >= a.sum_groups) {
     fill_rows<G>(a, __builtin_amdgcn_readfirstlane((blockIdx.x - a.sum_groups) * (ET / 64) + (threadIdx.x >> 6)),
                  (gridDim.x - a.sum_groups) * (ET / 64));
     return;
   }
-  const int lane = threadIdx.x % L;
-  const auto from = [&](int v, int t) {  // of the lane that has token t
-    if constexpr (L == 64) return __builtin_amdgcn_readlane(v, t);
-    else return __shfl(v, t, L);
-  };
-  int unit = blockIdx.x * (ET / L) + threadIdx.x / L;
-  if (L == 64) unit = __builtin_amdgcn_readfirstlane(unit);
-  const int range = unit / a.slabs, c = ((unit - range * a.slabs) * L + lane) * V;
-  if (range >= a.ranges) return;
-  const int left = max(a.channels - c, 0), first = range * a.each, last = min(first + a.each, a.count);
+  __shared__ float ends[2][V][ET];  // a share's sum of a run from before it, and of one that goes on behind it
+  __shared__ int firsts[SHARES];    // the first key of each share, -1 where it has no token
+  const int tid = threadIdx.x, share = L == 64 ? __builtin_amdgcn_readfirstlane(tid / L) : tid / L;
+  const int range = blockIdx.x / a.slabs, column = ((blockIdx.x - range * a.slabs) * L + tid % L) * V;
+  const bool in = column < a.channels;
+  const int c = min(column, a.channels - V), least = column - c;  // elements below `least` are the vector's before
+  const int begin = range * a.each, end = min(begin + a.each, a.count), each = a.each / SHARES;
+  const int first = begin + share * each, last = min(first + each, end);
+  const T* dy = (const T*)a.dy + c;
   float sum[V] = {};
-  int run = (int)a.keys[first];
-  bool before = first > 0 && (int)a.keys[first - 1] == run;
-  const int next = last < a.count ? (int)a.keys[last] : -1;
-  const auto end_run = [&](bool after) {
-    if (before || after) {
-      float* p = a.parts + ((size_t)range * 2 + (before ? 0 : 1)) * a.channels + c;
+  int run = -1;
+  bool before = false;
+  const auto write = [&](int key) {
+    G* p = (G*)a.grad + (size_t)key * a.ld_grad + c;
+    if (!in) return;
+    if (V > 1 && least > 0 && a.accumulate) {  // (what is shared is added to once)
 #pragma unroll
-      for (int h = 0; h < V; h += 4) {
-        const float f[4] = {sum[h], sum[h + 1], sum[h + 2], sum[h + 3]};
-        store_vec<float>(p + h, left - h, f);
-      }
+      for (int j = 0; j < V; j++)
+        if (j >= least) p[j] = to_t<G>(__builtin_fmaf(sum[j], a.scale, (float)p[j]));
     } else {
-      put<G, V>((G*)a.grad + (size_t)run * a.ld_grad + c, left, sum, a.scale, a.accumulate);
+      put<G, V>(p, V, sum, a.scale, a.accumulate);
     }
   };
-  for (int i0 = first; i0 < last; i0 += L) {
-    int key = a.vocab, place = 0;
-    if (i0 + lane < last) {
-      key = (int)a.keys[i0 + lane];
-      place = a.places[i0 + lane];
-    }
-#pragma unroll 1
-    for (int u = 0; u < L; u += AT_ONCE) {
-      if (i0 + u >= last || from(key, u) >= a.vocab) break;
-      typename RowVec<T>::type raw[AT_ONCE];
-      const bool whole = left >= V;
+  const auto keep = [&](int side) {
 #pragma unroll
-      for (int t = 0; t < AT_ONCE; t++) {
-        const int k = from(key, u + t), at = from(place, u + t);  // (of lanes that a branch on `whole` would switch off)
-        if (k < a.vocab && whole) raw[t] = *(const typename RowVec<T>::type*)((const T*)a.dy + (size_t)at * a.ld + c);
+    for (int j = 0; j < V; j++) ends[side][j][tid] = sum[j];
+  };
+  bool tail = false;  // a run that begins in this share goes on behind it
+  if (first < last) {
+    run = (int)a.keys[first];
+    before = first > 0 && (int)a.keys[first - 1] == run;
+    const int next = last < a.count ? (int)a.keys[last] : -1;
+    if (tid % L == 0) firsts[share] = run;
+    // (Every lane of a share reads the same eight keys and places at once; a share begins at a multiple of eight. Those past the last lie
+    // within the workspace.)
+    for (int i0 = first; i0 < last; i0 += AT_ONCE) {
+      int key[AT_ONCE], place[AT_ONCE];
+#pragma unroll
+      for (int t = 0; t < AT_ONCE; t += 4) {
+        const int4 k = *(const int4*)(a.keys + i0 + t), p = *(const int4*)(a.places + i0 + t);
+        key[t] = k.x, key[t + 1] = k.y, key[t + 2] = k.z, key[t + 3] = k.w;
+        place[t] = p.x, place[t + 1] = p.y, place[t + 2] = p.z, place[t + 3] = p.w;
       }
+      if (key[0] >= a.vocab) break;
+      float f[AT_ONCE][V];
+#pragma unroll
+      for (int t = 0; t < AT_ONCE; t++)
+        if (i0 + t < last && key[t] < a.vocab && in) load_columns<T, V>(dy + (size_t)place[t] * a.ld, f[t]);
 #pragma unroll
       for (int t = 0; t < AT_ONCE; t++) {
-        const int k = from(key, u + t), at = from(place, u + t);
-        if (k >= a.vocab) continue;
-        if (k != run) {
-          end_run(false);
+        if (i0 + t >= last || key[t] >= a.vocab) break;
+        if (key[t] != run) {
+          if (before) keep(0);
+          else write(run);
 #pragma unroll
           for (int j = 0; j < V; j++) sum[j] = 0.f;
-          run = k;
+          run = key[t];
           before = false;
         }
-        if (whole) {
 #pragma unroll
-          for (int j = 0; j < V; j++) sum[j] += widen1<T>(raw[t], j);
-        } else {
-          const T* p = (const T*)a.dy + (size_t)at * a.ld + c;
-#pragma unroll
-          for (int j = 0; j < V; j++) sum[j] += j < left ? (float)p[j] : 0.f;
-        }
+        for (int j = 0; j < V; j++) sum[j] += f[t][j];
       }
     }
+    if (run < a.vocab) {
+      tail = !before && next == run;
+      if (before) keep(0);
+      else if (!tail) write(run);
+    }
+  } else if (tid % L == 0) {
+    firsts[share] = -1;
   }
-  if (run < a.vocab) end_run(next == run);
+  __syncthreads();
+  // The first share's run from before the range, and each share's run that goes on: with its parts in the shares behind.
+  const bool from_before = share == 0 && first < last && first > 0 && firsts[0] < a.vocab && (int)a.keys[first - 1] == firsts[0];
+  const auto collect = [&](int key) {
+    int s = share + 1;
+    for (; s < SHARES && firsts[s] == key; s++) {
+#pragma unroll
+      for (int j = 0; j < V; j++) sum[j] += ends[0][j][s * L + tid % L];
+    }
+    return (s == SHARES || begin + s * each >= end) && end < a.count && (int)a.keys[end] == key;  // goes on behind the range
+  };
+  const auto leave = [&](int side) {
+    if (in) put<float, V>(a.parts + ((size_t)range * 2 + side) * a.channels + c, V, sum, 1.f, 0);
+  };
+  if (tail) {
+    if (collect(run)) leave(1);
+    else write(run);
+  }
+  if (from_before) {
+    const int key = firsts[0];
+#pragma unroll
+    for (int j = 0; j < V; j++) sum[j] = ends[0][j][tid];
+    // (Where it ends in the first share, the next one's first token may still be of the same key only if it did not end.)
+    collect(key);
+    leave(0);
+  }
 }
 
 // Runs over several ranges: a workgroup for up to JS slabs of 256 channels of each range that such a run begins in. Its waves are
@@ -397,7 +439,16 @@ struct Plan {
   int passes, bits, blocks, each_block, each, ranges;  // passes: 0 where the tokens are ranked
   size_t keys, places, counts, parts, bytes;
 };
-// (Ranges of as many tokens as leave some 2048 waves with a row's columns; a run's sum of more than 256 is cut.)
+// From one copy of the keys to the other: whole eights, which are read at once.
+size_t plan_stride(int count) { return ((size_t)count + 7) / 8 * 8; }
+// Lanes for a slab of `chunks` vectors.
+int lanes_of(int chunks) {
+  int lanes = 1;
+  while (lanes < chunks && lanes < 64) lanes *= 2;
+  return lanes;
+}
+// (A lane's share of the tokens leaves some 4096 waves, 8 tokens at least and 64 at most, a multiple of 8. It is that of the type whose
+// rows take the fewest lanes: ranges, and with them the workspace, are the same for every type.)
 Plan plan_of(int count, int vocab, int channels) {
   Plan p = {};
   if (count > kRanked) {
@@ -408,8 +459,9 @@ Plan plan_of(int count, int vocab, int channels) {
     p.each_block = (int)(rounds * ST);
     p.blocks = (int)(((long long)count + p.each_block - 1) / p.each_block);
   }
-  const long long slabs = ((long long)channels + 511) / 512;
-  p.each = (int)std::min(std::max((long long)count * std::min(slabs, 64ll) / 2048, 8ll) / 8 * 8, 256ll);
+  const int chunks = channels < 4 ? 8 : (channels + 7) / 8, lanes = channels < 4 ? 8 : channels < 8 ? 2 : lanes_of(chunks);
+  const long long waves = (long long)count * ((chunks + lanes - 1) / lanes) * lanes / 64;  // one token each
+  p.each = (int)std::min(std::max(waves / 4096 / 8 * 8, 8ll), 64ll) * (ET / lanes);
   p.ranges = (int)(((long long)count + p.each - 1) / p.each);
   const auto room = [&](size_t n) {
     const size_t at = p.bytes;
@@ -417,8 +469,8 @@ Plan plan_of(int count, int vocab, int channels) {
     return at;
   };
   const size_t copies = p.passes > 1 ? 2 : 1;
-  p.keys = room(copies * count * 4);
-  p.places = room(copies * count * 4);
+  p.keys = room(copies * plan_stride(count) * 4);
+  p.places = room(copies * plan_stride(count) * 4);
   p.counts = room((size_t)p.blocks * (4 << p.bits));
   p.parts = room((size_t)p.ranges * 2 * channels * 4);
   return p;
@@ -453,8 +505,8 @@ void sort_tokens(const kg_embedding_args& a, const Plan& plan, SumArgs& p, bool 
   for (int k = 0; k < plan.passes; k++) {
     const dim3 grid(t.blocks);
     t.shift = k * plan.bits;
-    t.keys_out = keys + (size_t)(k & 1) * a.count;
-    t.places_out = places + (size_t)(k & 1) * a.count;
+    t.keys_out = keys + (size_t)(k & 1) * plan_stride(a.count);
+    t.places_out = places + (size_t)(k & 1) * plan_stride(a.count);
     if (k == 0) {
       launch_k(sort_count_kernel<true>, dim3(t.blocks + more), ST, 0, s, t, fill);
       launch_k(sort_move_kernel<true>, grid, ST, 0, s, t);
@@ -467,25 +519,32 @@ void sort_tokens(const kg_embedding_args& a, const Plan& plan, SumArgs& p, bool 
   }
 }
 
-template <typename T, typename G, int L>
-void sums(SumArgs p, hipStream_t s) {
-  const int chunks = (p.channels + kVec<T> - 1) / kVec<T>;
+template <typename T, typename G, int V, int L>
+void sums(SumArgs p, int chunks, hipStream_t s) {
   p.slabs = (chunks + L - 1) / L;
-  p.sum_groups = (int)(((long long)p.ranges * p.slabs + ET / L - 1) / (ET / L));
+  p.sum_groups = p.ranges * p.slabs;
   const int fill = p.accumulate || p.filled ? 0 : (int)std::min(((long long)p.vocab + FR * ET / 64 - 1) / (FR * ET / 64), 8192ll);
-  launch_k(embedding_sums_kernel<T, G, L>, dim3(p.sum_groups + fill), ET, 0, s, p);
+  if (p.sum_groups + fill) launch_k(embedding_sums_kernel<T, G, V, L>, dim3(p.sum_groups + fill), ET, 0, s, p);
   if (p.ranges > 1) {
-    const int blocks = (p.channels + 256 * JS - 1) / (256 * JS);
+    const int blocks = (int)(((long long)p.channels + 256 * JS - 1) / (256 * JS));
     const int wide = p.channels <= 256 ? 1 : p.channels <= 512 ? 2 : p.channels <= 1024 ? 4 : JS;
     launch_k(embedding_join_kernel<G>, dim3((int)std::min((long long)(p.ranges - 1) * blocks, 1ll << 20)), JT, 0, s, p, blocks, wide);
   }
 }
 template <typename T, typename G>
 void backward_typed(const SumArgs& p, hipStream_t s) {
-  const int chunks = (p.channels + kVec<T> - 1) / kVec<T>;
-  if (chunks <= 16) sums<T, G, 16>(p, s);
-  else if (chunks <= 32) sums<T, G, 32>(p, s);
-  else sums<T, G, 64>(p, s);
+  constexpr int V = kVec<T>;
+  if (p.channels < V) return sums<T, G, 1, 8>(p, p.channels, s);
+  const int chunks = (int)(((long long)p.channels + V - 1) / V);
+  switch (lanes_of(chunks)) {
+    case 1: return sums<T, G, V, 1>(p, chunks, s);
+    case 2: return sums<T, G, V, 2>(p, chunks, s);
+    case 4: return sums<T, G, V, 4>(p, chunks, s);
+    case 8: return sums<T, G, V, 8>(p, chunks, s);
+    case 16: return sums<T, G, V, 16>(p, chunks, s);
+    case 32: return sums<T, G, V, 32>(p, chunks, s);
+    default: return sums<T, G, V, 64>(p, chunks, s);
+  }
 }
 
 }  // namespace
@@ -496,15 +555,18 @@ void launch_embedding(const kg_embedding_args& a, hipStream_t s) {
   const float scale = (float)a.scale;
   const auto go = [&](auto zero) {
     using T = decltype(zero);
-    const int chunks = (a.channels + kVec<T> - 1) / kVec<T>;
-    const long long columns = (long long)a.count * chunks;
-    const int past = columns * 16 > kPastBytes;
-    if (columns < kFewColumns)
-      launch_k(embedding_kernel<T, 1>, dim3(grid_of(columns)), ET, 0, s, a.tokens, (const T*)a.table, (T*)a.y, a.ld_table, a.ld_y, a.count,
-               a.vocab, a.channels, chunks, scale, past);
-    else
-      launch_k(embedding_kernel<T, 4>, dim3(grid_of((a.count + 3ll) / 4 * chunks)), ET, 0, s, a.tokens, (const T*)a.table, (T*)a.y,
-               a.ld_table, a.ld_y, a.count, a.vocab, a.channels, chunks, scale, past);
+    constexpr int V = kVec<T>;
+    const auto run = [&](auto kernel, int vec, int each) {
+      const int chunks = (a.channels + vec - 1) / vec;
+      const long long threads = ((long long)a.count + each - 1) / each * chunks;
+      const int past = (long long)a.count * a.channels * (long long)sizeof(T) > kPastBytes;
+      launch_k(kernel, dim3(grid_of(threads)), ET, 0, s, a.tokens, (const T*)a.table, (T*)a.y, a.ld_table, a.ld_y, a.count, a.vocab,
+               a.channels, chunks, scale, past);
+    };
+    const bool few = (long long)a.count * ((a.channels + V - 1) / V) < kFewColumns;
+    if (a.channels < V) run(embedding_kernel<T, 1, 4>, 1, 4);
+    else if (few) run(embedding_kernel<T, V, 1>, V, 1);
+    else run(embedding_kernel<T, V, 4>, V, 4);
   };
   switch (a.type) {
     case PREC_F32: go(0.f); break;

@@ -248,9 +248,9 @@ def distill_loss(logits, top_index, top_logits, *, legal=None, weight=None, logi
     if grad is not None:
         g, ld_g = _rows(grad, "grad", logits)
     elif want_grad:
-        grad = torch.empty((n, v), dtype=logits.dtype, device=logits.device)
+        grad = logits.new_empty((n, v))
         g, ld_g = grad.data_ptr(), v
-    loss = torch.empty(n, dtype=torch.float32, device=logits.device)
+    loss = logits.new_empty(n, dtype=torch.float32)
     L = _library()
     # (A board's rows need none: up to 448 columns with up to 256 entries.)
     work = _workspace(L.kg_distill_loss_workspace(n, v, k) if v > 448 or k > 256 else 0, logits.device)
@@ -382,17 +382,17 @@ def layer_norm(x, gamma=None, beta=None, *, eps=1e-5, rms=False, y=None):
     gm, bt = _vector(gamma, c, torch.float32, "gamma", dev), _vector(beta, c, torch.float32, "beta", dev)
     given = y
     if y is None:
-        y = torch.empty(shape, dtype=x.dtype, device=x.device)
+        y = x.new_empty(shape)
         yp, ldy = y.data_ptr(), c
     else:
         yp, ldy = _like(y, x, "y")
     L = _library()
     rows = shape[:-1]
     if rms:
-        mean, rstd = None, torch.empty(rows, dtype=torch.float32, device=x.device)
+        mean, rstd = None, x.new_empty(rows, dtype=torch.float32)
         mp, rp = 0, rstd.data_ptr()
     else:
-        mean, rstd = torch.empty((2, *rows), dtype=torch.float32, device=x.device).unbind()
+        mean, rstd = x.new_empty((2, *rows), dtype=torch.float32).unbind()
         mp = mean.data_ptr()
         rp = mp + 4 * n
     try:
@@ -417,7 +417,7 @@ def layer_norm_backward(dy, x, mean, rstd, gamma=None, *, dx=None):
     dyp, lddy = _like(dy, x, "dy")
     given = dx
     if dx is None:
-        dx = torch.empty(shape, dtype=x.dtype, device=x.device)
+        dx = x.new_empty(shape)
         dxp, lddx = dx.data_ptr(), c
     else:
         dxp, lddx = _like(dx, x, "dx")
@@ -428,7 +428,7 @@ def layer_norm_backward(dy, x, mean, rstd, gamma=None, *, dx=None):
             raise ValueError(f"{name} must be contiguous float32 of shape {tuple(shape[:-1])} on GPU {dev}")
     L = _library()
     work = _workspace(L.kg_layer_norm_workspace(n, c), x.device)
-    out = torch.empty((2, c), dtype=torch.float32, device=x.device)
+    out = x.new_empty((2, c), dtype=torch.float32)
     dgamma, dbeta = out.unbind()
     o = out.data_ptr()
     try:
@@ -459,7 +459,7 @@ def embedding(tokens, table, *, scale=1.0, y=None):
     shape = (*tokens.shape, c)
     given = y
     if y is None:
-        y = torch.empty(shape, dtype=table.dtype, device=table.device)
+        y = table.new_empty(shape)
         yp, ldy = y.data_ptr(), c
     else:
         if y.shape != shape or y.dtype is not table.dtype or y.get_device() != dev:
@@ -493,7 +493,7 @@ def embedding_backward(dy, tokens, vocab, *, scale=1.0, grad=None, dtype=None, a
             raise ValueError("accumulate needs grad")
         if not 1 <= vocab <= 1 << 30:
             raise ValueError("vocab must be in [1, 2^30]")
-        grad = torch.empty((vocab, c), dtype=dtype or dy.dtype, device=dy.device)
+        grad = dy.new_empty((vocab, c), dtype=dtype)
     elif grad.shape != (vocab, c) or grad.get_device() != dev or (dtype is not None and grad.dtype is not dtype):
         raise ValueError(f"grad must be [{vocab}, {c}] on GPU {dev}" + (f" of {dtype}" if dtype else ""))
     gp, ldg = _rows(grad, "grad")

@@ -490,15 +490,17 @@ __global__ __launch_bounds__(64) void distill_known_kernel(DistillRows a) {
 struct Copied : Listed {
   Known* known;
   __device__ __forceinline__ Copied(char* lds, int k_) : Listed(lds + sizeof(Known), k_) { known = (Known*)lds; }
-  static size_t bytes(int slots, int k) { return sizeof(Known) + Listed::bytes(slots, k); }
+  static size_t bytes(int slots, int k) { return (sizeof(Known) + Listed::bytes(slots, k) + 15) / 16 * 16; }
 };
+template <int NT>
+__device__ __forceinline__ int row_thread() { return NT == 64 ? threadIdx.x & 63 : threadIdx.x; }
 template <int NT>
 struct Asked {
   int c;
   double share, q;
   unsigned known;
   __device__ __forceinline__ Asked(const DistillRows& a, int row) {
-    const int i = threadIdx.x;
+    const int i = row_thread<NT>();
     const size_t at = (size_t)row * a.k + min(i, a.k - 1);
     c = a.column[at];
     share = a.share[at];
@@ -506,7 +508,7 @@ struct Asked {
     known = ((const unsigned*)(a.known + row))[min(i, (int)(sizeof(Known) / 4) - 1)];
   }
   __device__ __forceinline__ void begin(const DistillRows& a, int row, const Copied& l) const {
-    const int tid = threadIdx.x;
+    const int tid = row_thread<NT>();
     if (tid < (int)(sizeof(Known) / 4)) ((unsigned*)l.known)[tid] = known;
 #pragma unroll 1
     for (int i = tid; i < l.k; i += NT) {
@@ -521,7 +523,7 @@ struct Asked {
 template <typename T, int NT, int SLOTS>
 __device__ __forceinline__ void link_row(const Copied& l, const Chunks<T>& at) {
 #pragma unroll 1
-  for (int i = threadIdx.x; i < l.k; i += NT) {
+  for (int i = row_thread<NT>(); i < l.k; i += NT) {
     const int c = l.link[i].x;
     l.link[i] = placed<T>(at, c, c >= 0 ? atomicExch(&l.heads[at.of(c) % SLOTS], i + 1) : 0);
   }
@@ -529,20 +531,20 @@ __device__ __forceinline__ void link_row(const Copied& l, const Chunks<T>& at) {
 template <int NT>
 __device__ __forceinline__ void hot_row(const Copied& l, const DistillFactors& f) {
 #pragma unroll 1
-  for (int i = threadIdx.x; i < l.k; i += NT) l.hot[i] = hot_of(f, l.share[i], l.q[i]);
+  for (int i = row_thread<NT>(); i < l.k; i += NT) l.hot[i] = hot_of(f, l.share[i], l.q[i]);
 }
 
-// Longer rows that fit the registers of NT threads: a workgroup a row, one read.
+// Longer rows that fit the registers of NT threads: a wave a row without a barrier, or a workgroup; one read.
 template <typename T, int NT, int E>
-__global__ __launch_bounds__(NT, 6) void distill_row_kernel(DistillRows a) {
-  constexpr int WAVES = NT / 64;
+__global__ __launch_bounds__(NT == 64 ? 256 : NT, 6) void distill_row_kernel(DistillRows a) {
+  constexpr int WAVES = NT / 64, PER = NT == 64 ? 4 : 1;
   extern __shared__ __align__(16) char lds[];
   __shared__ float tops[WAVES], sums[WAVES];
   __shared__ DistillFactors box;
-  const int tid = threadIdx.x;
-  const Copied l(lds, a.k);
+  const int tid = row_thread<NT>(), wave = NT == 64 ? wave_row<64>() : 0;
+  const Copied l(lds + wave * a.list_bytes, a.k);
   const Base2 c2(a.scale);
-  for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
+  for (int row = blockIdx.x * PER + wave; row < a.rows; row += gridDim.x * PER) {
     const T* z = (const T*)a.logits + (size_t)row * a.ld;
     const unsigned char* legal = a.legal ? a.legal + (size_t)row * a.ld_legal : nullptr;
     T* g = a.grad ? (T*)a.grad + (size_t)row * a.ld_grad : nullptr;
@@ -550,39 +552,49 @@ __global__ __launch_bounds__(NT, 6) void distill_row_kernel(DistillRows a) {
     u32x4 raw[E], unused[1];
     const Asked<NT> asked(a, row);
     load_row<T, NT, E>(z, tid, at, raw);
-    lds_barrier();
+    row_sync<NT>();
     asked.begin(a, row, l);
 #pragma unroll
     for (int e = 0; e < E; e++) l.heads[tid + e * NT] = 0;
-    lds_barrier();
+    row_sync<NT>();
     link_row<T, NT, NT * E>(l, at);
     if (legal) remove_illegal<T, NT, E, false>(legal, tid, at, raw, unused);
     remove_past<T, NT, E>(tid, at, raw);
-    lds_barrier();
+    row_sync<NT>();
     remove_listed<T, NT, E>(l, tid, at, raw, 0);
     float top = wave_reduce<true>(own_top<T, NT, E>(at, raw));
-    if ((tid & 63) == 0) tops[tid >> 6] = top;
-    lds_barrier();
+    if constexpr (NT > 64) {
+      if ((tid & 63) == 0) tops[tid >> 6] = top;
+      lds_barrier();
 #pragma unroll
-    for (int k = 0; k < WAVES; k++) top = fmaxf(top, tops[k]);
+      for (int k = 0; k < WAVES; k++) top = fmaxf(top, tops[k]);
+    }
     const float base = top == -INFINITY ? 0.f : top, sum = wave_reduce<false>(own_sum<T, NT, E>(at, raw, base, c2));
-    if ((tid & 63) == 0) sums[tid >> 6] = sum;
-    lds_barrier();
-    if (tid < 64) {
+    double total = (double)sum;
+    if constexpr (NT > 64) {
+      if ((tid & 63) == 0) sums[tid >> 6] = sum;
+      lds_barrier();
+    }
+    DistillFactors f = {};
+    if (NT == 64 || tid < 64) {
       const Known known = *l.known;
-      double total = 0.0, all;
+      if constexpr (NT > 64) {
+        total = 0.0;
 #pragma unroll
-      for (int k = 0; k < WAVES; k++) total += (double)sums[k];
-      const DistillFactors f = distill_row(a, row, known, top, lead_of<true>(a, known, top), total, all);
+        for (int k = 0; k < WAVES; k++) total += (double)sums[k];
+      }
+      double all;
+      f = distill_row(a, row, known, top, lead_of<true>(a, known, top), total, all);
       if (tid == 0) {
-        box = f;
+        if (NT > 64) box = f;
         a.others[row] = Others{total, top};
       }
     }
-    lds_barrier();
-    hot_row<NT>(l, box);
-    lds_barrier();
-    if (g) own_gradient<T, NT, E>(g, tid, at, raw, l, base, c2, box.each, box.part, a.past);
+    if constexpr (NT > 64) lds_barrier();
+    const DistillFactors& shared = NT > 64 ? box : f;
+    hot_row<NT>(l, shared);
+    row_sync<NT>();
+    if (g) own_gradient<T, NT, E>(g, tid, at, raw, l, base, c2, shared.each, shared.part, a.past);
   }
 }
 
@@ -730,7 +742,10 @@ void distill_typed(DistillRows p, hipStream_t s) {
     return launch_k(distill_wave_kernel<T, 2>, dim3(row_grid(p.rows, 4)), 256, p.list_bytes * 4, s, p);
   }
   launch_k(distill_known_kernel<T>, groups, 64, Listed::bytes(kSlots, p.k), s, p);
-  if (r.threads == 64) launch_k(distill_row_kernel<T, 256, 2>, groups, 256, Copied::bytes(256 * 2, p.k), s, p);
+  if (r.threads == 64 && p.k <= kWaveEntries) {
+    p.list_bytes = (int)Copied::bytes(64 * 8, p.k);
+    launch_k(distill_row_kernel<T, 64, 8>, dim3(row_grid(p.rows, 4)), 256, p.list_bytes * 4, s, p);
+  } else if (r.threads == 64) launch_k(distill_row_kernel<T, 256, 2>, groups, 256, Copied::bytes(256 * 2, p.k), s, p);
   else if (r.threads == 256) launch_k(distill_row_kernel<T, 256, 8>, groups, 256, Copied::bytes(256 * 8, p.k), s, p);
   else if (r.threads == 512) launch_k(distill_row_kernel<T, 512, 8>, groups, 512, Copied::bytes(512 * 8, p.k), s, p);
   else {

@@ -400,17 +400,26 @@ __device__ __forceinline__ void own_gradient(T* g, int tid, const Chunks<T>& at,
                                              float each, int takes, int past) {
   forget<E>(raw);
   const bool part = __builtin_amdgcn_readfirstlane(takes);
+  // Mostly (z - base) log2 e as one multiply-add: what base log2 e's rounding makes of every term goes into the factor. Not where base is
+  // so large that this is a factor of its own, and not where the factor is no number, which columns without mass do not take.
+  const float shift = base * c2.hi, factor = each * __builtin_amdgcn_exp2f(__builtin_fmaf(-base, c2.hi, shift));
+  const bool plain = __builtin_amdgcn_readfirstlane(fabsf(shift) < 0x1p20f && fabsf(each) < INFINITY);
 #pragma unroll
   for (int e = 0; e < E; e++) {
     if (at.none(e * NT)) break;
     const int c = fresh(tid) + e * NT;
     float gf[kVec<T>] = {};
     if (part) {
-      // (A column without mass has no gradient, whatever the factor. A listed one's place is filled below.)
+      // (A listed column's place is filled below.)
+      if (plain) {
 #pragma unroll
-      for (int j = 0; j < kVec<T>; j++) {
-        const float ex = __builtin_amdgcn_exp2f((element<T>(raw[e], j) - base) * c2.hi);
-        gf[j] = ex == 0.f ? 0.f : ex * each;
+        for (int j = 0; j < kVec<T>; j++) gf[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(element<T>(raw[e], j), c2.hi, -shift)) * factor;
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVec<T>; j++) {
+          const float ex = __builtin_amdgcn_exp2f((element<T>(raw[e], j) - base) * c2.hi);
+          gf[j] = ex == 0.f ? 0.f : ex * each;
+        }
       }
       store_listed<T, NT * E>(g, l, tid + e * NT, c, at.whole(e * NT, NT), past, at, gf);
     } else {

@@ -18,7 +18,7 @@ namespace {
 constexpr int ET = 256;       // threads of a workgroup
 constexpr int ST = 1024;      // of the sort's
 constexpr int kDigit = 9;     // bits of a digit, at most
-constexpr int kMostBlocks = 128;  // of tokens, in the sort
+constexpr int kMostBlocks = 256;  // of tokens, in the sort
 constexpr long long kFewColumns = 1 << 20;  // two threads for each that the card holds
 constexpr int FR = 16;        // rows that a wave looks for at once
 
@@ -152,16 +152,33 @@ __global__ __launch_bounds__(ST) void sort_move_kernel(SortArgs a) {
   __shared__ int sums[WAVES];
   const int digits = 1 << a.bits, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, b = blockIdx.x;
   const auto key_at = [&](long long i) { return FIRST ? key_of(a.tokens[i], a.vocab) : a.keys[i]; };
-  for (int d = tid; d < digits * WAVES; d += ST) to[d >> a.bits][d & (digits - 1)] = 0;
+  // A digit's tokens in the blocks before this one, and in all, by as many groups of threads as there are for each digit.
   int before = 0, all = 0;
-  if (tid < digits) {
-#pragma unroll 16
-    for (int k = 0; k < a.blocks; k++) {
-      const int n = a.counts[k * digits + tid];
-      before += k < b ? n : 0;
-      all += n;
+  for (int k = tid >> a.bits; k < a.blocks; k += (ST >> a.bits) * 8) {
+    int n[8];
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      const int at = k + u * (ST >> a.bits);
+      n[u] = at < a.blocks ? a.counts[at * digits + (tid & (digits - 1))] : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      before += k + u * (ST >> a.bits) < b ? n[u] : 0;
+      all += n[u];
     }
   }
+  int* room = &to[0][0];  // (two numbers a thread)
+  room[tid] = before;
+  room[ST + tid] = all;
+  __syncthreads();
+  before = all = 0;
+  if (tid < digits)
+    for (int k = tid; k < ST; k += digits) {
+      before += room[k];
+      all += room[ST + k];
+    }
+  __syncthreads();
+  for (int d = tid; d < digits * WAVES; d += ST) to[d >> a.bits][d & (digits - 1)] = 0;
   // The tokens of lower digits: within a wave, then over the waves.
   int upto = all;
 #pragma unroll

@@ -63,18 +63,18 @@ __global__ __launch_bounds__(ET) void embedding_kernel(const int* tokens, const 
 // Tokens outside the table are behind all others.
 __device__ __forceinline__ unsigned key_of(int token, int vocab) { return min((unsigned)token, (unsigned)vocab); }
 
-// 0 in every row, by the workgroups behind those that sort, while these wait for memory: where most rows are not named, that is less
-// than finding them afterwards takes (100003 rows of 512 f16, 5003 tokens: @ us, @ otherwise).
+// 0 in every row, by workgroups behind those that sort, whose launches leave memory idle: the sums then write over the rows that are named.
+// (65536 tokens of 50257 rows of 1024 floats: @ us, 117 with the others looked for and filled beside the sums.)
 struct FillArgs {
   void* grad;
   long long ld;    // bytes
   long long bytes;
-  int rows, groups;  // groups: workgroups that sort
+  int first, rows, groups;  // this launch's rows; groups: workgroups that sort
 };
 __device__ __forceinline__ bool fills(const FillArgs& f) {
   if ((int)blockIdx.x < f.groups) return false;
   const int wave = (blockIdx.x - f.groups) * (ST / 64) + (threadIdx.x >> 6), waves = (gridDim.x - f.groups) * (ST / 64);
-  for (int row = wave; row < f.rows; row += waves) {
+  for (int row = f.first + wave; row < f.first + f.rows; row += waves) {
     char* p = (char*)f.grad + (size_t)row * f.ld;
     for (long long c = (threadIdx.x & 63) * 16; c < f.bytes; c += 1024) {
       if (c + 16 <= f.bytes) *(u32x4_any2*)(p + c) = u32x4{0, 0, 0, 0};
@@ -132,7 +132,7 @@ struct SortArgs {
 
 template <bool FIRST>
 __global__ __launch_bounds__(ST) void sort_count_kernel(SortArgs a, FillArgs fill) {
-  if (FIRST && fills(fill)) return;
+  if (fills(fill)) return;
   __shared__ int n[1 << kDigit];
   const int digits = 1 << a.bits, tid = threadIdx.x, b = blockIdx.x;
   for (int d = tid; d < digits; d += ST) n[d] = 0;
@@ -146,7 +146,8 @@ __global__ __launch_bounds__(ST) void sort_count_kernel(SortArgs a, FillArgs fil
 }
 
 template <bool FIRST>
-__global__ __launch_bounds__(ST) void sort_move_kernel(SortArgs a) {
+__global__ __launch_bounds__(ST) void sort_move_kernel(SortArgs a, FillArgs fill) {
+  if (fills(fill)) return;
   constexpr int WAVES = ST / 64;
   __shared__ int to[WAVES][1 << kDigit];  // where a wave's next token of a digit goes
   __shared__ int sums[WAVES];
@@ -504,15 +505,18 @@ void sort_tokens(const kg_embedding_args& a, const Plan& plan, SumArgs& p, bool 
   p.places = places;
   FillArgs fill = {};
   fill.groups = plan.passes ? plan.blocks : (a.count + RI - 1) / RI;
-  int more = 0;
-  if (filled) {
-    const int size = a.grad_type == PREC_F32 ? 4 : 2;
-    fill.grad = a.grad; fill.ld = a.ld_grad * size;
-    fill.rows = a.vocab; fill.bytes = (long long)a.channels * size;
-    more = std::min((a.vocab + ST / 64 - 1) / (ST / 64), 512);
-  }
+  const int size = a.grad_type == PREC_F32 ? 4 : 2, launches = plan.passes ? 2 * plan.passes : 1;
+  fill.grad = a.grad; fill.ld = a.ld_grad * size; fill.bytes = (long long)a.channels * size;
+  // The grid of the next launch, with its share of the rows.
+  const auto grid = [&](int launch) {
+    const auto upto = [&](int k) { return (int)((long long)a.vocab * k / launches); };
+    fill.first = upto(launch);
+    fill.rows = filled ? upto(launch + 1) - fill.first : 0;
+    return dim3(fill.groups + std::min((fill.rows + ST / 64 - 1) / (ST / 64), 512));
+  };
   if (!plan.passes) {
-    launch_k(sort_rank_kernel, dim3(fill.groups + more), ST, 0, s, a.tokens, keys, places, a.count, a.vocab, fill);
+    const dim3 all = grid(0);
+    launch_k(sort_rank_kernel, all, ST, 0, s, a.tokens, keys, places, a.count, a.vocab, fill);
     return;
   }
   SortArgs t = {};
@@ -520,17 +524,15 @@ void sort_tokens(const kg_embedding_args& a, const Plan& plan, SumArgs& p, bool 
   t.counts = (int*)(w + plan.counts);
   t.count = a.count; t.vocab = a.vocab; t.blocks = plan.blocks; t.each = plan.each_block; t.bits = plan.bits;
   for (int k = 0; k < plan.passes; k++) {
-    const dim3 grid(t.blocks);
     t.shift = k * plan.bits;
     t.keys_out = keys + (size_t)(k & 1) * plan_stride(a.count);
     t.places_out = places + (size_t)(k & 1) * plan_stride(a.count);
-    if (k == 0) {
-      launch_k(sort_count_kernel<true>, dim3(t.blocks + more), ST, 0, s, t, fill);
-      launch_k(sort_move_kernel<true>, grid, ST, 0, s, t);
-    } else {
-      launch_k(sort_count_kernel<false>, grid, ST, 0, s, t, fill);
-      launch_k(sort_move_kernel<false>, grid, ST, 0, s, t);
-    }
+    dim3 all = grid(2 * k);
+    if (k == 0) launch_k(sort_count_kernel<true>, all, ST, 0, s, t, fill);
+    else launch_k(sort_count_kernel<false>, all, ST, 0, s, t, fill);
+    all = grid(2 * k + 1);
+    if (k == 0) launch_k(sort_move_kernel<true>, all, ST, 0, s, t, fill);
+    else launch_k(sort_move_kernel<false>, all, ST, 0, s, t, fill);
     p.keys = t.keys = t.keys_out;
     p.places = t.places = t.places_out;
   }
@@ -604,7 +606,9 @@ void launch_embedding_backward(const kg_embedding_args& a, hipStream_t s) {
     p.parts = (float*)((char*)a.workspace + plan.parts);
     p.ranges = plan.ranges;
     p.each = plan.each;
-    p.filled = !p.accumulate && a.count <= a.vocab / 4;
+    // (A table of up to 128 MB is filled within the sort's time. A larger one where a good part of its rows is not named.)
+    const long long bytes = (long long)a.vocab * a.channels * (a.grad_type == PREC_F32 ? 4 : 2);
+    p.filled = !p.accumulate && (bytes <= 128ll << 20 || a.count <= 2ll * a.vocab);
     sort_tokens(a, plan, p, p.filled, s);
   }
   if (a.grad_type == a.type) {

@@ -468,7 +468,7 @@ __global__ __launch_bounds__(256) void distill_wave_kernel(DistillRows a) {
 }
 
 // What the workgroups of longer rows need of the entries, by a wave a row. (Its double arithmetic and its dependent loads in the row's own
-// launch, at 4093 x 32768 bf16: 240 us, and 175 by a wave of its own beside the row's; apart @.)
+// launch, at 4093 x 32768 bf16: 240 us, and 175 by a wave of its own beside the row's; apart 123, 10 of them here.)
 constexpr int kSlots = 256;
 template <typename T>
 __global__ __launch_bounds__(64) void distill_known_kernel(DistillRows a) {
@@ -632,7 +632,7 @@ __device__ __forceinline__ void losses_of_parts(const DistillRows& a, int first,
 
 // Longer rows: E chunks of each thread at a time relative to the running maximum, and again for the gradient, whose second reading comes
 // from the caches. Few such rows are cut into parts for as many workgroups: a launch for the parts' sums (PARTS), and one that joins
-// them and writes the gradient (JOIN): 301 rows of 100003 f16 @ us whole, @ in parts.
+// them and writes the gradient (JOIN): 301 rows of 100003 f16 62 us whole, 44 in parts.
 enum { WHOLE, PARTS, JOIN };
 template <typename T, int NT, int E, int STAGE>
 __global__ __launch_bounds__(NT) void distill_long_kernel(DistillRows a) {

@@ -64,7 +64,8 @@ __global__ __launch_bounds__(ET) void embedding_kernel(const int* tokens, const 
 __device__ __forceinline__ unsigned key_of(int token, int vocab) { return min((unsigned)token, (unsigned)vocab); }
 
 // 0 in every row, by workgroups behind those that sort, whose launches leave memory idle: the sums then write over the rows that are named.
-// (65536 tokens of 50257 rows of 1024 floats: @ us, 117 with the others looked for and filled beside the sums.)
+// Where few are named, or the table is small (5003 tokens of 100003 rows of 512 f16: 28 us, 32 with the others looked for and filled
+// beside the sums; but 65536 tokens of 50257 rows of 1024 floats, 206 MB: 113 against 104).
 struct FillArgs {
   void* grad;
   long long ld;    // bytes
@@ -85,7 +86,7 @@ __device__ __forceinline__ bool fills(const FillArgs& f) {
 }
 
 // Few tokens: each one's place is the number of tokens before it, counted. RI tokens a workgroup, whose threads share the tokens
-// that they are compared with, 64 ways: 5003 tokens in 5 us, where two launches for each digit take 20.
+// that they are compared with, 64 ways: 5003 tokens in 8 us, where two launches for each of two digits take 22.
 constexpr int kRanked = 8192, RI = 16;
 __global__ __launch_bounds__(ST) void sort_rank_kernel(const int* __restrict__ tokens, unsigned* __restrict__ keys, int* __restrict__ places,
                                                        int count, int vocab, FillArgs fill) {
@@ -294,12 +295,39 @@ __device__ __forceinline__ void fill_rows(const SumArgs& a, int wave, int waves)
   }
 }
 
-// A workgroup for L vectors of V elements over a range: L lanes take a share of its tokens each, eight tokens' loads at a time. A run that
+typedef unsigned short u16x4_any __attribute__((ext_vector_type(4), aligned(2)));
+// V elements of a row, as they were read.
+template <typename T, int V>
+struct Columns {
+  typename RowVec<T>::type raw;
+  __device__ __forceinline__ void load(const T* p) { raw = *(const typename RowVec<T>::type*)p; }
+  __device__ __forceinline__ float at(int j) const { return widen1<T>(raw, j); }
+};
+template <>
+struct Columns<f16, 4> {
+  u16x4_any raw;
+  __device__ __forceinline__ void load(const f16* p) { raw = *(const u16x4_any*)p; }
+  __device__ __forceinline__ float at(int j) const { return (float)__builtin_bit_cast(f16, (unsigned short)raw[j]); }
+};
+template <>
+struct Columns<bf16, 4> {
+  u16x4_any raw;
+  __device__ __forceinline__ void load(const bf16* p) { raw = *(const u16x4_any*)p; }
+  __device__ __forceinline__ float at(int j) const { return __uint_as_float((unsigned)raw[j] << 16); }
+};
+template <typename T>
+struct Columns<T, 1> {
+  T raw;
+  __device__ __forceinline__ void load(const T* p) { raw = *p; }
+  __device__ __forceinline__ float at(int) const { return (float)raw; }
+};
+
+// A workgroup for L vectors of V elements over a range: L lanes take a share of its tokens each. A run that
 // reaches over the ends of a share is added up in LDS; only one that reaches over the range's ends is left to the second launch. The
 // workgroups behind fill.
 template <typename T, typename G, int V, int L>
 __global__ __launch_bounds__(ET) void embedding_sums_kernel(SumArgs a) {
-  constexpr int AT_ONCE = 8, SHARES = ET / L;
+  constexpr int AT_ONCE = 4, SHARES = ET / L;
   if ((int)blockIdx.x >= a.sum_groups) {
     fill_rows<G>(a, __builtin_amdgcn_readfirstlane((blockIdx.x - a.sum_groups) * (ET / 64) + (threadIdx.x >> 6)),
                  (gridDim.x - a.sum_groups) * (ET / 64));
@@ -338,34 +366,56 @@ __global__ __launch_bounds__(ET) void embedding_sums_kernel(SumArgs a) {
     before = first > 0 && (int)a.keys[first - 1] == run;
     const int next = last < a.count ? (int)a.keys[last] : -1;
     if (tid % L == 0) firsts[share] = run;
-    // (Every lane of a share reads the same eight keys and places at once; a share begins at a multiple of eight. Those past the last lie
-    // within the workspace.)
-    for (int i0 = first; i0 < last; i0 += AT_ONCE) {
-      int key[AT_ONCE], place[AT_ONCE];
+    // Four tokens' columns are under way while those of the four before are added, and the keys and places of the four behind: a wait for
+    // what was asked for earlier does not wait for the sums written since. (Every lane of a share reads the same four; a share begins at a
+    // multiple of four. Keys past the last lie within the workspace.)
+    int4 key[2], place, keys_ahead, places_ahead;
+    Columns<T, V> f[2][AT_ONCE];
+    const auto look = [&](int i0) {
+      if (i0 >= last) return;
+      keys_ahead = *(const int4*)(a.keys + i0);
+      places_ahead = *(const int4*)(a.places + i0);
+    };
+    const auto ask = [&](int i0, int4& k, Columns<T, V>(&to)[AT_ONCE]) {
+      k = int4{a.vocab, a.vocab, a.vocab, a.vocab};
+      if (i0 >= last) return;
+      k = keys_ahead;
+      place = places_ahead;
+      if (i0 + 1 >= last) k.y = a.vocab;
+      if (i0 + 2 >= last) k.z = a.vocab;
+      if (i0 + 3 >= last) k.w = a.vocab;
+      if (!in) return;
+      if (k.x < a.vocab) to[0].load(dy + (size_t)place.x * a.ld);
+      if (k.y < a.vocab) to[1].load(dy + (size_t)place.y * a.ld);
+      if (k.z < a.vocab) to[2].load(dy + (size_t)place.z * a.ld);
+      if (k.w < a.vocab) to[3].load(dy + (size_t)place.w * a.ld);
+    };
+    const auto add = [&](int k, const Columns<T, V>& from) {
+      if (k >= a.vocab) return;
+      if (k != run) {
+        if (before) keep(0);
+        else write(run);
 #pragma unroll
-      for (int t = 0; t < AT_ONCE; t += 4) {
-        const int4 k = *(const int4*)(a.keys + i0 + t), p = *(const int4*)(a.places + i0 + t);
-        key[t] = k.x, key[t + 1] = k.y, key[t + 2] = k.z, key[t + 3] = k.w;
-        place[t] = p.x, place[t + 1] = p.y, place[t + 2] = p.z, place[t + 3] = p.w;
+        for (int j = 0; j < V; j++) sum[j] = 0.f;
+        run = k;
+        before = false;
       }
-      if (key[0] >= a.vocab) break;
-      float f[AT_ONCE][V];
 #pragma unroll
-      for (int t = 0; t < AT_ONCE; t++)
-        if (i0 + t < last && key[t] < a.vocab && in) load_columns<T, V>(dy + (size_t)place[t] * a.ld, f[t]);
+      for (int j = 0; j < V; j++) sum[j] += from.at(j);
+    };
+    look(first);
+    ask(first, key[0], f[0]);
+    look(first + AT_ONCE);
+    for (int i0 = first; i0 < last; i0 += 2 * AT_ONCE) {
 #pragma unroll
-      for (int t = 0; t < AT_ONCE; t++) {
-        if (i0 + t >= last || key[t] >= a.vocab) break;
-        if (key[t] != run) {
-          if (before) keep(0);
-          else write(run);
-#pragma unroll
-          for (int j = 0; j < V; j++) sum[j] = 0.f;
-          run = key[t];
-          before = false;
-        }
-#pragma unroll
-        for (int j = 0; j < V; j++) sum[j] += f[t][j];
+      for (int side = 0; side < 2; side++) {
+        const int i = i0 + side * AT_ONCE;
+        ask(i + AT_ONCE, key[1 - side], f[1 - side]);
+        look(i + 2 * AT_ONCE);
+        add(key[side].x, f[side][0]);
+        add(key[side].y, f[side][1]);
+        add(key[side].z, f[side][2]);
+        add(key[side].w, f[side][3]);
       }
     }
     if (run < a.vocab) {
@@ -552,7 +602,9 @@ void sums(SumArgs p, int chunks, hipStream_t s) {
 }
 template <typename T, typename G>
 void backward_typed(const SumArgs& p, hipStream_t s) {
-  constexpr int V = kVec<T>;
+  // (As many elements a lane as it stores in 16 bytes: with eight, a wave's stores of floats were halves of what it has, 65536 tokens of
+  // 1024 bf16 channels into floats 64 us of the sums' launch, now 57.)
+  constexpr int V = kVec<G>;
   if (p.channels < V) return sums<T, G, 1, 8>(p, p.channels, s);
   const int chunks = (int)(((long long)p.channels + V - 1) / V);
   switch (lanes_of(chunks)) {
@@ -606,9 +658,9 @@ void launch_embedding_backward(const kg_embedding_args& a, hipStream_t s) {
     p.parts = (float*)((char*)a.workspace + plan.parts);
     p.ranges = plan.ranges;
     p.each = plan.each;
-    // (A table of up to 128 MB is filled within the sort's time. A larger one where a good part of its rows is not named.)
+    // (A table of up to 64 MB is filled within the sort's time.)
     const long long bytes = (long long)a.vocab * a.channels * (a.grad_type == PREC_F32 ? 4 : 2);
-    p.filled = !p.accumulate && (bytes <= 128ll << 20 || a.count <= 2ll * a.vocab);
+    p.filled = !p.accumulate && (bytes <= 64ll << 20 || a.count <= a.vocab / 4);
     sort_tokens(a, plan, p, p.filled, s);
   }
   if (a.grad_type == a.type) {

@@ -202,7 +202,7 @@ __global__ __launch_bounds__((Row<T, L, E>::THREADS)) void layer_norm_held_kerne
 
 // Forward, a workgroup a row: its chunks lie along the lines of y (see Chunks), so that rows of odd strides are stored in whole ones, and
 // gamma and beta are read where they are used, which leaves a CU's registers to four rows and more: 2047 rows of 10007 f16 take
-// @ us (94 with chunks from the row's start and gamma and beta in registers, one row a CU).
+// 22 us (94 with chunks from the row's start and gamma and beta in registers, one row a CU).
 template <typename T, int NT, int E>
 __global__ __launch_bounds__(NT) void layer_norm_wide_kernel(LayerArgs a) {
   constexpr int V = kVec<T>;
@@ -379,7 +379,7 @@ __global__ __launch_bounds__(LT) void layer_norm_back_held_kernel(LayerArgs a) {
 }
 
 // The same for a workgroup a row. gamma lies in LDS, and the next row's words are asked for before this one's sums, as few workgroups
-// fit a CU beside the channels' sums (3051 rows of 16384 bf16: @ us, 205 with gamma in registers, some of which went to memory).
+// fit a CU beside the channels' sums (12207 rows of 4096 bf16: 72 us, 85 with gamma in registers and a row at a time).
 template <typename T, int NT, int E>
 __global__ __launch_bounds__(NT) void layer_norm_back_wide_kernel(LayerArgs a) {
   using R = Row<T, NT, E>;
@@ -661,8 +661,8 @@ Shape forward_shape(const LayerArgs& p) {
 }
 // Backward: few chunks a thread, whose sums of dy h and dy take four registers an element of 16 bits and more (97656 rows of 512 bf16
 // by 16 lanes with four chunks: 64 us, by 64 with one 49). Wider rows go by slabs (see layer_norm_back_slab_kernel): held, a row and its
-// channels' sums leave a CU one workgroup (3051 rows of 16384 bf16: 152 us, by slabs @; 6103 of 8192 bf16 109 and @, but 3051 of
-// 8192 f32 60 and @).
+// channels' sums leave a CU one workgroup (3051 rows of 16384 bf16: 152 us, by slabs 84; 6103 of 8192 bf16 109 and 86; rows of as many
+// floats hold half the sums and stay: 3051 of 8192 f32 59).
 Shape backward_shape(int channels, int vec) {
   const int chunks = (int)(((long long)channels + vec - 1) / vec);
   if (chunks <= 8) return {8, 1};

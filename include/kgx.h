@@ -585,10 +585,10 @@ int kg_layer_norm_backward(int device, void* stream, const kg_layer_norm_args* a
 size_t kg_layer_norm_workspace(int rows, int channels);
 
 /* The rows of a table that `count` tokens name, y[i] = scale table[tokens[i]], and the table's gradient,
- *   grad[v] = scale sum of dy[i] over the tokens i with tokens[i] = v, added up in their order,
- * 0 where there is none. A token outside [0, vocab) is padding: its row of y is 0, and its dy is not read. `accumulate`: the sums are
- * added to what grad holds, and rows that no token names are left as they are (a table that is the head's weight too). At most 2^30
- * tokens, rows and channels. */
+ *   grad[v] = scale sum of dy[i] over the tokens i with tokens[i] = v,
+ * 0 where there is none (added up in an order that the tokens alone decide: the same call gives the same bits). A token outside
+ * [0, vocab) is padding: its row of y is 0, and its dy is not read. `accumulate`: the sums are added to what grad holds, and rows
+ * that no token names are left as they are (a table that is the head's weight too). At most 2^30 tokens, rows and channels. */
 typedef struct {
   int count, vocab, channels;
   int type;                /* of table, y and dy */

@@ -42,6 +42,8 @@ EXPORTS = [
     "kg_featurize", "kg_featurize_rows", "kg_evaluate_positions",
     "kg_policy_loss", "kg_policy_loss_workspace", "kg_preference_loss", "kg_preference_loss_workspace", "kg_adamw_step", "kg_adamw_values",
     "kg_adamw_moments", "kg_group_norm", "kg_group_norm_backward", "kg_group_norm_workspace",
+    "kg_distill_loss", "kg_distill_loss_workspace", "kg_layer_norm", "kg_layer_norm_backward", "kg_layer_norm_workspace",
+    "kg_embedding", "kg_embedding_backward", "kg_embedding_backward_workspace",
 ]
 # Completion callback of kg_get_output_async: (user, status).
 DONE_FN = ctypes.CFUNCTYPE(None, ctypes.c_void_p, ctypes.c_int)

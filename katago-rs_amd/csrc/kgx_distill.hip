@@ -321,6 +321,7 @@ __device__ __forceinline__ void place_row(const Lists& l, const Chunks<T>& at) {
 template <typename T, int NT, int E>
 __device__ __forceinline__ void remove_listed(const Lists& l, int tid, const Chunks<T>& at, u32x4 (&raw)[E], int c0) {
   int head[E];
+  tid = fresh(tid);
 #pragma unroll
   for (int e = 0; e < E; e++) head[e] = l.heads[tid + e * NT];
 #pragma unroll
@@ -408,7 +409,7 @@ __device__ __forceinline__ void own_gradient(T* g, int tid, const Chunks<T>& at,
   for (int e = 0; e < E; e++) {
     if (at.none(e * NT)) break;
     const int c = fresh(tid) + e * NT;
-    float gf[kVec<T>] = {};
+    float gf[kVec<T>];
     if (part) {
       // (A listed column's place is filled below.)
       if (plain) {
@@ -423,6 +424,9 @@ __device__ __forceinline__ void own_gradient(T* g, int tid, const Chunks<T>& at,
       }
       store_listed<T, NT * E>(g, l, tid + e * NT, c, at.whole(e * NT, NT), past, at, gf);
     } else {
+      const float zero = __int_as_float(fresh(0));  // (four registers of zeros over the loop of rows are spilled)
+#pragma unroll
+      for (int j = 0; j < kVec<T>; j++) gf[j] = zero;
       store_gradient<T>(g, c, at.whole(e * NT, NT), past, at, gf);
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -764,7 +768,7 @@ void distill_typed(DistillRows p, hipStream_t s) {
     const size_t lds = Copied::bytes(512 * 4, p.k);
     if (p.split > 1) {
       launch_k(distill_long_kernel<T, 512, 4, PARTS>, dim3(p.rows * p.split), 512, lds, s, p);
-      return launch_k(distill_long_kernel<T, 512, 4, JOIN>, dim3(p.rows * p.split + 1), 512, lds, s, p);
+      return launch_k(distill_long_kernel<T, 512, 4, JOIN>, dim3(p.grad ? p.rows * p.split + 1 : 1), 512, lds, s, p);
     }
     launch_k(distill_long_kernel<T, 512, 4, WHOLE>, groups, 512, lds, s, p);
   }

@@ -1,10 +1,10 @@
 // The rows of a table that tokens name, scaled, and the table's gradient (kg_embedding, kg_embedding_backward).
 //
-// The gradient of a row is the sum of its tokens' gradients, in the order of the tokens whatever runs first: the tokens are sorted
-// with their places (stable, by digits of at most 9 bits; counts are whole numbers, so that their atomics have no order), and the sorted
-// places are cut into ranges of equal length, so that a token that comes often is no longer than many that come once. A range sums
-// its runs of one token each; a run that reaches over its range's ends leaves its sum to a second launch, which adds such sums up.
-// Rows that no token names are filled with 0 by other workgroups of the first.
+// The gradient of a row is the sum of its tokens' gradients, in an order that the tokens alone decide: they are sorted with their places
+// (stable, by counting where there are few, else by digits of at most 9 bits; counts are whole numbers, so that their atomics have no
+// order), and the sorted places are cut into ranges of equal length, so that a token that comes often takes no longer than many that come
+// once. A workgroup sums the runs of one token each in a range, in shares; a run that reaches over its range's ends leaves its sum to a
+// last launch, which adds such sums up. Rows that no token names are 0: filled beside the sums, or all of them beside the sort.
 #include <algorithm>
 
 #include "kgx_device.h"
@@ -448,8 +448,7 @@ __global__ __launch_bounds__(ET) void embedding_sums_kernel(SumArgs a) {
     const int key = firsts[0];
 #pragma unroll
     for (int j = 0; j < V; j++) sum[j] = ends[0][j][tid];
-    // (Where it ends in the first share, the next one's first token may still be of the same key only if it did not end.)
-    collect(key);
+    collect(key);  // (with the shares behind that begin with it)
     leave(0);
   }
 }

@@ -430,8 +430,8 @@ size_t kg_preference_loss_workspace(int rows);
  * weight T^2 to keep the gradients' size.) Where no other column has mass, rest is 0. Illegal columns take no part whatever they
  * hold, and their gradient is 0. A row without an entry that counts (padding: every index -1), or whose legal columns are all
  * -infinity, or all of whose teacher's logits are (without teacher_lse), takes no part: loss and gradient 0. A listed column with the logit
- * -infinity and q above 0 makes the loss infinite. NaN in a legal column or an entry that counts makes the row's loss NaN, and its gradient
- * wherever p is not 0. */
+ * -infinity and q above 0 makes the loss infinite (NaN with a weight of 0: it is a factor like any other). NaN or +infinity in a legal
+ * column or an entry that counts makes the row's loss NaN, and its gradient wherever p is not 0. */
 #define KG_DISTILL_MAX_K 1024
 typedef struct {
   int rows, columns, k;        /* k in [1, KG_DISTILL_MAX_K] */
@@ -554,8 +554,9 @@ size_t kg_group_norm_workspace(int batch, int points, int channels, int groups, 
 
 /* Layer norm over the `channels` of each of `rows` rows, and RMS norm (`rms`: mean 0, variance the mean of the squares):
  *   rstd = 1 / sqrt(variance + eps), y = (x - mean) rstd gamma + beta.
- * The statistics are outputs for the backward pass. NaN or infinity in a row makes that row NaN, and with it dgamma and dbeta's channels. At
- * most 2^30 rows of 2^30 channels. */
+ * The statistics are outputs for the backward pass. NaN in a row makes that row NaN, and its channel of dgamma; so does infinity (with `rms`
+ * the row's other elements of y are beta: rstd is 0). The sums are float: where the squares' passes its range rstd is 0 too. At most 2^30 rows
+ * of 2^30 channels. */
 typedef struct {
   int rows, channels;
   int type;                /* of x, y, dy and dx */

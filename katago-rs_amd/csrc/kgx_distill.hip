@@ -318,12 +318,12 @@ __device__ __forceinline__ void place_row(const Lists& l, const Chunks<T>& at) {
 }
 
 // -infinity in the place of listed columns, of the E chunks of a thread from chunk c0 on.
-template <typename T, int NT, int E>
+template <typename T, int NT, int E, int SLOTS = NT * E>
 __device__ __forceinline__ void remove_listed(const Lists& l, int tid, const Chunks<T>& at, u32x4 (&raw)[E], int c0) {
   int head[E];
   tid = fresh(tid);
 #pragma unroll
-  for (int e = 0; e < E; e++) head[e] = l.heads[tid + e * NT];
+  for (int e = 0; e < E; e++) head[e] = l.heads[tid + e * NT % SLOTS];
 #pragma unroll
   for (int e = 0; e < E; e++) {
     if (at.none(c0 + e * NT)) break;
@@ -337,7 +337,7 @@ __device__ __forceinline__ void remove_listed(const Lists& l, int tid, const Chu
 }
 
 // Stores the gradients f of chunk c, of head `slot`, with those of its listed columns.
-template <typename T, int SLOTS>
+template <typename T>
 __device__ __forceinline__ void store_listed(T* row, const Lists& l, int slot, int c, bool whole, int past, const Chunks<T>& at,
                                              const float (&f)[kVec<T>]) {
   typedef typename AnyWords<T>::type words_t;
@@ -396,7 +396,7 @@ __device__ __forceinline__ float own_sum(const Chunks<T>& at, u32x4 (&raw)[E], f
   }
   return sum;
 }
-template <typename T, int NT, int E>
+template <typename T, int NT, int E, int SLOTS = NT * E>
 __device__ __forceinline__ void own_gradient(T* g, int tid, const Chunks<T>& at, u32x4 (&raw)[E], const Lists& l, float base, Base2 c2,
                                              float each, int takes, int past) {
   forget<E>(raw);
@@ -422,7 +422,7 @@ __device__ __forceinline__ void own_gradient(T* g, int tid, const Chunks<T>& at,
           gf[j] = ex == 0.f ? 0.f : ex * each;
         }
       }
-      store_listed<T, NT * E>(g, l, tid + e * NT, c, at.whole(e * NT, NT), past, at, gf);
+      store_listed<T>(g, l, tid + e * NT % SLOTS, c, at.whole(e * NT, NT), past, at, gf);
     } else {
       const float zero = __int_as_float(fresh(0));  // (four registers of zeros over the loop of rows are spilled)
 #pragma unroll
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(256) void distill_wave_kernel(DistillRows a) {
 }
 
 // What the workgroups of longer rows need of the entries, by a wave a row. (Its double arithmetic and its dependent loads in the row's own
-// launch, at 4093 x 32768 bf16: 240 us, and 175 by a wave of its own beside the row's; apart 123, 10 of them here.)
+// launch, at 4093 x 32768 bf16: 240 us, and 175 by a wave of its own beside the row's; apart 112, 10 of them here.)
 constexpr int kSlots = 256;
 template <typename T>
 __global__ __launch_bounds__(64) void distill_known_kernel(DistillRows a) {
@@ -547,10 +547,11 @@ __device__ __forceinline__ void hot_row(const Copied& l, const DistillFactors& f
   for (int i = row_thread<NT>(); i < l.k; i += NT) l.hot[i] = hot_of(f, l.share[i], l.q[i]);
 }
 
-// Longer rows that fit the registers of NT threads: a wave a row without a barrier, or a workgroup; one read.
+// Longer rows that fit the registers of NT threads: a wave a row without a barrier, or a workgroup; one read. (Chunks that are 8 NT apart
+// share a list where there are more.)
 template <typename T, int NT, int E>
-__global__ __launch_bounds__(NT == 64 ? 256 : NT, 6) void distill_row_kernel(DistillRows a) {
-  constexpr int WAVES = NT / 64, PER = NT == 64 ? 4 : 1;
+__global__ __launch_bounds__(NT == 64 ? 256 : NT, E > 8 ? 4 : 6) void distill_row_kernel(DistillRows a) {
+  constexpr int WAVES = NT / 64, PER = NT == 64 ? 4 : 1, SLOTS = NT * (E < 8 ? E : 8);
   extern __shared__ __align__(16) char lds[];
   __shared__ float tops[WAVES], sums[WAVES];
   __shared__ DistillFactors box;
@@ -568,13 +569,13 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, 6) void distill_row_kernel(Dis
     row_sync<NT>();
     asked.begin(a, row, l);
 #pragma unroll
-    for (int e = 0; e < E; e++) l.heads[tid + e * NT] = 0;
+    for (int e = 0; e < SLOTS / NT; e++) l.heads[tid + e * NT] = 0;
     row_sync<NT>();
-    link_row<T, NT, NT * E>(l, at);
+    link_row<T, NT, SLOTS>(l, at);
     if (legal) remove_illegal<T, NT, E, false>(legal, tid, at, raw, unused);
     remove_past<T, NT, E>(tid, at, raw);
     row_sync<NT>();
-    remove_listed<T, NT, E>(l, tid, at, raw, 0);
+    remove_listed<T, NT, E, SLOTS>(l, tid, at, raw, 0);
     float top = wave_reduce<true>(own_top<T, NT, E>(at, raw));
     if constexpr (NT > 64) {
       if ((tid & 63) == 0) tops[tid >> 6] = top;
@@ -607,7 +608,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, 6) void distill_row_kernel(Dis
     const DistillFactors& shared = NT > 64 ? box : f;
     hot_row<NT>(l, shared);
     row_sync<NT>();
-    if (g) own_gradient<T, NT, E>(g, tid, at, raw, l, base, c2, shared.each, shared.part, a.past);
+    if (g) own_gradient<T, NT, E, SLOTS>(g, tid, at, raw, l, base, c2, shared.each, shared.part, a.past);
   }
 }
 
@@ -733,7 +734,7 @@ __global__ __launch_bounds__(NT) void distill_long_kernel(DistillRows a) {
             const float ex = __builtin_amdgcn_exp2f((element<T>(raw[e], j) - top) * c2.hi);
             gf[j] = ex == 0.f ? 0.f : ex * each;
           }
-          store_listed<T, SLOTS>(g, l, tid + e * NT, c, at.whole(c0 + e * NT, NT), a.past, at, gf);
+          store_listed<T>(g, l, tid + e * NT, c, at.whole(c0 + e * NT, NT), a.past, at, gf);
         } else {
           store_gradient<T>(g, c, at.whole(c0 + e * NT, NT), a.past, at, gf);
         }
@@ -770,7 +771,11 @@ void distill_typed(DistillRows p, hipStream_t s) {
       launch_k(distill_long_kernel<T, 512, 4, PARTS>, dim3(p.rows * p.split), 512, lds, s, p);
       return launch_k(distill_long_kernel<T, 512, 4, JOIN>, dim3(p.grad ? p.rows * p.split + 1 : 1), 512, lds, s, p);
     }
-    launch_k(distill_long_kernel<T, 512, 4, WHOLE>, groups, 512, lds, s, p);
+    // (As many chunks a thread again where rows are not cut: 4093 x 33000 bf16 204 us by pieces, 167 held, 2048 x 50257 bf16 151 and 136; but
+    // 300 x 50257 floats 58 in parts, 61 held, and rows twice as long by 1024 threads 325 where pieces take 313.)
+    const long long chunks = ((long long)p.columns + kVec<T> - 1) / kVec<T> + Chunks<T>::line(p.columns) / 16;
+    if (chunks <= 512 * 16) launch_k(distill_row_kernel<T, 512, 16>, groups, 512, Copied::bytes(512 * 8, p.k), s, p);
+    else launch_k(distill_long_kernel<T, 512, 4, WHOLE>, groups, 512, lds, s, p);
   }
   launch_k(distill_loss_kernel, dim3(row_grid(p.rows, 64)), 64, 0, s, p);
 }

@@ -20,11 +20,15 @@ def learn():
     return importlib.import_module("katago-rs_amd.learn")
 
 
-@pytest.mark.parametrize("n,v,dtype", [(389, 17001, torch.float32), (386, 33100, torch.bfloat16), (40, 70001, torch.float16)])
+@pytest.mark.parametrize("n,v,dtype", [(389, 17001, torch.float32), (386, 33100, torch.bfloat16), (40, 70001, torch.float16),
+                                       (390, 32736, torch.float32), (390, 32800, torch.float32), (385, 65473, torch.bfloat16)])
 @pytest.mark.parametrize("rest", [False, True])
 def test_long_rows(learn, n, v, dtype, rest):
     c = distill.make(n, v, 40, dtype, torch.float32, n, legal=rest, rest=rest, ld=6)
     c["index"][n // 2] = -1
+    # (Columns whose chunks lie 4096 apart: lists that may be shared.)
+    far = torch.arange(0, v, 4096 * 16 // c["z"].element_size())
+    c["index"][1, :len(far)] = far.int()
     distill.check(learn, c)
 
 

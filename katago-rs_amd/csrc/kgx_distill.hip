@@ -367,6 +367,32 @@ __device__ __forceinline__ void store_listed(T* row, const Lists& l, int slot, i
   }
 }
 
+// The gradients of a chunk's columns, listed ones aside: each e^((z - base) s).
+struct OtherGradients {
+  float base, shift, each, factor;
+  bool plain;
+  Base2 c2;
+  // Mostly (z - base) log2 e as one multiply-add: what base log2 e's rounding makes of every term goes into the factor. Not where base is
+  // so large that this is a factor of its own, and not where the factor is no number, which columns without mass do not take.
+  __device__ __forceinline__ OtherGradients(float base_, float each_, Base2 c) : base(base_), shift(base_ * c.hi), each(each_), c2(c) {
+    factor = each * __builtin_amdgcn_exp2f(__builtin_fmaf(-base, c.hi, shift));
+    plain = __builtin_amdgcn_readfirstlane(fabsf(shift) < 0x1p20f && fabsf(each) < INFINITY);
+  }
+  template <typename T>
+  __device__ __forceinline__ void of(const u32x4& raw, float (&f)[kVec<T>]) const {
+    if (plain) {
+#pragma unroll
+      for (int j = 0; j < kVec<T>; j++) f[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(element<T>(raw, j), c2.hi, -shift)) * factor;
+    } else {
+#pragma unroll
+      for (int j = 0; j < kVec<T>; j++) {
+        const float ex = __builtin_amdgcn_exp2f((element<T>(raw, j) - base) * c2.hi);
+        f[j] = ex == 0.f ? 0.f : ex * each;
+      }
+    }
+  }
+};
+
 // The maximum of a thread's chunks, their sum of e^((z - top) s) and their gradients, of rows that stay in registers.
 template <typename T, int NT, int E>
 __device__ __forceinline__ float own_top(const Chunks<T>& at, const u32x4 (&raw)[E]) {
@@ -401,27 +427,14 @@ __device__ __forceinline__ void own_gradient(T* g, int tid, const Chunks<T>& at,
                                              float each, int takes, int past) {
   forget<E>(raw);
   const bool part = __builtin_amdgcn_readfirstlane(takes);
-  // Mostly (z - base) log2 e as one multiply-add: what base log2 e's rounding makes of every term goes into the factor. Not where base is
-  // so large that this is a factor of its own, and not where the factor is no number, which columns without mass do not take.
-  const float shift = base * c2.hi, factor = each * __builtin_amdgcn_exp2f(__builtin_fmaf(-base, c2.hi, shift));
-  const bool plain = __builtin_amdgcn_readfirstlane(fabsf(shift) < 0x1p20f && fabsf(each) < INFINITY);
+  const OtherGradients others(base, each, c2);
 #pragma unroll
   for (int e = 0; e < E; e++) {
     if (at.none(e * NT)) break;
     const int c = fresh(tid) + e * NT;
     float gf[kVec<T>];
     if (part) {
-      // (A listed column's place is filled below.)
-      if (plain) {
-#pragma unroll
-        for (int j = 0; j < kVec<T>; j++) gf[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(element<T>(raw[e], j), c2.hi, -shift)) * factor;
-      } else {
-#pragma unroll
-        for (int j = 0; j < kVec<T>; j++) {
-          const float ex = __builtin_amdgcn_exp2f((element<T>(raw[e], j) - base) * c2.hi);
-          gf[j] = ex == 0.f ? 0.f : ex * each;
-        }
-      }
+      others.of<T>(raw[e], gf);  // (a listed column's place is filled below)
       store_listed<T>(g, l, tid + e * NT % SLOTS, c, at.whole(e * NT, NT), past, at, gf);
     } else {
       const float zero = __int_as_float(fresh(0));  // (four registers of zeros over the loop of rows are spilled)
@@ -718,7 +731,7 @@ __global__ __launch_bounds__(NT) void distill_long_kernel(DistillRows a) {
     hot_row<NT>(l, box);
     lds_barrier();
     const bool takes = __builtin_amdgcn_readfirstlane(box.part);
-    const float each = box.each, top = base;
+    const OtherGradients others(base, box.each, c2);
     for (int c0 = begin; c0 < end && !at.none(c0); c0 += SLOTS) {
       u32x4 raw[E];
       if (takes) piece(c0, raw);
@@ -728,12 +741,7 @@ __global__ __launch_bounds__(NT) void distill_long_kernel(DistillRows a) {
         const int c = fresh(tid) + c0 + e * NT;
         float gf[V] = {};
         if (takes) {
-          // (A column without mass has no gradient, whatever the factor. A listed one's place is filled below.)
-#pragma unroll
-          for (int j = 0; j < V; j++) {
-            const float ex = __builtin_amdgcn_exp2f((element<T>(raw[e], j) - top) * c2.hi);
-            gf[j] = ex == 0.f ? 0.f : ex * each;
-          }
+          others.of<T>(raw[e], gf);  // (a listed column's place is filled below)
           store_listed<T>(g, l, tid + e * NT, c, at.whole(c0 + e * NT, NT), a.past, at, gf);
         } else {
           store_gradient<T>(g, c, at.whole(c0 + e * NT, NT), a.past, at, gf);

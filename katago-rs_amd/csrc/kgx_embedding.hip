@@ -259,6 +259,18 @@ __device__ __forceinline__ void put(G* p, int left, const float (&sum)[N], float
   }
 }
 
+// A lane's vector, whose elements below `least` are the one's before too.
+template <typename G, int V>
+__device__ __forceinline__ void put_vector(G* p, int least, const float (&sum)[V], float scale, int accumulate) {
+  if (V > 1 && least > 0 && accumulate) {  // (what is shared is added to once)
+#pragma unroll
+    for (int j = 0; j < V; j++)
+      if (j >= least) p[j] = to_t<G>(__builtin_fmaf(sum[j], scale, (float)p[j]));
+  } else {
+    put<G, V>(p, V, sum, scale, accumulate);
+  }
+}
+
 // The first sorted place whose key is at least `key`, by seven probes at a time: each step waits for memory.
 __device__ __forceinline__ int lower_bound(const unsigned* keys, int count, unsigned key) {
   int lo = 0, hi = count;
@@ -346,15 +358,7 @@ __global__ __launch_bounds__(ET) void embedding_sums_kernel(SumArgs a) {
   int run = -1;
   bool before = false;
   const auto write = [&](int key) {
-    G* p = (G*)a.grad + (size_t)key * a.ld_grad + c;
-    if (!in) return;
-    if (V > 1 && least > 0 && a.accumulate) {  // (what is shared is added to once)
-#pragma unroll
-      for (int j = 0; j < V; j++)
-        if (j >= least) p[j] = to_t<G>(__builtin_fmaf(sum[j], a.scale, (float)p[j]));
-    } else {
-      put<G, V>(p, V, sum, a.scale, a.accumulate);
-    }
+    if (in) put_vector<G, V>((G*)a.grad + (size_t)key * a.ld_grad + c, least, sum, a.scale, a.accumulate);
   };
   const auto keep = [&](int side) {
 #pragma unroll
@@ -501,6 +505,112 @@ __global__ __launch_bounds__(JT) void embedding_join_kernel(SumArgs a, int block
   }
 }
 
+// Few tokens of a small table, in one launch: a workgroup for a slab of a few rows of the table finds their tokens by itself. It counts and
+// places them as the sort does, rows for digits; then L lanes take a row of few tokens each, and all of them one of many. 722 tokens of
+// 362 rows of 384 floats take 4 us of a graph (10 where they are all the same), 11 by the launches below; but of larger tables, where a
+// workgroup has more rows than it takes at once, 1024 skewed tokens of 16384 rows of 512 bf16 16 and 14.
+constexpr int NT = 1024, kFewTokens = NT, kFewRows = 16, kFewOfRow = 16;
+struct FewArgs {
+  const int* tokens;
+  const void* dy;
+  void* grad;
+  long long ld, ld_grad;
+  int count, vocab, channels, rows, slabs, lanes, accumulate;  // rows: of a workgroup; lanes: 2^lanes = L
+  float scale;
+};
+template <typename T, typename G, int V>
+__global__ __launch_bounds__(NT) void embedding_few_kernel(FewArgs a) {
+  constexpr int WAVES = NT / 64, AT_ONCE = 8;
+  __shared__ int to[WAVES][kFewRows];  // where a wave's tokens of a row go
+  __shared__ int firsts[kFewRows + 1], places[kFewTokens];
+  __shared__ float joined[V][NT];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int range = blockIdx.x / a.slabs, row0 = range * a.rows, rows = min(a.rows, a.vocab - row0);
+  // (A token before row0, or outside the table, is past `rows` as an unsigned difference.)
+  const unsigned row = tid < a.count ? (unsigned)a.tokens[tid] - (unsigned)row0 : ~0u;
+  const bool mine = row < (unsigned)rows;
+  if (lane < kFewRows) to[w][lane] = 0;
+  __syncthreads();
+  if (mine) atomicAdd(&to[w][row], 1);
+  __syncthreads();
+  if (tid < kFewRows) {
+    int n = 0;
+    for (int k = 0; k < WAVES; k++) {
+      const int here = to[k][tid];
+      to[k][tid] = n;
+      n += here;
+    }
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < kFewRows; o <<= 1) {
+      const int v = __shfl_up(upto, o);
+      upto += lane >= o ? v : 0;
+    }
+    firsts[tid + 1] = upto;
+    if (tid == 0) firsts[0] = 0;
+    for (int k = 0; k < WAVES; k++) to[k][tid] += upto - n;
+  }
+  __syncthreads();
+  unsigned long long same = __ballot(mine);
+  for (int k = 0; 1 << k < kFewRows; k++) {
+    const unsigned long long set = __ballot(row >> k & 1);
+    same &= row >> k & 1 ? set : ~set;
+  }
+  if (mine) places[to[w][row] + __popcll(same & ((1ull << lane) - 1))] = tid;
+  __syncthreads();
+
+  const int L = 1 << a.lanes, share = tid >> a.lanes, shares = NT >> a.lanes;
+  const int column = ((blockIdx.x - range * a.slabs) * L + (tid & (L - 1))) * V;
+  const bool in = column < a.channels;
+  const int c = min(column, a.channels - V), least = column - c;  // elements below `least` are the vector's before
+  const T* dy = (const T*)a.dy + c;
+  const auto add_up = [&](int first, int last, float(&sum)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; j++) sum[j] = 0.f;
+    for (int i = first; i < last; i += AT_ONCE) {
+      Columns<T, V> f[AT_ONCE];
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; k++)
+        if (i + k < last) f[k].load(dy + (size_t)places[i + k] * a.ld);
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; k++) {
+        if (i + k >= last) break;
+#pragma unroll
+        for (int j = 0; j < V; j++) sum[j] += f[k].at(j);
+      }
+    }
+  };
+  const auto write = [&](int r, const float(&sum)[V]) {
+    if (in) put_vector<G, V>((G*)a.grad + (size_t)(row0 + r) * a.ld_grad + c, least, sum, a.scale, a.accumulate);
+  };
+  for (int r = share; r < rows; r += shares) {
+    const int first = firsts[r], last = firsts[r + 1];
+    if (last - first > kFewOfRow || (a.accumulate && first == last)) continue;
+    float sum[V];
+    add_up(first, last, sum);
+    write(r, sum);
+  }
+  for (int r = 0; r < rows; r++) {
+    const int first = firsts[r], n = firsts[r + 1] - first;
+    if (n <= kFewOfRow) continue;
+    const int each = (n + shares - 1) / shares, used = (n + each - 1) / each, begin = first + share * each;
+    float sum[V];
+    add_up(begin, min(begin + each, first + n), sum);
+#pragma unroll
+    for (int j = 0; j < V; j++) joined[j][tid] = sum[j];
+    __syncthreads();
+    if (share == 0) {
+#pragma unroll 4
+      for (int k = 1; k < used; k++) {
+#pragma unroll
+        for (int j = 0; j < V; j++) sum[j] += joined[j][(k << a.lanes) + tid];
+      }
+      write(r, sum);
+    }
+    __syncthreads();
+  }
+}
+
 // How the tokens are sorted and cut, and where their parts of the workspace lie.
 struct Plan {
   int passes, bits, blocks, each_block, each, ranges;  // passes: 0 where the tokens are ranked
@@ -617,6 +727,29 @@ void backward_typed(const SumArgs& p, hipStream_t s) {
   }
 }
 
+// Returns whether there are few tokens, and the launch.
+template <typename T, typename G>
+bool few(const SumArgs& p, const int* tokens, hipStream_t s) {
+  constexpr int V = kVec<G>;
+  const bool narrow = p.channels < V;
+  FewArgs a = {};
+  a.lanes = 3;
+  const long long chunks = narrow ? p.channels : ((long long)p.channels + V - 1) / V;
+  while (1 << a.lanes < chunks && a.lanes < 6) a.lanes++;
+  const long long slabs = (chunks + (1 << a.lanes) - 1) >> a.lanes, groups = slabs * p.vocab;  // a row each
+  if (p.count > kFewTokens || groups > 512 * kFewRows) return false;
+  a.tokens = tokens;
+  a.dy = p.dy; a.ld = p.ld;
+  a.grad = p.grad; a.ld_grad = p.ld_grad;
+  a.count = p.count; a.vocab = p.vocab; a.channels = p.channels; a.accumulate = p.accumulate; a.scale = p.scale;
+  a.rows = (int)((groups + 511) / 512);
+  a.slabs = (int)slabs;
+  const dim3 grid((p.vocab + a.rows - 1) / a.rows * a.slabs);
+  if (narrow) launch_k(embedding_few_kernel<T, G, 1>, grid, NT, 0, s, a);
+  else launch_k(embedding_few_kernel<T, G, V>, grid, NT, 0, s, a);
+  return true;
+}
+
 }  // namespace
 
 size_t embedding_backward_workspace(int count, int vocab, int channels) { return count < 1 ? 0 : plan_of(count, vocab, channels).bytes; }
@@ -652,27 +785,27 @@ void launch_embedding_backward(const kg_embedding_args& a, hipStream_t s) {
   p.grad = a.grad; p.ld_grad = a.ld_grad;
   p.count = a.count; p.vocab = a.vocab; p.channels = a.channels; p.accumulate = a.accumulate != 0;
   p.scale = (float)a.scale;
-  if (a.count) {
-    const Plan plan = plan_of(a.count, a.vocab, a.channels);
-    p.parts = (float*)((char*)a.workspace + plan.parts);
-    p.ranges = plan.ranges;
-    p.each = plan.each;
-    // (A table of up to 64 MB is filled within the sort's time.)
-    const long long bytes = (long long)a.vocab * a.channels * (a.grad_type == PREC_F32 ? 4 : 2);
-    p.filled = !p.accumulate && (bytes <= 64ll << 20 || a.count <= a.vocab / 4);
-    sort_tokens(a, plan, p, p.filled, s);
-  }
-  if (a.grad_type == a.type) {
-    switch (a.type) {
-      case PREC_F32: backward_typed<float, float>(p, s); break;
-      case PREC_F16: backward_typed<f16, f16>(p, s); break;
-      default: backward_typed<bf16, bf16>(p, s); break;
+  const auto go = [&](auto of_dy, auto of_grad) {
+    using T = decltype(of_dy);
+    using G = decltype(of_grad);
+    if (few<T, G>(p, a.tokens, s)) return;
+    if (a.count) {
+      const Plan plan = plan_of(a.count, a.vocab, a.channels);
+      p.parts = (float*)((char*)a.workspace + plan.parts);
+      p.ranges = plan.ranges;
+      p.each = plan.each;
+      // (A table of up to 64 MB is filled within the sort's time.)
+      const long long bytes = (long long)a.vocab * a.channels * (long long)sizeof(G);
+      p.filled = !p.accumulate && (bytes <= 64ll << 20 || a.count <= a.vocab / 4);
+      sort_tokens(a, plan, p, p.filled, s);
     }
-  } else if (a.type == PREC_F16) {
-    backward_typed<f16, float>(p, s);
-  } else {
-    backward_typed<bf16, float>(p, s);
-  }
+    backward_typed<T, G>(p, s);
+  };
+  if (a.type == PREC_F32) go(0.f, 0.f);
+  else if (a.type == PREC_F16 && a.grad_type == a.type) go((f16)0.f, (f16)0.f);
+  else if (a.type == PREC_F16) go((f16)0.f, 0.f);
+  else if (a.grad_type == a.type) go((bf16)0.f, (bf16)0.f);
+  else go((bf16)0.f, 0.f);
   KGX_CHECK_LAUNCH();
 }
 

@@ -130,3 +130,26 @@ def test_infinite_logits_and_weights_of_zero(learn, v, rest):
     got = distill.run(learn, c)
     assert math.isnan(float(got.loss[1])) and math.isnan(float(got.loss[2])) and math.isfinite(float(got.loss[3]))
     assert torch.isfinite(got.grad[3]).all()
+
+
+# Up to 1024 tokens of up to 8192 rows and slabs of their columns go in one launch.
+@pytest.mark.parametrize("vocab", [1, 2, 63, 511, 513, 1025, 8192, 8193, 32769])
+@pytest.mark.parametrize("c,dtype,wide", [(1, torch.float32, False), (3, torch.bfloat16, True), (7, torch.float16, False), (31, torch.float16, False),
+                                          (36, torch.bfloat16, True), (257, torch.float32, False), (1030, torch.bfloat16, False)])
+def test_few_tokens(learn, vocab, c, dtype, wide):
+    g = torch.Generator().manual_seed(vocab + c)
+    grad_type = torch.float32 if wide else dtype
+    before = torch.randn(vocab, c, generator=g).to(grad_type)
+    before[vocab - 1] = math.inf
+    for n, kind in ((1, "even"), (17, "one"), (600, "likely"), (1023, "even"), (1024, "one"), (1025, "likely")):
+        tokens, dy = embedding.tokens_of(n, vocab, n, kind), torch.randn(n, c, generator=g).to(dtype)
+        dy[(tokens < 0) | (tokens >= vocab)] = math.nan
+        first = embedding.backward(learn, tokens, dy, vocab, 0.3, dtype=grad_type)
+        assert torch.equal(embedding.backward(learn, tokens, dy, vocab, 0.3, dtype=grad_type), first)
+        tokens[tokens == vocab - 1] = -1
+        dy[tokens == -1] = math.nan
+        embedding.backward(learn, tokens, dy, vocab, 0.3, before)
+        room = torch.full((vocab, c + 7), 7.0, dtype=grad_type, device="cuda")
+        given = learn.embedding_backward(dy.cuda(), tokens.cuda(), vocab, scale=0.3, grad=room[:, 3:c + 3])
+        assert torch.equal(given, learn.embedding_backward(dy.cuda(), tokens.cuda(), vocab, scale=0.3, dtype=grad_type))
+        assert (room[:, :3] == 7).all() and (room[:, c + 3:] == 7).all()

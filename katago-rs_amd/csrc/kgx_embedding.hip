@@ -4,7 +4,8 @@
 // (stable, by counting where there are few, else by digits of at most 9 bits; counts are whole numbers, so that their atomics have no
 // order), and the sorted places are cut into ranges of equal length, so that a token that comes often takes no longer than many that come
 // once. A workgroup sums the runs of one token each in a range, in shares; a run that reaches over its range's ends leaves its sum to a
-// last launch, which adds such sums up. Rows that no token names are 0: filled beside the sums, or all of them beside the sort.
+// last launch, which adds such sums up. Rows that no token names are 0: filled beside the sums, or all of them beside the sort. Few tokens
+// of a small table take one launch instead (embedding_few_kernel).
 #include <algorithm>
 
 #include "kgx_device.h"

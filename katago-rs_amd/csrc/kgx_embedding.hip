@@ -64,24 +64,41 @@ __global__ __launch_bounds__(ET) void embedding_kernel(const int* tokens, const 
 // Tokens outside the table are behind all others.
 __device__ __forceinline__ unsigned key_of(int token, int vocab) { return min((unsigned)token, (unsigned)vocab); }
 
-// 0 in every row, by workgroups behind those that sort, whose launches leave memory idle: the sums then write over the rows that are named.
-// Where few are named, or the table is small (5003 tokens of 100003 rows of 512 f16: 28 us, 32 with the others looked for and filled
-// beside the sums; but 65536 tokens of 50257 rows of 1024 floats, 206 MB: 113 against 104).
+// 0 in rows of the table by workgroups behind those that sort, whose launches leave memory idle. In every row, which the sums then write over,
+// where few are named or the table is small (5003 tokens of 100003 rows of 512 f16: 28 us, 32 with the others looked for and filled
+// beside the sums). Or in those that no token names, by marks that the first launch leaves: a row's is the place of any of its tokens, so that
+// what was in the marks' memory before is no mark unless it happens to be true (20000 tokens of 50257 rows of 1024 floats 62 -> 58 us
+// against filling beside the sums, 65536 of 200000 of 512 129 -> 120).
 struct FillArgs {
   void* grad;
-  long long ld;    // bytes
+  long long ld;     // bytes
   long long bytes;
-  int first, rows, groups;  // this launch's rows; groups: workgroups that sort
+  const int *tokens, *marks;  // marks: [vocab], or NULL: every row
+  int count, first, rows, groups;  // this launch's rows; groups: workgroups that sort
 };
+constexpr int kMarked = 8;  // rows whose marks a wave reads at once
+__device__ __forceinline__ void fill_row(const FillArgs& f, int row) {
+  char* p = (char*)f.grad + (size_t)row * f.ld;
+  for (long long c = (threadIdx.x & 63) * 16; c < f.bytes; c += 1024) {
+    if (c + 16 <= f.bytes) *(u32x4_any2*)(p + c) = u32x4{0, 0, 0, 0};
+    else for (long long k = c; k < f.bytes; k += 2) *(unsigned short*)(p + k) = 0;
+  }
+}
 __device__ __forceinline__ bool fills(const FillArgs& f) {
   if ((int)blockIdx.x < f.groups) return false;
-  const int wave = (blockIdx.x - f.groups) * (ST / 64) + (threadIdx.x >> 6), waves = (gridDim.x - f.groups) * (ST / 64);
-  for (int row = f.first + wave; row < f.first + f.rows; row += waves) {
-    char* p = (char*)f.grad + (size_t)row * f.ld;
-    for (long long c = (threadIdx.x & 63) * 16; c < f.bytes; c += 1024) {
-      if (c + 16 <= f.bytes) *(u32x4_any2*)(p + c) = u32x4{0, 0, 0, 0};
-      else for (long long k = c; k < f.bytes; k += 2) *(unsigned short*)(p + k) = 0;
+  const int lane = threadIdx.x & 63, end = f.first + f.rows, waves = (gridDim.x - f.groups) * (ST / 64);
+  const int wave = __builtin_amdgcn_readfirstlane((blockIdx.x - f.groups) * (ST / 64) + (threadIdx.x >> 6));
+  if (!f.marks) {
+    for (int row = f.first + wave; row < end; row += waves) fill_row(f, row);
+    return true;
+  }
+  for (long long row = f.first + (long long)wave * kMarked; row < end; row += (long long)waves * kMarked) {
+    bool none = false;
+    if (lane < kMarked && row + lane < end) {
+      const int at = f.marks[row + lane];
+      none = (unsigned)at >= (unsigned)f.count || f.tokens[at] != (int)row + lane;
     }
+    for (unsigned long long left = __ballot(none); left; left &= left - 1) fill_row(f, (int)row + __ffsll(left) - 1);
   }
   return true;
 }
@@ -129,6 +146,7 @@ struct SortArgs {
   unsigned* keys_out;
   int* places_out;
   int* counts;  // [blocks][2^bits]
+  int* marks;   // see FillArgs; or NULL
   int count, vocab, blocks, each, shift, bits;  // each: tokens of a block, a multiple of ST
 };
 
@@ -141,7 +159,11 @@ __global__ __launch_bounds__(ST) void sort_count_kernel(SortArgs a, FillArgs fil
   __syncthreads();
   for (int r = 0; r < a.each; r += ST) {
     const long long i = (long long)b * a.each + r + tid;
-    if (i < a.count) atomicAdd(&n[(FIRST ? key_of(a.tokens[i], a.vocab) : a.keys[i]) >> a.shift & (digits - 1)], 1);
+    if (i < a.count) {
+      const unsigned key = FIRST ? key_of(a.tokens[i], a.vocab) : a.keys[i];
+      atomicAdd(&n[key >> a.shift & (digits - 1)], 1);
+      if (FIRST && a.marks && key < (unsigned)a.vocab) a.marks[key] = (int)i;
+    }
   }
   __syncthreads();
   for (int d = tid; d < digits; d += ST) a.counts[b * digits + d] = n[d];
@@ -615,7 +637,8 @@ __global__ __launch_bounds__(NT) void embedding_few_kernel(FewArgs a) {
 // How the tokens are sorted and cut, and where their parts of the workspace lie.
 struct Plan {
   int passes, bits, blocks, each_block, each, ranges;  // passes: 0 where the tokens are ranked
-  size_t keys, places, counts, parts, bytes;
+  bool marked;  // rows that no token names are filled by marks
+  size_t keys, places, counts, marks, parts, bytes;
 };
 // From one copy of the keys to the other: whole eights, which are read at once.
 size_t plan_stride(int count) { return ((size_t)count + 7) / 8 * 8; }
@@ -632,7 +655,8 @@ Plan plan_of(int count, int vocab, int channels) {
   if (count > kRanked) {
     const int bits = 32 - __builtin_clz((unsigned)vocab);  // of the keys 0 ... vocab
     p.passes = (bits + kDigit - 1) / kDigit;
-    p.bits = (bits + p.passes - 1) / p.passes;
+    // (Six at least: a launch adds a digit's counts up by as many threads as there are digits, 11552 tokens of 3 rows 16 us with 2 bits.)
+    p.bits = std::max((bits + p.passes - 1) / p.passes, 6);
     const long long rounds = ((long long)count + (long long)ST * kMostBlocks - 1) / ((long long)ST * kMostBlocks);
     p.each_block = (int)(rounds * ST);
     p.blocks = (int)(((long long)count + p.each_block - 1) / p.each_block);
@@ -650,13 +674,16 @@ Plan plan_of(int count, int vocab, int channels) {
   p.keys = room(copies * plan_stride(count) * 4);
   p.places = room(copies * plan_stride(count) * 4);
   p.counts = room((size_t)p.blocks * (4 << p.bits));
+  // (Fewer: see FillArgs. More leave few rows without a token, and write each mark over and over: 1000000 tokens of 5000 rows 96 us, 92.)
+  p.marked = p.passes && count > vocab / 4 && count / 4 <= vocab;
+  p.marks = room(p.marked ? (size_t)vocab * 4 : 0);
   p.parts = room((size_t)p.ranges * 2 * channels * 4);
   return p;
 }
 
 inline int grid_of(long long threads) { return (int)std::min((threads + ET - 1) / ET, 1ll << 20); }
 
-// filled: whether the launch has set every row to 0.
+// filled: whether the launches fill rows.
 void sort_tokens(const kg_embedding_args& a, const Plan& plan, SumArgs& p, bool filled, hipStream_t s) {
   char* w = (char*)a.workspace;
   unsigned* keys = (unsigned*)(w + plan.keys);
@@ -667,12 +694,19 @@ void sort_tokens(const kg_embedding_args& a, const Plan& plan, SumArgs& p, bool 
   fill.groups = plan.passes ? plan.blocks : (a.count + RI - 1) / RI;
   const int size = a.grad_type == PREC_F32 ? 4 : 2, launches = plan.passes ? 2 * plan.passes : 1;
   fill.grad = a.grad; fill.ld = a.ld_grad * size; fill.bytes = (long long)a.channels * size;
-  // The grid of the next launch, with its share of the rows.
+  // The grid of the next launch, with its share of the rows: none for the one that leaves the marks.
+  const bool marks = filled && plan.marked;
+  if (marks) {
+    fill.marks = (const int*)(w + plan.marks);
+    fill.tokens = a.tokens;
+    fill.count = a.count;
+  }
   const auto grid = [&](int launch) {
-    const auto upto = [&](int k) { return (int)((long long)a.vocab * k / launches); };
+    const auto upto = [&](int k) { return k < marks ? 0 : (int)((long long)a.vocab * (k - marks) / (launches - marks)); };
     fill.first = upto(launch);
     fill.rows = filled ? upto(launch + 1) - fill.first : 0;
-    return dim3(fill.groups + std::min((fill.rows + ST / 64 - 1) / (ST / 64), 512));
+    const int each = marks ? kMarked * (ST / 64) : ST / 64;
+    return dim3(fill.groups + std::min((fill.rows + each - 1) / each, 512));
   };
   if (!plan.passes) {
     const dim3 all = grid(0);
@@ -682,6 +716,7 @@ void sort_tokens(const kg_embedding_args& a, const Plan& plan, SumArgs& p, bool 
   SortArgs t = {};
   t.tokens = a.tokens;
   t.counts = (int*)(w + plan.counts);
+  t.marks = marks ? (int*)(w + plan.marks) : nullptr;
   t.count = a.count; t.vocab = a.vocab; t.blocks = plan.blocks; t.each = plan.each_block; t.bits = plan.bits;
   for (int k = 0; k < plan.passes; k++) {
     t.shift = k * plan.bits;
@@ -797,7 +832,7 @@ void launch_embedding_backward(const kg_embedding_args& a, hipStream_t s) {
       p.each = plan.each;
       // (A table of up to 64 MB is filled within the sort's time.)
       const long long bytes = (long long)a.vocab * a.channels * (long long)sizeof(G);
-      p.filled = !p.accumulate && (bytes <= 64ll << 20 || a.count <= a.vocab / 4);
+      p.filled = !p.accumulate && (plan.marked || bytes <= 64ll << 20 || a.count <= a.vocab / 4);
       sort_tokens(a, plan, p, p.filled, s);
     }
     backward_typed<T, G>(p, s);

@@ -78,9 +78,10 @@ def test_sums_over_many_rows(learn, n, c, dtype):
         norm.both(learn, n, c, dtype, n + i, rms, params, ld)
 
 
-# Tables of more than 64 MB with more than a quarter as many tokens: rows that no token names are filled beside the sums.
+# Tables of more than 64 MB with more than a quarter as many tokens: rows that no token names are filled by marks or beside the sums.
 @pytest.mark.parametrize("n,vocab,c,dtype,wide", [(20001, 70000, 257, torch.float32, False), (40000, 140000, 257, torch.bfloat16, False),
-                                                  (20000, 70000, 250, torch.float16, True), (8192, 20000, 900, torch.float32, False)])
+                                                  (20000, 70000, 250, torch.float16, True), (8192, 20000, 900, torch.float32, False),
+                                                  (8200, 2000, 8500, torch.bfloat16, True)])
 def test_large_tables(learn, n, vocab, c, dtype, wide):
     g = torch.Generator().manual_seed(n)
     dy = torch.randn(n, c, generator=g).to(dtype)
@@ -153,3 +154,25 @@ def test_few_tokens(learn, vocab, c, dtype, wide):
         given = learn.embedding_backward(dy.cuda(), tokens.cuda(), vocab, scale=0.3, grad=room[:, 3:c + 3])
         assert torch.equal(given, learn.embedding_backward(dy.cuda(), tokens.cuda(), vocab, scale=0.3, dtype=grad_type))
         assert (room[:, :3] == 7).all() and (room[:, c + 3:] == 7).all()
+
+
+def test_marks_of_other_tokens(learn):
+    """What a call left in its workspace, where the next one with other tokens marks its rows: by a graph whose workspace stays."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    dy = torch.randn(20000, 40, generator=g, device="cuda")
+    tokens = torch.randint(0, 30000, (20000,), generator=g, device="cuda").int()
+    grad = torch.empty(30000, 40, device="cuda")
+    learn.embedding_backward(dy, tokens, 30000, grad=grad)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        learn.embedding_backward(dy, tokens, 30000, grad=grad)
+    for k in range(5):
+        tokens.copy_(torch.randint(0, (30000, 9, 15000, 40000, 1)[k], (20000,), generator=g, device="cuda") - k)
+        grad.fill_(math.nan)
+        graph.replay()
+        want = learn.embedding_backward(dy, tokens, 30000)
+        torch.cuda.synchronize()
+        assert torch.equal(grad, want)
+        named = torch.zeros(30000, dtype=torch.bool, device="cuda")
+        named[tokens[(tokens >= 0) & (tokens < 30000)].long()] = True
+        assert not grad[~named].any() and grad[named].any(1).all()

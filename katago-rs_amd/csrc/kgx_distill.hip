@@ -37,7 +37,7 @@ struct DistillRows {
   // Of rows that take a workgroup, by a launch before: what a wave knows of their entries (see Known).
   Known* known;
   Others *others, *parts;  // parts: of rows cut into `split` parts of `span` chunks
-  int split, span;
+  int split, span, knowing;  // knowing: workgroups ahead of the parts', a wave of four for the entries of a row (0: by a launch before)
   double *share, *q;  // [rows][k]
   int* column;        // [rows][k], -1 where an entry does not count
 };
@@ -488,27 +488,29 @@ __global__ __launch_bounds__(256) void distill_wave_kernel(DistillRows a) {
 // launch, at 4093 x 32768 bf16: 240 us, and 175 by a wave of its own beside the row's; apart 112, 10 of them here.)
 constexpr int kSlots = 256;
 template <typename T>
+__device__ __forceinline__ void know_row(const DistillRows& a, int row, const Listed& l) {
+  const int lane = threadIdx.x & 63;
+  const Entry mine(a, row, lane);
+  row_sync<64>();  // (the last row's lists have been read)
+#pragma unroll
+  for (int i = 0; i < kSlots / 64; i++) l.heads[lane + i * 64] = 0;
+  row_sync<64>();
+  list_row<T, 64>(a, row, (const T*)a.logits + (size_t)row * a.ld, a.legal ? a.legal + (size_t)row * a.ld_legal : nullptr, l, mine,
+                  [](int c) { return c % kSlots; });
+  const Known known = know(a, row, l);
+  if (lane == 0) a.known[row] = known;
+  for (int i = lane; i < a.k; i += 64) {
+    const size_t at = (size_t)row * a.k + i;
+    a.column[at] = l.link[i].x;
+    a.share[at] = l.share[i];
+    a.q[at] = l.q[i];
+  }
+}
+template <typename T>
 __global__ __launch_bounds__(64) void distill_known_kernel(DistillRows a) {
   extern __shared__ __align__(16) char lds[];
-  const int lane = threadIdx.x;
   const Listed l(lds, a.k);
-  for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const Entry mine(a, row, lane);
-    row_sync<64>();  // (the last row's lists have been read)
-#pragma unroll
-    for (int i = 0; i < kSlots / 64; i++) l.heads[lane + i * 64] = 0;
-    row_sync<64>();
-    list_row<T, 64>(a, row, (const T*)a.logits + (size_t)row * a.ld, a.legal ? a.legal + (size_t)row * a.ld_legal : nullptr, l, mine,
-                    [](int c) { return c % kSlots; });
-    const Known known = know(a, row, l);
-    if (lane == 0) a.known[row] = known;
-    for (int i = lane; i < a.k; i += 64) {
-      const size_t at = (size_t)row * a.k + i;
-      a.column[at] = l.link[i].x;
-      a.share[at] = l.share[i];
-      a.q[at] = l.q[i];
-    }
-  }
+  for (int row = blockIdx.x; row < a.rows; row += gridDim.x) know_row<T>(a, row, l);
 }
 
 // What a row's workgroup has of its entries in LDS, copied there by NT threads that ask for theirs before they ask for the row, as what is
@@ -652,6 +654,7 @@ __device__ __forceinline__ void losses_of_parts(const DistillRows& a, int first,
 // from the caches. Few such rows are cut into parts for as many workgroups: a launch for the parts' sums (PARTS), and one that joins
 // them and writes the gradient (JOIN): 301 rows of 100003 f16 62 us whole, 44 in parts.
 enum { WHOLE, PARTS, JOIN };
+constexpr int kKnowing = 4;
 template <typename T, int NT, int E, int STAGE>
 __global__ __launch_bounds__(NT) void distill_long_kernel(DistillRows a) {
   constexpr int V = kVec<T>, SLOTS = NT * E;
@@ -667,16 +670,30 @@ __global__ __launch_bounds__(NT) void distill_long_kernel(DistillRows a) {
     losses_of_parts(a, tid, NT, c2);
     return;
   }
-  for (int id = blockIdx.x; id < a.rows * (STAGE == WHOLE ? 1 : a.split); id += gridDim.x - (STAGE == JOIN)) {
+  if (STAGE == PARTS && (int)blockIdx.x < a.knowing) {
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (wave < kKnowing)
+      for (int row = blockIdx.x * kKnowing + wave; row < a.rows; row += a.knowing * kKnowing) know_row<T>(a, row, Listed(lds + wave * a.list_bytes, a.k));
+    return;
+  }
+  for (int id = blockIdx.x - (STAGE == PARTS ? a.knowing : 0); id < a.rows * (STAGE == WHOLE ? 1 : a.split); id += gridDim.x - (STAGE == JOIN)) {
     const int row = STAGE == WHOLE ? id : id / a.split, part = STAGE == WHOLE ? 0 : id - row * a.split;
     const int begin = part * a.span, end = STAGE == WHOLE ? INT_MAX : begin + a.span;  // its chunks, whole pieces of SLOTS
     const T* z = (const T*)a.logits + (size_t)row * a.ld;
     const unsigned char* legal = a.legal ? a.legal + (size_t)row * a.ld_legal : nullptr;
     T* g = a.grad ? (T*)a.grad + (size_t)row * a.ld_grad : nullptr;
     const Chunks<T> at(a.columns, g ? g : z);
-    const Asked<NT> asked(a, row);
-    lds_barrier();
-    asked.begin(a, row, l);
+    if (STAGE == PARTS) {  // (whether an entry counts is not asked: an illegal column is not among the others either)
+      lds_barrier();
+      for (int i = tid; i < l.k; i += NT) {
+        const int c = a.index[(size_t)row * a.ld_index + i];
+        l.link[i].x = (unsigned)c < (unsigned)a.columns ? c : -1;
+      }
+    } else {
+      const Asked<NT> asked(a, row);
+      lds_barrier();
+      asked.begin(a, row, l);
+    }
 #pragma unroll
     for (int e = 0; e < E; e++) l.heads[tid + e * NT] = 0;
     lds_barrier();
@@ -763,6 +780,18 @@ void distill_typed(DistillRows p, hipStream_t s) {
     p.list_bytes = (int)Listed::bytes(64 * 2, p.k);
     return launch_k(distill_wave_kernel<T, 2>, dim3(row_grid(p.rows, 4)), 256, p.list_bytes * 4, s, p);
   }
+  const RowParts cut = r.threads == 0 ? row_parts<T>(p.rows, p.columns, 512 * 4) : RowParts{1, 0};
+  if (cut.split > 1) {
+    const size_t lds = Copied::bytes(512 * 4, p.k);
+    p.split = cut.split;
+    p.span = cut.span;
+    p.list_bytes = (int)Listed::bytes(kSlots, p.k);
+    // (With few entries each row's are known beside the parts, which take the listed columns as they stand.)
+    if (p.k <= kWaveEntries) p.knowing = (p.rows + kKnowing - 1) / kKnowing;
+    else launch_k(distill_known_kernel<T>, groups, 64, p.list_bytes, s, p);
+    launch_k(distill_long_kernel<T, 512, 4, PARTS>, dim3(p.rows * p.split + p.knowing), 512, std::max(lds, (size_t)p.list_bytes * (p.knowing ? kKnowing : 0)), s, p);
+    return launch_k(distill_long_kernel<T, 512, 4, JOIN>, dim3(p.grad ? p.rows * p.split + 1 : 1), 512, lds, s, p);
+  }
   launch_k(distill_known_kernel<T>, groups, 64, Listed::bytes(kSlots, p.k), s, p);
   if (r.threads == 64 && p.k <= kWaveEntries) {
     p.list_bytes = (int)Copied::bytes(64 * 8, p.k);
@@ -771,19 +800,11 @@ void distill_typed(DistillRows p, hipStream_t s) {
   else if (r.threads == 256) launch_k(distill_row_kernel<T, 256, 8>, groups, 256, Copied::bytes(256 * 8, p.k), s, p);
   else if (r.threads == 512) launch_k(distill_row_kernel<T, 512, 8>, groups, 512, Copied::bytes(512 * 8, p.k), s, p);
   else {
-    const RowParts cut = row_parts<T>(p.rows, p.columns, 512 * 4);
-    p.split = cut.split;
-    p.span = cut.span;
-    const size_t lds = Copied::bytes(512 * 4, p.k);
-    if (p.split > 1) {
-      launch_k(distill_long_kernel<T, 512, 4, PARTS>, dim3(p.rows * p.split), 512, lds, s, p);
-      return launch_k(distill_long_kernel<T, 512, 4, JOIN>, dim3(p.grad ? p.rows * p.split + 1 : 1), 512, lds, s, p);
-    }
     // (As many chunks a thread again where rows are not cut: 4093 x 33000 bf16 204 us by pieces, 167 held, 2048 x 50257 bf16 151 and 136; but
     // 300 x 50257 floats 58 in parts, 61 held, and rows twice as long by 1024 threads 325 where pieces take 313.)
     const long long chunks = ((long long)p.columns + kVec<T> - 1) / kVec<T> + Chunks<T>::line(p.columns) / 16;
     if (chunks <= 512 * 16) launch_k(distill_row_kernel<T, 512, 16>, groups, 512, Copied::bytes(512 * 8, p.k), s, p);
-    else launch_k(distill_long_kernel<T, 512, 4, WHOLE>, groups, 512, lds, s, p);
+    else launch_k(distill_long_kernel<T, 512, 4, WHOLE>, groups, 512, Copied::bytes(512 * 4, p.k), s, p);
   }
   launch_k(distill_loss_kernel, dim3(row_grid(p.rows, 64)), 64, 0, s, p);
 }
@@ -834,6 +855,7 @@ void launch_distill_loss(const kg_distill_loss_args& a, hipStream_t s) {
   p.parts = (Others*)(w + plan.parts);
   p.split = 1;
   p.span = 0;
+  p.knowing = 0;
   p.share = (double*)(w + plan.share);
   p.q = (double*)(w + plan.q);
   p.column = (int*)(w + plan.column);

@@ -652,7 +652,8 @@ __device__ __forceinline__ void losses_of_parts(const DistillRows& a, int first,
 
 // Longer rows: E chunks of each thread at a time relative to the running maximum, and again for the gradient, whose second reading comes
 // from the caches. Few such rows are cut into parts for as many workgroups: a launch for the parts' sums (PARTS), and one that joins
-// them and writes the gradient (JOIN): 301 rows of 100003 f16 62 us whole, 44 in parts.
+// them and writes the gradient (JOIN): 301 rows of 100003 f16 62 us whole, 44 in parts (a call 49 with the entries in a launch
+// before, 45 with workgroups for them ahead of the parts').
 enum { WHOLE, PARTS, JOIN };
 constexpr int kKnowing = 4;
 template <typename T, int NT, int E, int STAGE>

@@ -172,8 +172,10 @@ __device__ __forceinline__ Known know(const DistillRows& a, int row, const Liste
   double sum = 0.0, t_sum = 0.0, weighed = 0.0;
 #pragma unroll 1
   for (int i = lane; i < l.k; i += 64) {
-    const double z = (double)*(const float*)(l.share + i) * s - z0, t = (double)*(const float*)(l.q + i) * s - (a.lse ? (double)a.lse[row] : t0);
-    const double e = exp(z), q = l.link[i].x < 0 ? 0.0 : exp(t);
+    const float top = *(const float*)(l.q + i);
+    const double z = (double)*(const float*)(l.share + i) * s - z0, t = (double)top * s - (a.lse ? (double)a.lse[row] : t0);
+    // (+infinity is no probability: NaN also where the normaliser leaves it infinite.)
+    const double e = exp(z), q = l.link[i].x < 0 ? 0.0 : top == INFINITY ? NAN : exp(t);
     sum += e;
     t_sum += q;
     weighed += q == 0.0 ? 0.0 : q * (t - z);

@@ -43,8 +43,8 @@ __device__ __forceinline__ double correction(double off, double squares) { retur
 
 // L lanes a row: neighbours of one wave (several rows a wave below 64), or a workgroup. Lane i holds chunks i, i + L, ... of 16
 // bytes. A chunk that reaches over the row's end is its last 16 bytes instead, so that no lane takes single elements: what it has of the
-// chunk before counts there alone (first), and is stored twice, with the same values. Rows shorter than a chunk are taken by elements,
-// 0 in the words behind them.
+// chunk before counts there alone (first), and is stored twice, with the same values. Rows shorter than a chunk are taken by elements;
+// in the places behind them is 0, or the row's first element (FIRST).
 template <typename T, int L, int E>
 struct Row {
   static constexpr int V = kVec<T>, THREADS = L <= 64 ? LT : L, ROWS = THREADS / L;  // of a workgroup
@@ -56,7 +56,8 @@ struct Row {
   static __device__ __forceinline__ int first(int channels, int e) { return column(e) - start(channels, e); }
   static __device__ __forceinline__ int limit(int channels) { return min(channels, V); }
   static __device__ __forceinline__ bool whole(int channels, int e) { return (e + 1) * L * V <= channels; }
-  static __device__ __forceinline__ void load(const T* row, int channels, bool in, u32x4 (&raw)[E]) {
+  enum Behind { ZERO, FIRST };
+  static __device__ __forceinline__ void load(const T* row, int channels, bool in, u32x4 (&raw)[E], Behind behind = ZERO) {
 #pragma unroll
     for (int e = 0; e < E; e++) {
       raw[e] = u32x4{0, 0, 0, 0};
@@ -66,10 +67,11 @@ struct Row {
       } else {
         unsigned w[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int j = 0; j < V - 1; j++)
-          if (j < channels) {
-            if constexpr (sizeof(T) == 4) w[j] = ((const unsigned*)row)[j];
-            else w[j >> 1] |= (unsigned)((const unsigned short*)row)[j] << (j & 1 ? 16 : 0);
+        for (int j = 0; j < V; j++)
+          if (j < channels || behind == FIRST) {
+            const int k = j < channels ? j : 0;
+            if constexpr (sizeof(T) == 4) w[j] = ((const unsigned*)row)[k];
+            else w[j >> 1] |= (unsigned)((const unsigned short*)row)[k] << (j & 1 ? 16 : 0);
           }
         raw[e] = u32x4{w[0], w[1], w[2], w[3]};
       }
@@ -303,7 +305,7 @@ __global__ __launch_bounds__(LT) void layer_norm_back_held_kernel(LayerArgs a) {
     const int row = first + threadIdx.x / L;
     const bool in = row < a.rows;
     u32x4 x[E], dy[E];
-    R::load((const T*)a.x + (size_t)row * a.ldx, a.channels, in, x);
+    R::load((const T*)a.x + (size_t)row * a.ldx, a.channels, in, x, R::FIRST);
     R::load((const T*)a.dy + (size_t)row * a.lddy, a.channels, in, dy);
     const float mean = a.rms || !in ? 0.f : a.mean[row], rstd = in ? a.rstd[row] : 0.f;
     float q[2] = {0.f, 0.f};
@@ -314,7 +316,7 @@ __global__ __launch_bounds__(LT) void layer_norm_back_held_kernel(LayerArgs a) {
       float t = 0.f, u = 0.f;
 #pragma unroll
       for (int j = 0; j < V; j++) {
-        // (Behind a short row's end dy is 0.)
+        // (Behind a short row's end dy is 0 and h is an element's: of 0 less a large mean it would be infinite, and their product NaN.)
         const float g = whole || j >= least ? element<T>(dy[e], j) : 0.f, d = g * gamma[e][j], h = (element<T>(x[e], j) - mean) * rstd;
         t += d;
         u = __builtin_fmaf(d, h, u);

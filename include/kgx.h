@@ -555,8 +555,9 @@ size_t kg_group_norm_workspace(int batch, int points, int channels, int groups, 
 /* Layer norm over the `channels` of each of `rows` rows, and RMS norm (`rms`: mean 0, variance the mean of the squares):
  *   rstd = 1 / sqrt(variance + eps), y = (x - mean) rstd gamma + beta.
  * The statistics are outputs for the backward pass. NaN in a row makes that row NaN, and its channel of dgamma; so does infinity (with `rms`
- * the row's other elements of y are beta: rstd is 0). The sums are float: where the squares' passes its range rstd is 0 too. At most 2^30 rows
- * of 2^30 channels. */
+ * the row's other elements of y are beta: rstd is 0). The squares' sum is float: where it passes float's range rstd is 0 too, and y beta
+ * (an element whose distance from the mean passes the range is NaN then); a mean is in the range as its elements are. At most
+ * 2^30 rows of 2^30 channels. */
 typedef struct {
   int rows, channels;
   int type;                /* of x, y, dy and dx */

@@ -6,6 +6,8 @@
 // The variance comes from the deviations d from the mean as a float sum gives it. Where that mean is far from 0, their own mean says
 // what its rounding left, and is taken out of both (correction).
 #include <algorithm>
+#include <cfloat>
+#include <cmath>
 
 #include "kgx_device.h"
 #include "kgx_learn.h"
@@ -29,7 +31,16 @@ struct LayerArgs {
   struct RowMeans* means;  // [rows], of wide rows
   int rows, channels, rms, past, split;
   double eps, inverse;  // inverse: 1 / channels
+  float shrink;         // of the elements in a sum for the mean: below 1 / channels, a power of 2, which changes no bit but an exponent's
+  double grow;          // 1 / (shrink channels)
 };
+
+// The mean from the sum of elements times shrink, which is in float's range as they are. (Rounded, the mean of elements near the range's end
+// may lie past it.)
+__device__ __forceinline__ float mean_of(const LayerArgs& a, double sum) {
+  const float mean = (float)(sum * a.grow);
+  return isinf(mean) && !isinf(sum) ? copysignf(FLT_MAX, mean) : mean;
+}
 
 // (NaN stays NaN: a comparison, not fmax.)
 __device__ __forceinline__ float root_of(double variance, double eps) { return (float)(1.0 / sqrt((variance < 0.0 ? 0.0 : variance) + eps)); }
@@ -161,11 +172,11 @@ __global__ __launch_bounds__((Row<T, L, E>::THREADS)) void layer_norm_held_kerne
         const int least = R::first(a.channels, e), limit = R::limit(a.channels);
         float t = 0.f;
 #pragma unroll
-        for (int j = 0; j < V; j++) t += whole || (j >= least && j < limit) ? element<T>(raw[e], j) : 0.f;
+        for (int j = 0; j < V; j++) t = __builtin_fmaf(whole || (j >= least && j < limit) ? element<T>(raw[e], j) : 0.f, a.shrink, t);
         s[0] += t;
       }
       R::sum(s, red[turn]);
-      mean = (float)((double)s[0] * a.inverse);
+      mean = mean_of(a, (double)s[0]);
     }
     float q[2] = {0.f, 0.f};  // of the deviations, and of their squares
 #pragma unroll
@@ -228,15 +239,15 @@ __global__ __launch_bounds__(NT) void layer_norm_wide_kernel(LayerArgs a) {
         float t = 0.f;
         if (at.whole(e * NT, NT)) {
 #pragma unroll
-          for (int j = 0; j < V; j++) t += element<T>(raw[e], j);
+          for (int j = 0; j < V; j++) t = __builtin_fmaf(element<T>(raw[e], j), a.shrink, t);
         } else {
 #pragma unroll
-          for (int j = 0; j < V; j++) t += j >= first && j < limit ? element<T>(raw[e], j) : 0.f;
+          for (int j = 0; j < V; j++) t = __builtin_fmaf(j >= first && j < limit ? element<T>(raw[e], j) : 0.f, a.shrink, t);
         }
         s[0] += t;
       }
       R::sum(s, red[turn]);
-      mean = (float)((double)s[0] * a.inverse);
+      mean = mean_of(a, (double)s[0]);
     }
     forget<E>(raw);
     float q[2] = {0.f, 0.f};  // of the deviations, and of their squares
@@ -479,8 +490,8 @@ __global__ __launch_bounds__(LT) void layer_norm_kernel(LayerArgs a) {
     float mean = 0.f;
     if (!a.rms) {
       float sum = 0.f;
-      for (int c = tid; c < a.channels; c += LT) sum += (float)x[c];
-      mean = (float)(row_sum<LT>(sum, red) * a.inverse);
+      for (int c = tid; c < a.channels; c += LT) sum = __builtin_fmaf((float)x[c], a.shrink, sum);
+      mean = mean_of(a, row_sum<LT>(sum, red));
     }
     float off = 0.f, square = 0.f;
     for (int c = tid; c < a.channels; c += LT) {
@@ -703,6 +714,8 @@ LayerArgs args_of(const kg_layer_norm_args& a) {
   p.split = 0;
   p.eps = a.eps;
   p.inverse = 1.0 / a.channels;
+  p.shrink = (float)std::ldexp(0.5, -(int)std::ceil(std::log2((double)a.channels)));
+  p.grow = p.inverse / (double)p.shrink;
   return p;
 }
 

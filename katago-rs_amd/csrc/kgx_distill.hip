@@ -102,7 +102,7 @@ struct Entry {
 };
 
 // Fills the lists of a row, whose heads are 0, with NT threads; slot: a column's head; mine: this thread's first entry. The logits of
-// both sides are left, as floats, in share and q.
+// both sides are left in share and q.
 template <typename T, int NT, typename Slot>
 __device__ __forceinline__ void list_row(const DistillRows& a, int row, const T* z, const unsigned char* legal, const Listed& l, const Entry& mine,
                                          const Slot& slot) {
@@ -128,8 +128,8 @@ __device__ __forceinline__ void list_row(const DistillRows& a, int row, const T*
         if (h - 1 < i && l.link[h - 1].x == own.c) counts = false;
       if (!counts) gone |= 1u << b;
     }
-    *(float*)(l.share + i) = counts ? v : -INFINITY;
-    *(float*)(l.q + i) = counts ? own.t : -INFINITY;
+    l.share[i] = (double)(counts ? v : -INFINITY);
+    l.q[i] = (double)(counts ? own.t : -INFINITY);
   }
   row_sync<NT>();
 #pragma unroll 1
@@ -160,8 +160,8 @@ __device__ __forceinline__ Known know(const DistillRows& a, int row, const Liste
   bool any = false;
 #pragma unroll 1
   for (int i = lane; i < l.k; i += 64) {
-    n.top = fmaxf(n.top, *(const float*)(l.share + i));
-    t_top = fmaxf(t_top, *(const float*)(l.q + i));
+    n.top = fmaxf(n.top, (float)l.share[i]);
+    t_top = fmaxf(t_top, (float)l.q[i]);
     any |= l.link[i].x >= 0;
   }
   n.any = __ballot(any) != 0;
@@ -172,8 +172,7 @@ __device__ __forceinline__ Known know(const DistillRows& a, int row, const Liste
   double sum = 0.0, t_sum = 0.0, weighed = 0.0;
 #pragma unroll 1
   for (int i = lane; i < l.k; i += 64) {
-    const float top = *(const float*)(l.q + i);
-    const double z = (double)*(const float*)(l.share + i) * s - z0, t = (double)top * s - (a.lse ? (double)a.lse[row] : t0);
+    const double top = l.q[i], z = l.share[i] * s - z0, t = top * s - (a.lse ? (double)a.lse[row] : t0);
     // (+infinity is no probability: NaN also where the normaliser leaves it infinite.)
     const double e = exp(z), q = l.link[i].x < 0 ? 0.0 : top == INFINITY ? NAN : exp(t);
     sum += e;
@@ -535,11 +534,11 @@ struct Asked {
     c = a.column[at];
     share = a.share[at];
     q = a.q[at];
-    known = ((const unsigned*)(a.known + row))[min(i, (int)(sizeof(Known) / 4) - 1)];
+    __builtin_memcpy(&known, (const char*)(a.known + row) + min(i, (int)(sizeof(Known) / 4) - 1) * 4, 4);
   }
   __device__ __forceinline__ void begin(const DistillRows& a, int row, const Copied& l) const {
     const int tid = row_thread<NT>();
-    if (tid < (int)(sizeof(Known) / 4)) ((unsigned*)l.known)[tid] = known;
+    if (tid < (int)(sizeof(Known) / 4)) __builtin_memcpy((char*)l.known + tid * 4, &known, 4);
 #pragma unroll 1
     for (int i = tid; i < l.k; i += NT) {
       const size_t at = (size_t)row * a.k + i;

@@ -2,8 +2,10 @@
 // current device restored.
 #include "kgx_learn.h"
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 #include <limits>
 #include <string>
 
@@ -58,6 +60,57 @@ void check_rows(const void* p, long long rows, long long width, long long ld, in
   if (rows > 1 && ld < width) bad(op, std::string("the row stride of ") + name + " is less than its row");
   if (ld < 0 || (rows > 1 && ld > std::numeric_limits<long long>::max() / 8 / rows)) bad(op, std::string("the row stride of ") + name + " is out of range");
   if (!aligned(p, size_of(type))) bad(op, std::string(name) + " is not aligned to its elements");
+}
+
+// What a call reads or writes: `rows` rows of `width` bytes, `step` bytes apart (width <= step where there are several).
+typedef __int128 wide;
+struct Region {
+  const char* name;
+  wide begin, end;  // end: past its last byte; begin where there is nothing
+  long long rows;
+  wide width, step;
+};
+Region matrix(const char* name, const void* p, long long rows, long long width, long long ld, int size) {
+  const wide begin = (wide)(uintptr_t)p, bytes = (wide)width * size, step = rows > 1 ? (wide)ld * size : bytes;
+  return {name, begin, p && rows > 0 ? begin + (rows - 1) * step + bytes : begin, rows, bytes, step};
+}
+Region vector(const char* name, const void* p, long long n, int size = 4) { return matrix(name, p, 1, n, 0, size); }
+
+// The least x >= 0 for which a x mod m is in [lo, hi], 0 < lo <= hi < m and 0 <= a < m; -1 where there is none. A multiple of a reaches lo before
+// it passes m, or none does without passing m: a x in [lo + m y, hi + m y] then, and the least y is such a question of m y mod a.
+wide first_within(wide a, wide m, wide lo, wide hi) {
+  if (a == 0) return -1;
+  const wide x = (lo + a - 1) / a;
+  if (x * a <= hi) return x;
+  // (No multiple of a is in [lo, hi]: -hi mod a is below -lo mod a, and neither is 0.)
+  const wide y = first_within(m % a, a, (a - hi % a) % a, (a - lo % a) % a);
+  return y < 0 ? -1 : (lo + m * y + a - 1) / a;
+}
+
+// Whether two regions share a byte: views side by side of one buffer do not, whatever their strides.
+bool share(const Region& a, const Region& b) {
+  if (b.begin >= a.end || a.begin >= b.end || a.begin == a.end || b.begin == b.end) return false;
+  const wide at = b.begin - a.begin;
+  // b's rows first ... last touch a's extent.
+  const wide first = at + b.width > 0 ? 0 : (-at - b.width) / b.step + 1, last = std::min((wide)b.rows - 1, (a.end - 1 - b.begin) / b.step);
+  if (first > last) return false;
+  // One that begins within a's extent lies between two of a's rows if its start is in [a.width, a.step - b.width] of one's.
+  const wide start = at + first * b.step;
+  if (start < 0 || a.width > a.step - b.width) return true;
+  const wide room = a.width + b.width - 2, r = (start + b.width - 1) % a.step;
+  if (r <= room) return true;
+  const wide next = first_within(b.step % a.step, a.step, a.step - r, a.step - r + room);
+  return next >= 0 && next <= last - first;
+}
+
+// Outputs, and what a call has of its own until it has run, share no memory with anything else of the call.
+void check_apart(std::initializer_list<Region> out, std::initializer_list<Region> in, const char* op) {
+  for (const Region* o = out.begin(); o != out.end(); o++) {
+    for (const Region* r = o + 1; r != out.end(); r++)
+      if (share(*o, *r)) bad(op, std::string(o->name) + " must not overlap " + r->name);
+    for (const Region& r : in)
+      if (share(*o, r)) bad(op, std::string(o->name) + " must not overlap " + r.name);
+  }
 }
 
 constexpr int kMaxRows = 1 << 30;     // a workgroup's step over them stays below 2^31
@@ -119,11 +172,18 @@ void check_distill(const kg_distill_loss_args& a) {
   if (a.grad) check_rows(a.grad, a.rows, a.columns, a.ld_grad, a.type, op, "grad");
   if (a.legal) need(a.ld_legal >= (a.rows > 1 ? a.columns : 0), op, "the row stride of legal is less than its row");
   need(a.loss, op, "null argument");
-  need(!a.grad || (a.grad != a.logits && a.grad != a.top_logits), op, "grad must not overlap an input");
-  if (kgx::distill_loss_workspace(a.rows, a.columns, a.k)) {
+  const size_t work = kgx::distill_loss_workspace(a.rows, a.columns, a.k);
+  if (work) {
     need(a.workspace, op, "workspace is null");
     need(aligned(a.workspace, 16), op, "workspace is not aligned to 16 bytes");
   }
+  const int size = (int)size_of(a.type);
+  check_apart({matrix("grad", a.grad, a.rows, a.columns, a.ld_grad, size), vector("loss", a.loss, a.rows), vector("workspace", a.workspace, work, 1)},
+              {matrix("logits", a.logits, a.rows, a.columns, a.ld, size), matrix("legal", a.legal, a.rows, a.columns, a.ld_legal, 1),
+               matrix("top_index", a.top_index, a.rows, a.k, a.ld_index, 4),
+               matrix("top_logits", a.top_logits, a.rows, a.k, a.ld_top, (int)size_of(a.top_type)), vector("teacher_lse", a.teacher_lse, a.rows),
+               vector("weight", a.weight, a.rows)},
+              op);
 }
 
 void check_state(const kg_adamw_state& s, const char* op) {
@@ -205,13 +265,20 @@ void check_layer_norm(const kg_layer_norm_args& a, bool backward) {
   if (backward) {
     check_rows(a.dy, a.rows, a.channels, a.lddy, a.type, op, "dy");
     check_rows(a.dx, a.rows, a.channels, a.lddx, a.type, op, "dx");
-    need(a.dx != a.x && a.dx != a.dy, op, "dx must not overlap an input");
     need(a.workspace, op, "workspace is null");
     need(aligned(a.workspace, 16), op, "workspace is not aligned to 16 bytes");
   } else {
     check_rows(a.y, a.rows, a.channels, a.ldy, a.type, op, "y");
-    need(a.y != a.x, op, "y must not overlap x");
   }
+  const int size = (int)size_of(a.type);
+  const Region x = matrix("x", a.x, a.rows, a.channels, a.ldx, size), gamma = vector("gamma", a.gamma, a.channels);
+  const Region mean = vector("mean", a.rms ? nullptr : a.mean, a.rows), rstd = vector("rstd", a.rstd, a.rows);
+  if (backward)
+    check_apart({matrix("dx", a.dx, a.rows, a.channels, a.lddx, size), vector("dgamma", a.dgamma, a.channels), vector("dbeta", a.dbeta, a.channels),
+                 vector("workspace", a.workspace, kgx::layer_norm_workspace(a.rows, a.channels), 1)},
+                {x, matrix("dy", a.dy, a.rows, a.channels, a.lddy, size), gamma, mean, rstd}, op);
+  else
+    check_apart({matrix("y", a.y, a.rows, a.channels, a.ldy, size), mean, rstd}, {x, gamma, vector("beta", a.beta, a.channels)}, op);
 }
 
 void check_embedding(const kg_embedding_args& a, bool backward) {
@@ -228,14 +295,20 @@ void check_embedding(const kg_embedding_args& a, bool backward) {
   need(a.tokens && aligned(a.tokens, 4), op, "tokens is null or not aligned to its elements");
   if (backward) {
     check_rows(a.dy, a.count, a.channels, a.ld_dy, a.type, op, "dy");
-    need(a.grad != a.dy, op, "grad must not overlap an input");
     need(a.workspace, op, "workspace is null");
     need(aligned(a.workspace, 16), op, "workspace is not aligned to 16 bytes");
   } else {
     check_rows(a.table, a.vocab, a.channels, a.ld_table, a.type, op, "table");
     check_rows(a.y, a.count, a.channels, a.ld_y, a.type, op, "y");
-    need(a.y != a.table, op, "y must not overlap the table");
   }
+  const int size = (int)size_of(a.type);
+  const Region tokens = vector("tokens", a.tokens, a.count);
+  if (backward)
+    check_apart({matrix("grad", a.grad, a.vocab, a.channels, a.ld_grad, (int)size_of(a.grad_type)),
+                 vector("workspace", a.workspace, kgx::embedding_backward_workspace(a.count, a.vocab, a.channels), 1)},
+                {matrix("dy", a.dy, a.count, a.channels, a.ld_dy, size), tokens}, op);
+  else
+    check_apart({matrix("y", a.y, a.count, a.channels, a.ld_y, size)}, {matrix("table", a.table, a.vocab, a.channels, a.ld_table, size), tokens}, op);
 }
 
 }  // namespace

@@ -62,6 +62,16 @@ void check_rows(const void* p, long long rows, long long width, long long ld, in
   if (!aligned(p, size_of(type))) bad(op, std::string(name) + " is not aligned to its elements");
 }
 
+// Vectors of floats, NULL where a call has none.
+struct Floats {
+  const char* name;
+  const float* p;
+};
+void check_floats(std::initializer_list<Floats> vectors, const char* op) {
+  for (const Floats& v : vectors)
+    if (!aligned(v.p, 4)) bad(op, std::string(v.name) + " is not aligned to its elements");
+}
+
 // What a call reads or writes: `rows` rows of `width` bytes, `step` bytes apart (width <= step where there are several).
 typedef __int128 wide;
 struct Region {
@@ -172,6 +182,7 @@ void check_distill(const kg_distill_loss_args& a) {
   if (a.grad) check_rows(a.grad, a.rows, a.columns, a.ld_grad, a.type, op, "grad");
   if (a.legal) need(a.ld_legal >= (a.rows > 1 ? a.columns : 0), op, "the row stride of legal is less than its row");
   need(a.loss, op, "null argument");
+  check_floats({{"loss", a.loss}, {"weight", a.weight}, {"teacher_lse", a.teacher_lse}}, op);
   const size_t work = kgx::distill_loss_workspace(a.rows, a.columns, a.k);
   if (work) {
     need(a.workspace, op, "workspace is null");
@@ -261,6 +272,9 @@ void check_layer_norm(const kg_layer_norm_args& a, bool backward) {
   if (!backward) need(usable_eps(a.eps), op, "eps must be positive, at least 2^-126");
   if (!a.rows) return;
   need((a.mean || a.rms) && a.rstd, op, "mean or rstd is null");
+  check_floats({{"gamma", a.gamma}, {"mean", a.rms ? nullptr : a.mean}, {"rstd", a.rstd}}, op);
+  if (backward) check_floats({{"dgamma", a.dgamma}, {"dbeta", a.dbeta}}, op);
+  else check_floats({{"beta", a.beta}}, op);
   check_rows(a.x, a.rows, a.channels, a.ldx, a.type, op, "x");
   if (backward) {
     check_rows(a.dy, a.rows, a.channels, a.lddy, a.type, op, "dy");

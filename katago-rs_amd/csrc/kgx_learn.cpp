@@ -426,7 +426,11 @@ int kg_group_norm_backward(int device, void* stream, const kg_group_norm_args* a
   });
 }
 
-size_t kg_distill_loss_workspace(int rows, int columns, int k) { return kgx::distill_loss_workspace(rows, columns, k); }
+// (Sizes that no call takes need none, and would overflow the sums.)
+size_t kg_distill_loss_workspace(int rows, int columns, int k) {
+  if (rows < 1 || rows > kMaxRows || columns < 1 || columns > kMaxColumns || k < 1 || k > KG_DISTILL_MAX_K) return 0;
+  return kgx::distill_loss_workspace(rows, columns, k);
+}
 
 int kg_distill_loss(int device, void* stream, const kg_distill_loss_args* args) {
   return guarded([&] {
@@ -438,7 +442,10 @@ int kg_distill_loss(int device, void* stream, const kg_distill_loss_args* args) 
   });
 }
 
-size_t kg_layer_norm_workspace(int rows, int channels) { return kgx::layer_norm_workspace(rows, channels); }
+size_t kg_layer_norm_workspace(int rows, int channels) {
+  if (rows < 1 || rows > kMaxRows || channels < 1 || channels > kMaxColumns) return 0;
+  return kgx::layer_norm_workspace(rows, channels);
+}
 
 int kg_layer_norm(int device, void* stream, const kg_layer_norm_args* args) {
   return guarded([&] {
@@ -460,7 +467,7 @@ int kg_layer_norm_backward(int device, void* stream, const kg_layer_norm_args* a
 }
 
 size_t kg_embedding_backward_workspace(int count, int vocab, int channels) {
-  if (count < 1 || vocab < 1 || channels < 1) return 0;
+  if (count < 1 || count > kMaxRows || vocab < 1 || vocab > kMaxRows || channels < 1 || channels > kMaxColumns) return 0;
   return kgx::embedding_backward_workspace(count, vocab, channels);
 }
 

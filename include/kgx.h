@@ -452,7 +452,7 @@ typedef struct {
   void* grad;                  /* [rows] rows of ld_grad (columns past `columns` stay as they are); or NULL */
   long long ld_grad;
   void* workspace;             /* kg_distill_loss_workspace(rows, columns, k) bytes, 16-byte aligned, this call's own until it has run;
-                                  NULL where that is 0 */
+                                  NULL where that is 0: up to 448 columns with up to 256 entries, whatever the rows */
 } kg_distill_loss_args;
 int kg_distill_loss(int device, void* stream, const kg_distill_loss_args* args);
 size_t kg_distill_loss_workspace(int rows, int columns, int k);

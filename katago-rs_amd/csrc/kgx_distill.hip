@@ -770,7 +770,7 @@ __global__ __launch_bounds__(NT) void distill_long_kernel(DistillRows a) {
   }
 }
 
-// Rows that a wave takes alone, whatever their type: they need no workspace.
+// Rows that a wave takes alone, whatever their type: they need no workspace, as the header promises.
 constexpr int kWaveColumns = 448, kWaveEntries = 256;
 
 template <typename T>

@@ -252,7 +252,7 @@ def distill_loss(logits, top_index, top_logits, *, legal=None, weight=None, logi
         g, ld_g = grad.data_ptr(), v
     loss = logits.new_empty(n, dtype=torch.float32)
     L = _library()
-    # (A board's rows need none: up to 448 columns with up to 256 entries.)
+    # (Rows for which the header promises that none is needed, a board's among them, are not asked about: a small call is its host time.)
     work = _workspace(L.kg_distill_loss_workspace(n, v, k) if v > 448 or k > 256 else 0, logits.device)
     try:
         args = _DISTILL_ARGS.pack(n, v, k, TYPES[logits.dtype], TYPES[top_logits.dtype], ptr, ld, lg, ld_lg, top_index.data_ptr(),

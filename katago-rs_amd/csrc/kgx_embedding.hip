@@ -368,7 +368,7 @@ __global__ __launch_bounds__(ET) void embedding_sums_kernel(SumArgs a) {
                  (gridDim.x - a.sum_groups) * (ET / 64));
     return;
   }
-  __shared__ float ends[2][V][ET];  // a share's sum of a run from before it, and of one that goes on behind it
+  __shared__ float ends[V][ET];     // a share's sum of a run from before it
   __shared__ int firsts[SHARES];    // the first key of each share, -1 where it has no token
   const int tid = threadIdx.x, share = L == 64 ? __builtin_amdgcn_readfirstlane(tid / L) : tid / L;
   const int range = blockIdx.x / a.slabs, column = ((blockIdx.x - range * a.slabs) * L + tid % L) * V;
@@ -383,9 +383,9 @@ __global__ __launch_bounds__(ET) void embedding_sums_kernel(SumArgs a) {
   const auto write = [&](int key) {
     if (in) put_vector<G, V>((G*)a.grad + (size_t)key * a.ld_grad + c, least, sum, a.scale, a.accumulate);
   };
-  const auto keep = [&](int side) {
+  const auto keep = [&] {
 #pragma unroll
-    for (int j = 0; j < V; j++) ends[side][j][tid] = sum[j];
+    for (int j = 0; j < V; j++) ends[j][tid] = sum[j];
   };
   bool tail = false;  // a run that begins in this share goes on behind it
   if (first < last) {
@@ -420,7 +420,7 @@ __global__ __launch_bounds__(ET) void embedding_sums_kernel(SumArgs a) {
     const auto add = [&](int k, const Columns<T, V>& from) {
       if (k >= a.vocab) return;
       if (k != run) {
-        if (before) keep(0);
+        if (before) keep();
         else write(run);
 #pragma unroll
         for (int j = 0; j < V; j++) sum[j] = 0.f;
@@ -447,7 +447,7 @@ __global__ __launch_bounds__(ET) void embedding_sums_kernel(SumArgs a) {
     }
     if (run < a.vocab) {
       tail = !before && next == run;
-      if (before) keep(0);
+      if (before) keep();
       else if (!tail) write(run);
     }
   } else if (tid % L == 0) {
@@ -460,7 +460,7 @@ __global__ __launch_bounds__(ET) void embedding_sums_kernel(SumArgs a) {
     int s = share + 1;
     for (; s < SHARES && firsts[s] == key; s++) {
 #pragma unroll
-      for (int j = 0; j < V; j++) sum[j] += ends[0][j][s * L + tid % L];
+      for (int j = 0; j < V; j++) sum[j] += ends[j][s * L + tid % L];
     }
     return (s == SHARES || begin + s * each >= end) && end < a.count && (int)a.keys[end] == key;  // goes on behind the range
   };
@@ -474,7 +474,7 @@ __global__ __launch_bounds__(ET) void embedding_sums_kernel(SumArgs a) {
   if (from_before) {
     const int key = firsts[0];
 #pragma unroll
-    for (int j = 0; j < V; j++) sum[j] = ends[0][j][tid];
+    for (int j = 0; j < V; j++) sum[j] = ends[j][tid];
     collect(key);  // (with the shares behind that begin with it)
     leave(0);
   }
@@ -648,8 +648,9 @@ int lanes_of(int chunks) {
   while (lanes < chunks && lanes < 64) lanes *= 2;
   return lanes;
 }
-// (A lane's share of the tokens leaves some 4096 waves, 8 tokens at least and 64 at most, a multiple of 8. It is that of the type whose
-// rows take the fewest lanes: ranges, and with them the workspace, are the same for every type.)
+// (A range is ET / lanes shares of tokens that leave some 4096 waves, 8 tokens at least and 64 at most, a multiple of 8, for the type whose
+// rows take the fewest lanes: ranges, and with them the workspace, are the same for every type. Where the sums' launch has other lanes a row, its
+// shares are as many times longer or shorter: 4 to 256 tokens, a multiple of 4.)
 Plan plan_of(int count, int vocab, int channels) {
   Plan p = {};
   if (count > kRanked) {

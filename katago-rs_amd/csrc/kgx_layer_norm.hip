@@ -667,7 +667,6 @@ Shape forward_shape(const LayerArgs& p) {
   if (least <= 256) return {64, (least + 63) / 64};
   if (chunks <= 512) return {256, 2};
   if (chunks <= 1024) return {256, 4};
-  if (chunks <= 1536) return {512, 3};
   if (chunks <= 2048) return {512, 4};
   if (chunks <= 4096) return {1024, 4};
   return {};
@@ -737,7 +736,6 @@ void forward_typed(const LayerArgs& p, hipStream_t s) {
   else if (r.lanes == 64) forward_held<T, 64, 4>(p, s);
   else if (r.lanes == 256 && r.each == 2) launch_k(layer_norm_wide_kernel<T, 256, 2>, grid, 256, 0, s, p);
   else if (r.lanes == 256) launch_k(layer_norm_wide_kernel<T, 256, 4>, grid, 256, 0, s, p);
-  else if (r.lanes == 512 && r.each == 3) launch_k(layer_norm_wide_kernel<T, 512, 3>, grid, 512, 0, s, p);
   else if (r.lanes == 512) launch_k(layer_norm_wide_kernel<T, 512, 4>, grid, 512, 0, s, p);
   else if (r.lanes == 1024) launch_k(layer_norm_wide_kernel<T, 1024, 4>, grid, 1024, 0, s, p);
   else launch_k(layer_norm_kernel<T>, grid, LT, 0, s, p);

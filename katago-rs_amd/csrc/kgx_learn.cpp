@@ -270,11 +270,15 @@ void check_layer_norm(const kg_layer_norm_args& a, bool backward) {
        "rows must be in [0, 2^30] and channels in [1, 2^30]");
   check_type(a.type, op);
   if (!backward) need(usable_eps(a.eps), op, "eps must be positive, at least 2^-126");
+  const Region dgamma = vector("dgamma", a.dgamma, a.channels), dbeta = vector("dbeta", a.dbeta, a.channels);
+  if (backward) {  // (written for no rows too: 0)
+    check_floats({{"dgamma", a.dgamma}, {"dbeta", a.dbeta}}, op);
+    check_apart({dgamma, dbeta}, {}, op);
+  }
   if (!a.rows) return;
   need((a.mean || a.rms) && a.rstd, op, "mean or rstd is null");
   check_floats({{"gamma", a.gamma}, {"mean", a.rms ? nullptr : a.mean}, {"rstd", a.rstd}}, op);
-  if (backward) check_floats({{"dgamma", a.dgamma}, {"dbeta", a.dbeta}}, op);
-  else check_floats({{"beta", a.beta}}, op);
+  if (!backward) check_floats({{"beta", a.beta}}, op);
   check_rows(a.x, a.rows, a.channels, a.ldx, a.type, op, "x");
   if (backward) {
     check_rows(a.dy, a.rows, a.channels, a.lddy, a.type, op, "dy");
@@ -288,7 +292,7 @@ void check_layer_norm(const kg_layer_norm_args& a, bool backward) {
   const Region x = matrix("x", a.x, a.rows, a.channels, a.ldx, size), gamma = vector("gamma", a.gamma, a.channels);
   const Region mean = vector("mean", a.rms ? nullptr : a.mean, a.rows), rstd = vector("rstd", a.rstd, a.rows);
   if (backward)
-    check_apart({matrix("dx", a.dx, a.rows, a.channels, a.lddx, size), vector("dgamma", a.dgamma, a.channels), vector("dbeta", a.dbeta, a.channels),
+    check_apart({matrix("dx", a.dx, a.rows, a.channels, a.lddx, size), dgamma, dbeta,
                  vector("workspace", a.workspace, kgx::layer_norm_workspace(a.rows, a.channels), 1)},
                 {x, matrix("dy", a.dy, a.rows, a.channels, a.lddy, size), gamma, mean, rstd}, op);
   else

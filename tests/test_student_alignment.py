@@ -28,3 +28,13 @@ def test_vectors_that_are_not_aligned(kgx, name, kind, base, vectors):
 def test_what_a_call_does_not_use_is_not_looked_at(kgx):
     assert "aligned" not in said(kgx, "kg_layer_norm", abi.LayerArgs(**{**LAYER, "rms": 1, "mean": 3, "dgamma": 5, "dbeta": 6}))
     assert "aligned" not in said(kgx, "kg_layer_norm_backward", abi.LayerArgs(**{**LAYER, "rms": 1, "mean": 3, "beta": 7}))
+
+
+def test_sums_over_no_rows_are_written_too(kgx):
+    """dgamma and dbeta: they are looked at without a row as well."""
+    none = {**LAYER, "rows": 0, "x": None, "dy": None, "dx": None, "mean": None, "rstd": None, "workspace": None}
+    assert "dgamma is not aligned" in said(kgx, "kg_layer_norm_backward", abi.LayerArgs(**{**none, "dgamma": LAYER["dgamma"] + 2}))
+    assert "dbeta is not aligned" in said(kgx, "kg_layer_norm_backward", abi.LayerArgs(**{**none, "dbeta": LAYER["dbeta"] + 1}))
+    assert "dgamma must not overlap dbeta" in said(kgx, "kg_layer_norm_backward", abi.LayerArgs(**{**none, "dbeta": LAYER["dgamma"] + 44}))
+    text = said(kgx, "kg_layer_norm_backward", abi.LayerArgs(**none))
+    assert "aligned" not in text and "overlap" not in text

@@ -342,7 +342,7 @@ int kg_rmsnorm_rows_of(int rows, int channels, int region, int workgroup, int* g
  * without waiting. It allocates nothing, copies nothing and keeps nothing for a later call, so it may be captured into a
  * graph, and calls on different streams may overlap as long as their buffers differ. The argument structures are read
  * before the call returns; every pointer in them is memory of `device` unless it says otherwise, aligned to its elements.
- * The caller's current device is left as it was. Outputs must not overlap inputs. Element types are KG_PRECISION_F32, _F16
+ * The caller's current device is left as it was. Outputs must not overlap inputs (nor each other or a workspace). Element types are KG_PRECISION_F32, _F16
  * and _BF16; all sums and row statistics are float or wider. The losses take at most 2^30 rows of 2^30 columns.
  * ------------------------------------------------------------------------------------------------------------------ */
 
@@ -556,8 +556,8 @@ size_t kg_group_norm_workspace(int batch, int points, int channels, int groups, 
  *   rstd = 1 / sqrt(variance + eps), y = (x - mean) rstd gamma + beta.
  * The statistics are outputs for the backward pass. NaN in a row makes that row NaN, and its channel of dgamma; so does infinity (with `rms`
  * the row's other elements of y are beta: rstd is 0). The squares' sum is float: where it passes float's range rstd is 0 too, and y beta
- * (an element whose distance from the mean passes the range is NaN then); a mean is in the range as its elements are. At most
- * 2^30 rows of 2^30 channels. */
+ * (an element whose distance from the mean passes the range is NaN then); a mean is in the range as its elements are. The backward
+ * pass's sums, over a row and over the rows, are float: infinite, or NaN, past its range. At most 2^30 rows of 2^30 channels. */
 typedef struct {
   int rows, channels;
   int type;                /* of x, y, dy and dx */

@@ -215,7 +215,7 @@ __global__ __launch_bounds__((Row<T, L, E>::THREADS)) void layer_norm_held_kerne
 
 // Forward, a workgroup a row: its chunks lie along the lines of y (see Chunks), so that rows of odd strides are stored in whole ones, and
 // gamma and beta are read where they are used, which leaves a CU's registers to four rows and more: 2047 rows of 10007 f16 take
-// 22 us (94 with chunks from the row's start and gamma and beta in registers, one row a CU).
+// 22 us among other calls, 23 to 28 in a graph by how many buffers take turns (94 with chunks from the row's start and gamma and beta in registers, one row a CU).
 template <typename T, int NT, int E>
 __global__ __launch_bounds__(NT) void layer_norm_wide_kernel(LayerArgs a) {
   constexpr int V = kVec<T>;
